@@ -1,18 +1,16 @@
-"""Build recipe for the gfx950 GEMM library.
+"""Build recipe for the gfx950 library.
 
     python 5_amd/csrc/build.py [-v]
 
-compiles 5_amd/csrc/hcg_gemm.hip, hcg_tile.hip and hcg_mfma.hip (kernels +
-the C ABI declared in include/hcg_gemm.h, include/hcg_tile_ops.h and
-include/hcg_mfma.h) with hipcc for
-gfx950 into
-5_amd/hc/gfx950/libhcg_gfx950.so, next to the Python code that loads it
-(and, with -DHCG_STAMPS, libhcg_gfx950_stamps.so, whose GEMM kernels record
-per-workgroup timestamps for bench.py --stamps), and hcg_probe.hip (the hardware ceiling probes of include/hcg_probe.h, used
-by bench.py) into 5_amd/hc/gfx950/libhcg_probe.so, and hcg_torch.cpp (host
-code: the device-tensor binding of hcg_gemm_algo as a Python extension,
-linked against libhcg_gfx950.so) with g++ against the installed PyTorch into
-5_amd/hc/gfx950/_hcg_torch<EXT_SUFFIX>.
+compiles SRCS (the kernels and the C ABI declared in include/hcg_*.h) with
+hipcc for gfx950, each to an object of its own, in parallel, and links them
+into 5_amd/hc/gfx950/libhcg_gfx950.so, next to the Python code that loads it;
+STAMPED_SRCS again with -DHCG_STAMPS into libhcg_gfx950_stamps.so, whose GEMM
+kernels record per-workgroup timestamps for bench.py --stamps; hcg_probe.hip
+(the hardware ceiling probes of include/hcg_probe.h, used by bench.py) into
+libhcg_probe.so; and hcg_torch.cpp (host code: the device-tensor binding of
+hcg_gemm_algo as a Python extension, linked against libhcg_gfx950.so) with
+g++ against the installed PyTorch into _hcg_torch<EXT_SUFFIX>.
 hipcc cross-compiles, so this runs on a machine without a GPU.
 """
 
@@ -23,14 +21,18 @@ import shutil
 import subprocess
 import sys
 import sysconfig
+import tempfile
+from collections.abc import Callable
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 PKG = os.path.dirname(HERE)
 ROOT = os.path.dirname(PKG)
-SRCS = [os.path.join(HERE, f) for f in ("hcg_gemm.hip", "hcg_tile.hip", "hcg_mfma.hip")]
+STAMPED_SRCS = [os.path.join(HERE, f) for f in ("hcg_gemm.hip", "hcg_tile.hip", "hcg_mfma.hip")]
+SRCS = STAMPED_SRCS + [os.path.join(HERE, f) for f in ("hcg_embed.hip", "hcg_norm.hip", "hcg_loss.hip")]
 INCLUDE = os.path.join(ROOT, "include")
 OUT = os.path.join(PKG, "hc", "gfx950", "libhcg_gfx950.so")
-# The same sources with -DHCG_STAMPS: the tiled and streaming kernels record
+# The products' sources with -DHCG_STAMPS: the tiled and streaming kernels record
 # per-workgroup timestamps (bench.py --stamps); never loaded by the package.
 STAMPS_OUT = os.path.join(PKG, "hc", "gfx950", "libhcg_gfx950_stamps.so")
 PROBE_SRCS = [os.path.join(HERE, "hcg_probe.hip")]
@@ -53,7 +55,6 @@ def flags() -> list[str]:
         "-O3",
         "-std=c++20",
         "-fPIC",
-        "-shared",
         # Packed fp32 VALU forms stay disabled for all device code.
         "-Xclang",
         "-target-feature",
@@ -64,29 +65,36 @@ def flags() -> list[str]:
     ]
 
 
-def _start(srcs: list[str], out: str, extra: list[str], verbose: bool) -> tuple[subprocess.Popen, str]:
-    os.makedirs(os.path.dirname(out), exist_ok=True)
-    tmp = out + ".tmp"
-    cmd = [hipcc(), *flags(), *extra, *srcs, "-o", tmp]
+def _run(cmd: list[str], what: str, verbose: bool) -> None:
     if verbose:
         print(" ".join(cmd), flush=True)
-    proc = subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True)
-    return proc, out
-
-
-def _finish(job: tuple[subprocess.Popen, str], verbose: bool) -> str:
-    proc, out = job
-    _, stderr = proc.communicate()
+    proc = subprocess.run(cmd, capture_output=True, text=True)
     # The host pass does not know the device-only target feature; that
     # warning is expected and harmless.  Anything else is shown.
     noise = "'-packed-fp32-ops' is not a recognized feature for this target"
-    err = "\n".join(line for line in stderr.splitlines() if noise not in line)
+    err = "\n".join(line for line in proc.stderr.splitlines() if noise not in line)
     if proc.returncode != 0:
-        raise RuntimeError(f"hipcc failed for {os.path.basename(out)} ({proc.returncode}):\n{err}")
+        raise RuntimeError(f"hipcc failed for {what} ({proc.returncode}):\n{err}")
     if verbose and err.strip():
         print(err)
-    os.replace(out + ".tmp", out)
-    return out
+
+
+def _build_library(pool: ThreadPoolExecutor, srcs: list[str], out: str, extra: list[str], scratch: str,
+                   verbose: bool) -> Callable[[], str]:
+    """Starts compiling srcs; the result waits for that and links them into out."""
+    os.makedirs(os.path.dirname(out), exist_ok=True)
+    objs = [os.path.join(scratch, f"{os.path.basename(out)}.{os.path.basename(s)}.o") for s in srcs]
+    jobs = [pool.submit(_run, [hipcc(), *flags(), *extra, "-c", s, "-o", o], os.path.basename(s), verbose)
+            for s, o in zip(srcs, objs)]
+
+    def link() -> str:
+        for job in jobs:
+            job.result()
+        _run([hipcc(), *flags(), "-shared", *objs, "-o", out + ".tmp"], os.path.basename(out), verbose)
+        os.replace(out + ".tmp", out)
+        return out
+
+    return link
 
 
 def _compile_torch_binding(verbose: bool) -> str:
@@ -117,12 +125,13 @@ def _compile_torch_binding(verbose: bool) -> str:
 
 
 def build(verbose: bool = False) -> str:
-    """Builds the GEMM library, its timestamped variant, the probe library
-    and the device-tensor binding (the three hipcc runs in parallel);
-    returns the first."""
-    jobs = [_start(SRCS, OUT, [], verbose), _start(SRCS, STAMPS_OUT, ["-DHCG_STAMPS"], verbose),
-            _start(PROBE_SRCS, PROBE_OUT, [], verbose)]
-    outs = [_finish(job, verbose) for job in jobs]
+    """Builds the library, the products' timestamped variant, the probe
+    library and the device-tensor binding; returns the first."""
+    with tempfile.TemporaryDirectory() as scratch, ThreadPoolExecutor(os.cpu_count() or 4) as pool:
+        links = [_build_library(pool, srcs, out, extra, scratch, verbose)
+                 for srcs, out, extra in ((SRCS, OUT, []), (STAMPED_SRCS, STAMPS_OUT, ["-DHCG_STAMPS"]),
+                                          (PROBE_SRCS, PROBE_OUT, []))]
+        outs = [link() for link in links]
     _compile_torch_binding(verbose)
     return outs[0]
 

@@ -1,0 +1,493 @@
+// hcg_head.h -- the products of a linear head's loss on gfx950 (device code).
+//
+// Three products share one kernel: with W (vocab x width), X (tokens x width)
+// and the probabilities P (tokens x vocab),
+//   logits^T = W X^T,  dX^T = W^T P^T,  dW^T = X^T P.
+// Each is computed transposed, its "N" index (a token, or a vocabulary row)
+// across the lanes of an accumulator and its "M" index in the registers
+// (32x32x16 layout: register r of lane l is row 8 (r/4) + 4 (l/32) + r%4,
+// column l%32).  So a lane holds runs of one output row: a softmax's maximum
+// and sum over the vocabulary are reductions over registers plus one exchange
+// between the wave's halves (across lanes they would take five exchanges per
+// row and register), and outputs leave as 16-byte pieces of a row.
+//
+// TM x TN tiles by WM x WN waves; K advances 64 at a time through a ring of
+// STAGES LDS stages filled by global-to-LDS DMA.  One barrier per stage: past
+// it every wave has read the stage before, which is refilled STAGES stages
+// ahead while the next one multiplies.  Operand layouts, swizzles and fragment
+// reads are those of hcg_wg8.h.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <type_traits>
+
+#include "hcg_lm.h"
+#include "hcg_tile.h"
+
+namespace hcg {
+namespace head {
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kStep = 64;  // K per stage
+
+enum Epilogue {
+  kStats,    // softmax statistics of the logits
+  kExp,      // and exp(logit - block maximum) as f16
+  kRound,    // scaled, rounded to DT, as rows of the output
+  kPartial,  // float32, into scratch
+};
+
+struct Args {
+  const uint16_t* A;  // M side
+  const uint16_t* B;  // N side
+  int64_t lda, ldb;   // elements between rows as stored
+  int M, N, K;
+  // The live tokens, on the device: N (or, COUNT_K, K) is at most *count - count0.
+  const int* count;
+  int count0;
+  int tiles_m;
+  int splits, kchunk;  // K split s covers k [s * kchunk, (s + 1) * kchunk)
+  // kRound, kPartial: row n of the output is out + (row_of ? row_of[n] : n) * ldo
+  // (kPartial: out + split * split_stride + n * ldo).
+  void* out;
+  int64_t ldo, split_stride;
+  const int* row_of;
+  const float* add;    // [N][M] floats added to the sums, or null
+  const float* scale;  // kRound: the factor *scale * post
+  float post;
+  // kStats, kExp: per token n and block of TM / WM vocabulary rows its maximum
+  // and the sum of exp(logit - maximum), and the target's logit.
+  f32x2* stats;
+  int64_t ld_stats;
+  const int* target;
+  float* hit;
+};
+
+template <int DT>
+__device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
+  if constexpr (DT == HCG_F16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0,
+                                                  0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
+                                                   0, 0);
+}
+
+template <int N>
+__device__ __forceinline__ void wait_vm() {
+  static_assert(N >= 0 && N < 64, "vmcnt range");
+  __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | ((N >> 4) << 14));
+}
+__device__ __forceinline__ void wait_lgkm() { __builtin_amdgcn_s_waitcnt(0xc07f); }
+
+// Each stage is an LDS object of its own, named at compile time, so that the
+// compiler does not serialize a DMA into one with reads of another.
+template <int BYTES, int S>
+__device__ __forceinline__ unsigned char* ring_stage() {
+  __shared__ __attribute__((aligned(1024))) unsigned char buf[BYTES];
+  return buf;
+}
+
+// Two floats rounded to DT, packed.
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (DT == HCG_F16)
+    return __builtin_bit_cast(uint32_t, f16x2{(_Float16)a, (_Float16)b});
+  else
+    return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)a, (__bf16)b});
+}
+
+// blockIdx -> (K split, tile): each XCD (id % 8) takes a contiguous run of
+// units, within a split in groups of 4 tile rows, so that the workgroups
+// sharing an L2 share operand rows (as hcg_wg8.h's unit_of).
+__device__ __forceinline__ void unit_of(int tiles_m, int tiles_n, int splits, int wg, int& split, int& tm, int& tn) {
+  const int nt = tiles_m * tiles_n, n = nt * splits;
+  const int per = n >> 3, rem = n & 7, xcd = wg & 7, idx = wg >> 3;
+  const int unit = xcd < rem ? xcd * (per + 1) + idx : rem * (per + 1) + (xcd - rem) * per + idx;
+  split = unit / nt;
+  const int logical = unit - split * nt;
+  const int span = 4 * tiles_n;
+  const int group = logical / span, first = group * 4;
+  const int size = min(tiles_m - first, 4);
+  const int in_group = logical - group * span;
+  tm = first + in_group % size;
+  tn = in_group / size;
+}
+
+// One operand's part of a stage, T rows of the output's M or N by kStep of K,
+// loaded by NW waves.  KC: K-contiguous rows as stored (LDS rows of 64
+// elements, one per output row, a fragment is one ds_read_b128).  Otherwise K
+// rows of T contiguous output rows (LDS rows of T elements, one per k, a
+// fragment is two transposing reads).  The 16-byte chunks of an LDS row are
+// XOR-swizzled to cover all banks.
+template <int T, bool KC, int NW>
+struct Operand {
+  static constexpr int kBytes = T * kStep * 2;
+  static constexpr int kInst = kBytes / 1024 / NW;  // DMA instructions per wave per stage
+  static constexpr int kRowBytes = KC ? kStep * 2 : T * 2;
+  static constexpr int kChunks = kRowBytes / 16;
+  static constexpr int kRowsPerInst = 64 / kChunks;
+  static_assert(kInst >= 1 && kInst * NW * 1024 == kBytes, "a stage is whole DMA instructions of every wave");
+  static_assert(KC || T >= 128, "swizzle");
+
+  static __device__ __forceinline__ int swz(int row, int c) {
+    if constexpr (KC) {
+      return c ^ ((row >> 1) & 7);
+    } else {
+      const int m = row & 3;
+      return c ^ ((m >> 1) * 10 + (m & 1) * 4);
+    }
+  }
+
+  int off[kInst];  // byte offset of the lane's chunk from the stage's first element, or kOobOffset
+  int key[kInst];  // the chunk's first k from the stage's first
+
+  // extent: output rows from the tile's first on.
+  __device__ __forceinline__ void init(int wave, int lane, int extent, int64_t ld) {
+#pragma unroll
+    for (int i = 0; i < kInst; ++i) {
+      const int row = (wave * kInst + i) * kRowsPerInst + lane / kChunks;
+      const int c = swz(row, lane % kChunks);
+      const bool live = KC ? row < extent : c * 8 < extent;
+      off[i] = live ? (row * (int)ld + c * 8) * 2 : kOobOffset;
+      key[i] = KC ? c * 8 : row;
+    }
+  }
+
+  // The stage whose first element is at p, `left` of K from there on (FULL: a
+  // whole stage).  The resource starts at the stage, so offsets stay in 31
+  // bits whatever the matrix's size; chunks out of range are redirected past
+  // its extent and load zeros.
+  template <bool FULL>
+  __device__ __forceinline__ void issue(const uint16_t* p, unsigned char* st, int wave, int left) const {
+    const __amdgpu_buffer_rsrc_t r = make_rsrc(p, 0x7fffffe0);
+#pragma unroll
+    for (int i = 0; i < kInst; ++i) {
+      lds_void* dst = (lds_void*)(st + (wave * kInst + i) * 1024);
+      if constexpr (FULL)
+        dma16(r, dst, off[i]);
+      else
+        dma16(r, dst, dma_offset(key[i] < left, off[i]));
+    }
+  }
+
+  int fa;
+  int fb[2];
+  __device__ __forceinline__ void frag_init(int lane, int first) {
+    if constexpr (KC) {
+      const int row = first + (lane & 31);
+      fa = row * kRowBytes + swz(row, lane >> 5) * 16;
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int sl = lane & 15, grp = lane >> 4;
+        const int krow = 8 * (grp >> 1) + 4 * h + (sl >> 2);
+        const int col = first + 16 * (grp & 1) + 4 * (sl & 3);
+        fb[h] = krow * kRowBytes + swz(krow, col >> 3) * 16 + (col & 7) * 2;
+      }
+    }
+  }
+  // Fragment of 32-row block b and 16-wide K step s.
+  __device__ __forceinline__ u32x4 frag(const unsigned char* st, int b, int s) const {
+    if constexpr (KC) {
+      return *reinterpret_cast<const u32x4*>(st + (fa ^ (s * 32)) + b * 32 * kRowBytes);
+    } else {
+      const int x = s * 16 * kRowBytes;
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (__attribute__((address_space(3))) s16x4*)(st + (fb[0] ^ (b * 64)) + x));
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (__attribute__((address_space(3))) s16x4*)(st + (fb[1] ^ (b * 64)) + x));
+      const uint64_t l = __builtin_bit_cast(uint64_t, lo), h = __builtin_bit_cast(uint64_t, hi);
+      return u32x4{(uint32_t)l, (uint32_t)(l >> 32), (uint32_t)h, (uint32_t)(h >> 32)};
+    }
+  }
+};
+
+template <int S>
+using StageC = std::integral_constant<int, S>;
+
+// 16-bit outputs of rows n (one per lane), M columns m0 .. m0 + 31: value(r)
+// is accumulator register r.  The wave's halves exchange 4-value groups, so
+// that each lane stores whole 16-byte pieces.  `row`: the output row's
+// element 0, `extent`: its columns; a piece past them is cut (CUT) or, in
+// padded scratch, stored whole.
+template <int DT, bool CUT, class F>
+__device__ __forceinline__ void store_row16(uint16_t* row, int m0, int extent, int half, bool live, F value) {
+  typedef uint32_t u32x4u __attribute__((ext_vector_type(4), aligned(2)));
+#pragma unroll
+  for (int p = 0; p < 2; ++p) {
+    uint32_t w[2][2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t a = pack2<DT>(value(8 * p + 2 * i), value(8 * p + 2 * i + 1));
+      const uint32_t b = pack2<DT>(value(8 * p + 4 + 2 * i), value(8 * p + 5 + 2 * i));
+      const auto s = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+      w[0][i] = s[0];
+      w[1][i] = s[1];
+    }
+    const u32x4 v{w[0][0], w[0][1], w[1][0], w[1][1]};
+    const int m = m0 + 16 * p + 8 * half;
+    if (!live || m >= extent) continue;
+    if (!CUT || m + 8 <= extent) {
+      *reinterpret_cast<u32x4u*>(row + m) = v;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (m + e < extent) row[m + e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
+    }
+  }
+}
+
+// AKC, BKC: the operand is stored with K contiguous.  COUNT_K: the live
+// tokens bound K, else N.
+template <int DT, int TM, int TN, int WM, int WN, int STAGES, bool AKC, bool BKC, int EPI, bool COUNT_K>
+__global__ __launch_bounds__(64 * WM * WN, 1) void head_kernel(Args g) {
+  constexpr int NW = WM * WN;
+  constexpr int MI = TM / WM / 32, NI = TN / WN / 32;
+  static_assert(MI >= 1 && NI >= 1 && MI * WM * 32 == TM && NI * WN * 32 == TN, "wave tile");
+  constexpr int NSUB = kStep / 16;
+  using OpA = Operand<TM, AKC, NW>;
+  using OpB = Operand<TN, BKC, NW>;
+  constexpr int kStageBytes = OpA::kBytes + OpB::kBytes;
+  constexpr int kDma = OpA::kInst + OpB::kInst;
+  static_assert(STAGES >= 2 && STAGES <= 4, "stages");
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+
+  const int live = min(max(*g.count - g.count0, 0), COUNT_K ? g.K : g.N);
+  const int N = COUNT_K ? g.N : live;
+  const int tiles_n = (N + TN - 1) / TN;
+  if ((int)blockIdx.x >= g.tiles_m * tiles_n * g.splits) return;
+  int split, tm, tn;
+  unit_of(g.tiles_m, tiles_n, g.splits, blockIdx.x, split, tm, tn);
+  const int m0 = tm * TM, n0 = tn * TN;
+  const int kbeg = split * g.kchunk;
+  const int K = min((COUNT_K ? live : g.K) - kbeg, g.kchunk);
+  const int nk = max((K + kStep - 1) / kStep, 0);
+
+  const uint16_t* pa = g.A + (AKC ? (int64_t)m0 * g.lda + kbeg : (int64_t)kbeg * g.lda + m0);
+  const uint16_t* pb = g.B + (BKC ? (int64_t)n0 * g.ldb + kbeg : (int64_t)kbeg * g.ldb + n0);
+  const int64_t step_a = AKC ? kStep : kStep * g.lda, step_b = BKC ? kStep : kStep * g.ldb;
+  OpA a;
+  OpB b;
+  a.init(wave, lane, g.M - m0, g.lda);
+  b.init(wave, lane, N - n0, g.ldb);
+  a.frag_init(lane, wm * (TM / WM));
+  b.frag_init(lane, wn * (TN / WN));
+
+  f32x16 acc[MI][NI];
+#pragma unroll
+  for (int i = 0; i < MI; ++i)
+#pragma unroll
+    for (int j = 0; j < NI; ++j) acc[i][j] = f32x16{};
+
+  u32x4 fa[2][MI], fb[2][NI];
+  // Requests the next stage into ring stage S.
+  int to_issue = 0;
+  auto issue = [&](auto sc, auto full) {
+    unsigned char* st = ring_stage<kStageBytes, decltype(sc)::value>();
+    const int left = K - to_issue * kStep;
+    a.template issue<decltype(full)::value>(pa, st, wave, left);
+    b.template issue<decltype(full)::value>(pb, st + OpA::kBytes, wave, left);
+    pa += step_a;
+    pb += step_b;
+    ++to_issue;
+  };
+  auto read = [&](auto sc, int s) {
+    const unsigned char* st = ring_stage<kStageBytes, decltype(sc)::value>();
+#pragma unroll
+    for (int i = 0; i < MI; ++i) fa[s & 1][i] = a.frag(st, i, s);
+#pragma unroll
+    for (int j = 0; j < NI; ++j) fb[s & 1][j] = b.frag(st + OpA::kBytes, j, s);
+  };
+  auto multiply = [&](int s) {
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NI; ++j) acc[i][j] = mfma<DT>(fa[s & 1][i], fb[s & 1][j], acc[i][j]);
+  };
+  constexpr int kReads = MI * (AKC ? 1 : 2) + NI * (BKC ? 1 : 2);
+  constexpr int kMfmas = MI * NI;
+  // Instruction order of one 16-wide K step: fragment reads behind the first
+  // MFMAs, DMA loads spread over all.
+  auto schedule = [&](auto nv_c) {
+    constexpr int nv = decltype(nv_c)::value;
+    constexpr int per = (kReads + kMfmas - 1) / kMfmas > 2 ? (kReads + kMfmas - 1) / kMfmas : 2;
+#pragma unroll
+    for (int m = 0; m < kMfmas; ++m) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      if (per * m < kReads) __builtin_amdgcn_sched_group_barrier(0x100, per, 0);
+      int loads = 0;
+#pragma unroll
+      for (int v = 0; v < nv; ++v) loads += (v * kMfmas / (nv > 0 ? nv : 1) == m) ? 1 : 0;
+      if (loads == 1) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+      if (loads == 2) __builtin_amdgcn_sched_group_barrier(0x020, 2, 0);
+      if (loads > 2) __builtin_amdgcn_sched_group_barrier(0x020, 4, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  using Full = std::true_type;
+  using Checked = std::false_type;
+  // One stage: on entry fragment 0 is in registers, on exit the next stage's.
+  auto iteration = [&](auto sc, auto full) {
+    constexpr int S = decltype(sc)::value;
+#pragma unroll
+    for (int s = 0; s < NSUB - 1; ++s) {
+      read(sc, s + 1);
+      multiply(s);
+      schedule(std::integral_constant<int, 0>{});
+    }
+    wait_vm<(STAGES - 2) * kDma>();  // the next stage has landed
+    wait_lgkm();
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    read(StageC<(S + 1) % STAGES>{}, 0);
+    issue(sc, full);
+    multiply(NSUB - 1);
+    schedule(std::integral_constant<int, kDma>{});
+  };
+
+  issue(StageC<0>{}, Checked{});
+  issue(StageC<1>{}, Checked{});
+  if constexpr (STAGES > 2) issue(StageC<2 % STAGES>{}, Checked{});
+  if constexpr (STAGES > 3) issue(StageC<3 % STAGES>{}, Checked{});
+  wait_vm<(STAGES - 1) * kDma>();
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+  read(StageC<0>{}, 0);
+
+  int kt = 0;
+  const int nfull = K / kStep;
+  for (; kt + 2 * STAGES <= nfull; kt += STAGES) {
+    iteration(StageC<0>{}, Full{});
+    iteration(StageC<1>{}, Full{});
+    if constexpr (STAGES > 2) iteration(StageC<2 % STAGES>{}, Full{});
+    if constexpr (STAGES > 3) iteration(StageC<3 % STAGES>{}, Full{});
+  }
+  for (; kt + STAGES <= nk; kt += STAGES) {
+    iteration(StageC<0>{}, Checked{});
+    iteration(StageC<1>{}, Checked{});
+    if constexpr (STAGES > 2) iteration(StageC<2 % STAGES>{}, Checked{});
+    if constexpr (STAGES > 3) iteration(StageC<3 % STAGES>{}, Checked{});
+  }
+  if (kt < nk) iteration(StageC<0>{}, Checked{}), ++kt;
+  if constexpr (STAGES > 2)
+    if (kt < nk) iteration(StageC<1>{}, Checked{}), ++kt;
+  if constexpr (STAGES > 3)
+    if (kt < nk) iteration(StageC<2 % STAGES>{}, Checked{}), ++kt;
+  wait_vm<0>();  // no DMA may still be writing LDS when the workgroup ends
+
+  // Accumulator block (mi, ni) of a lane: row n of the output, columns
+  // m = mfirst + 32 mi + 8 (r / 4) + 4 (lane / 32) + r % 4.
+  const int half = lane >> 5;
+  const int mfirst = m0 + wm * (TM / WM);
+#pragma unroll
+  for (int ni = 0; ni < NI; ++ni) {
+    const int n = n0 + wn * (TN / WN) + ni * 32 + (lane & 31);
+    const bool live_n = n < N;
+    if constexpr (EPI == kStats || EPI == kExp) {
+      constexpr float kLog2e = 1.44269504088896341f;
+      constexpr int kBlock = TM / WM;
+      const bool edge = mfirst + kBlock > g.M;
+      if (edge) {
+#pragma unroll
+        for (int mi = 0; mi < MI; ++mi)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (mfirst + mi * 32 + 8 * (r / 4) + 4 * half + r % 4 >= g.M) acc[mi][ni][r] = -__builtin_inff();
+      }
+      // The target's logit, where it lies in this block (few waves have one).
+      const int t = live_n ? g.target[n] : -1;
+      const int at = t - mfirst;
+      if (__any(at >= 0 && at < kBlock && live_n)) {
+        float v = 0.f;
+#pragma unroll
+        for (int mi = 0; mi < MI; ++mi)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (at == mi * 32 + 8 * (r / 4) + 4 * half + r % 4) v = acc[mi][ni][r];
+        if (live_n && at >= 0 && at < kBlock && ((at >> 2) & 1) == half) g.hit[n] = v;
+      }
+      float top = -__builtin_inff();
+#pragma unroll
+      for (int mi = 0; mi < MI; ++mi)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, acc[mi][ni][r]);
+      top = fmaxf(top, __shfl_xor(top, 32));
+      // (a block without a finite maximum: exp(-inf - 0) = 0)
+      const float ref = top == -__builtin_inff() ? 0.f : top;
+      float sum = 0.f;
+#pragma unroll
+      for (int mi = 0; mi < MI; ++mi)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float e = __builtin_amdgcn_exp2f((acc[mi][ni][r] - ref) * kLog2e);
+          acc[mi][ni][r] = e;
+          sum += e;
+        }
+      sum += __shfl_xor(sum, 32);
+      if (half == 0 && live_n) g.stats[(int64_t)n * g.ld_stats + tm * WM + wm] = f32x2{top, sum};
+      if constexpr (EPI == kExp) {
+        uint16_t* row = static_cast<uint16_t*>(g.out) + (int64_t)n * g.ldo;
+#pragma unroll
+        for (int mi = 0; mi < MI; ++mi)
+          store_row16<HCG_F16, false>(row, mfirst + mi * 32, g.M, half, live_n, [&](int r) { return acc[mi][ni][r]; });
+      }
+    } else {
+      if (g.add && live_n) {
+#pragma unroll
+        for (int mi = 0; mi < MI; ++mi)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int m = mfirst + mi * 32 + 8 * q + 4 * half;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (m + e < g.M) acc[mi][ni][4 * q + e] += g.add[(int64_t)n * g.M + m + e];
+          }
+      }
+      if constexpr (EPI == kRound) {
+        const float f = *g.scale * g.post;
+        uint16_t* row =
+            static_cast<uint16_t*>(g.out) + (int64_t)(live_n && g.row_of ? g.row_of[n] : n) * g.ldo;
+#pragma unroll
+        for (int mi = 0; mi < MI; ++mi)
+          store_row16<DT, true>(row, mfirst + mi * 32, g.M, half, live_n,
+                                [&](int r) { return acc[mi][ni][r] * f; });
+      } else {
+        typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+        float* row = static_cast<float*>(g.out) + split * g.split_stride + (int64_t)n * g.ldo;
+        if (live_n) {
+#pragma unroll
+          for (int mi = 0; mi < MI; ++mi)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const int m = mfirst + mi * 32 + 8 * q + 4 * half;
+              const f32x4 v{acc[mi][ni][4 * q], acc[mi][ni][4 * q + 1], acc[mi][ni][4 * q + 2], acc[mi][ni][4 * q + 3]};
+              if (m + 4 <= g.M) {
+                *reinterpret_cast<f32x4u*>(row + m) = v;
+              } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  if (m + e < g.M) row[m + e] = v[e];
+              }
+            }
+        }
+      }
+    }
+  }
+}
+
+}  // namespace head
+}  // namespace hcg

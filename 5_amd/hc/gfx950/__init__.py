@@ -383,6 +383,14 @@ def _gemm_torch(torch: Any, a: Any, b: Any, out: Any | None, algo: int) -> Any:
     return out
 
 
+from .lm import (  # noqa: E402  (a language model's ends and norm, with their gradients)
+    embedding,
+    embedding_grad,
+    layer_norm,
+    layer_norm_grad,
+    linear_cross_entropy,
+    linear_cross_entropy_grad,
+)
 from .tiles import tile_load, tile_store  # noqa: E402  (masked tile gather / scatter)
 
 
@@ -398,11 +406,17 @@ __all__ = [
     "Gfx950Target",
     "TARGET_NAME",
     "device_available",
+    "embedding",
+    "embedding_grad",
     "find_lowering",
     "gemm",
     "launch",
+    "layer_norm",
+    "layer_norm_grad",
     "library_available",
     "library_path",
+    "linear_cross_entropy",
+    "linear_cross_entropy_grad",
     "register_kernel",
     "run",
     "tile_load",

@@ -1,4 +1,5 @@
-"""ctypes binding of libhcg_gfx950.so (the C ABI in include/hcg_gemm.h).
+"""ctypes binding of libhcg_gfx950.so (the C ABI in include/hcg_gemm.h and
+the other headers beside it).
 
 The library is built in-tree by 5_amd/csrc/build.py.  There is no fallback:
 if it is missing or cannot be loaded, every gfx950 launch raises
@@ -27,6 +28,7 @@ HCG_EDECLINED = 3
 
 HCG_F16 = 0
 HCG_BF16 = 1
+HCG_F32 = 2  # include/hcg_lm.h
 
 HCG_ALGO_AUTO = 0
 HCG_ALGO_TILED = 1
@@ -55,6 +57,11 @@ ALGOS = {
 # Every symbol include/hcg_gemm.h, include/hcg_tile_ops.h and include/hcg_mfma.h declare.
 EXPORTS = ("hcg_init", "hcg_gemm", "hcg_gemm_algo", "hcg_gemm_noalloc", "hcg_gemm_trans", "hcg_last_error", "hcg_version",
            "hcg_operand_in_place", "hcg_tile_load", "hcg_tile_store", "hcg_mfma_step")
+
+# Every symbol include/hcg_lm.h declares.
+LM_EXPORTS = ("hcg_embedding", "hcg_embedding_grad", "hcg_embedding_grad_workspace", "hcg_layer_norm",
+              "hcg_layer_norm_grad", "hcg_layer_norm_grad_workspace", "hcg_linear_cross_entropy",
+              "hcg_linear_cross_entropy_grad", "hcg_linear_cross_entropy_workspace")
 
 NOALLOC_SCRATCH_BYTES = 32 << 20  # HCG_NOALLOC_SCRATCH_BYTES
 
@@ -89,6 +96,21 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.hcg_tile_store.restype = c_int
     lib.hcg_mfma_step.argtypes = [c_int, c_int, c_int, c_int, vp, vp, vp, vp, vp, vp, vp]
     lib.hcg_mfma_step.restype = c_int
+    f32 = ctypes.c_float
+    lib.hcg_embedding.argtypes = [c_int, vp, i64, i64, i64, c_int, vp, i64, f32, vp, i64, vp]
+    lib.hcg_embedding_grad_workspace.argtypes = [i64, i64, i64]
+    lib.hcg_embedding_grad.argtypes = [c_int, vp, i64, i64, i64, c_int, vp, i64, i64, f32, c_int, vp, i64, vp, i64, vp]
+    lib.hcg_layer_norm.argtypes = [c_int, vp, i64, i64, i64, c_int, vp, vp, f32, vp, i64, vp, vp, vp]
+    lib.hcg_layer_norm_grad_workspace.argtypes = [i64, i64]
+    lib.hcg_layer_norm_grad.argtypes = [c_int, vp, i64, vp, i64, i64, i64, vp, vp, c_int, vp, vp, i64, vp, vp, vp,
+                                        i64, vp]
+    lib.hcg_linear_cross_entropy_workspace.argtypes = [i64, i64, i64, vp, i64, c_int]
+    lib.hcg_linear_cross_entropy.argtypes = [c_int, vp, i64, i64, vp, i64, i64, i64, c_int, vp, i64, vp, vp, vp, i64,
+                                             vp]
+    lib.hcg_linear_cross_entropy_grad.argtypes = [c_int, vp, i64, i64, vp, i64, i64, i64, c_int, vp, i64, c_int, f32,
+                                                  vp, vp, i64, vp, i64, vp, i64, vp]
+    for name in LM_EXPORTS:
+        getattr(lib, name).restype = i64 if name.endswith("_workspace") else c_int
 
 
 def load() -> ctypes.CDLL:
