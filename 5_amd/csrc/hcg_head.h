@@ -11,11 +11,11 @@
 // between the wave's halves (across lanes they would take five exchanges per
 // row and register), and outputs leave as 16-byte pieces of a row.
 //
-// TM x TN tiles by WM x WN waves; K advances 64 at a time through a ring of
-// STAGES LDS stages filled by global-to-LDS DMA.  One barrier per stage: past
-// it every wave has read the stage before, which is refilled STAGES stages
-// ahead while the next one multiplies.  Operand layouts, swizzles and fragment
-// reads are those of hcg_wg8.h.
+// TM x TN tiles by WM x WN waves; K advances 64 at a time.  A stage is two
+// units, A's part and B's; a ring of UNITS LDS units is filled by
+// global-to-LDS DMA.  One barrier per stage: past it every wave has read the
+// stage before, whose two units are refilled UNITS units ahead.  Operand
+// layouts, swizzles and fragment reads are those of hcg_wg8.h.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -45,6 +45,7 @@ enum Epilogue {
   kExp,      // and exp(logit - block maximum) as f16
   kRound,    // scaled, rounded to DT, as rows of the output
   kPartial,  // float32, into scratch
+  kSplit,    // kRound, or with K split kPartial
 };
 
 struct Args {
@@ -56,11 +57,15 @@ struct Args {
   const int* count;
   int count0;
   int tiles_m;
-  int splits, kchunk;  // K split s covers k [s * kchunk, (s + 1) * kchunk)
-  // kRound, kPartial: row n of the output is out + (row_of ? row_of[n] : n) * ldo
-  // (kPartial: out + split * split_stride + n * ldo).
+  // kSplit: K is split while there are fewer tiles (of live tokens) than units,
+  // into at most max_splits parts.
+  int units, max_splits;
+  // kRound: row n of the output is out + (row_of ? row_of[n] : n) * ldo;
+  // kPartial: part + (split * N + n) * ld_part.
   void* out;
-  int64_t ldo, split_stride;
+  int64_t ldo;
+  float* part;
+  int64_t ld_part;
   const int* row_of;
   const float* add;    // [N][M] floats added to the sums, or null
   const float* scale;  // kRound: the factor *scale * post
@@ -90,10 +95,10 @@ __device__ __forceinline__ void wait_vm() {
 }
 __device__ __forceinline__ void wait_lgkm() { __builtin_amdgcn_s_waitcnt(0xc07f); }
 
-// Each stage is an LDS object of its own, named at compile time, so that the
+// Each unit is an LDS object of its own, named at compile time, so that the
 // compiler does not serialize a DMA into one with reads of another.
 template <int BYTES, int S>
-__device__ __forceinline__ unsigned char* ring_stage() {
+__device__ __forceinline__ unsigned char* ring_unit() {
   __shared__ __attribute__((aligned(1024))) unsigned char buf[BYTES];
   return buf;
 }
@@ -105,6 +110,14 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     return __builtin_bit_cast(uint32_t, f16x2{(_Float16)a, (_Float16)b});
   else
     return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)a, (__bf16)b});
+}
+
+// The parts that K is split into, of *chunk (a multiple of kStep) each but the
+// last.
+__device__ __forceinline__ int splits_of(int units, int max_splits, int tiles, int K, int* chunk) {
+  const int want = max(1, min(units / max(tiles, 1), max_splits));
+  *chunk = ((K + want - 1) / want + kStep - 1) / kStep * kStep;
+  return max(1, (K + *chunk - 1) / max(*chunk, 1));
 }
 
 // blockIdx -> (K split, tile): each XCD (id % 8) takes a contiguous run of
@@ -168,11 +181,12 @@ struct Operand {
   // whole stage).  The resource starts at the stage, so offsets stay in 31
   // bits whatever the matrix's size; chunks out of range are redirected past
   // its extent and load zeros.
-  template <bool FULL>
+  // Instructions FROM to TO - 1 of the wave's.
+  template <bool FULL, int FROM, int TO>
   __device__ __forceinline__ void issue(const uint16_t* p, unsigned char* st, int wave, int left) const {
     const __amdgpu_buffer_rsrc_t r = make_rsrc(p, 0x7fffffe0);
 #pragma unroll
-    for (int i = 0; i < kInst; ++i) {
+    for (int i = FROM; i < TO; ++i) {
       lds_void* dst = (lds_void*)(st + (wave * kInst + i) * 1024);
       if constexpr (FULL)
         dma16(r, dst, off[i]);
@@ -213,44 +227,70 @@ struct Operand {
   }
 };
 
-template <int S>
-using StageC = std::integral_constant<int, S>;
+template <int I>
+using Int = std::integral_constant<int, I>;
 
-// 16-bit outputs of rows n (one per lane), M columns m0 .. m0 + 31: value(r)
-// is accumulator register r.  The wave's halves exchange 4-value groups, so
-// that each lane stores whole 16-byte pieces.  `row`: the output row's
-// element 0, `extent`: its columns; a piece past them is cut (CUT) or, in
-// padded scratch, stored whole.
-template <int DT, bool CUT, class F>
-__device__ __forceinline__ void store_row16(uint16_t* row, int m0, int extent, int half, bool live, F value) {
-  typedef uint32_t u32x4u __attribute__((ext_vector_type(4), aligned(2)));
+// A wave's 32 rows by 32 * MI columns of 16-bit results on their way out, in
+// LDS: row r's 16-byte chunk c lies at chunk c ^ (r % the row's chunks), so that
+// both the writes (a lane per row) and the reads (a row per group of lanes)
+// cover all banks.
+template <int MI>
+struct RowStage {
+  static constexpr int kChunks = 4 * MI;  // 16-byte chunks per row
+  static constexpr int kBytes = 32 * kChunks * 16;
+  static __device__ __forceinline__ int at(int row, int chunk) {
+    return (row * kChunks + (chunk ^ (row & (kChunks - 1)))) * 16;
+  }
+  // value(r), r = 0 .. 15: the lane's accumulator registers of block mi, in
+  // row lane % 32, columns 32 mi + 8 (r / 4) + 4 (lane / 32) + r % 4.  The
+  // wave's halves exchange groups of four, so that each lane holds whole
+  // chunks.
+  template <int DT, class F>
+  static __device__ __forceinline__ void put(unsigned char* st, int lane, int mi, F value) {
+    const int row = lane & 31, half = lane >> 5;
 #pragma unroll
-  for (int p = 0; p < 2; ++p) {
-    uint32_t w[2][2];
+    for (int p = 0; p < 2; ++p) {
+      uint32_t w[2][2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint32_t a = pack2<DT>(value(8 * p + 2 * i), value(8 * p + 2 * i + 1));
-      const uint32_t b = pack2<DT>(value(8 * p + 4 + 2 * i), value(8 * p + 5 + 2 * i));
-      const auto s = __builtin_amdgcn_permlane32_swap(a, b, false, false);
-      w[0][i] = s[0];
-      w[1][i] = s[1];
-    }
-    const u32x4 v{w[0][0], w[0][1], w[1][0], w[1][1]};
-    const int m = m0 + 16 * p + 8 * half;
-    if (!live || m >= extent) continue;
-    if (!CUT || m + 8 <= extent) {
-      *reinterpret_cast<u32x4u*>(row + m) = v;
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (m + e < extent) row[m + e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t a = pack2<DT>(value(8 * p + 2 * i), value(8 * p + 2 * i + 1));
+        const uint32_t b = pack2<DT>(value(8 * p + 4 + 2 * i), value(8 * p + 5 + 2 * i));
+        const auto x = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+        w[0][i] = x[0];
+        w[1][i] = x[1];
+      }
+      *reinterpret_cast<u32x4*>(st + at(row, 4 * mi + 2 * p + half)) = u32x4{w[0][0], w[0][1], w[1][0], w[1][1]};
     }
   }
-}
+  // The wave's rows as 16-byte stores, a row's chunks in neighbouring lanes.
+  // base(row): the output row's element 0, or null; columns m0 ... below
+  // `extent` (a chunk that reaches past it is cut, or, in padded scratch,
+  // stored whole).
+  template <bool CUT, class F>
+  static __device__ __forceinline__ void store(const unsigned char* st, int lane, int m0, int extent, F base) {
+    typedef uint32_t u32x4u __attribute__((ext_vector_type(4), aligned(2)));
+    constexpr int kPer = 64 / kChunks;  // rows per instruction
+    const int chunk = lane % kChunks, m = m0 + chunk * 8;
+#pragma unroll
+    for (int i = 0; i < 32 / kPer; ++i) {
+      const int row = i * kPer + lane / kChunks;
+      const u32x4 v = *reinterpret_cast<const u32x4*>(st + at(row, chunk));
+      uint16_t* p = base(row);
+      if (p == nullptr || m >= extent) continue;
+      if (!CUT || m + 8 <= extent) {
+        *reinterpret_cast<u32x4u*>(p + m) = v;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (m + e < extent) p[m + e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
+      }
+    }
+  }
+};
 
 // AKC, BKC: the operand is stored with K contiguous.  COUNT_K: the live
 // tokens bound K, else N.
-template <int DT, int TM, int TN, int WM, int WN, int STAGES, bool AKC, bool BKC, int EPI, bool COUNT_K>
+template <int DT, int TM, int TN, int WM, int WN, int UNITS, bool AKC, bool BKC, int EPI, bool COUNT_K>
 __global__ __launch_bounds__(64 * WM * WN, 1) void head_kernel(Args g) {
   constexpr int NW = WM * WN;
   constexpr int MI = TM / WM / 32, NI = TN / WN / 32;
@@ -258,9 +298,9 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void head_kernel(Args g) {
   constexpr int NSUB = kStep / 16;
   using OpA = Operand<TM, AKC, NW>;
   using OpB = Operand<TN, BKC, NW>;
-  constexpr int kStageBytes = OpA::kBytes + OpB::kBytes;
-  constexpr int kDma = OpA::kInst + OpB::kInst;
-  static_assert(STAGES >= 2 && STAGES <= 4, "stages");
+  constexpr int kUnitBytes = OpA::kBytes > OpB::kBytes ? OpA::kBytes : OpB::kBytes;
+  static_assert(UNITS >= 4 && kUnitBytes * UNITS <= 160 * 1024, "ring");
+  constexpr int kPeriod = UNITS % 2 ? UNITS : UNITS / 2;  // stages until the units' places repeat
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -269,12 +309,15 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void head_kernel(Args g) {
   const int live = min(max(*g.count - g.count0, 0), COUNT_K ? g.K : g.N);
   const int N = COUNT_K ? g.N : live;
   const int tiles_n = (N + TN - 1) / TN;
-  if ((int)blockIdx.x >= g.tiles_m * tiles_n * g.splits) return;
+  const int K_all = COUNT_K ? live : g.K;
+  int chunk = K_all, splits = 1;
+  if constexpr (EPI == kSplit) splits = splits_of(g.units, g.max_splits, g.tiles_m * tiles_n, K_all, &chunk);
+  if ((int)blockIdx.x >= g.tiles_m * tiles_n * splits) return;
   int split, tm, tn;
-  unit_of(g.tiles_m, tiles_n, g.splits, blockIdx.x, split, tm, tn);
+  unit_of(g.tiles_m, tiles_n, splits, blockIdx.x, split, tm, tn);
   const int m0 = tm * TM, n0 = tn * TN;
-  const int kbeg = split * g.kchunk;
-  const int K = min((COUNT_K ? live : g.K) - kbeg, g.kchunk);
+  const int kbeg = split * chunk;
+  const int K = min(K_all - kbeg, chunk);
   const int nk = max((K + kStep - 1) / kStep, 0);
 
   const uint16_t* pa = g.A + (AKC ? (int64_t)m0 * g.lda + kbeg : (int64_t)kbeg * g.lda + m0);
@@ -294,23 +337,35 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void head_kernel(Args g) {
     for (int j = 0; j < NI; ++j) acc[i][j] = f32x16{};
 
   u32x4 fa[2][MI], fb[2][NI];
-  // Requests the next stage into ring stage S.
-  int to_issue = 0;
-  auto issue = [&](auto sc, auto full) {
-    unsigned char* st = ring_stage<kStageBytes, decltype(sc)::value>();
-    const int left = K - to_issue * kStep;
-    a.template issue<decltype(full)::value>(pa, st, wave, left);
-    b.template issue<decltype(full)::value>(pb, st + OpA::kBytes, wave, left);
-    pa += step_a;
-    pb += step_b;
-    ++to_issue;
+  // Instructions FROM to TO - 1 of the next unit U of its operand (even units
+  // are A's).
+  int left_a = K, left_b = K;
+  auto issue = [&](auto uc, auto full, auto from, auto to) {
+    constexpr int U = decltype(uc)::value, F = decltype(from)::value, T = decltype(to)::value;
+    constexpr bool kFull = decltype(full)::value;
+    unsigned char* st = ring_unit<kUnitBytes, U % UNITS>();
+    if constexpr (U % 2 == 0) {
+      a.template issue<kFull, F, T>(pa, st, wave, left_a);
+      if constexpr (T == OpA::kInst) pa += step_a, left_a -= kStep;
+    } else {
+      b.template issue<kFull, F, T>(pb, st, wave, left_b);
+      if constexpr (T == OpB::kInst) pb += step_b, left_b -= kStep;
+    }
   };
-  auto read = [&](auto sc, int s) {
-    const unsigned char* st = ring_stage<kStageBytes, decltype(sc)::value>();
+  // DMA instructions of n units from unit u on.
+  constexpr auto dmas = [](int u, int n) {
+    int c = 0;
+    for (int i = 0; i < n; ++i) c += (u + i) % 2 ? OpB::kInst : OpA::kInst;
+    return c;
+  };
+  auto read = [&](auto kc, int s) {
+    constexpr int K0 = decltype(kc)::value;
+    const unsigned char* sa = ring_unit<kUnitBytes, 2 * K0 % UNITS>();
+    const unsigned char* sb = ring_unit<kUnitBytes, (2 * K0 + 1) % UNITS>();
 #pragma unroll
-    for (int i = 0; i < MI; ++i) fa[s & 1][i] = a.frag(st, i, s);
+    for (int i = 0; i < MI; ++i) fa[s & 1][i] = a.frag(sa, i, s);
 #pragma unroll
-    for (int j = 0; j < NI; ++j) fb[s & 1][j] = b.frag(st + OpA::kBytes, j, s);
+    for (int j = 0; j < NI; ++j) fb[s & 1][j] = b.frag(sb, j, s);
   };
   auto multiply = [&](int s) {
 #pragma unroll
@@ -340,54 +395,97 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void head_kernel(Args g) {
   };
   using Full = std::true_type;
   using Checked = std::false_type;
-  // One stage: on entry fragment 0 is in registers, on exit the next stage's.
-  auto iteration = [&](auto sc, auto full) {
-    constexpr int S = decltype(sc)::value;
-#pragma unroll
-    for (int s = 0; s < NSUB - 1; ++s) {
-      read(sc, s + 1);
+  // Stage k (known modulo kPeriod): on entry fragment 0 is in registers, on
+  // exit the next stage's.  The DMA of unit 2 k + UNITS goes out behind the
+  // barrier, that of the unit after it over the next stage's K steps: 64 DMA
+  // instructions take the CU's address unit 1024 cycles, and issued within one
+  // K step (512 cycles of MFMA) they held the waves up.
+  auto iteration = [&](auto kc, auto full) {
+    constexpr int k = decltype(kc)::value;
+    constexpr int kLast = 2 * k + UNITS - 1;  // the unit that the stage before left to issue
+    constexpr int kParts = kLast % 2 ? OpB::kInst : OpA::kInst;
+    constexpr int kNext = 2 * k + UNITS;
+    constexpr int kNextParts = kNext % 2 ? OpB::kInst : OpA::kInst;
+    auto step = [&](auto sc) {
+      constexpr int s = decltype(sc)::value;
+      constexpr int from = kParts * s / (NSUB - 1), to = kParts * (s + 1) / (NSUB - 1);
+      read(Int<k>{}, s + 1);
+      if constexpr (to > from) issue(Int<kLast>{}, full, Int<from>{}, Int<to>{});
       multiply(s);
-      schedule(std::integral_constant<int, 0>{});
-    }
-    wait_vm<(STAGES - 2) * kDma>();  // the next stage has landed
+      schedule(Int<to - from>{});
+    };
+    step(Int<0>{});
+    step(Int<1>{});
+    step(Int<2>{});
+    static_assert(NSUB == 4, "K steps");
+    wait_vm<dmas(2 * k + 4, UNITS - 4)>();  // the next stage's two units have landed
     wait_lgkm();
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
-    read(StageC<(S + 1) % STAGES>{}, 0);
-    issue(sc, full);
+    read(Int<k + 1>{}, 0);
+    issue(Int<kNext>{}, full, Int<0>{}, Int<kNextParts>{});
     multiply(NSUB - 1);
-    schedule(std::integral_constant<int, kDma>{});
+    schedule(Int<kNextParts>{});
   };
 
-  issue(StageC<0>{}, Checked{});
-  issue(StageC<1>{}, Checked{});
-  if constexpr (STAGES > 2) issue(StageC<2 % STAGES>{}, Checked{});
-  if constexpr (STAGES > 3) issue(StageC<3 % STAGES>{}, Checked{});
-  wait_vm<(STAGES - 1) * kDma>();
+  auto first = [&](auto uc) {
+    constexpr int U = decltype(uc)::value;
+    if constexpr (U < UNITS - 1) issue(uc, Checked{}, Int<0>{}, Int<(U % 2 ? OpB::kInst : OpA::kInst)>{});
+  };
+  first(Int<0>{});
+  first(Int<1>{});
+  first(Int<2>{});
+  first(Int<3>{});
+  first(Int<4>{});
+  first(Int<5>{});
+  first(Int<6>{});
+  first(Int<7>{});
+  first(Int<8>{});
+  static_assert(UNITS <= 10, "ring");
+  wait_vm<dmas(2, UNITS - 3)>();
   __builtin_amdgcn_s_barrier();
   __builtin_amdgcn_sched_barrier(0);
-  read(StageC<0>{}, 0);
+  read(Int<0>{}, 0);
 
   int kt = 0;
   const int nfull = K / kStep;
-  for (; kt + 2 * STAGES <= nfull; kt += STAGES) {
-    iteration(StageC<0>{}, Full{});
-    iteration(StageC<1>{}, Full{});
-    if constexpr (STAGES > 2) iteration(StageC<2 % STAGES>{}, Full{});
-    if constexpr (STAGES > 3) iteration(StageC<3 % STAGES>{}, Full{});
+  for (; kt + kPeriod + UNITS / 2 <= nfull; kt += kPeriod) {
+    iteration(Int<0>{}, Full{});
+    iteration(Int<1>{}, Full{});
+    if constexpr (kPeriod > 2) iteration(Int<2>{}, Full{});
+    if constexpr (kPeriod > 3) iteration(Int<3>{}, Full{});
+    if constexpr (kPeriod > 4) iteration(Int<4>{}, Full{});
   }
-  for (; kt + STAGES <= nk; kt += STAGES) {
-    iteration(StageC<0>{}, Checked{});
-    iteration(StageC<1>{}, Checked{});
-    if constexpr (STAGES > 2) iteration(StageC<2 % STAGES>{}, Checked{});
-    if constexpr (STAGES > 3) iteration(StageC<3 % STAGES>{}, Checked{});
+  static_assert(kPeriod <= 5, "ring");
+  while (kt < nk) {
+    iteration(Int<0>{}, Checked{});
+    if (++kt >= nk) break;
+    iteration(Int<1>{}, Checked{});
+    if (++kt >= nk) break;
+    if constexpr (kPeriod > 2) {
+      iteration(Int<2>{}, Checked{});
+      if (++kt >= nk) break;
+    }
+    if constexpr (kPeriod > 3) {
+      iteration(Int<3>{}, Checked{});
+      if (++kt >= nk) break;
+    }
+    if constexpr (kPeriod > 4) {
+      iteration(Int<4>{}, Checked{});
+      ++kt;
+    }
   }
-  if (kt < nk) iteration(StageC<0>{}, Checked{}), ++kt;
-  if constexpr (STAGES > 2)
-    if (kt < nk) iteration(StageC<1>{}, Checked{}), ++kt;
-  if constexpr (STAGES > 3)
-    if (kt < nk) iteration(StageC<2 % STAGES>{}, Checked{}), ++kt;
-  wait_vm<0>();  // no DMA may still be writing LDS when the workgroup ends
+  wait_vm<0>();  // no DMA may still be writing LDS
+  wait_lgkm();
+  __builtin_amdgcn_s_barrier();  // every wave has read its last fragments: the stages are free
+  // Rows on their way out: a part of the first units for each wave.
+  typedef RowStage<MI> Stage;
+  constexpr int kWavesPerUnit = kUnitBytes / Stage::kBytes;
+  static_assert(kWavesPerUnit * 3 >= NW, "staging");
+  unsigned char* const rows_out =
+      (wave < kWavesPerUnit ? ring_unit<kUnitBytes, 0>()
+                            : wave < 2 * kWavesPerUnit ? ring_unit<kUnitBytes, 1>() : ring_unit<kUnitBytes, 2>()) +
+      wave % kWavesPerUnit * Stage::kBytes;
 
   // Accumulator block (mi, ni) of a lane: row n of the output, columns
   // m = mfirst + 32 mi + 8 (r / 4) + 4 (lane / 32) + r % 4.
@@ -395,7 +493,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void head_kernel(Args g) {
   const int mfirst = m0 + wm * (TM / WM);
 #pragma unroll
   for (int ni = 0; ni < NI; ++ni) {
-    const int n = n0 + wn * (TN / WN) + ni * 32 + (lane & 31);
+    const int nfirst = n0 + wn * (TN / WN) + ni * 32, n = nfirst + (lane & 31);
     const bool live_n = n < N;
     if constexpr (EPI == kStats || EPI == kExp) {
       constexpr float kLog2e = 1.44269504088896341f;
@@ -440,13 +538,16 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void head_kernel(Args g) {
       sum += __shfl_xor(sum, 32);
       if (half == 0 && live_n) g.stats[(int64_t)n * g.ld_stats + tm * WM + wm] = f32x2{top, sum};
       if constexpr (EPI == kExp) {
-        uint16_t* row = static_cast<uint16_t*>(g.out) + (int64_t)n * g.ldo;
 #pragma unroll
         for (int mi = 0; mi < MI; ++mi)
-          store_row16<HCG_F16, false>(row, mfirst + mi * 32, g.M, half, live_n, [&](int r) { return acc[mi][ni][r]; });
+          Stage::template put<HCG_F16>(rows_out, lane, mi, [&](int r) { return acc[mi][ni][r]; });
+        Stage::template store<false>(rows_out, lane, mfirst, g.M, [&](int row) -> uint16_t* {
+          const int to = nfirst + row;
+          return to < N ? static_cast<uint16_t*>(g.out) + (int64_t)to * g.ldo : nullptr;
+        });
       }
     } else {
-      if (g.add && live_n) {
+      if (EPI != kSplit && g.add && live_n) {
 #pragma unroll
         for (int mi = 0; mi < MI; ++mi)
 #pragma unroll
@@ -457,17 +558,19 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void head_kernel(Args g) {
               if (m + e < g.M) acc[mi][ni][4 * q + e] += g.add[(int64_t)n * g.M + m + e];
           }
       }
-      if constexpr (EPI == kRound) {
+      if (EPI == kRound || (EPI == kSplit && splits == 1)) {
         const float f = *g.scale * g.post;
-        uint16_t* row =
-            static_cast<uint16_t*>(g.out) + (int64_t)(live_n && g.row_of ? g.row_of[n] : n) * g.ldo;
 #pragma unroll
         for (int mi = 0; mi < MI; ++mi)
-          store_row16<DT, true>(row, mfirst + mi * 32, g.M, half, live_n,
-                                [&](int r) { return acc[mi][ni][r] * f; });
+          Stage::template put<DT>(rows_out, lane, mi, [&](int r) { return acc[mi][ni][r] * f; });
+        Stage::template store<true>(rows_out, lane, mfirst, g.M, [&](int row) -> uint16_t* {
+          const int to = nfirst + row;
+          if (to >= N) return nullptr;
+          return static_cast<uint16_t*>(g.out) + (int64_t)(g.row_of ? g.row_of[to] : to) * g.ldo;
+        });
       } else {
         typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
-        float* row = static_cast<float*>(g.out) + split * g.split_stride + (int64_t)n * g.ldo;
+        float* row = g.part + ((int64_t)split * N + n) * g.ld_part;
         if (live_n) {
 #pragma unroll
           for (int mi = 0; mi < MI; ++mi)

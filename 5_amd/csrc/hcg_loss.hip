@@ -43,74 +43,113 @@ constexpr float kF16Scale = 4096.f;
 struct PackArgs {
   const void* targets;
   int64_t ignore, vocab;
-  int tokens, mean;
+  int tokens, per_wg, mean;
   float grad_scale;
-  int* slot;    // per token: its place among those that count, or -1
-  int* token;   // per place: the token
+  int* token;   // per place among those that count: the token
   int* target;  // per place: its target, -1 outside the vocabulary
   int* count;
   float* scale;  // [0]: the gradient's factor, [1]: the loss's
   float* loss;   // per token, zeroed where ignored (or null)
   float* lse;
+  // The rows: x to its place, zeros past the width; zeros in dx where ignored.
+  const uint16_t* x;
+  int64_t ldx;
+  uint16_t* rows;
+  int64_t ldr;
+  int width, vecs;
+  uint16_t* dx;  // or null
+  int64_t lddx;
 };
 
-// One workgroup; each thread a contiguous run of tokens.
+constexpr int kPackThreads = 256;
+constexpr int kPackRun = 128;  // tokens per workgroup at most: their places are in LDS
+
+// A workgroup packs a run of tokens.  It counts the tokens before its run
+// itself, from the L2 (64 KB of targets at 8192 tokens), so that packing is one
+// launch without anything to wait for.
 template <class I>
-__global__ __launch_bounds__(1024) void pack_kernel(PackArgs g) {
-  __shared__ int waves[16];
+__global__ __launch_bounds__(kPackThreads) void pack_kernel(PackArgs g) {
+  __shared__ int waves[kPackThreads / 64];
+  __shared__ int slot[kPackRun];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int per = (g.tokens + 1023) / 1024;
-  const int from = min(tid * per, g.tokens), to = min(from + per, g.tokens);
+  const int from = blockIdx.x * g.per_wg, n = min(g.per_wg, g.tokens - from);
   const I* targets = static_cast<const I*>(g.targets);
-  int mine = 0;
-  for (int t = from; t < to; ++t) mine += (int64_t)targets[t] != g.ignore;
-  int sum = mine;
+  int before = 0;
+  for (int t0 = tid; t0 < from; t0 += kPackThreads * 8) {
 #pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
-    const int up = __shfl_up(sum, m);
-    if (lane >= m) sum += up;
-  }
-  if (lane == 63) waves[wave] = sum;
-  __syncthreads();
-  int place = sum - mine, total = 0;
-#pragma unroll
-  for (int w = 0; w < 16; ++w) {
-    if (w < wave) place += waves[w];
-    total += waves[w];
-  }
-  for (int t = from; t < to; ++t) {
-    const int64_t y = (int64_t)targets[t];
-    if (y == g.ignore) {
-      g.slot[t] = -1;
-      if (g.loss) g.loss[t] = 0.f;
-      if (g.lse) g.lse[t] = 0.f;
-    } else {
-      g.slot[t] = place;
-      g.token[place] = t;
-      g.target[place] = y >= 0 && y < g.vocab ? (int)y : -1;
-      ++place;
+    for (int u = 0; u < 8; ++u) {
+      const int t = t0 + u * kPackThreads;
+      before += t < from && (int64_t)targets[t] != g.ignore;
     }
   }
-  if (tid == 0) {
-    *g.count = total;
-    const float share = g.mean ? 1.f / (float)max(total, 1) : 1.f;
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) before += __shfl_xor(before, m);
+  if (lane == 0) waves[wave] = before;
+  __syncthreads();
+  int place = 0;
+#pragma unroll
+  for (int w = 0; w < kPackThreads / 64; ++w) place += waves[w];
+  // Every wave places the run; the first one writes it down.
+  for (int j0 = 0; j0 < n; j0 += 64) {
+    const int j = j0 + lane, t = from + j;
+    const int64_t y = j < n ? (int64_t)targets[t] : g.ignore;
+    const uint64_t counts = __ballot(y != g.ignore);
+    if (wave == 0 && j < n) {
+      const int at = place + __popcll(counts & (((uint64_t)1 << lane) - 1));
+      slot[j] = y == g.ignore ? -1 : at;
+      if (y == g.ignore) {
+        if (g.loss) g.loss[t] = 0.f;
+        if (g.lse) g.lse[t] = 0.f;
+      } else {
+        g.token[at] = t;
+        g.target[at] = y >= 0 && y < g.vocab ? (int)y : -1;
+      }
+    }
+    place += __popcll(counts);
+  }
+  if (tid == 0 && from + n == g.tokens) {
+    *g.count = place;
+    const float share = g.mean ? 1.f / (float)max(place, 1) : 1.f;
     g.scale[0] = g.grad_scale * share;
     g.scale[1] = share;
+  }
+  __syncthreads();
+  typedef _Float16 h;
+  const int total = n * g.vecs;
+  constexpr int kPer = 8;  // loads in flight
+  for (int i0 = tid; i0 < total; i0 += kPackThreads * kPer) {
+    raw4 v[kPer];
+    int row[kPer], col[kPer], to[kPer];
+#pragma unroll
+    for (int u = 0; u < kPer; ++u) {
+      const int i = i0 + u * kPackThreads;
+      row[u] = i / g.vecs;
+      col[u] = (i - row[u] * g.vecs) * 8;
+      to[u] = i < total ? slot[row[u]] : -2;
+      v[u] = raw4{0, 0, 0, 0};
+      if (to[u] >= 0)
+        v[u] = hcg::load_raw(reinterpret_cast<const h*>(g.x + (int64_t)(from + row[u]) * g.ldx + col[u]),
+                             g.width - col[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < kPer; ++u) {
+      if (to[u] >= 0)
+        *reinterpret_cast<raw4*>(g.rows + (int64_t)to[u] * g.ldr + col[u]) = v[u];
+      else if (to[u] == -1 && g.dx)
+        hcg::store_raw(reinterpret_cast<h*>(g.dx + (int64_t)(from + row[u]) * g.lddx + col[u]), v[u],
+                       g.width - col[u]);
+    }
   }
 }
 
 // Rows of 16-bit elements into rows of `ldo` (a multiple of 8) elements, zeros
-// past the width.  With `slot`, row t goes to place slot[t], or (-1) leaves
-// zeros in row t of dx.
+// past the width.
 struct CopyArgs {
   const uint16_t* src;
   int64_t lds;
   uint16_t* dst;
   int64_t ldo;
   int rows, width, vecs;
-  const int* slot;
-  uint16_t* dx;  // or null
-  int64_t lddx;
 };
 
 __global__ __launch_bounds__(256) void copy_rows_kernel(CopyArgs g) {
@@ -118,14 +157,9 @@ __global__ __launch_bounds__(256) void copy_rows_kernel(CopyArgs g) {
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
     const int64_t row = i / g.vecs;
     const int c = (int)(i - row * g.vecs) * 8;
-    const int64_t to = g.slot ? g.slot[row] : row;
     typedef _Float16 h;
-    if (to >= 0) {
-      const raw4 v = hcg::load_raw(reinterpret_cast<const h*>(g.src + row * g.lds + c), g.width - c);
-      *reinterpret_cast<raw4*>(g.dst + to * g.ldo + c) = v;
-    } else if (g.dx) {
-      hcg::store_raw(reinterpret_cast<h*>(g.dx + row * g.lddx + c), raw4{0, 0, 0, 0}, g.width - c);
-    }
+    *reinterpret_cast<raw4*>(g.dst + row * g.ldo + c) =
+        hcg::load_raw(reinterpret_cast<const h*>(g.src + row * g.lds + c), g.width - c);
   }
 }
 
@@ -216,11 +250,12 @@ __global__ __launch_bounds__(1024) void loss_sum_kernel(const float* loss, const
   }
 }
 
-// Rows of dx from the K splits' sums.
+// Rows of dx from the K splits' sums (where head_kernel split K).
 struct JoinArgs {
-  const float* part;  // [splits][rows][ld]
-  int64_t ld, stride;
-  int splits, width, vecs;
+  const float* part;  // [splits][live tokens][ld]
+  int64_t ld;
+  int units, max_splits, tiles_m, tile_n, tokens, K;  // as head_kernel has them
+  int width, vecs;
   const int* count;
   int count0;
   const int* token;
@@ -232,17 +267,25 @@ struct JoinArgs {
 
 template <int DT>
 __global__ __launch_bounds__(256) void join_kernel(JoinArgs g) {
-  const int n = blockIdx.x;
-  if (n >= *g.count - g.count0) return;
+  const int live = min(max(*g.count - g.count0, 0), g.tokens);
+  int chunk;
+  const int splits =
+      head::splits_of(g.units, g.max_splits, g.tiles_m * ((live + g.tile_n - 1) / g.tile_n), g.K, &chunk);
+  if (splits == 1) return;
   const float f = *g.scale * g.post;
   typedef typename ElemOf<DT>::type T;
-  T* row = reinterpret_cast<T*>(g.dx) + (int64_t)g.token[n] * g.lddx;
-  for (int i = blockIdx.y * 256 + threadIdx.x; i < g.vecs; i += gridDim.y * 256) {
+  const int64_t total = (int64_t)live * g.vecs;
+  for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < total; at += (int64_t)gridDim.x * 256) {
+    const int n = (int)(at / g.vecs), i = (int)(at - (int64_t)n * g.vecs);
+    T* row = reinterpret_cast<T*>(g.dx) + (int64_t)g.token[n] * g.lddx;
     const float* p = g.part + (int64_t)n * g.ld + i * 8;  // (rows are padded to 8)
     float sum[8] = {};
-    for (int s = 0; s < g.splits; ++s) {
+#pragma unroll 4
+    for (int s = 0; s < splits; ++s) {
+      const head::f32x4 a = *reinterpret_cast<const head::f32x4*>(p + (int64_t)s * live * g.ld);
+      const head::f32x4 b = *reinterpret_cast<const head::f32x4*>(p + (int64_t)s * live * g.ld + 4);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum[e] += p[s * g.stride + e];
+      for (int e = 0; e < 4; ++e) sum[e] += a[e], sum[4 + e] += b[e];
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) sum[e] *= f;
@@ -257,21 +300,57 @@ __global__ __launch_bounds__(256) void join_kernel(JoinArgs g) {
 int64_t round_up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Tile shapes of head_kernel: rows of M and N, waves over them, LDS stages.
+// Tile shapes of head_kernel: rows of M and N, waves over M in the softmax's
+// product, and a model of its time in us: a tile's start and end, and one
+// stage of K on an idle and on a busy chip, per round of workgroups
+// (per_cu of which share a CU).  Fitted to 11 sizes with every shape and 1 to 16
+// K splits.  Both sides, us: dx of 1300 x 50000 x 1032 large in 8 parts 141,
+// medium in 2 208; of 256 x 4096 x 512 large in 16 parts 18, medium in 8 9; of
+// 64 x 32768 x 4096 medium in 8 parts 43, few in 8 49; logits of 32 x 50000 x
+// 1024 medium 22, few 17; of 1024 x 32768 x 2048 large 117, medium 167.
 enum Shape { kLarge, kMedium, kFew };
 struct ShapeInfo {
-  int tm, tn, wm;
+  int tm, tn, wm, per_cu;
+  double fixed, lo, hi;
 };
-constexpr ShapeInfo kShapes[] = {{256, 256, 2}, {128, 128, 2}, {128, 32, 4}};
-
-// The whole chip is 256 CUs with one workgroup each.
+constexpr ShapeInfo kShapes[] = {
+    {256, 256, 2, 1, 12.0, 0.95, 1.55}, {128, 128, 2, 1, 5.0, 0.31, 0.52}, {128, 32, 4, 2, 4.0, 0.33, 0.66}};
+constexpr int kNumShapes = 3;
 constexpr int kCus = 256;
+constexpr int kMaxSplits = 32;
+constexpr int kMinKPerSplit = 256;
 
 int64_t tiles(Shape s, int64_t m, int64_t n) { return ceil_div(m, kShapes[s].tm) * ceil_div(n, kShapes[s].tn); }
 
-Shape pick_shape(int64_t m, int64_t n, bool few) {
-  if (few && n <= 32) return kFew;
-  return tiles(kLarge, m, n) >= kCus / 2 ? kLarge : kMedium;
+double cost_of(Shape s, int64_t m, int64_t n, int64_t k, int splits) {
+  const ShapeInfo& t = kShapes[s];
+  const int64_t units = tiles(s, m, n) * splits, room = kCus * t.per_cu;
+  const double busy = units < room ? (double)units / room : 1.0;
+  const double stages = (double)ceil_div(ceil_div(k, splits), head::kStep);
+  double us = (double)ceil_div(units, room) * (t.fixed + stages * (t.lo + (t.hi - t.lo) * busy));
+  if (splits > 1) us += 4.0 + 2.0 * splits * m * n * 4 / 6.0e6;  // the parts written and read, and a launch
+  return us;
+}
+
+// The shape with the least modelled time; few: the 32-token tiles may be taken
+// (their N is K-contiguous); *units: workgroups to split K up to, or null.
+Shape pick_shape(int64_t m, int64_t n, int64_t k, bool few, int* units) {
+  Shape best = kLarge;
+  double best_cost = -1;
+  for (int i = 0; i < kNumShapes; ++i) {
+    const Shape s = (Shape)i;
+    if (s == kFew && !few) continue;
+    for (int splits = 1; splits <= kMaxSplits; ++splits) {
+      if (splits > 1 && (!units || k / splits < kMinKPerSplit)) break;
+      const double cost = cost_of(s, m, n, k, splits);
+      if (best_cost >= 0 && cost >= best_cost) continue;
+      best_cost = cost;
+      best = s;
+      // (fewer tokens that count leave fewer tiles and more splits)
+      if (units) *units = (int)std::max<int64_t>(kCus * kShapes[s].per_cu, std::min<int64_t>(tiles(s, m, n) * splits, 1 << 20));
+    }
+  }
+  return best;
 }
 
 struct Plan {
@@ -281,10 +360,10 @@ struct Plan {
   int64_t piece;       // tokens per piece
   int pieces;
   Shape logits, dx, dw;
-  int splits, kchunk;  // of dx
+  int units, max_splits;  // of dx
   int64_t blocks;      // statistics per token
   // Offsets into the workspace.
-  int64_t slot, token, target, count, scale, rows, weight, stats, hit, loss, exps, part, sums, total;
+  int64_t token, target, count, scale, rows, weight, stats, hit, loss, exps, part, sums, total;
 };
 
 Plan make_plan(int64_t tokens, int64_t vocab, int64_t width, bool copy_weight, bool grad) {
@@ -299,16 +378,12 @@ Plan make_plan(int64_t tokens, int64_t vocab, int64_t width, bool copy_weight, b
   p.piece = tokens;
   if (grad) p.piece = std::min(tokens, std::max<int64_t>(256, kPieceBytes / (p.lde * 2) / 256 * 256));
   p.pieces = (int)ceil_div(tokens, p.piece);
-  p.logits = pick_shape(vocab, p.piece, true);
+  p.logits = pick_shape(vocab, p.piece, width, true, nullptr);
   p.blocks = ceil_div(vocab, kShapes[p.logits].tm) * kShapes[p.logits].wm;
-  p.splits = 1;
   if (grad) {
-    p.dx = pick_shape(width, p.piece, true);
-    p.dw = pick_shape(width, vocab, false);
-    const int64_t t = tiles(p.dx, width, p.piece);
-    if (t < kCus) p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(kCus / t, 32), vocab / 512));
-    p.kchunk = (int)round_up(ceil_div(vocab, p.splits), head::kStep);
-    p.splits = (int)ceil_div(vocab, p.kchunk);
+    p.dx = pick_shape(width, p.piece, vocab, true, &p.units);
+    p.dw = pick_shape(width, vocab, p.piece, false, nullptr);
+    p.max_splits = (int)std::max<int64_t>(1, std::min<int64_t>(kMaxSplits, vocab / kMinKPerSplit));
   }
   int64_t at = 0;
   const auto take = [&](int64_t bytes) {
@@ -316,7 +391,6 @@ Plan make_plan(int64_t tokens, int64_t vocab, int64_t width, bool copy_weight, b
     at += round_up(bytes, 256);
     return here;
   };
-  p.slot = take(tokens * 4);
   p.token = take(tokens * 4);
   p.target = take(tokens * 4);
   p.count = take(4);
@@ -328,7 +402,11 @@ Plan make_plan(int64_t tokens, int64_t vocab, int64_t width, bool copy_weight, b
   if (grad) {
     p.loss = take(tokens * 4);
     p.exps = take(p.piece * p.lde * 2);
-    p.part = take(p.splits > 1 ? p.splits * p.piece * p.ldx * 4 : 0);
+    // K is split while the parts' tiles are at most `units`: no more rows than
+    // those tiles have (nor than max_splits times the tokens).
+    const ShapeInfo& t = kShapes[p.dx];
+    const int64_t rows = std::min(p.units / ceil_div(width, t.tm) * t.tn, p.max_splits * p.piece);
+    p.part = take(p.max_splits > 1 ? rows * p.ldx * 4 : 0);
     p.sums = take(p.pieces > 1 ? vocab * width * 4 : 0);
   }
   p.total = at;
@@ -343,12 +421,18 @@ bool weight_in_place(const void* w, int64_t ldw, int64_t vocab, int64_t width) {
 template <int DT, int EPI, bool AKC, bool BKC, bool COUNT_K>
 void launch_head(Shape shape, const head::Args& a, int64_t wgs, hipStream_t s) {
   const dim3 grid((unsigned)wgs);
+  // Large tiles: four waves read the least LDS (128 KB per stage against 192 KB
+  // by eight), and the board runs at its power limit; the softmax's epilogue is
+  // faster by eight.  8192 x 65536 x 4096 bf16, us, four / eight waves: logits
+  // 3598 / 3513, dx 3096 / 3150, dw 3243 / 3259.
+  constexpr bool kSoftmax = EPI == head::kStats || EPI == head::kExp;
   if (shape == kLarge) {
-    head::head_kernel<DT, 256, 256, 2, 4, 2, AKC, BKC, EPI, COUNT_K><<<grid, 512, 0, s>>>(a);
+    head::head_kernel<DT, 256, 256, 2, kSoftmax ? 4 : 2, 5, AKC, BKC, EPI, COUNT_K>
+        <<<grid, kSoftmax ? 512 : 256, 0, s>>>(a);
   } else if (shape == kMedium) {
-    head::head_kernel<DT, 128, 128, 2, 4, 4, AKC, BKC, EPI, COUNT_K><<<grid, 512, 0, s>>>(a);
+    head::head_kernel<DT, 128, 128, 2, 4, 8, AKC, BKC, EPI, COUNT_K><<<grid, 512, 0, s>>>(a);
   } else if constexpr (BKC) {
-    head::head_kernel<DT, 128, 32, 4, 1, 4, AKC, BKC, EPI, COUNT_K><<<grid, 256, 0, s>>>(a);
+    head::head_kernel<DT, 128, 32, 4, 1, 5, AKC, BKC, EPI, COUNT_K><<<grid, 256, 0, s>>>(a);
   }
 }
 
@@ -381,23 +465,40 @@ int run_loss(const Plan& p, const Call& c, hipStream_t s) {
   uint16_t* rows = static_cast<uint16_t*>(at(p.rows));
   const int T = (int)p.tokens, V = (int)p.vocab, D = (int)p.width;
 
-  PackArgs pk{c.targets, c.ignore, p.vocab, T, c.mean, c.grad_scale, static_cast<int*>(at(p.slot)), token, target,
-              count, scale, p.grad ? nullptr : c.loss, p.grad ? nullptr : c.lse};
+  // At most 1024 runs, four workgroups per CU, while a run fits.
+  const int per_wg = (int)std::min<int64_t>(kPackRun, ceil_div(T, 1024));
+  const PackArgs pk{c.targets,
+                    c.ignore,
+                    p.vocab,
+                    T,
+                    per_wg,
+                    c.mean,
+                    c.grad_scale,
+                    token,
+                    target,
+                    count,
+                    scale,
+                    p.grad ? nullptr : c.loss,
+                    p.grad ? nullptr : c.lse,
+                    static_cast<const uint16_t*>(c.x),
+                    c.ldx,
+                    rows,
+                    p.ldx,
+                    D,
+                    (int)(p.ldx / 8),
+                    static_cast<uint16_t*>(c.dx),
+                    c.lddx};
+  const dim3 runs((unsigned)ceil_div(T, per_wg));
   if (c.id_bytes == 8)
-    pack_kernel<int64_t><<<1, 1024, 0, s>>>(pk);
+    pack_kernel<int64_t><<<runs, kPackThreads, 0, s>>>(pk);
   else
-    pack_kernel<int32_t><<<1, 1024, 0, s>>>(pk);
-  const auto copy = [&](const CopyArgs& a) {
-    const int64_t wgs = std::min<int64_t>(ceil_div((int64_t)a.rows * a.vecs, 256), 16384);
-    copy_rows_kernel<<<dim3((unsigned)wgs), 256, 0, s>>>(a);
-  };
-  copy(CopyArgs{static_cast<const uint16_t*>(c.x), c.ldx, rows, p.ldx, T, D, (int)(p.ldx / 8),
-                static_cast<const int*>(at(p.slot)), static_cast<uint16_t*>(c.dx), c.lddx});
+    pack_kernel<int32_t><<<runs, kPackThreads, 0, s>>>(pk);
   const uint16_t* weight = static_cast<const uint16_t*>(c.weight);
   int64_t ldw = p.vocab == 1 ? p.ldx : c.ldw;
   if (p.copy_weight) {
-    copy(CopyArgs{weight, c.ldw, static_cast<uint16_t*>(at(p.weight)), p.ldx, V, D, (int)(p.ldx / 8), nullptr,
-                  nullptr, 0});
+    const CopyArgs a{weight, c.ldw, static_cast<uint16_t*>(at(p.weight)), p.ldx, V, D, (int)(p.ldx / 8)};
+    const int64_t wgs = std::min<int64_t>(ceil_div((int64_t)V * a.vecs, 256), 16384);
+    copy_rows_kernel<<<dim3((unsigned)wgs), 256, 0, s>>>(a);
     weight = static_cast<const uint16_t*>(at(p.weight));
     ldw = p.ldx;
   }
@@ -418,8 +519,6 @@ int run_loss(const Plan& p, const Call& c, hipStream_t s) {
     a.K = (int)p.ldx;
     a.count = count;
     a.count0 = (int)t0;
-    a.splits = 1;
-    a.kchunk = a.K;
     a.tiles_m = (int)ceil_div(V, kShapes[p.logits].tm);
     a.stats = static_cast<f32x2*>(at(p.stats));
     a.ld_stats = p.blocks;
@@ -454,25 +553,24 @@ int run_loss(const Plan& p, const Call& c, hipStream_t s) {
     d.K = V;
     d.count = count;
     d.count0 = (int)t0;
-    d.splits = p.splits;
-    d.kchunk = p.kchunk;
+    d.units = p.units;
+    d.max_splits = p.max_splits;
     d.tiles_m = (int)ceil_div(D, kShapes[p.dx].tm);
     d.scale = scale;
     d.post = post;
-    const int64_t dx_wgs = tiles(p.dx, D, n) * p.splits;
-    if (p.splits == 1) {
-      d.out = c.dx;
-      d.ldo = c.lddx;
-      d.row_of = token + t0;
-      launch_head<DT, head::kRound, false, true, false>(p.dx, d, dx_wgs, s);
-    } else {
-      d.out = at(p.part);
-      d.ldo = p.ldx;
-      d.split_stride = p.piece * p.ldx;
-      launch_head<DT, head::kPartial, false, true, false>(p.dx, d, dx_wgs, s);
-      const JoinArgs j{static_cast<const float*>(d.out), p.ldx, d.split_stride, p.splits, D, (int)(p.ldx / 8), count,
-                       (int)t0, token + t0, scale, post, static_cast<uint16_t*>(c.dx), c.lddx};
-      join_kernel<DT><<<dim3((unsigned)n, (unsigned)ceil_div(p.ldx / 8, 256)), 256, 0, s>>>(j);
+    d.out = c.dx;
+    d.ldo = c.lddx;
+    d.row_of = token + t0;
+    d.part = static_cast<float*>(at(p.part));
+    d.ld_part = p.ldx;
+    // (as many workgroups as any number of live tokens takes)
+    launch_head<DT, head::kSplit, false, true, false>(p.dx, d, std::max<int64_t>(tiles(p.dx, D, n), p.units), s);
+    if (p.max_splits > 1) {
+      const JoinArgs j{d.part,    p.ldx, d.units,    d.max_splits, d.tiles_m, kShapes[p.dx].tn,
+                       n,         V,     D,          (int)(p.ldx / 8), count, (int)t0,
+                       token + t0, scale, post,      static_cast<uint16_t*>(c.dx), c.lddx};
+      const int64_t wgs = std::min<int64_t>(ceil_div((int64_t)n * j.vecs, 256), 4 * kCus);
+      join_kernel<DT><<<dim3((unsigned)wgs), 256, 0, s>>>(j);
     }
 
     head::Args w{};
@@ -485,8 +583,6 @@ int run_loss(const Plan& p, const Call& c, hipStream_t s) {
     w.K = n;
     w.count = count;
     w.count0 = (int)t0;
-    w.splits = 1;
-    w.kchunk = n;
     w.tiles_m = (int)ceil_div(D, kShapes[p.dw].tm);
     w.scale = scale;
     w.post = post;
@@ -497,8 +593,8 @@ int run_loss(const Plan& p, const Call& c, hipStream_t s) {
       w.ldo = c.lddw;
       launch_head<DT, head::kRound, false, false, true>(p.dw, w, dw_wgs, s);
     } else {
-      w.out = sums;
-      w.ldo = D;
+      w.part = sums;
+      w.ld_part = D;
       launch_head<DT, head::kPartial, false, false, true>(p.dw, w, dw_wgs, s);
     }
   }
@@ -532,7 +628,7 @@ int check_call(int dtype, const Call& c, int64_t tokens, int64_t vocab, int64_t 
   *plan = make_plan(tokens, vocab, width, !weight_in_place(c.weight, c.ldw, vocab, width), grad);
   HCG_LM_REQUIRE(tiles(plan->logits, vocab, plan->piece) < ((int64_t)1 << 31) &&
                      tiles(plan->dw, width, vocab) < ((int64_t)1 << 31) &&
-                     tiles(plan->dx, width, plan->piece) * std::max(plan->splits, 1) < ((int64_t)1 << 31),
+                     tiles(plan->dx, width, plan->piece) < ((int64_t)1 << 31),
                  "too many tiles");
   HCG_LM_REQUIRE(c.ws && ws_bytes >= plan->total && hcg::elem_aligned(c.ws, 256),
                  "workspace of %lld bytes, %lld needed (256-byte aligned)", (long long)ws_bytes,
