@@ -88,16 +88,24 @@ __global__ __launch_bounds__(256) void embed_kernel(EmbedArgs g) {
 // Gradient
 // ---------------------------------------------------------------------------
 
-constexpr int kGradThreads = 256;
+constexpr int kGradThreads = 512;
 constexpr int kGradWaves = kGradThreads / 64;
 constexpr int kScan = 8;           // ids in flight per lane
 constexpr int kMaxRows = 64;       // table rows per workgroup
-constexpr int kListPerWave = 512;  // ids of a workgroup's rows kept in LDS, per wave that scans
-constexpr int kLong = 32;
-constexpr int kWindow = 64;
+constexpr int kListPerWave = 256;  // ids of a workgroup's rows kept in LDS, per wave that scans
+// Rows of dy in flight per thread.  (16 take registers that leave two workgroups
+// per CU instead of four: 999 tokens of 515 f32 into 5003 rows 10.9 us with 8,
+// 12.7 with 16.)
+constexpr int kSumLoads = 8;
+constexpr int kLong = 16;
+constexpr int kWindow = 32;
 // Runs of long rows in one window: those that lie inside it have more than
 // kLong entries each, and one more may enter and one leave.
 constexpr int kRuns = kWindow / (kLong + 1) + 2;
+// Up to so many tokens of rows of at most half as many items as threads, a
+// workgroup sums its long rows too, in parts that meet in LDS: then one launch
+// does it all.
+constexpr int kOneLaunch = 2048;
 
 struct EmbedGradArgs {
   const void* dy;
@@ -105,11 +113,12 @@ struct EmbedGradArgs {
   void* grad;
   int64_t lddy, ldg, vocab, padding;
   int n;
-  int width, vecs;  // vecs: 16-byte vectors of dy in a row
+  int width, items;  // items: dy's whole 16-byte vectors in a row, and the elements past them
   int rows;         // table rows per workgroup
   float scale;
+  bool lines;       // the gradient's rows are whole 128-byte lines
   // Lists over the tokens in the order of (row, i).
-  int* token;     // i
+  int* token;     // i (null: one launch)
   int* row;       // the long row it belongs to, or -1
   int* run_len;   // (at a long row's first entry) its tokens
   int* found;     // tokens of a workgroup's rows in the order of i, where LDS is too small ...
@@ -122,21 +131,76 @@ __device__ __forceinline__ int lanes_below(uint64_t mask) {
 }
 
 // f[0..E) of dy scaled, as the sum's rounding to G and one 16- or 32-byte store.
-template <class T, class G>
-__device__ __forceinline__ void store_grad(G* p, const float (&f)[kVec<T>], float scale, int valid) {
+// nt: the rows are whole 128-byte lines, so non-temporal stores leave no partial
+// ones (65536 x 4096 bf16: 170 us without, 135 with).
+template <bool WHOLE, class T, class G>
+__device__ __forceinline__ void store_grad(G* p, const float (&f)[kVec<T>], float scale, bool nt) {
   constexpr int E = kVec<T>, EG = kVec<G>;
+  if constexpr (!WHOLE) {
+    *p = (G)(f[0] * scale);
+  } else {
 #pragma unroll
-  for (int h = 0; h < E / EG; ++h) {
-    float o[EG];
+    for (int h = 0; h < E / EG; ++h) {
+      float o[EG];
 #pragma unroll
-    for (int e = 0; e < EG; ++e) o[e] = f[h * EG + e] * scale;
-    if (h * EG < valid) hcg::store_raw(p + h * EG, hcg::pack<G>(o), valid - h * EG);
+      for (int e = 0; e < EG; ++e) o[e] = f[h * EG + e] * scale;
+      if (nt)
+        hcg::store_raw<true>(p + h * EG, hcg::pack<G>(o), EG);
+      else
+        hcg::store_raw(p + h * EG, hcg::pack<G>(o), EG);
+    }
   }
 }
 
-template <class T, class G, class I>
-__global__ __launch_bounds__(kGradThreads) void embed_grad_kernel(EmbedGradArgs g) {
+// A row as whole vectors and, one by one, the elements past them: items
+// 0 .. items - 1.  A thread's item is WHOLE (E elements) or one element, so that
+// no load asks how much of it is in the row.
+struct Items {
+  int whole, items;
+  __device__ Items(int width, int E) : whole(width / E), items(width / E + width % E) {}
+};
+
+// sum[e] += the rows of dy (from the item's first element on) that entries
+// 0 .. n - 1 name, in order.
+template <bool WHOLE, class T, class F>
+__device__ __forceinline__ void sum_rows(float (&sum)[kVec<T>], const T* dy, int64_t lddy, int n, F entry) {
+  constexpr int E = kVec<T>, W = WHOLE ? E : 1;
+  int j = 0;
+  auto batch = [&](auto count) {
+    constexpr int N = decltype(count)::value;
+    raw4 raw[N];
+    T one[N];
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      const T* p = dy + (int64_t)entry(j + u) * lddy;
+      if constexpr (WHOLE)
+        raw[u] = hcg::load_raw(p, E);
+      else
+        one[u] = *p;
+    }
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      float f[E];
+      if constexpr (WHOLE)
+        hcg::unpack<T>(raw[u], f);
+      else
+        f[0] = (float)one[u];
+#pragma unroll
+      for (int e = 0; e < W; ++e) sum[e] += f[e];
+    }
+    j += N;
+  };
+  while (n - j >= kSumLoads) batch(std::integral_constant<int, kSumLoads>{});
+  if (n - j >= 4) batch(std::integral_constant<int, 4>{});
+  if (n - j >= 2) batch(std::integral_constant<int, 2>{});
+  if (n - j >= 1) batch(std::integral_constant<int, 1>{});
+}
+
+// ONE: no lists are kept (g.token is null), the workgroup sums its long rows too.
+template <class T, class G, class I, bool ONE>
+__global__ __launch_bounds__(kGradThreads, 8) void embed_grad_kernel(EmbedGradArgs g) {
   constexpr int E = kVec<T>;
+  __shared__ float meet[ONE ? kGradThreads * E : 1];
   __shared__ int found[kGradWaves * kListPerWave], grouped[kGradWaves * kListPerWave];
   __shared__ uint8_t found_row[kGradWaves * kListPerWave];
   __shared__ int wave_found[kGradWaves], wave_below[kGradWaves];
@@ -192,7 +256,7 @@ __global__ __launch_bounds__(kGradThreads) void embed_grad_kernel(EmbedGradArgs 
     below += wave_below[w];
     fits = fits && wave_found[w] <= kListPerWave;
   }
-  if (!fits) {
+  if (!ONE && !fits) {
     // (wave_found and wave_below are written again with the same values)
     scan([&](int at, int i, int r) {
       g.found[below + before + at] = i;
@@ -203,7 +267,7 @@ __global__ __launch_bounds__(kGradThreads) void embed_grad_kernel(EmbedGradArgs 
 
   // Find number j of wave w.
   auto find = [&](int w, int off, int j, int& i) -> int {
-    if (fits) {
+    if (ONE || fits) {
       i = found[w * kListPerWave + j];
       return found_row[w * kListPerWave + j];
     }
@@ -238,105 +302,132 @@ __global__ __launch_bounds__(kGradThreads) void embed_grad_kernel(EmbedGradArgs 
         const uint64_t hit = __ballot(mine);
         if (mine) {
           const int at = put + lanes_below(hit);
-          if (fits) grouped[at] = i;
-          if (g.token) g.token[below + at] = i;
+          if (ONE || fits) grouped[at] = i;
+          if (!ONE) g.token[below + at] = i;
         }
         put += __popcll(hit);
       }
       off += wave_found[w];
     }
-    if (g.row) {
+    if (!ONE) {
       for (int j = lane; j < c; j += 64) g.row[below + start[r] + j] = c > kLong ? (int)(lo + r) : -1;
       if (c > kLong && lane == 0) g.run_len[below + start[r]] = c;
     }
   }
   // The places past all tokens (ids that name no row) belong to no long row.
-  if (g.row && lo + rows == g.vocab)
+  if (!ONE && lo + rows == g.vocab)
     for (int j = below + total + tid; j < g.n; j += kGradThreads) g.row[j] = -1;
   __syncthreads();
 
-  // Every row that is not long, as vectors over the threads.
+  // Every row that is not long, its items over the threads.
   const T* dy = static_cast<const T*>(g.dy);
   G* grad = static_cast<G*>(g.grad);
-  const int work = rows * g.vecs;
+  const Items it(g.width, E);
+  const auto entry = [&](int j) { return ONE || fits ? grouped[j] : g.token[below + j]; };
+  const int work = rows * it.items;
   for (int at = tid; at < work; at += kGradThreads) {
-    const int r = at / g.vecs, c = (at - r * g.vecs) * E;
-    const int n = count[r];
+    const int r = at / it.items, i = at - r * it.items;
+    const int n = count[r], first = start[r];
     if (n > kLong) continue;
-    float sum[E];
+    const auto one_item = [&](auto whole, int c) {
+      constexpr bool WHOLE = decltype(whole)::value;
+      float sum[E] = {};
+      sum_rows<WHOLE, T>(sum, dy + c, g.lddy, n, [&](int j) { return entry(first + j); });
+      store_grad<WHOLE, T, G>(grad + (lo + r) * g.ldg + c, sum, g.scale, g.lines);
+    };
+    if (i < it.whole)
+      one_item(std::true_type{}, i * E);
+    else
+      one_item(std::false_type{}, it.whole * E + i - it.whole);
+  }
+  if constexpr (!ONE) return;
+
+  // A long row's entries in `parts` runs, a group of threads each (the row's
+  // items are at most half the threads, and few tokens always fit the lists).
+  const int parts = kGradThreads / it.items, part = tid / it.items, i = tid - part * it.items;
+  for (int r = 0; r < rows; ++r) {
+    const int n = count[r];
+    if (n <= kLong) continue;
+    const int first = start[r] + n * part / parts, len = start[r] + n * (part + 1) / parts - first;
+    const auto one_item = [&](auto whole, int c) {
+      constexpr bool WHOLE = decltype(whole)::value;
+      constexpr int W = WHOLE ? E : 1;
+      float sum[E] = {};
+      if (part < parts)
+        sum_rows<WHOLE, T>(sum, dy + c, g.lddy, len, [&](int j) { return entry(first + j); });
 #pragma unroll
-    for (int e = 0; e < E; ++e) sum[e] = 0.f;
-    const int first = start[r];
-    for (int j0 = 0; j0 < n; j0 += 4) {
-      raw4 raw[4];
+      for (int e = 0; e < W; ++e) meet[e * kGradThreads + tid] = sum[e];
+    };
+    const bool whole = i < it.whole;
+    const int c = whole ? i * E : it.whole * E + i - it.whole;
+    if (whole)
+      one_item(std::true_type{}, c);
+    else
+      one_item(std::false_type{}, c);
+    __syncthreads();
+    if (part == 0) {
+      float sum[E];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        if (j0 + u < n) {
-          const int i = fits ? grouped[first + j0 + u] : g.token[below + first + j0 + u];
-          raw[u] = hcg::load_raw(dy + (int64_t)i * g.lddy + c, g.width - c);
-        }
-      }
+      for (int e = 0; e < E; ++e) sum[e] = meet[e * kGradThreads + tid];
+      for (int q = 1; q < parts; ++q)
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        if (j0 + u < n) {
-          float f[E];
-          hcg::unpack<T>(raw[u], f);
-#pragma unroll
-          for (int e = 0; e < E; ++e) sum[e] += f[e];
-        }
-      }
+        for (int e = 0; e < E; ++e) sum[e] += meet[e * kGradThreads + q * it.items + tid];
+      G* p = grad + (lo + r) * g.ldg + c;
+      if (whole)
+        store_grad<true, T, G>(p, sum, g.scale, g.lines);
+      else
+        store_grad<false, T, G>(p, sum, g.scale, g.lines);
     }
-    store_grad<T, G>(grad + (lo + r) * g.ldg + c, sum, g.scale, g.width - c);
+    __syncthreads();
   }
 }
 
-// Window blockIdx.x of the lists, vectors blockIdx.y * 256 ...: the sum of
+// The entries of a window (a lane each): which belong to a long row, and of
+// these which are the first of a run in the window.
+struct Window {
+  uint64_t in_long, starts;
+};
+__device__ __forceinline__ Window window_of(const EmbedGradArgs& g, int from, int n, int lane, int* row) {
+  const int mine = lane < n ? g.row[from + lane] : -1;
+  const int left = __shfl_up(mine, 1);
+  *row = mine;
+  return Window{__ballot(mine >= 0), __ballot(mine >= 0 && (lane == 0 || mine != left))};
+}
+
+// Window blockIdx.x of the lists, items blockIdx.y * 256 ...: the sum of
 // each run of one long row in it.
 template <class T>
 __global__ __launch_bounds__(256) void embed_window_kernel(EmbedGradArgs g) {
   constexpr int E = kVec<T>;
-  __shared__ int token[kWindow], row[kWindow];
-  const int from = blockIdx.x * kWindow, n = min(kWindow, g.n - from);
-  if ((int)threadIdx.x < n) {
-    token[threadIdx.x] = g.token[from + threadIdx.x];
-    row[threadIdx.x] = g.row[from + threadIdx.x];
-  }
+  __shared__ int token[kWindow];
+  const int from = blockIdx.x * kWindow, n = min(kWindow, g.n - from), lane = threadIdx.x & 63;
+  int row;
+  const Window w = window_of(g, from, n, lane, &row);
+  if (w.in_long == 0) return;
+  if ((int)threadIdx.x < n) token[threadIdx.x] = g.token[from + threadIdx.x];
   __syncthreads();
-  const int c = (blockIdx.y * 256 + threadIdx.x) * E;
-  if (c >= g.width) return;
-  const T* dy = static_cast<const T*>(g.dy) + c;
+  const Items it(g.width, E);
+  const int i = blockIdx.y * 256 + threadIdx.x;
+  if (i >= it.items) return;
+  const bool whole = i < it.whole;
+  const int c = whole ? i * E : it.whole * E + i - it.whole;
   float* part = g.part + (int64_t)blockIdx.x * kRuns * g.width + c;
-  const int left = g.width - c;
-  int j = 0;
-  while (j < n) {
-    const int r = row[j];
-    if (r < 0) {
-      ++j;
-      continue;
+  for (uint64_t starts = w.starts; starts; starts &= starts - 1) {
+    const int first = __ffsll((unsigned long long)starts) - 1;
+    // The run ends before the next start or the next entry of no long row.
+    const uint64_t ends = ((starts & (starts - 1)) | ~w.in_long) >> first >> 1;
+    const int len = __ffsll((unsigned long long)ends);
+    const T* dy = static_cast<const T*>(g.dy) + c;
+    const auto entry = [&](int j) { return token[first + j]; };
+    float sum[E] = {};
+    if (whole) {
+      sum_rows<true, T>(sum, dy, g.lddy, len, entry);
+#pragma unroll
+      for (int e = 0; e < E; ++e) part[e] = sum[e];
+    } else {
+      sum_rows<false, T>(sum, dy, g.lddy, len, entry);
+      part[0] = sum[0];
     }
-    float sum[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) sum[e] = 0.f;
-    int end = j + 1;
-    while (end < n && row[end] == r) ++end;
-    for (; j < end; j += 8) {
-      raw4 raw[8];
-#pragma unroll
-      for (int u = 0; u < 8; ++u)
-        if (j + u < end) raw[u] = hcg::load_raw(dy + (int64_t)token[j + u] * g.lddy, left);
-#pragma unroll
-      for (int u = 0; u < 8; ++u)
-        if (j + u < end) {
-          float f[E];
-          hcg::unpack<T>(raw[u], f);
-#pragma unroll
-          for (int e = 0; e < E; ++e) sum[e] += f[e];
-        }
-    }
-    j = end;
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-      if (e < left) part[e] = sum[e];
     part += g.width;
   }
 }
@@ -345,24 +436,26 @@ __global__ __launch_bounds__(256) void embed_window_kernel(EmbedGradArgs g) {
 // their windows' sums, in order.
 template <class G>
 __global__ __launch_bounds__(256) void embed_long_kernel(EmbedGradArgs g) {
-  __shared__ int row[kWindow + 1];  // [0]: the entry before the window
-  const int from = blockIdx.x * kWindow, n = min(kWindow, g.n - from);
-  for (int j = threadIdx.x; j <= n; j += 256) row[j] = from + j > 0 ? g.row[from + j - 1] : -1;
-  __syncthreads();
+  const int from = blockIdx.x * kWindow, n = min(kWindow, g.n - from), lane = threadIdx.x & 63;
+  int row;
+  const Window w = window_of(g, from, n, lane, &row);
+  // A run that goes on from the window before is that window's business.
+  const int before = from > 0 ? g.row[from - 1] : -1;
+  uint64_t starts = w.starts;
+  int run = 0;
+  if ((starts & 1) && before == __shfl(row, 0)) starts &= ~(uint64_t)1, run = 1;
   const int64_t c = (int64_t)blockIdx.y * 256 + threadIdx.x;
-  if (c >= g.width) return;
-  int run = row[1] >= 0 ? 0 : -1;  // of the entry looked at, counted over the long rows of the window
-  for (int j = 1; j <= n; ++j) {
-    const bool starts = row[j] >= 0 && row[j] != row[j - 1];
-    if (j > 1 && starts) ++run;
-    if (!starts) continue;
-    const int len = g.run_len[from + j - 1];
-    const int windows = (from + j - 1 + len - 1) / kWindow - (int)blockIdx.x;  // after this one
+  for (; starts; starts &= starts - 1, ++run) {
+    const int first = __ffsll((unsigned long long)starts) - 1;
+    const int v = __shfl(row, first);
+    if (c >= g.width) continue;
+    const int len = g.run_len[from + first];
+    const int windows = (from + first + len - 1) / kWindow - (int)blockIdx.x;  // after this one
     float sum = g.part[((int64_t)blockIdx.x * kRuns + run) * g.width + c];
     const float* next = g.part + (int64_t)(blockIdx.x + 1) * kRuns * g.width + c;
-#pragma unroll 8
-    for (int w = 0; w < windows; ++w) sum += next[(int64_t)w * kRuns * g.width];
-    static_cast<G*>(g.grad)[(int64_t)row[j] * g.ldg + c] = (G)(sum * g.scale);
+#pragma unroll 16
+    for (int q = 0; q < windows; ++q) sum += next[(int64_t)q * kRuns * g.width];
+    static_cast<G*>(g.grad)[(int64_t)v * g.ldg + c] = (G)(sum * g.scale);
   }
 }
 
@@ -372,6 +465,13 @@ __global__ __launch_bounds__(256) void embed_long_kernel(EmbedGradArgs g) {
 
 constexpr int64_t kMaxTokens = (int64_t)1 << 30;
 
+int64_t items_of(int dtype, int64_t width) {
+  const int64_t e = 16 / hcg::elem_bytes(dtype);
+  return width / e + width % e;
+}
+bool one_launch(int64_t n, int64_t items) {
+  return n <= kLong || (n <= kOneLaunch && items <= kGradThreads / 2);
+}
 int64_t windows_of(int64_t n) { return (n + kWindow - 1) / kWindow; }
 int64_t round256(int64_t b) { return (b + 255) / 256 * 256; }
 
@@ -387,10 +487,14 @@ void with_elem(int dtype, F f) {
 
 template <class T, class G, class I>
 void run_embed_grad(const EmbedGradArgs& a, hipStream_t s) {
-  embed_grad_kernel<T, G, I><<<dim3((unsigned)((a.vocab + a.rows - 1) / a.rows)), kGradThreads, 0, s>>>(a);
-  if (a.token == nullptr) return;  // too few tokens for a long row
+  const dim3 grid((unsigned)((a.vocab + a.rows - 1) / a.rows));
+  if (a.token == nullptr) {
+    embed_grad_kernel<T, G, I, true><<<grid, kGradThreads, 0, s>>>(a);
+    return;
+  }
+  embed_grad_kernel<T, G, I, false><<<grid, kGradThreads, 0, s>>>(a);
   const unsigned windows = (unsigned)windows_of(a.n);
-  embed_window_kernel<T><<<dim3(windows, (unsigned)((a.vecs + 255) / 256)), 256, 0, s>>>(a);
+  embed_window_kernel<T><<<dim3(windows, (unsigned)((a.items + 255) / 256)), 256, 0, s>>>(a);
   embed_long_kernel<G><<<dim3(windows, (unsigned)((a.width + 255) / 256)), 256, 0, s>>>(a);
 }
 
@@ -428,8 +532,8 @@ int hcg_embedding(int dtype, const void* table, int64_t ldt, int64_t vocab, int6
   return HCG_OK;
 }
 
-int64_t hcg_embedding_grad_workspace(int64_t n, int64_t vocab, int64_t width) {
-  if (n <= kLong || vocab <= 0 || width <= 0 || n >= kMaxTokens) return 0;
+int64_t hcg_embedding_grad_workspace(int dtype, int64_t n, int64_t vocab, int64_t width) {
+  if (vocab <= 0 || width <= 0 || n >= kMaxTokens || one_launch(n, items_of(dtype, width))) return 0;
   return 4 * round256(n * 4) + round256(n * 2) + windows_of(n) * kRuns * width * 4;
 }
 
@@ -451,7 +555,7 @@ int hcg_embedding_grad(int dtype, const void* dy, int64_t lddy, int64_t n, int64
   HCG_LM_REQUIRE(hcg::elem_aligned(dy, eb) && hcg::elem_aligned(grad, hcg::elem_bytes(grad_dtype)) &&
                      hcg::elem_aligned(ids, id_bytes),
                  "rows and ids must be aligned to their elements");
-  const int64_t need = hcg_embedding_grad_workspace(n, vocab, width);
+  const int64_t need = hcg_embedding_grad_workspace(dtype, n, vocab, width);
   HCG_LM_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && hcg::elem_aligned(workspace, 256)),
                  "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
   EmbedGradArgs a{};
@@ -464,9 +568,15 @@ int hcg_embedding_grad(int dtype, const void* dy, int64_t lddy, int64_t n, int64
   a.padding = padding_idx < 0 ? -1 : padding_idx;
   a.n = (int)n;
   a.width = (int)width;
-  a.vecs = (int)((width * eb + 15) / 16);
-  a.rows = (int)std::min<int64_t>(kMaxRows, (vocab + 1023) / 1024);
+  a.items = (int)items_of(dtype, width);
+  // A small table in one round of workgroups (1024), a large one in up to four,
+  // so that some scan the ids while others write (65536 x 4096 bf16: 1024
+  // workgroups 135 us, 4096 123).
+  const int64_t quick = std::min((vocab + 1023) / 1024, std::max<int64_t>(1, (128 << 10) / (width * eb)));
+  a.rows = (int)std::min<int64_t>(kMaxRows, std::max((vocab + 4095) / 4096, quick));
   a.scale = scale;
+  const int gb = hcg::elem_bytes(grad_dtype);
+  a.lines = hcg::elem_aligned(grad, 128) && (vocab == 1 || ldg * gb % 128 == 0);
   if (need > 0) {
     char* p = static_cast<char*>(workspace);
     a.token = reinterpret_cast<int*>(p);

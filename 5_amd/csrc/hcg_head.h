@@ -289,8 +289,12 @@ struct RowStage {
 };
 
 // AKC, BKC: the operand is stored with K contiguous.  COUNT_K: the live
-// tokens bound K, else N.
-template <int DT, int TM, int TN, int WM, int WN, int UNITS, bool AKC, bool BKC, int EPI, bool COUNT_K>
+// tokens bound K, else N.  ROTATE (few tokens, bound by reading A's rows): a
+// workgroup starts at a stage of its own (a golden-ratio sequence) and wraps.
+// With all of them at one k, rows a power of two apart put every piece that is
+// read at one offset, and the reads pile onto a few HBM channels: logits of 16 x
+// 65536 x 4096 bf16 110 us, rotated 90 (5.96 TB/s).
+template <int DT, int TM, int TN, int WM, int WN, int UNITS, bool AKC, bool BKC, int EPI, bool COUNT_K, bool ROTATE>
 __global__ __launch_bounds__(64 * WM * WN, 1) void head_kernel(Args g) {
   constexpr int NW = WM * WN;
   constexpr int MI = TM / WM / 32, NI = TN / WN / 32;
@@ -298,8 +302,14 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void head_kernel(Args g) {
   constexpr int NSUB = kStep / 16;
   using OpA = Operand<TM, AKC, NW>;
   using OpB = Operand<TN, BKC, NW>;
-  constexpr int kUnitBytes = OpA::kBytes > OpB::kBytes ? OpA::kBytes : OpB::kBytes;
-  static_assert(UNITS >= 4 && kUnitBytes * UNITS <= 160 * 1024, "ring");
+  // (In a ring of an even number of units a place holds units of one operand.)
+  constexpr int kUnitA = UNITS % 2 && OpB::kBytes > OpA::kBytes ? OpB::kBytes : OpA::kBytes;
+  constexpr int kUnitB = UNITS % 2 && OpA::kBytes > OpB::kBytes ? OpA::kBytes : OpB::kBytes;
+  static_assert(UNITS >= 4 && kUnitA * ((UNITS + 1) / 2) + kUnitB * (UNITS / 2) <= 160 * 1024, "ring");
+  auto place = [](auto uc) {
+    constexpr int P = decltype(uc)::value % UNITS;
+    return ring_unit<P % 2 ? kUnitB : kUnitA, P>();
+  };
   constexpr int kPeriod = UNITS % 2 ? UNITS : UNITS / 2;  // stages until the units' places repeat
 
   const int tid = threadIdx.x, lane = tid & 63;
@@ -340,16 +350,36 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void head_kernel(Args g) {
   // Instructions FROM to TO - 1 of the next unit U of its operand (even units
   // are A's).
   int left_a = K, left_b = K;
+  const int stage0 = ROTATE ? (int)(((uint64_t)((uint32_t)tm * 2654435769u) * (uint32_t)nk) >> 32) : 0;
+  int at_a = stage0, at_b = stage0, issued_a = 0, issued_b = 0;
+  if constexpr (ROTATE) {
+    pa += stage0 * step_a;
+    pb += stage0 * step_b;
+    left_a -= stage0 * kStep;
+    left_b = left_a;
+  }
+  auto advance = [&](const uint16_t*& p, int64_t step, int& left, int& at, int& issued) {
+    p += step;
+    left -= kStep;
+    if constexpr (ROTATE) {
+      if (++at == nk) {
+        at = 0;
+        p -= nk * step;
+        left = K;
+      }
+      if (++issued >= nk) left = 0;
+    }
+  };
   auto issue = [&](auto uc, auto full, auto from, auto to) {
     constexpr int U = decltype(uc)::value, F = decltype(from)::value, T = decltype(to)::value;
     constexpr bool kFull = decltype(full)::value;
-    unsigned char* st = ring_unit<kUnitBytes, U % UNITS>();
+    unsigned char* st = place(uc);
     if constexpr (U % 2 == 0) {
       a.template issue<kFull, F, T>(pa, st, wave, left_a);
-      if constexpr (T == OpA::kInst) pa += step_a, left_a -= kStep;
+      if constexpr (T == OpA::kInst) advance(pa, step_a, left_a, at_a, issued_a);
     } else {
       b.template issue<kFull, F, T>(pb, st, wave, left_b);
-      if constexpr (T == OpB::kInst) pb += step_b, left_b -= kStep;
+      if constexpr (T == OpB::kInst) advance(pb, step_b, left_b, at_b, issued_b);
     }
   };
   // DMA instructions of n units from unit u on.
@@ -360,8 +390,8 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void head_kernel(Args g) {
   };
   auto read = [&](auto kc, int s) {
     constexpr int K0 = decltype(kc)::value;
-    const unsigned char* sa = ring_unit<kUnitBytes, 2 * K0 % UNITS>();
-    const unsigned char* sb = ring_unit<kUnitBytes, (2 * K0 + 1) % UNITS>();
+    const unsigned char* sa = place(Int<2 * K0>{});
+    const unsigned char* sb = place(Int<2 * K0 + 1>{});
 #pragma unroll
     for (int i = 0; i < MI; ++i) fa[s & 1][i] = a.frag(sa, i, s);
 #pragma unroll
@@ -448,7 +478,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void head_kernel(Args g) {
   read(Int<0>{}, 0);
 
   int kt = 0;
-  const int nfull = K / kStep;
+  const int nfull = ROTATE ? 0 : K / kStep;  // (a rotated walk may pass the partial stage anywhere)
   for (; kt + kPeriod + UNITS / 2 <= nfull; kt += kPeriod) {
     iteration(Int<0>{}, Full{});
     iteration(Int<1>{}, Full{});
@@ -480,12 +510,12 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void head_kernel(Args g) {
   __builtin_amdgcn_s_barrier();  // every wave has read its last fragments: the stages are free
   // Rows on their way out: a part of the first units for each wave.
   typedef RowStage<MI> Stage;
-  constexpr int kWavesPerUnit = kUnitBytes / Stage::kBytes;
-  static_assert(kWavesPerUnit * 3 >= NW, "staging");
-  unsigned char* const rows_out =
-      (wave < kWavesPerUnit ? ring_unit<kUnitBytes, 0>()
-                            : wave < 2 * kWavesPerUnit ? ring_unit<kUnitBytes, 1>() : ring_unit<kUnitBytes, 2>()) +
-      wave % kWavesPerUnit * Stage::kBytes;
+  constexpr int kWavesPerUnit = kUnitA / Stage::kBytes;  // (in the places 0, 2, 4 of A's units)
+  static_assert(kWavesPerUnit * ((UNITS + 1) / 2) >= NW && kWavesPerUnit * 3 >= NW, "staging");
+  unsigned char* const rows_out = (wave < kWavesPerUnit       ? place(Int<0>{})
+                                   : wave < 2 * kWavesPerUnit ? place(Int<2>{})
+                                                              : place(Int<4 % UNITS>{})) +
+                                  wave % kWavesPerUnit * Stage::kBytes;
 
   // Accumulator block (mi, ni) of a lane: row n of the output, columns
   // m = mfirst + 32 mi + 8 (r / 4) + 4 (lane / 32) + r % 4.

@@ -427,12 +427,16 @@ void launch_head(Shape shape, const head::Args& a, int64_t wgs, hipStream_t s) {
   // 3598 / 3513, dx 3096 / 3150, dw 3243 / 3259.
   constexpr bool kSoftmax = EPI == head::kStats || EPI == head::kExp;
   if (shape == kLarge) {
-    head::head_kernel<DT, 256, 256, 2, kSoftmax ? 4 : 2, 5, AKC, BKC, EPI, COUNT_K>
+    head::head_kernel<DT, 256, 256, 2, kSoftmax ? 4 : 2, 5, AKC, BKC, EPI, COUNT_K, false>
         <<<grid, kSoftmax ? 512 : 256, 0, s>>>(a);
   } else if (shape == kMedium) {
-    head::head_kernel<DT, 128, 128, 2, 4, 8, AKC, BKC, EPI, COUNT_K><<<grid, 512, 0, s>>>(a);
+    // (one tile of tokens: bound by reading the weights)
+    if (kSoftmax && a.N <= 128)
+      head::head_kernel<DT, 128, 128, 2, 4, 8, AKC, BKC, EPI, COUNT_K, kSoftmax><<<grid, 512, 0, s>>>(a);
+    else
+      head::head_kernel<DT, 128, 128, 2, 4, 8, AKC, BKC, EPI, COUNT_K, false><<<grid, 512, 0, s>>>(a);
   } else if constexpr (BKC) {
-    head::head_kernel<DT, 128, 32, 4, 1, 5, AKC, BKC, EPI, COUNT_K><<<grid, 256, 0, s>>>(a);
+    head::head_kernel<DT, 128, 32, 4, 1, 6, AKC, BKC, EPI, COUNT_K, kSoftmax><<<grid, 256, 0, s>>>(a);
   }
 }
 

@@ -36,19 +36,25 @@ template <class T>
 constexpr int kVec = 16 / (int)sizeof(T);
 
 typedef uint32_t raw4 __attribute__((ext_vector_type(4)));
-typedef uint32_t raw4u __attribute__((ext_vector_type(4), aligned(2)));
+// The same at an address aligned to an element only.
+template <int BYTES>
+struct RawAt;
+template <>
+struct RawAt<2> {
+  typedef uint32_t type __attribute__((ext_vector_type(4), aligned(2)));
+};
+template <>
+struct RawAt<4> {
+  typedef uint32_t type __attribute__((ext_vector_type(4), aligned(4)));
+};
 
 // 16 bytes at an element-aligned address, of which the first `valid` elements
 // are in the row (the rest zero, not read).
 template <class T>
 __device__ __forceinline__ raw4 load_raw(const T* p, int valid) {
   if (valid >= kVec<T>) {
-    if constexpr (sizeof(T) == 4) {
-      typedef uint32_t raw4w __attribute__((ext_vector_type(4), aligned(4)));
-      return *reinterpret_cast<const raw4w*>(p);
-    } else {
-      return *reinterpret_cast<const raw4u*>(p);
-    }
+    typedef typename RawAt<sizeof(T)>::type raw4a;
+    return *reinterpret_cast<const raw4a*>(p);
   }
   raw4 r{0, 0, 0, 0};
   if constexpr (sizeof(T) == 4) {
@@ -65,15 +71,16 @@ __device__ __forceinline__ raw4 load_raw(const T* p, int valid) {
   return r;
 }
 
-template <class T>
+// NT: non-temporal, for outputs much larger than the caches (they leave no
+// dirty lines for the launch's end to write back).
+template <bool NT = false, class T>
 __device__ __forceinline__ void store_raw(T* p, raw4 v, int valid) {
   if (valid >= kVec<T>) {
-    if constexpr (sizeof(T) == 4) {
-      typedef uint32_t raw4w __attribute__((ext_vector_type(4), aligned(4)));
-      *reinterpret_cast<raw4w*>(p) = v;
-    } else {
-      *reinterpret_cast<raw4u*>(p) = v;
-    }
+    typedef typename RawAt<sizeof(T)>::type raw4a;
+    if constexpr (NT)
+      __builtin_nontemporal_store((raw4a)v, reinterpret_cast<raw4a*>(p));
+    else
+      *reinterpret_cast<raw4a*>(p) = v;
     return;
   }
   if constexpr (sizeof(T) == 4) {

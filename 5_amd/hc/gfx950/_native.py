@@ -98,7 +98,7 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.hcg_mfma_step.restype = c_int
     f32 = ctypes.c_float
     lib.hcg_embedding.argtypes = [c_int, vp, i64, i64, i64, c_int, vp, i64, f32, vp, i64, vp]
-    lib.hcg_embedding_grad_workspace.argtypes = [i64, i64, i64]
+    lib.hcg_embedding_grad_workspace.argtypes = [c_int, i64, i64, i64]
     lib.hcg_embedding_grad.argtypes = [c_int, vp, i64, i64, i64, c_int, vp, i64, i64, f32, c_int, vp, i64, vp, i64, vp]
     lib.hcg_layer_norm.argtypes = [c_int, vp, i64, i64, i64, c_int, vp, vp, f32, vp, i64, vp, vp, vp]
     lib.hcg_layer_norm_grad_workspace.argtypes = [i64, i64]

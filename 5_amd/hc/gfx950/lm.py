@@ -33,6 +33,27 @@ def _torch() -> Any:
     return torch
 
 
+_FAST: Any = None  # _hcg_torch once loaded; False where it is not built
+
+
+def _fast(name: str, *args: Any) -> Any:
+    """The compiled binding's result for contiguous tensors on the current
+    device (a call costs about 10 us less host time than below), or None: the
+    general path below takes the call, or says what is wrong with it."""
+    global _FAST
+    if _FAST is None:
+        _FAST = _PKG._fast_gemm() and sys.modules[__package__ + "._hcg_torch"]
+    if not _FAST:
+        return None
+    try:
+        result = getattr(_FAST, name)(*args)
+    except TypeError:  # an argument that is no tensor or number
+        return None
+    if type(result) is int:
+        _native.check(_native.lib(), result, "hcg_" + name)
+    return result
+
+
 def _name(dtype: Any) -> str:
     return str(dtype).replace("torch.", "")
 
@@ -140,6 +161,10 @@ def embedding(tokens: Any, table: Any, *, scale: float = 1.0, out: Any | None = 
     float16, bfloat16 or float32) that ``tokens`` (int32 or int64, any shape)
     name, of shape ``tokens.shape + (width,)``.  A token outside the
     vocabulary gives a row of NaN."""
+    if out is None:
+        r = _fast("embedding", tokens, table, scale)
+        if r is not None:
+            return r
     torch = _torch()
     index = _check_tensor(torch, table, "table")
     code = _code(table, "table", _ANY)
@@ -169,6 +194,10 @@ def embedding_grad(dy: Any, tokens: Any, vocab: int, *, scale: float = 1.0, padd
     tokens; zeros where there is none and in row ``padding_idx``.  ``dtype``:
     that of ``dy`` (the default) or float32.  Tokens outside the vocabulary
     reach no row."""
+    if padding_idx is None and dtype is None and out is None:
+        r = _fast("embedding_grad", dy, tokens, vocab, scale)
+        if r is not None:
+            return r
     torch = _torch()
     index = _check_tensor(torch, dy, "dy")
     code = _code(dy, "dy", _ANY)
@@ -194,7 +223,7 @@ def embedding_grad(dy: Any, tokens: Any, vocab: int, *, scale: float = 1.0, padd
         out, m = _out_rows(torch, out, (vocab, width), dtype, "out", index)
         ldg = _ld(m)
     lib = _native.lib()
-    need = lib.hcg_embedding_grad_workspace(n, vocab, width)
+    need = lib.hcg_embedding_grad_workspace(code, n, vocab, width)
     ws = _workspace(torch, need, dy.device)
     _call(torch, index, lib.hcg_embedding_grad, "hcg_embedding_grad", code, _ptr(rows), _ld(rows), n, width, size,
           _ptr(ids), vocab, -1 if padding_idx is None else padding_idx, scale, _CODES[dtype], _ptr(m), ldg, _ptr(ws),
@@ -229,6 +258,10 @@ def layer_norm(x: Any, weight: Any | None = None, bias: Any | None = None, *, ep
     bias`` of x's type and the rows' mean and ``rstd = 1 / sqrt(var + eps)``
     as float32, which :func:`layer_norm_grad` takes.  ``weight`` and ``bias``:
     vectors of x's type or float32, or None."""
+    if out is None:
+        r = _fast("layer_norm", x, weight, bias, eps)
+        if r is not None:
+            return r
     torch = _torch()
     index = _check_tensor(torch, x, "x")
     code = _code(x, "x", _ANY)
@@ -263,6 +296,10 @@ def layer_norm_grad(dy: Any, x: Any, mean: Any, rstd: Any, weight: Any | None = 
     ``dy`` (x's shape and type) and what the forward call returned.  dweight
     and dbias have the type of ``weight`` (x's without one), or
     ``param_dtype``: x's type or float32."""
+    if param_dtype is None:
+        r = _fast("layer_norm_grad", dy, x, mean, rstd, weight)
+        if r is not None:
+            return r
     torch = _torch()
     index = _check_tensor(torch, x, "x")
     code = _code(x, "x", _ANY)
@@ -333,6 +370,9 @@ def linear_cross_entropy(x: Any, weight: Any, targets: Any, *, ignore_index: int
     bfloat16; targets: int32 or int64.  Tokens whose target is
     ``ignore_index`` have loss and lse 0, whatever x holds there; other
     targets outside the vocabulary give NaN.  The logits are never written."""
+    r = _fast("linear_cross_entropy", x, weight, targets, ignore_index)
+    if r is not None:
+        return r
     torch = _torch()
     index, code, rows, w, ids, size = _head_args(torch, x, weight, targets)
     n, width = rows.shape
@@ -358,6 +398,11 @@ def linear_cross_entropy_grad(x: Any, weight: Any, targets: Any, *, ignore_index
     The probabilities are held for up to 1 GiB of tokens at a time, in the
     operands' type.  float16 gradients of a mean over many tokens reach the
     type's subnormals: scale them (``grad_scale``) as loss scaling does."""
+    if reduction in ("mean", "sum"):
+        r = _fast("linear_cross_entropy_grad", x, weight, targets, ignore_index, reduction == "mean",
+                  grad_scale)
+        if r is not None:
+            return r
     torch = _torch()
     if reduction not in ("mean", "sum"):
         raise LaunchError(f"unknown reduction {reduction!r}; expected 'mean' or 'sum'")

@@ -40,7 +40,7 @@ int hcg_embedding(int dtype, const void* table, int64_t ldt, int64_t vocab, int6
  * none; an id outside [0, vocab) reaches no row).  dy is n x width of dtype,
  * grad vocab x width of grad_dtype (dtype or HCG_F32).  The sum of a row is
  * float32 over ascending i, in fixed pieces where it is long. */
-int64_t hcg_embedding_grad_workspace(int64_t n, int64_t vocab, int64_t width);
+int64_t hcg_embedding_grad_workspace(int dtype, int64_t n, int64_t vocab, int64_t width);
 int hcg_embedding_grad(int dtype, const void* dy, int64_t ldy, int64_t n, int64_t width, int id_bytes,
                        const void* ids, int64_t vocab, int64_t padding_idx, float scale, int grad_dtype,
                        void* grad, int64_t ldg, void* workspace, int64_t workspace_bytes, void* stream);

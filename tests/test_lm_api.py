@@ -54,7 +54,7 @@ def test_embedding_arguments(change, match):
     ({"ws": P + 8}, "workspace")])
 def test_embedding_grad_arguments(change, match):
     lib = _native.load()
-    a = dict(dtype=BF16, dy=P, lddy=8, n=300, width=8, id_bytes=8, ids=P, vocab=5, padding=-1, scale=1.0,
+    a = dict(dtype=BF16, dy=P, lddy=8, n=3000, width=8, id_bytes=8, ids=P, vocab=5, padding=-1, scale=1.0,
              grad_dtype=BF16, grad=P, ldg=8, ws=P, ws_bytes=1 << 20, stream=None)
     a.update(change)
     _refused(lib.hcg_embedding_grad(*a.values()), match)
@@ -110,9 +110,12 @@ def test_linear_cross_entropy_grad_arguments(change, match):
 
 def test_workspace_sizes():
     lib = _native.load()
-    assert lib.hcg_embedding_grad_workspace(32, 1000, 64) == 0  # too few tokens for a long row
-    assert lib.hcg_embedding_grad_workspace(33, 1000, 64) > 0
-    assert lib.hcg_embedding_grad_workspace(0, 0, 0) == 0
+    assert lib.hcg_embedding_grad_workspace(BF16, 16, 1000, 1 << 20) == 0  # too few tokens for a long row
+    assert lib.hcg_embedding_grad_workspace(BF16, 17, 1000, 1 << 20) > 0
+    assert lib.hcg_embedding_grad_workspace(BF16, 2048, 1000, 2048) == 0  # one launch
+    assert lib.hcg_embedding_grad_workspace(F32, 2048, 1000, 2048) > 0
+    assert lib.hcg_embedding_grad_workspace(BF16, 2049, 1000, 64) > 0
+    assert lib.hcg_embedding_grad_workspace(BF16, 0, 0, 0) == 0
     assert lib.hcg_layer_norm_grad_workspace(0, 64) == 0
     size = lib.hcg_linear_cross_entropy_workspace
     assert size(0, 100, 64, P, 64, 1) == 0
