@@ -24,6 +24,7 @@
 #include <type_traits>
 
 #include "hcg_lm.h"
+#include "hcg_splitsum.h"
 #include "hcg_tile.h"
 
 namespace hcg {
@@ -45,8 +46,14 @@ enum Epilogue {
   kExp,      // and exp(logit - block maximum) as f16
   kRound,    // scaled, rounded to DT, as rows of the output
   kPartial,  // float32, into scratch
-  kSplit,    // kRound, or with K split kPartial
+  kSplit,    // kRound, where K is split of the parts' sum (can_fuse) or kPartial
 };
+
+// Tiles whose K splits the tile's last workgroup sums itself (hcg_splitsum.h);
+// larger ones are added up by a launch of their own (dx of 256 x 4096 x 512 in
+// 128x128 tiles and 8 parts: 16.0 us by the last workgroup, 12.6 by a launch; in
+// 128x32 tiles of 128 x 6000 x 700 11.2 by the last one).
+constexpr bool can_fuse(int tm, int tn) { return tm * tn <= 128 * 32; }
 
 struct Args {
   const uint16_t* A;  // M side
@@ -60,6 +67,8 @@ struct Args {
   // kSplit: K is split while there are fewer tiles (of live tokens) than units,
   // into at most max_splits parts.
   int units, max_splits;
+  unsigned* counters;  // can_fuse: one per tile, kSplitCounterStride apart, all zero
+  int part_bytes;
   // kRound: row n of the output is out + (row_of ? row_of[n] : n) * ldo;
   // kPartial: part + (split * N + n) * ld_part.
   void* out;
@@ -70,12 +79,18 @@ struct Args {
   const float* add;    // [N][M] floats added to the sums, or null
   const float* scale;  // kRound: the factor *scale * post
   float post;
-  // kStats, kExp: per token n and block of TM / WM vocabulary rows its maximum
-  // and the sum of exp(logit - maximum), and the target's logit.
+  // kStats, kExp: per token n and block of TM / WM vocabulary rows its largest
+  // logit times log2 e, c, and the sum of 2^(logit * log2 e - c), and the
+  // target's logit.
   f32x2* stats;
   int64_t ld_stats;
   const int* target;
   float* hit;
+  // kRound, where loss_out is not null: one workgroup more, which adds up the
+  // losses of the live tokens.
+  const float* loss;
+  const float* loss_scale;
+  float* loss_out;
 };
 
 template <int DT>
@@ -151,13 +166,14 @@ struct Operand {
   static constexpr int kChunks = kRowBytes / 16;
   static constexpr int kRowsPerInst = 64 / kChunks;
   static_assert(kInst >= 1 && kInst * NW * 1024 == kBytes, "a stage is whole DMA instructions of every wave");
-  static_assert(KC || T >= 128, "swizzle");
+  static_assert(KC || T >= 64, "swizzle");
 
   static __device__ __forceinline__ int swz(int row, int c) {
     if constexpr (KC) {
       return c ^ ((row >> 1) & 7);
     } else {
       const int m = row & 3;
+      if constexpr (T == 64) return c ^ ((m >> 1) * 4);
       return c ^ ((m >> 1) * 10 + (m & 1) * 4);
     }
   }
@@ -295,7 +311,7 @@ struct RowStage {
 // read at one offset, and the reads pile onto a few HBM channels: logits of 16 x
 // 65536 x 4096 bf16 110 us, rotated 90 (5.96 TB/s).
 template <int DT, int TM, int TN, int WM, int WN, int UNITS, bool AKC, bool BKC, int EPI, bool COUNT_K, bool ROTATE>
-__global__ __launch_bounds__(64 * WM * WN, 1) void head_kernel(Args g) {
+__device__ __forceinline__ void head_tile(Args g, int wg) {
   constexpr int NW = WM * WN;
   constexpr int MI = TM / WM / 32, NI = TN / WN / 32;
   static_assert(MI >= 1 && NI >= 1 && MI * WM * 32 == TM && NI * WN * 32 == TN, "wave tile");
@@ -322,9 +338,9 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void head_kernel(Args g) {
   const int K_all = COUNT_K ? live : g.K;
   int chunk = K_all, splits = 1;
   if constexpr (EPI == kSplit) splits = splits_of(g.units, g.max_splits, g.tiles_m * tiles_n, K_all, &chunk);
-  if ((int)blockIdx.x >= g.tiles_m * tiles_n * splits) return;
+  if (wg >= g.tiles_m * tiles_n * splits) return;
   int split, tm, tn;
-  unit_of(g.tiles_m, tiles_n, splits, blockIdx.x, split, tm, tn);
+  unit_of(g.tiles_m, tiles_n, splits, wg, split, tm, tn);
   const int m0 = tm * TM, n0 = tn * TN;
   const int kbeg = split * chunk;
   const int K = min(K_all - kbeg, chunk);
@@ -478,7 +494,8 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void head_kernel(Args g) {
   read(Int<0>{}, 0);
 
   int kt = 0;
-  const int nfull = ROTATE ? 0 : K / kStep;  // (a rotated walk may pass the partial stage anywhere)
+  // (A rotated walk passes a partial stage somewhere inside.)
+  const int nfull = ROTATE && K % kStep ? 0 : K / kStep;
   for (; kt + kPeriod + UNITS / 2 <= nfull; kt += kPeriod) {
     iteration(Int<0>{}, Full{});
     iteration(Int<1>{}, Full{});
@@ -517,6 +534,25 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void head_kernel(Args g) {
                                                               : place(Int<4 % UNITS>{})) +
                                   wave % kWavesPerUnit * Stage::kBytes;
 
+  if constexpr (EPI == kSplit && can_fuse(TM, TN)) {
+    if (splits > 1) {
+      constexpr int P = MI * NI * 4;
+      split_f32x4 v[P];
+#pragma unroll
+      for (int p = 0; p < P; ++p)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[p][e] = acc[p / 4 / NI][p / 4 % NI][p % 4 * 4 + e];
+      if (!sum_splits<P, 64 * NW>(v, make_rsrc(g.part, g.part_bytes), g.tiles_m * tiles_n, tm * tiles_n + tn, splits,
+                                  split, g.counters, reinterpret_cast<unsigned*>(place(Int<1>{}))))
+        return;
+#pragma unroll
+      for (int p = 0; p < P; ++p)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[p / 4 / NI][p / 4 % NI][p % 4 * 4 + e] = v[p][e];
+      splits = 1;
+    }
+  }
+
   // Accumulator block (mi, ni) of a lane: row n of the output, columns
   // m = mfirst + 32 mi + 8 (r / 4) + 4 (lane / 32) + r % 4.
   const int half = lane >> 5;
@@ -548,20 +584,23 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void head_kernel(Args g) {
             if (at == mi * 32 + 8 * (r / 4) + 4 * half + r % 4) v = acc[mi][ni][r];
         if (live_n && at >= 0 && at < kBlock && ((at >> 2) & 1) == half) g.hit[n] = v;
       }
+      // In powers of two: exp(l) = 2^(l log2 e), relative to the block's largest
+      // exponent c, whose float32 value is the reference itself, so that one
+      // fused multiply-add per logit loses nothing.
       float top = -__builtin_inff();
 #pragma unroll
       for (int mi = 0; mi < MI; ++mi)
 #pragma unroll
         for (int r = 0; r < 16; ++r) top = fmaxf(top, acc[mi][ni][r]);
-      top = fmaxf(top, __shfl_xor(top, 32));
-      // (a block without a finite maximum: exp(-inf - 0) = 0)
+      top = fmaxf(top, __shfl_xor(top, 32)) * kLog2e;
+      // (a block without a finite maximum: 2^(-inf - 0) = 0)
       const float ref = top == -__builtin_inff() ? 0.f : top;
       float sum = 0.f;
 #pragma unroll
       for (int mi = 0; mi < MI; ++mi)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const float e = __builtin_amdgcn_exp2f((acc[mi][ni][r] - ref) * kLog2e);
+          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[mi][ni][r], kLog2e, -ref));
           acc[mi][ni][r] = e;
           sum += e;
         }
@@ -620,6 +659,31 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void head_kernel(Args g) {
       }
     }
   }
+}
+
+// The sum of the losses over the live tokens by one wave, in one order, into
+// *out (times *scale).  It runs beside the tiles of a product.
+__device__ __forceinline__ void sum_losses(const float* loss, int n, const float* scale, float* out) {
+  float sum = 0.f;
+#pragma unroll 16
+  for (int i = threadIdx.x; i < n; i += 64) sum += loss[i];
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) sum += __shfl_xor(sum, m);
+  if (threadIdx.x == 0) *out = sum * *scale;
+}
+
+// Waves per SIMD: two workgroups per CU where the ring takes at most half its LDS.
+constexpr int waves_per_simd(int tm, int tn, int waves, int units) {
+  return waves / 4 * ((tm + tn) * kStep * 2 * units / 2 <= 80 * 1024 ? 2 : 1);
+}
+
+template <int DT, int TM, int TN, int WM, int WN, int UNITS, bool AKC, bool BKC, int EPI, bool COUNT_K, bool ROTATE>
+__global__ __launch_bounds__(64 * WM * WN, waves_per_simd(TM, TN, WM * WN, UNITS)) void head_kernel(Args g) {
+  if (EPI == kRound && g.loss_out && blockIdx.x + 1 == gridDim.x) {
+    if (threadIdx.x < 64) sum_losses(g.loss, *g.count, g.loss_scale, g.loss_out);
+    return;
+  }
+  head_tile<DT, TM, TN, WM, WN, UNITS, AKC, BKC, EPI, COUNT_K, ROTATE>(g, blockIdx.x);
 }
 
 }  // namespace head

@@ -59,6 +59,8 @@ struct PackArgs {
   int width, vecs;
   uint16_t* dx;  // or null
   int64_t lddx;
+  unsigned* counters;  // cleared for the dx product
+  int num_counters;
 };
 
 constexpr int kPackThreads = 256;
@@ -74,6 +76,8 @@ __global__ __launch_bounds__(kPackThreads) void pack_kernel(PackArgs g) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int from = blockIdx.x * g.per_wg, n = min(g.per_wg, g.tokens - from);
   const I* targets = static_cast<const I*>(g.targets);
+  for (int i = blockIdx.x * kPackThreads + tid; i < g.num_counters; i += gridDim.x * kPackThreads)
+    g.counters[i * hcg::kSplitCounterStride] = 0;
   int before = 0;
   for (int t0 = tid; t0 < from; t0 += kPackThreads * 8) {
 #pragma unroll
@@ -189,7 +193,7 @@ struct SoftmaxArgs {
 // (GRAD) the probabilities in place of the exponentials.
 template <int DT, bool GRAD>
 __global__ __launch_bounds__(256) void softmax_kernel(SoftmaxArgs g) {
-  constexpr float kLog2e = 1.44269504088896341f;
+  constexpr double kLn2 = 0.693147180559945309;
   __shared__ float slots[2][4];
   const int n = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   if (n >= *g.count - g.count0) return;
@@ -205,13 +209,14 @@ __global__ __launch_bounds__(256) void softmax_kernel(SoftmaxArgs g) {
   for (int j = tid; j < g.blocks; j += 256) {
     const f32x2 s = stats[j];
     // (a block of -inf alone has sum 0, a NaN sum stays)
-    sum += s.y * __builtin_amdgcn_exp2f((s.x == -__builtin_inff() ? -1e30f : s.x - ref) * kLog2e);
+    sum += s.y * __builtin_amdgcn_exp2f(s.x == -__builtin_inff() ? -1e30f : s.x - ref);
   }
   sum = hcg::wave_sum(sum);
   if (lane == 0) slots[1][wave] = sum;
   __syncthreads();
   sum = (slots[1][0] + slots[1][1]) + (slots[1][2] + slots[1][3]);
-  const float lse = ref + logf(sum);
+  // (in doubles: one rounding of a value that may be some hundreds)
+  const float lse = (float)(((double)ref + (double)log2f(sum)) * kLn2);
   const int target = g.target[n];
   if (tid == 0) {
     const int64_t to = g.token ? g.token[n] : n;
@@ -224,29 +229,13 @@ __global__ __launch_bounds__(256) void softmax_kernel(SoftmaxArgs g) {
     const float rest = scale / sum;
     for (int c = tid * 8; c < g.vocab; c += 256 * 8) {
       const float m = stats[c / g.block].x;
-      const float f = rest * __builtin_amdgcn_exp2f((m == -__builtin_inff() ? -1e30f : m - ref) * kLog2e);
+      const float f = rest * __builtin_amdgcn_exp2f(m == -__builtin_inff() ? -1e30f : m - ref);
       float v[8];
       hcg::unpack<_Float16>(*reinterpret_cast<const raw4*>(row + c), v);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = v[e] * f - (c + e == target ? scale : 0.f);
       *reinterpret_cast<raw4*>(row + c) = hcg::pack<typename ElemOf<DT>::type>(v);
     }
-  }
-}
-
-// The loss over all places, in one order.
-__global__ __launch_bounds__(1024) void loss_sum_kernel(const float* loss, const int* count, const float* scale,
-                                                        float* out) {
-  __shared__ float waves[16];
-  float sum = 0.f;
-  for (int n = threadIdx.x; n < *count; n += 1024) sum += loss[n];
-  sum = hcg::wave_sum(sum);
-  if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = sum;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    sum = 0.f;
-    for (int w = 0; w < 16; ++w) sum += waves[w];
-    *out = sum * scale[1];
   }
 }
 
@@ -308,14 +297,17 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // medium in 2 208; of 256 x 4096 x 512 large in 16 parts 18, medium in 8 9; of
 // 64 x 32768 x 4096 medium in 8 parts 43, few in 8 49; logits of 32 x 50000 x
 // 1024 medium 22, few 17; of 1024 x 32768 x 2048 large 117, medium 167.
-enum Shape { kLarge, kMedium, kFew };
+enum Shape { kLarge, kMedium, kSmall, kFew };
 struct ShapeInfo {
   int tm, tn, wm, per_cu;
   double fixed, lo, hi;
 };
 constexpr ShapeInfo kShapes[] = {
-    {256, 256, 2, 1, 12.0, 0.95, 1.55}, {128, 128, 2, 1, 5.0, 0.31, 0.52}, {128, 32, 4, 2, 4.0, 0.33, 0.66}};
-constexpr int kNumShapes = 3;
+    {256, 256, 2, 1, 12.0, 0.95, 1.55},
+    {128, 128, 2, 1, 4.0, 0.31, 0.52},
+    {128, 64, 4, 2, 3.5, 0.25, 0.50},   // (not dx: its split sums want more registers than two per CU leave)
+    {128, 32, 4, 2, 3.5, 0.22, 0.60}};  // (not dw: its rows of vocabulary are read 64 at a time)
+constexpr int kNumShapes = 4;
 constexpr int kCus = 256;
 constexpr int kMaxSplits = 32;
 constexpr int kMinKPerSplit = 256;
@@ -328,26 +320,35 @@ double cost_of(Shape s, int64_t m, int64_t n, int64_t k, int splits) {
   const double busy = units < room ? (double)units / room : 1.0;
   const double stages = (double)ceil_div(ceil_div(k, splits), head::kStep);
   double us = (double)ceil_div(units, room) * (t.fixed + stages * (t.lo + (t.hi - t.lo) * busy));
-  if (splits > 1) us += 4.0 + 2.0 * splits * m * n * 4 / 6.0e6;  // the parts written and read, and a launch
+  if (splits > 1) {
+    // The parts written and read, and a launch, or their reading by one CU.
+    us += 2.0 * splits * m * n * 4 / 6.0e6;
+    us += head::can_fuse(t.tm, t.tn) ? 1.0 + (splits - 1) * std::max(0.234, t.tm * t.tn * 4 / 1.0e5) : 4.0;
+  }
   return us;
 }
 
-// The shape with the least modelled time; few: the 32-token tiles may be taken
-// (their N is K-contiguous); *units: workgroups to split K up to, or null.
-Shape pick_shape(int64_t m, int64_t n, int64_t k, bool few, int* units) {
+int max_splits_of(Shape s, int64_t k) {
+  const int64_t most = head::can_fuse(kShapes[s].tm, kShapes[s].tn) ? hcg::kMaxSummedSplits : kMaxSplits;
+  return (int)std::max<int64_t>(1, std::min(most, k / kMinKPerSplit));
+}
+
+// The shape with the least modelled time; *units: workgroups to split K up to, or null.
+enum Product { kLogits, kDx, kDw };
+Shape pick_shape(Product product, int64_t m, int64_t n, int64_t k, int* units) {
   Shape best = kLarge;
   double best_cost = -1;
   for (int i = 0; i < kNumShapes; ++i) {
     const Shape s = (Shape)i;
-    if (s == kFew && !few) continue;
-    for (int splits = 1; splits <= kMaxSplits; ++splits) {
-      if (splits > 1 && (!units || k / splits < kMinKPerSplit)) break;
+    if (product == kDx ? s == kSmall : product == kDw && s == kFew) continue;
+    for (int splits = 1; splits <= max_splits_of(s, k); ++splits) {
+      if (splits > 1 && !units) break;
       const double cost = cost_of(s, m, n, k, splits);
       if (best_cost >= 0 && cost >= best_cost) continue;
       best_cost = cost;
       best = s;
       // (fewer tokens that count leave fewer tiles and more splits)
-      if (units) *units = (int)std::max<int64_t>(kCus * kShapes[s].per_cu, std::min<int64_t>(tiles(s, m, n) * splits, 1 << 20));
+      if (units) *units = (int)(splits > 1 ? tiles(s, m, n) * splits : (int64_t)kCus * kShapes[s].per_cu);
     }
   }
   return best;
@@ -361,9 +362,11 @@ struct Plan {
   int pieces;
   Shape logits, dx, dw;
   int units, max_splits;  // of dx
+  int counters;           // its tiles, where their last workgroup sums the splits
   int64_t blocks;      // statistics per token
   // Offsets into the workspace.
-  int64_t token, target, count, scale, rows, weight, stats, hit, loss, exps, part, sums, total;
+  int64_t token, target, count, scale, rows, weight, stats, hit, loss, exps, part, counter, sums, total;
+  int64_t part_bytes;
 };
 
 Plan make_plan(int64_t tokens, int64_t vocab, int64_t width, bool copy_weight, bool grad) {
@@ -378,12 +381,13 @@ Plan make_plan(int64_t tokens, int64_t vocab, int64_t width, bool copy_weight, b
   p.piece = tokens;
   if (grad) p.piece = std::min(tokens, std::max<int64_t>(256, kPieceBytes / (p.lde * 2) / 256 * 256));
   p.pieces = (int)ceil_div(tokens, p.piece);
-  p.logits = pick_shape(vocab, p.piece, width, true, nullptr);
+  p.logits = pick_shape(kLogits, vocab, p.piece, width, nullptr);
   p.blocks = ceil_div(vocab, kShapes[p.logits].tm) * kShapes[p.logits].wm;
   if (grad) {
-    p.dx = pick_shape(width, p.piece, vocab, true, &p.units);
-    p.dw = pick_shape(width, vocab, p.piece, false, nullptr);
-    p.max_splits = (int)std::max<int64_t>(1, std::min<int64_t>(kMaxSplits, vocab / kMinKPerSplit));
+    p.dx = pick_shape(kDx, width, p.piece, vocab, &p.units);
+    p.dw = pick_shape(kDw, width, vocab, p.piece, nullptr);
+    p.max_splits = max_splits_of(p.dx, vocab);
+    if (head::can_fuse(kShapes[p.dx].tm, kShapes[p.dx].tn) && p.max_splits > 1) p.counters = (int)std::min<int64_t>(p.units, tiles(p.dx, width, p.piece));
   }
   int64_t at = 0;
   const auto take = [&](int64_t bytes) {
@@ -404,9 +408,12 @@ Plan make_plan(int64_t tokens, int64_t vocab, int64_t width, bool copy_weight, b
     p.exps = take(p.piece * p.lde * 2);
     // K is split while the parts' tiles are at most `units`: no more rows than
     // those tiles have (nor than max_splits times the tokens).
+    // (Where a tile's last workgroup sums, the parts are whole tiles.)
     const ShapeInfo& t = kShapes[p.dx];
     const int64_t rows = std::min(p.units / ceil_div(width, t.tm) * t.tn, p.max_splits * p.piece);
-    p.part = take(p.max_splits > 1 ? rows * p.ldx * 4 : 0);
+    p.part_bytes = p.max_splits == 1 ? 0 : p.counters ? (int64_t)p.units * t.tm * t.tn * 4 : rows * p.ldx * 4;
+    p.part = take(p.part_bytes);
+    p.counter = take((int64_t)p.counters * hcg::kSplitCounterStride * 4);
     p.sums = take(p.pieces > 1 ? vocab * width * 4 : 0);
   }
   p.total = at;
@@ -430,11 +437,15 @@ void launch_head(Shape shape, const head::Args& a, int64_t wgs, hipStream_t s) {
     head::head_kernel<DT, 256, 256, 2, kSoftmax ? 4 : 2, 5, AKC, BKC, EPI, COUNT_K, false>
         <<<grid, kSoftmax ? 512 : 256, 0, s>>>(a);
   } else if (shape == kMedium) {
-    // (one tile of tokens: bound by reading the weights)
-    if (kSoftmax && a.N <= 128)
-      head::head_kernel<DT, 128, 128, 2, 4, 8, AKC, BKC, EPI, COUNT_K, kSoftmax><<<grid, 512, 0, s>>>(a);
-    else
-      head::head_kernel<DT, 128, 128, 2, 4, 8, AKC, BKC, EPI, COUNT_K, false><<<grid, 512, 0, s>>>(a);
+    head::head_kernel<DT, 128, 128, 2, 4, 8, AKC, BKC, EPI, COUNT_K, false><<<grid, 512, 0, s>>>(a);
+  } else if (shape == kSmall) {
+    if constexpr (EPI != head::kSplit) {
+      // (one tile of tokens: bound by reading the weights)
+      if (kSoftmax && a.N <= 64)
+        head::head_kernel<DT, 128, 64, 4, 2, 6, AKC, BKC, EPI, COUNT_K, kSoftmax><<<grid, 512, 0, s>>>(a);
+      else
+        head::head_kernel<DT, 128, 64, 4, 2, 6, AKC, BKC, EPI, COUNT_K, false><<<grid, 512, 0, s>>>(a);
+    }
   } else if constexpr (BKC) {
     head::head_kernel<DT, 128, 32, 4, 1, 6, AKC, BKC, EPI, COUNT_K, kSoftmax><<<grid, 256, 0, s>>>(a);
   }
@@ -491,7 +502,9 @@ int run_loss(const Plan& p, const Call& c, hipStream_t s) {
                     D,
                     (int)(p.ldx / 8),
                     static_cast<uint16_t*>(c.dx),
-                    c.lddx};
+                    c.lddx,
+                    static_cast<unsigned*>(at(p.counter)),
+                    p.counters};
   const dim3 runs((unsigned)ceil_div(T, per_wg));
   if (c.id_bytes == 8)
     pack_kernel<int64_t><<<runs, kPackThreads, 0, s>>>(pk);
@@ -567,9 +580,12 @@ int run_loss(const Plan& p, const Call& c, hipStream_t s) {
     d.row_of = token + t0;
     d.part = static_cast<float*>(at(p.part));
     d.ld_part = p.ldx;
+    d.counters = static_cast<unsigned*>(at(p.counter));
+    d.part_bytes = (int)p.part_bytes;
     // (as many workgroups as any number of live tokens takes)
-    launch_head<DT, head::kSplit, false, true, false>(p.dx, d, std::max<int64_t>(tiles(p.dx, D, n), p.units), s);
-    if (p.max_splits > 1) {
+    const int64_t dx_wgs = std::max<int64_t>(tiles(p.dx, D, n), p.max_splits > 1 ? p.units : 0);
+    launch_head<DT, head::kSplit, false, true, false>(p.dx, d, dx_wgs, s);
+    if (p.max_splits > 1 && !p.counters) {
       const JoinArgs j{d.part,    p.ldx, d.units,    d.max_splits, d.tiles_m, kShapes[p.dx].tn,
                        n,         V,     D,          (int)(p.ldx / 8), count, (int)t0,
                        token + t0, scale, post,      static_cast<uint16_t*>(c.dx), c.lddx};
@@ -595,15 +611,16 @@ int run_loss(const Plan& p, const Call& c, hipStream_t s) {
     if (i + 1 == p.pieces) {
       w.out = c.dw;
       w.ldo = c.lddw;
-      launch_head<DT, head::kRound, false, false, true>(p.dw, w, dw_wgs, s);
+      w.loss = static_cast<const float*>(at(p.loss));
+      w.loss_scale = scale + 1;
+      w.loss_out = c.loss;
+      launch_head<DT, head::kRound, false, false, true>(p.dw, w, dw_wgs + 1, s);
     } else {
       w.part = sums;
       w.ld_part = D;
       launch_head<DT, head::kPartial, false, false, true>(p.dw, w, dw_wgs, s);
     }
   }
-  if (p.grad)
-    loss_sum_kernel<<<1, 1024, 0, s>>>(static_cast<const float*>(at(p.loss)), count, scale, c.loss);
   HCG_LM_HIP_CHECK(hipGetLastError());
   return HCG_OK;
 }
