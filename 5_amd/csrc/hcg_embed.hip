@@ -90,7 +90,7 @@ __global__ __launch_bounds__(256) void embed_kernel(EmbedArgs g) {
 
 constexpr int kGradThreads = 512;
 constexpr int kGradWaves = kGradThreads / 64;
-constexpr int kScan = 8;           // ids in flight per lane
+constexpr int kScan = 4;           // pairs of ids in flight per lane
 constexpr int kMaxRows = 64;       // table rows per workgroup
 constexpr int kListPerWave = 256;  // ids of a workgroup's rows kept in LDS, per wave that scans
 // Rows of dy in flight per thread.  (16 take registers that leave two workgroups
@@ -106,6 +106,14 @@ constexpr int kRuns = kWindow / (kLong + 1) + 2;
 // workgroup sums its long rows too, in parts that meet in LDS: then one launch
 // does it all.
 constexpr int kOneLaunch = 2048;
+// Past so many tokens they are first parted by ranges of the table (a launch of
+// kBuckets workgroups, stable), and a workgroup scans its range's tokens only:
+// 4096 workgroups that scan them all read 1 GB from the L2s at 32768 tokens.
+// us, all scanned / parted: 32768 into 108888 x 512 f16 86 / 70, 65536 into 32768
+// x 1024 bf16 185 / 140, 8192 into 65536 x 4096 150 / 149, 5000 into 5000 x 512
+// f32 26.2 / 27.1.
+constexpr int kBucketTokens = 8192;
+constexpr int kBuckets = 64;
 
 struct EmbedGradArgs {
   const void* dy;
@@ -124,6 +132,12 @@ struct EmbedGradArgs {
   int* found;     // tokens of a workgroup's rows in the order of i, where LDS is too small ...
   uint16_t* found_row;  // ... and which of its rows
   float* part;    // [windows][kRuns][width]
+  // Parted tokens, or null: their rows and indexes by bucket of bucket_rows
+  // table rows, and each bucket's first place and number of tokens.
+  int* bucket_id;
+  int* bucket_token;
+  int* bucket;  // [kBuckets][2]
+  int bucket_rows;
 };
 
 __device__ __forceinline__ int lanes_below(uint64_t mask) {
@@ -193,8 +207,108 @@ __device__ __forceinline__ void sum_rows(float (&sum)[kVec<T>], const T* dy, int
   }
 }
 
+// The ids [from, to) by one wave, two neighbours per lane: f(i, a, b) with the
+// ids of i and i + 1, -1 past the end and for the padding row; kScan loads in
+// flight.
+template <class I, class F>
+__device__ __forceinline__ void scan_ids(const I* ids, int from, int to, int64_t padding, F f) {
+  typedef I pair __attribute__((ext_vector_type(2), aligned(sizeof(I))));
+  const int lane = threadIdx.x & 63;
+  for (int i0 = from; i0 < to; i0 += 128 * kScan) {
+    int64_t a[kScan], b[kScan];
+#pragma unroll
+    for (int u = 0; u < kScan; ++u) {
+      const int i = i0 + u * 128 + lane * 2;
+      a[u] = b[u] = -1;
+      if (i + 1 < to) {
+        const pair v = *reinterpret_cast<const pair*>(ids + i);
+        a[u] = (int64_t)v.x;
+        b[u] = (int64_t)v.y;
+      } else if (i < to) {
+        a[u] = (int64_t)ids[i];
+      }
+      if (a[u] == padding) a[u] = -1;
+      if (b[u] == padding) b[u] = -1;
+    }
+#pragma unroll
+    for (int u = 0; u < kScan; ++u)
+      if (i0 + u * 128 < to) f(i0 + u * 128 + lane * 2, a[u], b[u]);
+  }
+}
+
+// Over scan_ids: counts the ids below `lo` into *below and those in [lo, hi)
+// into *finds, which it hands over in order: keep(number, i, id).
+template <class I, class F>
+__device__ __forceinline__ void find_ids(const I* ids, int from, int to, int64_t padding, int64_t lo, int64_t hi,
+                                         int* finds, int* below, F keep) {
+  const int lane = threadIdx.x & 63;
+  int found = 0, under = 0;
+  scan_ids<I>(ids, from, to, padding, [&](int i, int64_t a, int64_t b) {
+    under += __popcll(__ballot(a >= 0 && a < lo)) + __popcll(__ballot(b >= 0 && b < lo));
+    const uint64_t hit_a = __ballot(a >= lo && a < hi), hit_b = __ballot(b >= lo && b < hi);
+    if (hit_a | hit_b) {
+      const int at = found + lanes_below(hit_a) + lanes_below(hit_b);
+      const bool mine_a = hit_a >> lane & 1;
+      if (mine_a) keep(at, i, a);
+      if (hit_b >> lane & 1) keep(at + mine_a, i + 1, b);
+      found += __popcll(hit_a) + __popcll(hit_b);
+    }
+  });
+  *finds = found;
+  *below = under;
+}
+
+// Parts the tokens: workgroup b takes those of its bucket_rows rows of the
+// table, in order, to the places after all of lower rows.  The finds wait in
+// LDS until their place is known; where they do not fit (a hot row) the ids are
+// scanned again, from the L2.
+constexpr int kPartThreads = 1024;
+constexpr int kPartWaves = kPartThreads / 64;
+constexpr int kPartList = 512;  // finds per wave
+template <class I>
+__global__ __launch_bounds__(kPartThreads) void embed_bucket_kernel(EmbedGradArgs g) {
+  __shared__ int wave_found[kPartWaves], wave_below[kPartWaves];
+  __shared__ int list_id[kPartWaves * kPartList], list_token[kPartWaves * kPartList];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t lo = (int64_t)blockIdx.x * g.bucket_rows, hi = min(lo + g.bucket_rows, g.vocab);
+  const I* ids = static_cast<const I*>(g.ids);
+  const int quota = (g.n + kPartWaves * 128 - 1) / (kPartWaves * 128) * 128;
+  const int from = min(wave * quota, g.n), to = min(from + quota, g.n);
+  int finds, below;
+  find_ids<I>(ids, from, to, g.padding, lo, hi, &finds, &below, [&](int at, int i, int64_t id) {
+    if (at < kPartList) {
+      list_id[wave * kPartList + at] = (int)id;
+      list_token[wave * kPartList + at] = i;
+    }
+  });
+  if (lane == 0) wave_found[wave] = finds, wave_below[wave] = below;
+  __syncthreads();
+  int total = 0, first = 0, base = 0;
+#pragma unroll
+  for (int w = 0; w < kPartWaves; ++w) {
+    if (w < wave) first += wave_found[w];
+    total += wave_found[w];
+    base += wave_below[w];
+  }
+  if (threadIdx.x == 0) g.bucket[2 * blockIdx.x] = base, g.bucket[2 * blockIdx.x + 1] = total;
+  first += base;
+  if (finds <= kPartList) {  // (this wave's own finds)
+    for (int j = lane; j < finds; j += 64) {
+      g.bucket_id[first + j] = list_id[wave * kPartList + j];
+      g.bucket_token[first + j] = list_token[wave * kPartList + j];
+    }
+  } else {
+    find_ids<I>(ids, from, to, g.padding, lo, hi, &finds, &below, [&](int at, int i, int64_t id) {
+      g.bucket_id[first + at] = (int)id;
+      g.bucket_token[first + at] = i;
+    });
+  }
+}
+
 // ONE: no lists are kept (g.token is null), the workgroup sums its long rows too.
-template <class T, class G, class I, bool ONE>
+// PARTED: the tokens come from the workgroup's bucket (I is int).
+template <class T, class G, class I, bool ONE, bool PARTED>
 __global__ __launch_bounds__(kGradThreads, 8) void embed_grad_kernel(EmbedGradArgs g) {
   constexpr int E = kVec<T>;
   __shared__ float meet[ONE ? kGradThreads * E : 1];
@@ -206,35 +320,21 @@ __global__ __launch_bounds__(kGradThreads, 8) void embed_grad_kernel(EmbedGradAr
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t lo = (int64_t)blockIdx.x * g.rows;
   const int rows = (int)min((int64_t)g.rows, g.vocab - lo);
-  const I* ids = static_cast<const I*>(g.ids);
+  const int bucket = PARTED ? (int)(lo / g.bucket_rows) : 0;
+  const int base = PARTED ? g.bucket[2 * bucket] : 0, tokens = PARTED ? g.bucket[2 * bucket + 1] : g.n;
+  const I* ids = PARTED ? reinterpret_cast<const I*>(g.bucket_id + base) : static_cast<const I*>(g.ids);
   for (int r = tid; r < kMaxRows; r += kGradThreads) count[r] = 0;
 
   // Wave w scans the tokens [w * quota, (w + 1) * quota): its finds and, for
   // the place of this workgroup's tokens in the lists, how many name a row
   // before the first of these.  `keep` takes the find at its place.
-  const int quota = (g.n + kGradWaves * 64 - 1) / (kGradWaves * 64) * 64;
-  const int from = min(wave * quota, g.n), to = min(from + quota, g.n);
+  const int quota = (tokens + kGradWaves * 128 - 1) / (kGradWaves * 128) * 128;
+  const int from = min(wave * quota, tokens), to = min(from + quota, tokens);
   auto scan = [&](auto keep) {
-    int finds = 0, below = 0;
-    for (int i0 = from; i0 < to; i0 += 64 * kScan) {
-      int64_t id[kScan];
-#pragma unroll
-      for (int u = 0; u < kScan; ++u) {
-        const int i = i0 + u * 64 + lane;
-        id[u] = i < to ? (int64_t)ids[i] : -1;
-        if (id[u] == g.padding) id[u] = -1;
-      }
-#pragma unroll
-      for (int u = 0; u < kScan; ++u) {
-        const int64_t r = id[u] - lo;
-        below += __popcll(__ballot(id[u] >= 0 && r < 0));
-        const uint64_t hit = __ballot(r >= 0 && r < rows);
-        if (hit) {
-          if (hit >> lane & 1) keep(finds + lanes_below(hit), i0 + u * 64 + lane, (int)r);
-          finds += __popcll(hit);
-        }
-      }
-    }
+    int finds, below;
+    find_ids<I>(ids, from, to, g.padding, lo, lo + rows, &finds, &below, [&](int at, int i, int64_t id) {
+      keep(at, PARTED ? g.bucket_token[base + i] : i, (int)(id - lo));
+    });
     if (lane == 0) wave_found[wave] = finds, wave_below[wave] = below;
   };
   scan([&](int at, int i, int r) {
@@ -244,7 +344,7 @@ __global__ __launch_bounds__(kGradThreads, 8) void embed_grad_kernel(EmbedGradAr
     }
   });
   __syncthreads();
-  int total = 0, before = 0, below = 0;
+  int total = 0, before = 0, below = base;
   bool fits = true;
 #pragma unroll
   for (int w = 0; w < kGradWaves; ++w) {
@@ -486,10 +586,16 @@ template <class T, class G, class I>
 void run_embed_grad(const EmbedGradArgs& a, hipStream_t s) {
   const dim3 grid((unsigned)((a.vocab + a.rows - 1) / a.rows));
   if (a.token == nullptr) {
-    embed_grad_kernel<T, G, I, true><<<grid, kGradThreads, 0, s>>>(a);
+    embed_grad_kernel<T, G, I, true, false><<<grid, kGradThreads, 0, s>>>(a);
     return;
   }
-  embed_grad_kernel<T, G, I, false><<<grid, kGradThreads, 0, s>>>(a);
+  if (a.bucket) {
+    const dim3 buckets((unsigned)((a.vocab + a.bucket_rows - 1) / a.bucket_rows));
+    embed_bucket_kernel<I><<<buckets, kPartThreads, 0, s>>>(a);
+    embed_grad_kernel<T, G, int32_t, false, true><<<grid, kGradThreads, 0, s>>>(a);
+  } else {
+    embed_grad_kernel<T, G, I, false, false><<<grid, kGradThreads, 0, s>>>(a);
+  }
   const unsigned windows = (unsigned)windows_of(a.n);
   embed_window_kernel<T><<<dim3(windows, (unsigned)((a.items + 255) / 256)), 256, 0, s>>>(a);
   embed_long_kernel<G><<<dim3(windows, (unsigned)((a.width + 255) / 256)), 256, 0, s>>>(a);
@@ -531,7 +637,8 @@ int hcg_embedding(int dtype, const void* table, int64_t ldt, int64_t vocab, int6
 
 int64_t hcg_embedding_grad_workspace(int dtype, int64_t n, int64_t vocab, int64_t width) {
   if (vocab <= 0 || width <= 0 || n >= kMaxTokens || one_launch(n, items_of(dtype, width))) return 0;
-  return 4 * round256(n * 4) + round256(n * 2) + windows_of(n) * kRuns * width * 4;
+  const int64_t parted = n > kBucketTokens ? 2 * round256(n * 4) + round256(kBuckets * 8) : 0;
+  return 4 * round256(n * 4) + round256(n * 2) + parted + windows_of(n) * kRuns * width * 4;
 }
 
 int hcg_embedding_grad(int dtype, const void* dy, int64_t lddy, int64_t n, int64_t width, int id_bytes,
@@ -581,7 +688,16 @@ int hcg_embedding_grad(int dtype, const void* dy, int64_t lddy, int64_t n, int64
     a.run_len = reinterpret_cast<int*>(p += round256(n * 4));
     a.found = reinterpret_cast<int*>(p += round256(n * 4));
     a.found_row = reinterpret_cast<uint16_t*>(p += round256(n * 4));
-    a.part = reinterpret_cast<float*>(p + round256(n * 2));
+    p += round256(n * 2);
+    if (n > kBucketTokens) {
+      a.bucket_id = reinterpret_cast<int*>(p);
+      a.bucket_token = reinterpret_cast<int*>(p += round256(n * 4));
+      a.bucket = reinterpret_cast<int*>(p += round256(n * 4));
+      p += round256(kBuckets * 8);
+      // (whole workgroups' rows: a workgroup's lie in one bucket)
+      a.bucket_rows = (int)((vocab + (int64_t)kBuckets * a.rows - 1) / ((int64_t)kBuckets * a.rows) * a.rows);
+    }
+    a.part = reinterpret_cast<float*>(p);
   }
   const hipStream_t s = static_cast<hipStream_t>(stream);
   with_elem(dtype, [&](auto t) {
