@@ -305,8 +305,8 @@ struct ShapeInfo {
 constexpr ShapeInfo kShapes[] = {
     {256, 256, 2, 1, 12.0, 0.95, 1.55},
     {128, 128, 2, 1, 4.0, 0.31, 0.52},
-    {128, 64, 4, 2, 3.5, 0.25, 0.50},   // (not dx: its split sums want more registers than two per CU leave)
-    {128, 32, 4, 2, 3.5, 0.22, 0.60}};  // (not dw: its rows of vocabulary are read 64 at a time)
+    {128, 64, 4, 2, 3.5, 0.30, 0.82},   // (not dx: its split sums want more registers than two per CU leave)
+    {128, 32, 4, 2, 3.5, 0.26, 0.74}};  // (not dw: its rows of vocabulary are read 64 at a time)
 constexpr int kNumShapes = 4;
 constexpr int kCus = 256;
 constexpr int kMaxSplits = 32;
@@ -316,10 +316,15 @@ int64_t tiles(Shape s, int64_t m, int64_t n) { return ceil_div(m, kShapes[s].tm)
 
 double cost_of(Shape s, int64_t m, int64_t n, int64_t k, int splits) {
   const ShapeInfo& t = kShapes[s];
-  const int64_t units = tiles(s, m, n) * splits, room = kCus * t.per_cu;
-  const double busy = units < room ? (double)units / room : 1.0;
+  const int64_t units = tiles(s, m, n) * splits, room = kCus * t.per_cu, rest = units % room;
   const double stages = (double)ceil_div(ceil_div(k, splits), head::kStep);
-  double us = (double)ceil_div(units, room) * (t.fixed + stages * (t.lo + (t.hi - t.lo) * busy));
+  // Full rounds, and what is left: with one workgroup per CU a stage slows as the
+  // chip fills, with two once CUs are shared.
+  double us = (double)(units / room) * (t.fixed + stages * t.hi);
+  if (rest) {
+    const double busy = t.per_cu == 1 ? (double)rest / room : std::max(0.0, (double)(rest - kCus) / kCus);
+    us += t.fixed + stages * (t.lo + (t.hi - t.lo) * busy);
+  }
   if (splits > 1) {
     // The parts written and read, and a launch, or their reading by one CU.
     us += 2.0 * splits * m * n * 4 / 6.0e6;
@@ -377,9 +382,12 @@ Plan make_plan(int64_t tokens, int64_t vocab, int64_t width, bool copy_weight, b
   p.grad = grad;
   p.copy_weight = copy_weight;
   p.ldx = round_up(width, 8);
-  p.lde = round_up(vocab, 8);
+  // Whole 128-byte lines, and not a multiple of 1 KB: rows a power of two apart
+  // put the pieces that are read at one k on a few HBM channels (dx of 4096 x
+  // 32768 x 512 bf16 145 us, so 118).
+  p.lde = round_up(vocab, 64) + (round_up(vocab, 64) % 512 ? 0 : 64);
   p.piece = tokens;
-  if (grad) p.piece = std::min(tokens, std::max<int64_t>(256, kPieceBytes / (p.lde * 2) / 256 * 256));
+  if (grad) p.piece = std::min(tokens, std::max<int64_t>(256, kPieceBytes / (vocab * 2) / 256 * 256));
   p.pieces = (int)ceil_div(tokens, p.piece);
   p.logits = pick_shape(kLogits, vocab, p.piece, width, nullptr);
   p.blocks = ceil_div(vocab, kShapes[p.logits].tm) * kShapes[p.logits].wm;
