@@ -46,14 +46,14 @@ enum Epilogue {
   kExp,      // and exp(logit - block maximum) as f16
   kRound,    // scaled, rounded to DT, as rows of the output
   kPartial,  // float32, into scratch
-  kSplit,    // kRound, where K is split of the parts' sum (can_fuse) or kPartial
+  kSplit,    // kRound, or where K is split and the tile too large to fuse kPartial
 };
 
 // Tiles whose K splits the tile's last workgroup sums itself (hcg_splitsum.h);
 // larger ones are added up by a launch of their own (dx of 256 x 4096 x 512 in
 // 128x128 tiles and 8 parts: 16.0 us by the last workgroup, 12.6 by a launch; in
 // 128x32 tiles of 128 x 6000 x 700 11.2 by the last one).
-constexpr bool can_fuse(int tm, int tn) { return tm * tn <= 128 * 32; }
+constexpr bool can_fuse(int tm, int tn) { return tm * tn <= 128 * 64; }
 
 struct Args {
   const uint16_t* A;  // M side
@@ -64,8 +64,8 @@ struct Args {
   const int* count;
   int count0;
   int tiles_m;
-  // kSplit: K is split while there are fewer tiles (of live tokens) than units,
-  // into at most max_splits parts.
+  // kSplit, and tiles that can_fuse: K is split while there are fewer tiles (of
+  // live tokens) than units, into at most max_splits parts.
   int units, max_splits;
   unsigned* counters;  // can_fuse: one per tile, kSplitCounterStride apart, all zero
   int part_bytes;
@@ -337,7 +337,8 @@ __device__ __forceinline__ void head_tile(Args g, int wg) {
   const int tiles_n = (N + TN - 1) / TN;
   const int K_all = COUNT_K ? live : g.K;
   int chunk = K_all, splits = 1;
-  if constexpr (EPI == kSplit) splits = splits_of(g.units, g.max_splits, g.tiles_m * tiles_n, K_all, &chunk);
+  constexpr bool kFuse = can_fuse(TM, TN) && EPI != kPartial;
+  if constexpr (EPI == kSplit || kFuse) splits = splits_of(g.units, g.max_splits, g.tiles_m * tiles_n, K_all, &chunk);
   if (wg >= g.tiles_m * tiles_n * splits) return;
   int split, tm, tn;
   unit_of(g.tiles_m, tiles_n, splits, wg, split, tm, tn);
@@ -534,7 +535,7 @@ __device__ __forceinline__ void head_tile(Args g, int wg) {
                                                               : place(Int<4 % UNITS>{})) +
                                   wave % kWavesPerUnit * Stage::kBytes;
 
-  if constexpr (EPI == kSplit && can_fuse(TM, TN)) {
+  if constexpr (kFuse) {
     if (splits > 1) {
       constexpr int P = MI * NI * 4;
       split_f32x4 v[P];
@@ -542,7 +543,7 @@ __device__ __forceinline__ void head_tile(Args g, int wg) {
       for (int p = 0; p < P; ++p)
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[p][e] = acc[p / 4 / NI][p / 4 % NI][p % 4 * 4 + e];
-      if (!sum_splits<P, 64 * NW>(v, make_rsrc(g.part, g.part_bytes), g.tiles_m * tiles_n, tm * tiles_n + tn, splits,
+      if (!sum_splits<P, 64 * NW, 16>(v, make_rsrc(g.part, g.part_bytes), g.tiles_m * tiles_n, tm * tiles_n + tn, splits,
                                   split, g.counters, reinterpret_cast<unsigned*>(place(Int<1>{}))))
         return;
 #pragma unroll

@@ -305,12 +305,12 @@ struct ShapeInfo {
 constexpr ShapeInfo kShapes[] = {
     {256, 256, 2, 1, 12.0, 0.95, 1.55},
     {128, 128, 2, 1, 4.0, 0.31, 0.52},
-    {128, 64, 4, 2, 3.5, 0.30, 0.82},   // (not dx: its split sums want more registers than two per CU leave)
+    {128, 64, 4, 2, 3.5, 0.30, 0.82},
     {128, 32, 4, 2, 3.5, 0.26, 0.74}};  // (not dw: its rows of vocabulary are read 64 at a time)
 constexpr int kNumShapes = 4;
 constexpr int kCus = 256;
 constexpr int kMaxSplits = 32;
-constexpr int kMinKPerSplit = 256;
+constexpr int kMinKPerSplit = 256, kMinKPerFusedSplit = 128;
 
 int64_t tiles(Shape s, int64_t m, int64_t n) { return ceil_div(m, kShapes[s].tm) * ceil_div(n, kShapes[s].tn); }
 
@@ -333,27 +333,52 @@ double cost_of(Shape s, int64_t m, int64_t n, int64_t k, int splits) {
   return us;
 }
 
-int max_splits_of(Shape s, int64_t k) {
-  const int64_t most = head::can_fuse(kShapes[s].tm, kShapes[s].tn) ? hcg::kMaxSummedSplits : kMaxSplits;
-  return (int)std::max<int64_t>(1, std::min(most, k / kMinKPerSplit));
-}
+bool fuses(Shape s) { return head::can_fuse(kShapes[s].tm, kShapes[s].tn); }
 
-// The shape with the least modelled time; *units: workgroups to split K up to, or null.
-enum Product { kLogits, kDx, kDw };
-Shape pick_shape(Product product, int64_t m, int64_t n, int64_t k, int* units) {
-  Shape best = kLarge;
+enum ProductKind { kLogits, kDx, kDw };
+
+// How a product of m x n over k runs: the shape with the least modelled time, and
+// into how many parts K may be split (by the tile's last workgroup, or, dx in
+// large tiles, by a launch).
+struct Product {
+  Shape shape;
+  int units, max_splits;  // as head::Args has them
+  int counters;           // tiles that may be split and summed by their last workgroup
+  int64_t part_bytes;
+  int64_t wgs(int64_t m, int64_t n) const {
+    return std::max<int64_t>(tiles(shape, m, n), max_splits > 1 ? units : 0);
+  }
+};
+
+Product pick_product(ProductKind kind, int64_t m, int64_t n, int64_t k) {
+  Product best{};
   double best_cost = -1;
   for (int i = 0; i < kNumShapes; ++i) {
     const Shape s = (Shape)i;
-    if (product == kDx ? s == kSmall : product == kDw && s == kFew) continue;
-    for (int splits = 1; splits <= max_splits_of(s, k); ++splits) {
-      if (splits > 1 && !units) break;
+    if (kind == kDw && s == kFew) continue;
+    const int64_t most = fuses(s) ? std::min<int64_t>(hcg::kMaxSummedSplits, k / kMinKPerFusedSplit)
+                         : kind == kDx ? std::min<int64_t>(kMaxSplits, k / kMinKPerSplit)
+                                       : 1;
+    for (int splits = 1; splits <= std::max<int64_t>(1, most); ++splits) {
       const double cost = cost_of(s, m, n, k, splits);
       if (best_cost >= 0 && cost >= best_cost) continue;
       best_cost = cost;
-      best = s;
-      // (fewer tokens that count leave fewer tiles and more splits)
-      if (units) *units = (int)(splits > 1 ? tiles(s, m, n) * splits : (int64_t)kCus * kShapes[s].per_cu);
+      best.shape = s;
+      best.max_splits = (int)std::max<int64_t>(1, most);
+      // (where fewer tokens count, the fewer tiles are split up to as many)
+      best.units = (int)std::min<int64_t>(tiles(s, m, n) * splits, 0x7fffffff);
+    }
+  }
+  if (best.max_splits > 1) {
+    const ShapeInfo& t = kShapes[best.shape];
+    if (fuses(best.shape)) {
+      // Whole tiles of at most `units` workgroups.
+      best.counters = (int)std::min<int64_t>(best.units, tiles(best.shape, m, n));
+      best.part_bytes = (int64_t)best.units * t.tm * t.tn * 4;
+    } else {
+      // K is split while the parts' tiles are at most `units`: no more rows
+      // (padded to 8) than those tiles have, nor than max_splits times n.
+      best.part_bytes = std::min(best.units / ceil_div(m, t.tm) * t.tn, best.max_splits * n) * round_up(m, 8) * 4;
     }
   }
   return best;
@@ -365,13 +390,11 @@ struct Plan {
   int64_t ldx, lde;    // padded rows of X and of the probabilities
   int64_t piece;       // tokens per piece
   int pieces;
-  Shape logits, dx, dw;
-  int units, max_splits;  // of dx
-  int counters;           // its tiles, where their last workgroup sums the splits
+  Product logits, dx, dw;
+  int counters;        // of the products (which run one after the other), the most
   int64_t blocks;      // statistics per token
   // Offsets into the workspace.
   int64_t token, target, count, scale, rows, weight, stats, hit, loss, exps, part, counter, sums, total;
-  int64_t part_bytes;
 };
 
 Plan make_plan(int64_t tokens, int64_t vocab, int64_t width, bool copy_weight, bool grad) {
@@ -389,14 +412,14 @@ Plan make_plan(int64_t tokens, int64_t vocab, int64_t width, bool copy_weight, b
   p.piece = tokens;
   if (grad) p.piece = std::min(tokens, std::max<int64_t>(256, kPieceBytes / (vocab * 2) / 256 * 256));
   p.pieces = (int)ceil_div(tokens, p.piece);
-  p.logits = pick_shape(kLogits, vocab, p.piece, width, nullptr);
-  p.blocks = ceil_div(vocab, kShapes[p.logits].tm) * kShapes[p.logits].wm;
+  p.logits = pick_product(kLogits, vocab, p.piece, width);
+  p.blocks = ceil_div(vocab, kShapes[p.logits.shape].tm) * kShapes[p.logits.shape].wm;
   if (grad) {
-    p.dx = pick_shape(kDx, width, p.piece, vocab, &p.units);
-    p.dw = pick_shape(kDw, width, vocab, p.piece, nullptr);
-    p.max_splits = max_splits_of(p.dx, vocab);
-    if (head::can_fuse(kShapes[p.dx].tm, kShapes[p.dx].tn) && p.max_splits > 1) p.counters = (int)std::min<int64_t>(p.units, tiles(p.dx, width, p.piece));
+    p.dx = pick_product(kDx, width, p.piece, vocab);
+    p.dw = pick_product(kDw, width, vocab, p.piece);
   }
+  p.counters = std::max({p.logits.counters, p.dx.counters, p.dw.counters});
+  const int64_t part_bytes = std::max({p.logits.part_bytes, p.dx.part_bytes, p.dw.part_bytes});
   int64_t at = 0;
   const auto take = [&](int64_t bytes) {
     const int64_t here = at;
@@ -414,16 +437,10 @@ Plan make_plan(int64_t tokens, int64_t vocab, int64_t width, bool copy_weight, b
   if (grad) {
     p.loss = take(tokens * 4);
     p.exps = take(p.piece * p.lde * 2);
-    // K is split while the parts' tiles are at most `units`: no more rows than
-    // those tiles have (nor than max_splits times the tokens).
-    // (Where a tile's last workgroup sums, the parts are whole tiles.)
-    const ShapeInfo& t = kShapes[p.dx];
-    const int64_t rows = std::min(p.units / ceil_div(width, t.tm) * t.tn, p.max_splits * p.piece);
-    p.part_bytes = p.max_splits == 1 ? 0 : p.counters ? (int64_t)p.units * t.tm * t.tn * 4 : rows * p.ldx * 4;
-    p.part = take(p.part_bytes);
-    p.counter = take((int64_t)p.counters * hcg::kSplitCounterStride * 4);
     p.sums = take(p.pieces > 1 ? vocab * width * 4 : 0);
   }
+  p.part = take(part_bytes);
+  p.counter = take((int64_t)p.counters * hcg::kSplitCounterStride * 4);
   p.total = at;
   return p;
 }
@@ -433,9 +450,15 @@ bool weight_in_place(const void* w, int64_t ldw, int64_t vocab, int64_t width) {
          ldw <= kMaxExtent;
 }
 
+// extra: workgroups beside the product's.
 template <int DT, int EPI, bool AKC, bool BKC, bool COUNT_K>
-void launch_head(Shape shape, const head::Args& a, int64_t wgs, hipStream_t s) {
-  const dim3 grid((unsigned)wgs);
+void launch_head(const Product& p, head::Args a, hipStream_t s, int extra = 0) {
+  const Shape shape = p.shape;
+  a.tiles_m = (int)ceil_div(a.M, kShapes[shape].tm);
+  a.units = p.units;
+  a.max_splits = p.max_splits;
+  a.part_bytes = (int)p.part_bytes;
+  const dim3 grid((unsigned)(p.wgs(a.M, a.N) + extra));
   // Large tiles: four waves read the least LDS (128 KB per stage against 192 KB
   // by eight), and the board runs at its power limit; the softmax's epilogue is
   // faster by eight.  8192 x 65536 x 4096 bf16, us, four / eight waves: logits
@@ -447,13 +470,11 @@ void launch_head(Shape shape, const head::Args& a, int64_t wgs, hipStream_t s) {
   } else if (shape == kMedium) {
     head::head_kernel<DT, 128, 128, 2, 4, 8, AKC, BKC, EPI, COUNT_K, false><<<grid, 512, 0, s>>>(a);
   } else if (shape == kSmall) {
-    if constexpr (EPI != head::kSplit) {
-      // (one tile of tokens: bound by reading the weights)
-      if (kSoftmax && a.N <= 64)
-        head::head_kernel<DT, 128, 64, 4, 2, 6, AKC, BKC, EPI, COUNT_K, kSoftmax><<<grid, 512, 0, s>>>(a);
-      else
-        head::head_kernel<DT, 128, 64, 4, 2, 6, AKC, BKC, EPI, COUNT_K, false><<<grid, 512, 0, s>>>(a);
-    }
+    // (one tile of tokens: bound by reading the weights)
+    if (kSoftmax && a.N <= 64)
+      head::head_kernel<DT, 128, 64, 4, 2, 6, AKC, BKC, EPI, COUNT_K, kSoftmax><<<grid, 512, 0, s>>>(a);
+    else
+      head::head_kernel<DT, 128, 64, 4, 2, 6, AKC, BKC, EPI, COUNT_K, false><<<grid, 512, 0, s>>>(a);
   } else if constexpr (BKC) {
     head::head_kernel<DT, 128, 32, 4, 1, 6, AKC, BKC, EPI, COUNT_K, kSoftmax><<<grid, 256, 0, s>>>(a);
   }
@@ -544,20 +565,20 @@ int run_loss(const Plan& p, const Call& c, hipStream_t s) {
     a.K = (int)p.ldx;
     a.count = count;
     a.count0 = (int)t0;
-    a.tiles_m = (int)ceil_div(V, kShapes[p.logits].tm);
+    a.part = static_cast<float*>(at(p.part));
+    a.counters = static_cast<unsigned*>(at(p.counter));
     a.stats = static_cast<f32x2*>(at(p.stats));
     a.ld_stats = p.blocks;
     a.target = target + t0;
     a.hit = static_cast<float*>(at(p.hit));
     a.out = p.grad ? at(p.exps) : nullptr;
     a.ldo = p.lde;
-    const int64_t wgs = tiles(p.logits, V, n);
     if (p.grad)
-      launch_head<DT, head::kExp, true, true, false>(p.logits, a, wgs, s);
+      launch_head<DT, head::kExp, true, true, false>(p.logits, a, s);
     else
-      launch_head<DT, head::kStats, true, true, false>(p.logits, a, wgs, s);
+      launch_head<DT, head::kStats, true, true, false>(p.logits, a, s);
 
-    SoftmaxArgs sm{a.stats, p.blocks, (int)p.blocks, kShapes[p.logits].tm / kShapes[p.logits].wm, a.hit, a.target,
+    SoftmaxArgs sm{a.stats, p.blocks, (int)p.blocks, kShapes[p.logits.shape].tm / kShapes[p.logits.shape].wm, a.hit, a.target,
                    count, (int)t0, p.grad ? nullptr : token + t0, p.grad ? static_cast<float*>(at(p.loss)) + t0 : c.loss,
                    p.grad ? nullptr : c.lse, static_cast<uint16_t*>(a.out), p.lde, V, 1.f};
     if (!p.grad) {
@@ -578,25 +599,21 @@ int run_loss(const Plan& p, const Call& c, hipStream_t s) {
     d.K = V;
     d.count = count;
     d.count0 = (int)t0;
-    d.units = p.units;
-    d.max_splits = p.max_splits;
-    d.tiles_m = (int)ceil_div(D, kShapes[p.dx].tm);
     d.scale = scale;
     d.post = post;
     d.out = c.dx;
     d.ldo = c.lddx;
     d.row_of = token + t0;
-    d.part = static_cast<float*>(at(p.part));
+    d.part = a.part;
     d.ld_part = p.ldx;
-    d.counters = static_cast<unsigned*>(at(p.counter));
-    d.part_bytes = (int)p.part_bytes;
-    // (as many workgroups as any number of live tokens takes)
-    const int64_t dx_wgs = std::max<int64_t>(tiles(p.dx, D, n), p.max_splits > 1 ? p.units : 0);
-    launch_head<DT, head::kSplit, false, true, false>(p.dx, d, dx_wgs, s);
-    if (p.max_splits > 1 && !p.counters) {
-      const JoinArgs j{d.part,    p.ldx, d.units,    d.max_splits, d.tiles_m, kShapes[p.dx].tn,
-                       n,         V,     D,          (int)(p.ldx / 8), count, (int)t0,
-                       token + t0, scale, post,      static_cast<uint16_t*>(c.dx), c.lddx};
+    d.counters = a.counters;
+    launch_head<DT, head::kSplit, false, true, false>(p.dx, d, s);
+    if (p.dx.max_splits > 1 && !fuses(p.dx.shape)) {
+      const ShapeInfo& t = kShapes[p.dx.shape];
+      const JoinArgs j{d.part,     p.ldx, p.dx.units, p.dx.max_splits,  (int)ceil_div(D, t.tm),
+                       t.tn,       n,     V,          D,                (int)(p.ldx / 8),
+                       count,      (int)t0, token + t0, scale,          post,
+                       static_cast<uint16_t*>(c.dx), c.lddx};
       const int64_t wgs = std::min<int64_t>(ceil_div((int64_t)n * j.vecs, 256), 4 * kCus);
       join_kernel<DT><<<dim3((unsigned)wgs), 256, 0, s>>>(j);
     }
@@ -611,22 +628,22 @@ int run_loss(const Plan& p, const Call& c, hipStream_t s) {
     w.K = n;
     w.count = count;
     w.count0 = (int)t0;
-    w.tiles_m = (int)ceil_div(D, kShapes[p.dw].tm);
+    w.counters = a.counters;
+    w.part = a.part;
     w.scale = scale;
     w.post = post;
     w.add = i > 0 ? sums : nullptr;
-    const int64_t dw_wgs = tiles(p.dw, D, V);
     if (i + 1 == p.pieces) {
       w.out = c.dw;
       w.ldo = c.lddw;
       w.loss = static_cast<const float*>(at(p.loss));
       w.loss_scale = scale + 1;
       w.loss_out = c.loss;
-      launch_head<DT, head::kRound, false, false, true>(p.dw, w, dw_wgs + 1, s);
+      launch_head<DT, head::kRound, false, false, true>(p.dw, w, s, 1);
     } else {
       w.part = sums;
       w.ld_part = D;
-      launch_head<DT, head::kPartial, false, false, true>(p.dw, w, dw_wgs, s);
+      launch_head<DT, head::kPartial, false, false, true>(p.dw, w, s);
     }
   }
   HCG_LM_HIP_CHECK(hipGetLastError());
@@ -655,9 +672,9 @@ int check_call(int dtype, const Call& c, int64_t tokens, int64_t vocab, int64_t 
                  "rows and targets must be aligned to their elements");
   if (tokens == 0 || vocab == 0 || width == 0) return HCG_OK;
   *plan = make_plan(tokens, vocab, width, !weight_in_place(c.weight, c.ldw, vocab, width), grad);
-  HCG_LM_REQUIRE(tiles(plan->logits, vocab, plan->piece) < ((int64_t)1 << 31) &&
-                     tiles(plan->dw, width, vocab) < ((int64_t)1 << 31) &&
-                     tiles(plan->dx, width, plan->piece) < ((int64_t)1 << 31),
+  const int64_t most = ((int64_t)1 << 31) - 1;
+  HCG_LM_REQUIRE(plan->logits.wgs(vocab, plan->piece) < most &&
+                     (!grad || (plan->dw.wgs(width, vocab) < most && plan->dx.wgs(width, plan->piece) < most)),
                  "too many tiles");
   HCG_LM_REQUIRE(c.ws && ws_bytes >= plan->total && hcg::elem_aligned(c.ws, 256),
                  "workspace of %lld bytes, %lld needed (256-byte aligned)", (long long)ws_bytes,

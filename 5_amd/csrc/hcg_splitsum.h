@@ -30,8 +30,9 @@ constexpr int kMaxSummedSplits = 16;
 // the last workgroup of the block to arrive, with v summed over the splits in
 // the order 0, 1, ...; false in the others.  flag: an LDS word that no wave
 // still uses when all have reached the first barrier here.  splits <=
-// kMaxSummedSplits; the workspace stays below 2^31 bytes.
-template <int P, int THREADS>
+// kMaxSummedSplits; the workspace stays below 2^31 bytes.  PIECES: loads in
+// flight per thread (of 16 bytes, four registers each).
+template <int P, int THREADS, int PIECES = 32>
 __device__ __forceinline__ bool sum_splits(split_f32x4 (&v)[P], __amdgpu_buffer_rsrc_t ws, int blocks, int block,
                                            int splits, int split, unsigned* counters, unsigned* flag) {
   constexpr int kAgent = 16;  // SC1: the cache policy of an agent-scope access
@@ -52,8 +53,8 @@ __device__ __forceinline__ bool sum_splits(split_f32x4 (&v)[P], __amdgpu_buffer_
   split_f32x4 own[P];
 #pragma unroll
   for (int p = 0; p < P; ++p) own[p] = v[p];
-  // Splits whose loads are in flight together (at most 32 of 16 bytes a thread).
-  constexpr int kBatch = P >= 4 ? 32 / P : 8;
+  // Splits whose loads are in flight together.
+  constexpr int kBatch = P >= 4 ? PIECES / P : 8;
   for (int s0 = 0; s0 < splits; s0 += kBatch) {
     u32x4 part[kBatch][P];
 #pragma unroll
