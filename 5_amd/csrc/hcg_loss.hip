@@ -186,7 +186,6 @@ struct SoftmaxArgs {
   uint16_t* e;  // exponentials in, probabilities out
   int64_t lde;
   int vocab;
-  float scale;
 };
 
 // One row by one workgroup: lse from the blocks' statistics, the loss, and
@@ -292,21 +291,23 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // Tile shapes of head_kernel: rows of M and N, waves over M in the softmax's
 // product, and a model of its time in us: a tile's start and end, and one
 // stage of K on an idle and on a busy chip, per round of workgroups
-// (per_cu of which share a CU).  Fitted to 11 sizes with every shape and 1 to 16
-// K splits.  Both sides, us: dx of 1300 x 50000 x 1032 large in 8 parts 141,
-// medium in 2 208; of 256 x 4096 x 512 large in 16 parts 18, medium in 8 9; of
-// 64 x 32768 x 4096 medium in 8 parts 43, few in 8 49; logits of 32 x 50000 x
-// 1024 medium 22, few 17; of 1024 x 32768 x 2048 large 117, medium 167.
+// (per_cu of which share a CU).  Fitted to 10 sizes with every shape and 1 to 8
+// K splits: its choice is the fastest, or within 8% of it, at nine of them.  Both
+// sides, us: dx of 1300 x 50000 x 1032 large in 8 parts 150, medium in 4 189; of
+// 256 x 4096 x 512 large in 8 parts 28, few in 4 10; of 1000 x 30000 x 1000
+// large in 8 parts 87, medium in 4 73; logits of 128 x 6000 x 700 large 20, few
+// 7; of 1024 x 32768 x 2048 large 117, medium 147; dw of 64 x 32768 x 4096 large
+// 111, medium 78, small 125; of 4096 x 32768 x 512 109, 140, 190.
 enum Shape { kLarge, kMedium, kSmall, kFew };
 struct ShapeInfo {
   int tm, tn, wm, per_cu;
   double fixed, lo, hi;
 };
 constexpr ShapeInfo kShapes[] = {
-    {256, 256, 2, 1, 12.0, 0.95, 1.55},
-    {128, 128, 2, 1, 4.0, 0.31, 0.52},
-    {128, 64, 4, 2, 3.5, 0.30, 0.82},
-    {128, 32, 4, 2, 3.5, 0.26, 0.74}};  // (not dw: its rows of vocabulary are read 64 at a time)
+    {256, 256, 2, 1, 10.0, 0.92, 1.5},
+    {128, 128, 2, 2, 4.0, 0.55, 1.05},
+    {128, 64, 4, 2, 3.2, 0.35, 0.78},
+    {128, 32, 4, 2, 3.5, 0.28, 0.74}};  // (not dw: its rows of vocabulary are read 64 at a time)
 constexpr int kNumShapes = 4;
 constexpr int kCus = 256;
 constexpr int kMaxSplits = 32;
@@ -468,7 +469,11 @@ void launch_head(const Product& p, head::Args a, hipStream_t s, int extra = 0) {
     head::head_kernel<DT, 256, 256, 2, kSoftmax ? 4 : 2, 5, AKC, BKC, EPI, COUNT_K, false>
         <<<grid, kSoftmax ? 512 : 256, 0, s>>>(a);
   } else if (shape == kMedium) {
-    head::head_kernel<DT, 128, 128, 2, 4, 8, AKC, BKC, EPI, COUNT_K, false><<<grid, 512, 0, s>>>(a);
+    // A ring of 5 units, 80 KB: two workgroups share a CU, and one computes while
+    // the other starts or ends.  Eight units at one per CU / five, us: logits of
+    // 4096 x 32768 x 512 251 / 198, dw of 64 x 32768 x 4096 130 / 78, dx of 1024 x
+    // 32768 x 2048 134 / 133.
+    head::head_kernel<DT, 128, 128, 2, 4, 5, AKC, BKC, EPI, COUNT_K, false><<<grid, 512, 0, s>>>(a);
   } else if (shape == kSmall) {
     // (one tile of tokens: bound by reading the weights)
     if (kSoftmax && a.N <= 64)
@@ -580,7 +585,7 @@ int run_loss(const Plan& p, const Call& c, hipStream_t s) {
 
     SoftmaxArgs sm{a.stats, p.blocks, (int)p.blocks, kShapes[p.logits.shape].tm / kShapes[p.logits.shape].wm, a.hit, a.target,
                    count, (int)t0, p.grad ? nullptr : token + t0, p.grad ? static_cast<float*>(at(p.loss)) + t0 : c.loss,
-                   p.grad ? nullptr : c.lse, static_cast<uint16_t*>(a.out), p.lde, V, 1.f};
+                   p.grad ? nullptr : c.lse, static_cast<uint16_t*>(a.out), p.lde, V};
     if (!p.grad) {
       softmax_kernel<DT, false><<<dim3((unsigned)n), 256, 0, s>>>(sm);
       continue;
