@@ -43,7 +43,8 @@ constexpr int kEmbedPer = 4;  // vectors per thread and turn
 template <class T, class I>
 __global__ __launch_bounds__(256) void embed_kernel(EmbedArgs g) {
   constexpr int E = kVec<T>;
-  const int64_t row0 = (int64_t)blockIdx.x * g.rows_per_wg;
+  const int64_t row0 = hcg::workgroup() * g.rows_per_wg;
+  if (row0 >= g.n) return;
   const int rows = (int)min((int64_t)g.rows_per_wg, g.n - row0);
   const int total = rows * g.vecs;
   const I* ids = static_cast<const I*>(g.ids) + row0;
@@ -561,6 +562,8 @@ __global__ __launch_bounds__(256) void embed_long_kernel(EmbedGradArgs g) {
 // ---------------------------------------------------------------------------
 
 constexpr int64_t kMaxTokens = (int64_t)1 << 30;
+// Tokens and rows of the gradient: fewer than 2^32 threads to a launch.
+constexpr int64_t kMaxGrad = (int64_t)1 << 28;
 
 int64_t items_of(int dtype, int64_t width) {
   const int64_t e = 16 / hcg::elem_bytes(dtype);
@@ -622,7 +625,7 @@ int hcg_embedding(int dtype, const void* table, int64_t ldt, int64_t vocab, int6
   EmbedArgs a{table, ids, out, ldt, ldo, vocab, n, (int)width, 0, 0, scale};
   a.vecs = (int)((width * eb + 15) / 16);
   a.rows_per_wg = std::max(1, 256 * kEmbedPer / a.vecs);
-  const dim3 grid((unsigned)((n + a.rows_per_wg - 1) / a.rows_per_wg));
+  const dim3 grid = hcg::grid_of((n + a.rows_per_wg - 1) / a.rows_per_wg);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   with_elem(dtype, [&](auto t) {
     using T = decltype(t);
@@ -636,7 +639,7 @@ int hcg_embedding(int dtype, const void* table, int64_t ldt, int64_t vocab, int6
 }
 
 int64_t hcg_embedding_grad_workspace(int dtype, int64_t n, int64_t vocab, int64_t width) {
-  if (vocab <= 0 || width <= 0 || n >= kMaxTokens || one_launch(n, items_of(dtype, width))) return 0;
+  if (vocab <= 0 || width <= 0 || n >= kMaxGrad || one_launch(n, items_of(dtype, width))) return 0;
   const int64_t parted = n > kBucketTokens ? 2 * round256(n * 4) + round256(kBuckets * 8) : 0;
   return 4 * round256(n * 4) + round256(n * 2) + parted + windows_of(n) * kRuns * width * 4;
 }
@@ -647,7 +650,7 @@ int hcg_embedding_grad(int dtype, const void* dy, int64_t lddy, int64_t n, int64
   HCG_LM_REQUIRE(hcg::elem_ok(dtype), "dtype %d is not HCG_F16, HCG_BF16 or HCG_F32", dtype);
   HCG_LM_REQUIRE(grad_dtype == dtype || grad_dtype == HCG_F32, "the gradient has the type of dy or float32");
   HCG_LM_REQUIRE(id_bytes == 4 || id_bytes == 8, "ids are 4 or 8 bytes, not %d", id_bytes);
-  HCG_LM_REQUIRE(n >= 0 && n < kMaxTokens && vocab >= 0 && vocab < kMaxTokens && width >= 0 &&
+  HCG_LM_REQUIRE(n >= 0 && n < kMaxGrad && vocab >= 0 && vocab < kMaxGrad && width >= 0 &&
                      width < ((int64_t)1 << 23),
                  "%lld ids into %lld rows of %lld elements are out of range", (long long)n, (long long)vocab,
                  (long long)width);

@@ -663,14 +663,15 @@ __device__ __forceinline__ void head_tile(Args g, int wg) {
 }
 
 // The sum of the losses over the live tokens by one wave, in one order, into
-// *out (times *scale).  It runs beside the tiles of a product.
+// *out (times *scale).  It runs beside the tiles of a product.  In doubles: a lane
+// adds up n / 64 values, and like ones would all be rounded the same way.
 __device__ __forceinline__ void sum_losses(const float* loss, int n, const float* scale, float* out) {
-  float sum = 0.f;
+  double sum = 0.0;
 #pragma unroll 16
   for (int i = threadIdx.x; i < n; i += 64) sum += loss[i];
 #pragma unroll
   for (int m = 32; m >= 1; m >>= 1) sum += __shfl_xor(sum, m);
-  if (threadIdx.x == 0) *out = sum * *scale;
+  if (threadIdx.x == 0) *out = (float)(sum * (double)*scale);
 }
 
 // Waves per SIMD: two workgroups per CU where the ring takes at most half its LDS.

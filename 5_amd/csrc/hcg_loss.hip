@@ -30,6 +30,9 @@ namespace head = hcg::head;
 typedef head::f32x2 f32x2;
 
 constexpr int64_t kPieceBytes = (int64_t)1 << 30;
+// ... and no more than so many tokens, whose launches stay below 2^32 threads
+// (a loss alone holds no probabilities, and its pieces kPieceLogits logits).
+constexpr int64_t kPieceTokens = (int64_t)1 << 22, kPieceLogits = (int64_t)1 << 32;
 constexpr int64_t kMaxTokens = (int64_t)1 << 26;
 constexpr int64_t kMaxExtent = 4000000;  // of vocabulary and width: a tile's offsets stay in 31 bits
 // f16 probabilities are held times 2^12 (a uniform one over a vocabulary past
@@ -48,6 +51,7 @@ struct PackArgs {
   int* token;   // per place among those that count: the token
   int* target;  // per place: its target, -1 outside the vocabulary
   int* count;
+  const int* counts;  // how many count among each kCountRun tokens, where there are more (or null)
   float* scale;  // [0]: the gradient's factor, [1]: the loss's
   float* loss;   // per token, zeroed where ignored (or null)
   float* lse;
@@ -66,6 +70,29 @@ struct PackArgs {
 constexpr int kPackThreads = 256;
 constexpr int kPackRun = 128;  // tokens per workgroup at most: their places are in LDS
 
+// Past so many tokens, a launch counts them by runs of that many first.  us of
+// hcg_linear_cross_entropy over 64 x 16, counted first / not: 98304 tokens 161 /
+// 182, 262144 319 / 470, 1048576 1092 / 4624.
+constexpr int kCountRun = 1 << 16;
+constexpr int kCountThreads = 1024;
+template <class I>
+__global__ __launch_bounds__(kCountThreads) void count_kernel(const I* targets, int tokens, int64_t ignore,
+                                                              int* counts) {
+  __shared__ int waves[kCountThreads / 64];
+  const int from = blockIdx.x * kCountRun, to = min(from + kCountRun, tokens);
+  int sum = 0;
+#pragma unroll 8
+  for (int t = from + threadIdx.x; t < to; t += kCountThreads) sum += (int64_t)targets[t] != ignore;
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) sum += __shfl_xor(sum, m);
+  if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < kCountThreads / 64; ++w) sum += waves[w];
+    counts[blockIdx.x] = sum;
+  }
+}
+
 // A workgroup packs a run of tokens.  It counts the tokens before its run
 // itself, from the L2 (64 KB of targets at 8192 tokens), so that packing is one
 // launch without anything to wait for.
@@ -78,8 +105,12 @@ __global__ __launch_bounds__(kPackThreads) void pack_kernel(PackArgs g) {
   const I* targets = static_cast<const I*>(g.targets);
   for (int i = blockIdx.x * kPackThreads + tid; i < g.num_counters; i += gridDim.x * kPackThreads)
     g.counters[i * hcg::kSplitCounterStride] = 0;
-  int before = 0;
-  for (int t0 = tid; t0 < from; t0 += kPackThreads * 8) {
+  int before = 0, counted = 0;
+  if (g.counts) {
+    counted = from / kCountRun * kCountRun;
+    for (int i = tid; i < from / kCountRun; i += kPackThreads) before += g.counts[i];
+  }
+  for (int t0 = counted + tid; t0 < from; t0 += kPackThreads * 8) {
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
       const int t = t0 + u * kPackThreads;
@@ -366,8 +397,9 @@ Product pick_product(ProductKind kind, int64_t m, int64_t n, int64_t k) {
       best_cost = cost;
       best.shape = s;
       best.max_splits = (int)std::max<int64_t>(1, most);
-      // (where fewer tokens count, the fewer tiles are split up to as many)
-      best.units = (int)std::min<int64_t>(tiles(s, m, n) * splits, 0x7fffffff);
+      // (where fewer tokens count, the fewer tiles are split up to as many; more
+      // than some rounds of workgroups gain nothing and would take scratch)
+      best.units = (int)std::min<int64_t>(tiles(s, m, n) * splits, 8 * kCus);
     }
   }
   if (best.max_splits > 1) {
@@ -395,7 +427,7 @@ struct Plan {
   int counters;        // of the products (which run one after the other), the most
   int64_t blocks;      // statistics per token
   // Offsets into the workspace.
-  int64_t token, target, count, scale, rows, weight, stats, hit, loss, exps, part, counter, sums, total;
+  int64_t token, target, count, counts, scale, rows, weight, stats, hit, loss, exps, part, counter, sums, total;
 };
 
 Plan make_plan(int64_t tokens, int64_t vocab, int64_t width, bool copy_weight, bool grad) {
@@ -410,8 +442,8 @@ Plan make_plan(int64_t tokens, int64_t vocab, int64_t width, bool copy_weight, b
   // put the pieces that are read at one k on a few HBM channels (dx of 4096 x
   // 32768 x 512 bf16 145 us, so 118).
   p.lde = round_up(vocab, 64) + (round_up(vocab, 64) % 512 ? 0 : 64);
-  p.piece = tokens;
-  if (grad) p.piece = std::min(tokens, std::max<int64_t>(256, kPieceBytes / (vocab * 2) / 256 * 256));
+  const int64_t fit = (grad ? kPieceBytes / 2 : kPieceLogits) / vocab / 256 * 256;
+  p.piece = std::min({tokens, std::max<int64_t>(256, fit), kPieceTokens});
   p.pieces = (int)ceil_div(tokens, p.piece);
   p.logits = pick_product(kLogits, vocab, p.piece, width);
   p.blocks = ceil_div(vocab, kShapes[p.logits.shape].tm) * kShapes[p.logits.shape].wm;
@@ -430,6 +462,7 @@ Plan make_plan(int64_t tokens, int64_t vocab, int64_t width, bool copy_weight, b
   p.token = take(tokens * 4);
   p.target = take(tokens * 4);
   p.count = take(4);
+  p.counts = take(tokens > kCountRun ? ceil_div(tokens, kCountRun) * 4 : 0);
   p.scale = take(8);
   p.rows = take(tokens * p.ldx * 2);
   p.weight = take(copy_weight ? vocab * p.ldx * 2 : 0);
@@ -507,12 +540,13 @@ struct Call {
 template <int DT>
 int run_loss(const Plan& p, const Call& c, hipStream_t s) {
   const auto at = [&](int64_t offset) { return static_cast<void*>(c.ws + offset); };
+  const int T = (int)p.tokens, V = (int)p.vocab, D = (int)p.width;
   int* token = static_cast<int*>(at(p.token));
   int* target = static_cast<int*>(at(p.target));
   int* count = static_cast<int*>(at(p.count));
+  int* counts = T > kCountRun ? static_cast<int*>(at(p.counts)) : nullptr;
   float* scale = static_cast<float*>(at(p.scale));
   uint16_t* rows = static_cast<uint16_t*>(at(p.rows));
-  const int T = (int)p.tokens, V = (int)p.vocab, D = (int)p.width;
 
   // At most 1024 runs, four workgroups per CU, while a run fits.
   const int per_wg = (int)std::min<int64_t>(kPackRun, ceil_div(T, 1024));
@@ -526,6 +560,7 @@ int run_loss(const Plan& p, const Call& c, hipStream_t s) {
                     token,
                     target,
                     count,
+                    counts,
                     scale,
                     p.grad ? nullptr : c.loss,
                     p.grad ? nullptr : c.lse,
@@ -540,6 +575,13 @@ int run_loss(const Plan& p, const Call& c, hipStream_t s) {
                     static_cast<unsigned*>(at(p.counter)),
                     p.counters};
   const dim3 runs((unsigned)ceil_div(T, per_wg));
+  if (counts) {
+    const dim3 grid((unsigned)ceil_div(T, kCountRun));
+    if (c.id_bytes == 8)
+      count_kernel<<<grid, kCountThreads, 0, s>>>(static_cast<const int64_t*>(c.targets), T, c.ignore, counts);
+    else
+      count_kernel<<<grid, kCountThreads, 0, s>>>(static_cast<const int32_t*>(c.targets), T, c.ignore, counts);
+  }
   if (c.id_bytes == 8)
     pack_kernel<int64_t><<<runs, kPackThreads, 0, s>>>(pk);
   else

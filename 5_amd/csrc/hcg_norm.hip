@@ -56,7 +56,7 @@ __global__ __launch_bounds__(norm_threads<WPR>()) void norm_kernel(NormArgs g) {
   __shared__ float slots[2][kRowsPerWg * WPR];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int group = wave / WPR, wir = wave % WPR;
-  const int64_t row = (int64_t)blockIdx.x * kRowsPerWg + group;
+  const int64_t row = hcg::workgroup() * kRowsPerWg + group;
   const bool live = row < g.rows;
   const T* x = static_cast<const T*>(g.x) + (live ? row : 0) * g.ldx;
   const int first = (wir * 64 + lane) * E;
@@ -119,7 +119,8 @@ __global__ __launch_bounds__(1024) void norm_wide_kernel(NormArgs g) {
   constexpr int E = kVec<T>;
   __shared__ float slots[2][16];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t row = blockIdx.x;
+  const int64_t row = hcg::workgroup();
+  if (row >= g.rows) return;
   const T* x = static_cast<const T*>(g.x) + row * g.ldx;
   float sum = 0.f;
   for (int64_t c = (int64_t)threadIdx.x * E; c < g.width; c += 1024 * E) {
@@ -338,7 +339,8 @@ __global__ __launch_bounds__(1024) void norm_grad_wide_kernel(NormGradArgs g) {
   constexpr int E = kVec<T>;
   __shared__ float slots[2][16];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t row = blockIdx.x;
+  const int64_t row = hcg::workgroup();
+  if (row >= g.rows) return;
   const T* x = static_cast<const T*>(g.x) + row * g.ldx;
   const T* dy = static_cast<const T*>(g.dy) + row * g.lddy;
   T* dx = static_cast<T*>(g.dx) + row * g.lddx;
@@ -427,7 +429,7 @@ constexpr int64_t kMaxWidth = 1 << 30;
 template <class T, class P, int WPR, int NV>
 void launch_norm(const NormArgs& a, hipStream_t s) {
   constexpr int rows = norm_threads<WPR>() / 64 / WPR;
-  norm_kernel<T, P, WPR, NV><<<dim3((unsigned)((a.rows + rows - 1) / rows)), norm_threads<WPR>(), 0, s>>>(a);
+  norm_kernel<T, P, WPR, NV><<<hcg::grid_of((a.rows + rows - 1) / rows), norm_threads<WPR>(), 0, s>>>(a);
 }
 
 template <class T, class P>
@@ -438,7 +440,7 @@ void run_norm(const NormArgs& a, hipStream_t s) {
   if (vecs <= 512) return launch_norm<T, P, 4, 2>(a, s);
   if (vecs <= 1024) return launch_norm<T, P, 4, 4>(a, s);
   if (vecs <= 4096) return launch_norm<T, P, 16, 4>(a, s);
-  norm_wide_kernel<T, P><<<dim3((unsigned)a.rows), 1024, 0, s>>>(a);
+  norm_wide_kernel<T, P><<<hcg::grid_of(a.rows), 1024, 0, s>>>(a);
 }
 
 template <class T, class P, int WPR, int NV, int GROUPS, bool LEAN = false>
@@ -457,7 +459,7 @@ int run_norm_grad(const NormGradArgs& a, hipStream_t s) {
   if (vecs <= 512) return launch_norm_grad<T, P, 8, 1, 2>(a, s);
   if (vecs <= 1024) return launch_norm_grad<T, P, 8, 2, 1>(a, s);
   if (vecs <= 2048) return launch_norm_grad<T, P, 16, 2, 1, sizeof(T) == 2>(a, s);
-  norm_grad_wide_kernel<T, P><<<dim3((unsigned)a.rows), 1024, 0, s>>>(a);
+  norm_grad_wide_kernel<T, P><<<hcg::grid_of(a.rows), 1024, 0, s>>>(a);
   const int parts = (int)std::min<int64_t>(64, a.rows);
   if (a.part)
     norm_columns_kernel<T><<<dim3((unsigned)((a.width + 255) / 256), parts), 256, 0, s>>>(a);
@@ -467,13 +469,11 @@ int run_norm_grad(const NormGradArgs& a, hipStream_t s) {
 template <class F>
 int with_types(int dtype, int param_dtype, F f) {
   const auto inner = [&](auto t) {
-    using T = decltype(t);
     switch (param_dtype) {
       case HCG_F16: return f(t, ElemOf<HCG_F16>::type{});
       case HCG_BF16: return f(t, ElemOf<HCG_BF16>::type{});
       default: return f(t, float{});
     }
-    (void)sizeof(T);
   };
   switch (dtype) {
     case HCG_F16: return inner(ElemOf<HCG_F16>::type{});

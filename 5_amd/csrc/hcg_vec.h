@@ -153,6 +153,15 @@ __device__ __forceinline__ float wave_max(float v) {
   return v;
 }
 
+// The grid of n workgroups, in two dimensions past 2^20 of them (a launch's
+// threads along one are fewer than 2^32), and a workgroup's number in it, which
+// may be n or more.
+inline dim3 grid_of(int64_t n) {
+  const int64_t x = n < (1 << 20) ? n : 1 << 20;
+  return dim3((unsigned)x, (unsigned)((n + x - 1) / x));
+}
+__device__ __forceinline__ int64_t workgroup() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
+
 // Host: the shape and pointer rules that every row-wise entry point has.
 inline int elem_bytes(int dtype) { return dtype == HCG_F32 ? 4 : 2; }
 inline bool elem_ok(int dtype) { return dtype == HCG_F16 || dtype == HCG_BF16 || dtype == HCG_F32; }

@@ -266,6 +266,23 @@ def test_layer_norm_grad(rows, width, dtype, pdtype):
         _close(got, wt, tol + U[pdtype] * (wt.abs() + tol) + TINY[pdtype])
 
 
+def test_layer_norm_of_more_rows_than_one_grid_dimension():
+    """More workgroups than 2^32 threads along one dimension of a grid have,
+    and offsets past 2^31."""
+    rows, width = (1 << 26) + 4100, 33
+    x = torch.arange(rows, device=DEV).remainder_(251).to(F16)[:, None].repeat(1, width)
+    x[:, ::2] += 3
+    y, mean, rstd = g.layer_norm(x)
+    m, var = 3 * 17 / 33, 9 * (17 / 33) * (16 / 33)
+    want = torch.arange(rows, device=DEV).remainder_(251).double() + m
+    assert ((mean.double() - want).abs() <= 40 * E32 * 256).all()
+    del want
+    r = 1 / math.sqrt(var + 1e-5)
+    assert ((rstd.double() - r).abs() <= 200 * E32 * 256 * r).all()
+    for c, v in ((0, (3 - m) * r), (31, -m * r), (32, (3 - m) * r)):
+        assert ((y[:, c].double() - v).abs() <= U[F16] * abs(v) + 200 * E32 * 256 * r).all()
+
+
 def test_layer_norm_grad_against_differences():
     """<dx, d> = d/dh of <dy, y(x + h d)>, and the same for the weight: central
     differences of the forward call itself in float32, summed in 64 bits."""
@@ -501,6 +518,27 @@ def test_more_tokens_than_one_piece(ignored):
     keep[::ignored] = False
     lse, loss, slack, gz, p = _head_want(x, w, y, keep)
     got = g.linear_cross_entropy_grad(x, w, torch.where(keep, y, -100), reduction="sum")
+    tol = _loss_tol(slack, lse)[keep].sum() + (t / 1024 + 30) * E32 * loss[keep].abs().sum()
+    assert abs(float(got[0]) - float(loss[keep].sum())) <= float(tol)
+    (dx, tx), (dw, tw) = _grad_tols(x, w, gz, p, slack, keep, 1.0, BF16)
+    _close(got[1], dx, tx)
+    _close(got[2], dw, tw)
+
+
+@pytest.mark.parametrize("t,v,d,ignored", [(65537, 5, 8, 3), (200003, 70, 16, 2), ((1 << 24) + 5000, 3, 8, 4)])
+def test_many_tokens(t, v, d, ignored):
+    """More tokens than one launch counts in one go, and than one piece has."""
+    x, w, y = _head(t, v, d, BF16, 12)
+    keep = torch.ones((t,), dtype=torch.bool, device=DEV)
+    keep[::ignored] = False
+    keep[70000 : min(t, 140000)] = False
+    lse, loss, slack, gz, p = _head_want(x, w, y, keep)
+    targets = torch.where(keep, y, -100)
+    got = g.linear_cross_entropy(x, w, targets)
+    for a, want in zip(got, (loss, lse)):
+        _close(a[keep], want[keep], _loss_tol(slack, lse)[keep])
+        assert (a[~keep] == 0).all()
+    got = g.linear_cross_entropy_grad(x, w, targets, reduction="sum")
     tol = _loss_tol(slack, lse)[keep].sum() + (t / 1024 + 30) * E32 * loss[keep].abs().sum()
     assert abs(float(got[0]) - float(loss[keep].sum())) <= float(tol)
     (dx, tx), (dw, tw) = _grad_tols(x, w, gz, p, slack, keep, 1.0, BF16)
