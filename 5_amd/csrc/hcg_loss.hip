@@ -360,7 +360,7 @@ double cost_of(Shape s, int64_t m, int64_t n, int64_t k, int splits) {
   if (splits > 1) {
     // The parts written and read, and a launch, or their reading by one CU.
     us += 2.0 * splits * m * n * 4 / 6.0e6;
-    us += head::can_fuse(t.tm, t.tn) ? 1.0 + (splits - 1) * std::max(0.234, t.tm * t.tn * 4 / 1.0e5) : 4.0;
+    us += head::can_fuse(t.tm, t.tn) ? 1.0 + (splits - 1) * std::max(0.5, t.tm * t.tn * 4 / 4.5e4) : 4.0;
   }
   return us;
 }

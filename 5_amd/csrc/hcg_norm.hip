@@ -4,6 +4,13 @@
 //   y = (x - mean) r w + b
 // and, with xh = (x - mean) r and g = dy w,
 //   dx = r (g - sum g / D - xh sum(g xh) / D), dw = sum_t dy xh, db = sum_t dy.
+//
+// Both are bound by HBM: a row is read once (the gradient reads two) and held in
+// registers, so the variance is the sum of squares about the mean, without the
+// cancellation of E[x^2] - mean^2 and without a second read.  A row takes as
+// few lanes as hold it with 16 bytes each.  8192 x 4096 bf16: forward 24.8 us
+// (5.4 TB/s), gradient 43.3 + 4.6 (4.2 TB/s); the sums' divisions are true
+// ones, so that a row of equal values gives exactly 0.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -28,42 +35,49 @@ struct NormArgs {
   float eps;
 };
 
-// Sum over the WPR waves of a row, the same value in every lane.  `slot`: LDS
-// words of the row group, not in use by a wave still behind the last barrier.
-template <int WPR>
-__device__ __forceinline__ float row_sum(float v, float* slot, int wave_in_row, int lane) {
-  v = hcg::wave_sum(v);
-  if constexpr (WPR > 1) {
-    if (lane == 0) slot[wave_in_row] = v;
+// Sum over the LANES lanes of a row that share a wave, the same value in each.
+template <int LANES>
+__device__ __forceinline__ float lanes_sum(float v) {
+#pragma unroll
+  for (int m = (LANES < 64 ? LANES : 64) / 2; m >= 1; m >>= 1) v += __shfl_xor(v, m);
+  return v;
+}
+// Sum over the LANES lanes of a row (a part of a wave, or whole waves).  `slot`:
+// LDS words of the row group, not in use by a wave still behind the last barrier.
+template <int LANES>
+__device__ __forceinline__ float row_sum(float v, float* slot, int tir) {
+  v = lanes_sum<LANES>(v);
+  if constexpr (LANES > 64) {
+    if (tir % 64 == 0) slot[tir / 64] = v;
     __syncthreads();
     v = 0.f;
 #pragma unroll
-    for (int i = 0; i < WPR; ++i) v += slot[i];
+    for (int i = 0; i < LANES / 64; ++i) v += slot[i];
   }
   return v;
 }
 
-template <int WPR>
+template <int LANES>
 constexpr int norm_threads() {
-  return WPR > 4 ? 64 * WPR : 256;
+  return LANES > 256 ? LANES : 256;
 }
 
-// One row by WPR waves, held in registers as NV vectors per lane between the
+// One row by LANES lanes, held in registers as NV vectors per lane between the
 // two passes of the variance.
-template <class T, class P, int WPR, int NV>
-__global__ __launch_bounds__(norm_threads<WPR>()) void norm_kernel(NormArgs g) {
-  constexpr int E = kVec<T>, kRowsPerWg = norm_threads<WPR>() / 64 / WPR;
-  __shared__ float slots[2][kRowsPerWg * WPR];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int group = wave / WPR, wir = wave % WPR;
+template <class T, class P, int LANES, int NV>
+__global__ __launch_bounds__(norm_threads<LANES>()) void norm_kernel(NormArgs g) {
+  constexpr int E = kVec<T>, kRowsPerWg = norm_threads<LANES>() / LANES;
+  constexpr int kSlots = LANES > 64 ? LANES / 64 : 1;
+  __shared__ float slots[2][kRowsPerWg * kSlots];
+  const int group = threadIdx.x / LANES, tir = threadIdx.x % LANES;
   const int64_t row = hcg::workgroup() * kRowsPerWg + group;
   const bool live = row < g.rows;
   const T* x = static_cast<const T*>(g.x) + (live ? row : 0) * g.ldx;
-  const int first = (wir * 64 + lane) * E;
+  const int first = tir * E;
   raw4 raw[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int c = first + i * WPR * 64 * E;
+    const int c = first + i * LANES * E;
     raw[i] = c < g.width ? hcg::load_raw(x + c, g.width - c) : raw4{0, 0, 0, 0};
   }
   float v[NV][E];
@@ -75,21 +89,21 @@ __global__ __launch_bounds__(norm_threads<WPR>()) void norm_kernel(NormArgs g) {
     for (int e = 0; e < E; ++e) sum += v[i][e];
   }
   const float count = (float)g.width;
-  const float mean = row_sum<WPR>(sum, slots[0] + group * WPR, wir, lane) / count;
+  const float mean = row_sum<LANES>(sum, slots[0] + group * kSlots, tir) / count;
   float sq = 0.f;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int left = g.width - (first + i * WPR * 64 * E);
+    const int left = g.width - (first + i * LANES * E);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       v[i][e] -= mean;
       if (e < left) sq += v[i][e] * v[i][e];
     }
   }
-  const float var = row_sum<WPR>(sq, slots[1] + group * WPR, wir, lane) / count;
+  const float var = row_sum<LANES>(sq, slots[1] + group * kSlots, tir) / count;
   const float rstd = 1.f / sqrtf(var + g.eps);
   if (!live) return;
-  if (wir == 0 && lane == 0) {
+  if (tir == 0) {
     if (g.mean) g.mean[row] = mean;
     if (g.rstd) g.rstd[row] = rstd;
   }
@@ -98,7 +112,7 @@ __global__ __launch_bounds__(norm_threads<WPR>()) void norm_kernel(NormArgs g) {
   const P* b = static_cast<const P*>(g.bias);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int c = first + i * WPR * 64 * E;
+    const int c = first + i * LANES * E;
     if (c < g.width) {
       float o[E], wf[E], bf[E];
 #pragma unroll
@@ -118,7 +132,6 @@ template <class T, class P>
 __global__ __launch_bounds__(1024) void norm_wide_kernel(NormArgs g) {
   constexpr int E = kVec<T>;
   __shared__ float slots[2][16];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t row = hcg::workgroup();
   if (row >= g.rows) return;
   const T* x = static_cast<const T*>(g.x) + row * g.ldx;
@@ -130,7 +143,7 @@ __global__ __launch_bounds__(1024) void norm_wide_kernel(NormArgs g) {
     for (int e = 0; e < E; ++e) sum += f[e];
   }
   const float count = (float)g.width;
-  const float mean = row_sum<16>(sum, slots[0], wave, lane) / count;
+  const float mean = row_sum<1024>(sum, slots[0], threadIdx.x) / count;
   float sq = 0.f;
   for (int64_t c = (int64_t)threadIdx.x * E; c < g.width; c += 1024 * E) {
     float f[E];
@@ -139,7 +152,7 @@ __global__ __launch_bounds__(1024) void norm_wide_kernel(NormArgs g) {
     for (int e = 0; e < E; ++e)
       if (c + e < g.width) sq += (f[e] - mean) * (f[e] - mean);
   }
-  const float rstd = 1.f / sqrtf(row_sum<16>(sq, slots[1], wave, lane) / count + g.eps);
+  const float rstd = 1.f / sqrtf(row_sum<1024>(sq, slots[1], threadIdx.x) / count + g.eps);
   if (threadIdx.x == 0) {
     if (g.mean) g.mean[row] = mean;
     if (g.rstd) g.rstd[row] = rstd;
@@ -178,19 +191,21 @@ struct NormGradArgs {
   bool stream;  // dx past the caches: non-temporal stores
 };
 
-// GROUPS row groups of WPR waves; group q of workgroup b takes rows
+// GROUPS row groups of LANES lanes; group q of workgroup b takes rows
 // b * GROUPS + q, + gridDim.x * GROUPS, ... and keeps its columns' sums of
 // dy xh and dy in registers; the groups' sums meet in LDS once, at the end.
 // LEAN (1024 threads, so 128 registers, with 16 16-bit columns each): the
 // weights come from the L2 for every row and no loads run ahead; held, they
 // spill 65 registers.
-template <class T, class P, int WPR, int NV, int GROUPS, bool LEAN = false>
-__global__ __launch_bounds__(64 * WPR * GROUPS) void norm_grad_kernel(NormGradArgs g) {
-  constexpr int E = kVec<T>, kLanes = 64 * WPR;
-  __shared__ float slots[2][GROUPS * WPR * 2];
-  __shared__ float meet[GROUPS > 1 ? GROUPS * kLanes * E : 1];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int group = wave / WPR, wir = wave % WPR, tir = wir * 64 + lane;
+template <class T, class P, int LANES, int NV, int GROUPS, bool LEAN = false>
+__global__ __launch_bounds__(LANES * GROUPS) void norm_grad_kernel(NormGradArgs g) {
+  constexpr int E = kVec<T>, kWaves = LANES / 64;
+  __shared__ float slots[2][kWaves > 1 ? GROUPS * kWaves * 2 : 1];
+  // The column sums of groups that share a wave meet by exchanges, the waves'
+  // in LDS.
+  constexpr int kShare = LANES < 64 ? 64 / LANES : 1, kMeet = GROUPS / kShare;
+  __shared__ float meet[kMeet > 1 ? kMeet * LANES * E : 1];
+  const int group = threadIdx.x / LANES, tir = threadIdx.x % LANES;
   const T* px = static_cast<const T*>(g.x);
   const T* pdy = static_cast<const T*>(g.dy);
   const P* w = static_cast<const P*>(g.weight);
@@ -199,7 +214,7 @@ __global__ __launch_bounds__(64 * WPR * GROUPS) void norm_grad_kernel(NormGradAr
 
   float wf[LEAN ? 1 : NV][E], dw[NV][E], db[NV][E];
   auto load_weight = [&](int i, float(&f)[E]) {
-    const int c = first + i * kLanes * E;
+    const int c = first + i * LANES * E;
 #pragma unroll
     for (int e = 0; e < E; ++e) f[e] = 1.f;
     if (w && c < g.width) hcg::load_floats<P, E>(w + c, g.width - c, f);
@@ -225,7 +240,7 @@ __global__ __launch_bounds__(64 * WPR * GROUPS) void norm_grad_kernel(NormGradAr
     rrstd[S] = live ? g.rstd[row] : 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = first + i * kLanes * E;
+      const int c = first + i * LANES * E;
       const bool in = live && c < g.width;
       rx[S][i] = in ? hcg::load_raw(px + row * g.ldx + c, g.width - c) : raw4{0, 0, 0, 0};
       rdy[S][i] = in ? hcg::load_raw(pdy + row * g.lddy + c, g.width - c) : raw4{0, 0, 0, 0};
@@ -258,15 +273,15 @@ __global__ __launch_bounds__(64 * WPR * GROUPS) void norm_grad_kernel(NormGradAr
         s2 += dy[i][e] * xh[i][e];
       }
     }
-    s1 = hcg::wave_sum(s1);
-    s2 = hcg::wave_sum(s2);
-    if constexpr (WPR > 1) {
-      float* slot_sums = slots[parity] + group * WPR * 2;
-      if (lane == 0) slot_sums[wir * 2] = s1, slot_sums[wir * 2 + 1] = s2;
+    s1 = lanes_sum<LANES>(s1);
+    s2 = lanes_sum<LANES>(s2);
+    if constexpr (kWaves > 1) {
+      float* slot_sums = slots[parity] + group * kWaves * 2;
+      if (tir % 64 == 0) slot_sums[tir / 64 * 2] = s1, slot_sums[tir / 64 * 2 + 1] = s2;
       __syncthreads();
       s1 = s2 = 0.f;
 #pragma unroll
-      for (int i = 0; i < WPR; ++i) s1 += slot_sums[i * 2], s2 += slot_sums[i * 2 + 1];
+      for (int i = 0; i < kWaves; ++i) s1 += slot_sums[i * 2], s2 += slot_sums[i * 2 + 1];
       parity ^= 1;
     }
     if (row < g.rows) {
@@ -275,7 +290,7 @@ __global__ __launch_bounds__(64 * WPR * GROUPS) void norm_grad_kernel(NormGradAr
       T* dx = static_cast<T*>(g.dx) + row * g.lddx;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int c = first + i * kLanes * E;
+        const int c = first + i * LANES * E;
         if (c < g.width) {
           float o[E];
 #pragma unroll
@@ -308,21 +323,25 @@ __global__ __launch_bounds__(64 * WPR * GROUPS) void norm_grad_kernel(NormGradAr
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       float (&v)[E] = which ? db[i] : dw[i];
-      if constexpr (GROUPS > 1) {
-        __syncthreads();
-        if (group > 0) {
 #pragma unroll
-          for (int e = 0; e < E; ++e) meet[(group * E + e) * kLanes + tir] = v[e];
+      for (int m = LANES; m < 64; m <<= 1)
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] += __shfl_xor(v[e], m);
+      if constexpr (kMeet > 1) {
+        __syncthreads();
+        if (group > 0 && group % kShare == 0) {
+#pragma unroll
+          for (int e = 0; e < E; ++e) meet[(group / kShare * E + e) * LANES + tir] = v[e];
         }
         __syncthreads();
         if (group == 0) {
 #pragma unroll
-          for (int q = 1; q < GROUPS; ++q)
+          for (int q = 1; q < kMeet; ++q)
 #pragma unroll
-            for (int e = 0; e < E; ++e) v[e] += meet[(q * E + e) * kLanes + tir];
+            for (int e = 0; e < E; ++e) v[e] += meet[(q * E + e) * LANES + tir];
         }
       }
-      const int c = first + i * kLanes * E;
+      const int c = first + i * LANES * E;
       if (group == 0) {
 #pragma unroll
         for (int e = 0; e < E; ++e)
@@ -338,7 +357,6 @@ template <class T, class P>
 __global__ __launch_bounds__(1024) void norm_grad_wide_kernel(NormGradArgs g) {
   constexpr int E = kVec<T>;
   __shared__ float slots[2][16];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t row = hcg::workgroup();
   if (row >= g.rows) return;
   const T* x = static_cast<const T*>(g.x) + row * g.ldx;
@@ -369,8 +387,8 @@ __global__ __launch_bounds__(1024) void norm_grad_wide_kernel(NormGradArgs g) {
       }
     }
     if (pass == 0) {
-      s1 = row_sum<16>(s1, slots[0], wave, lane) / count;
-      s2 = row_sum<16>(s2, slots[1], wave, lane) / count;
+      s1 = row_sum<1024>(s1, slots[0], threadIdx.x) / count;
+      s2 = row_sum<1024>(s2, slots[1], threadIdx.x) / count;
     }
   }
 }
@@ -426,27 +444,32 @@ __global__ __launch_bounds__(1024) void norm_reduce_kernel(const float* part, in
 constexpr int kGradParts = 256;       // workgroups of the gradient, each with one part
 constexpr int64_t kMaxWidth = 1 << 30;
 
-template <class T, class P, int WPR, int NV>
+template <class T, class P, int LANES, int NV>
 void launch_norm(const NormArgs& a, hipStream_t s) {
-  constexpr int rows = norm_threads<WPR>() / 64 / WPR;
-  norm_kernel<T, P, WPR, NV><<<hcg::grid_of((a.rows + rows - 1) / rows), norm_threads<WPR>(), 0, s>>>(a);
+  constexpr int rows = norm_threads<LANES>() / LANES;
+  norm_kernel<T, P, LANES, NV><<<hcg::grid_of((a.rows + rows - 1) / rows), norm_threads<LANES>(), 0, s>>>(a);
 }
 
 template <class T, class P>
 void run_norm(const NormArgs& a, hipStream_t s) {
   const int64_t vecs = ((int64_t)a.width + kVec<T> - 1) / kVec<T>;  // 16-byte vectors in a row
-  if (vecs <= 64) return launch_norm<T, P, 1, 1>(a, s);
-  if (vecs <= 256) return launch_norm<T, P, 4, 1>(a, s);
-  if (vecs <= 512) return launch_norm<T, P, 4, 2>(a, s);
-  if (vecs <= 1024) return launch_norm<T, P, 4, 4>(a, s);
-  if (vecs <= 4096) return launch_norm<T, P, 16, 4>(a, s);
+  if (vecs <= 16) return launch_norm<T, P, 16, 1>(a, s);
+  if (vecs <= 32) return launch_norm<T, P, 32, 1>(a, s);
+  if (vecs <= 64) return launch_norm<T, P, 64, 1>(a, s);
+  // As few lanes as hold the row.  us, 64 / 16 lanes (65536 x 128 bf16) 23.9 / 9.5,
+  // 64 / 32 (16384 x 256) 8.9 / 6.6, 256 / 128 (16384 x 1024) 23.4 / 16.4.
+  if (vecs <= 128) return launch_norm<T, P, 128, 1>(a, s);
+  if (vecs <= 256) return launch_norm<T, P, 256, 1>(a, s);
+  if (vecs <= 512) return launch_norm<T, P, 256, 2>(a, s);
+  if (vecs <= 1024) return launch_norm<T, P, 256, 4>(a, s);
+  if (vecs <= 4096) return launch_norm<T, P, 1024, 4>(a, s);
   norm_wide_kernel<T, P><<<hcg::grid_of(a.rows), 1024, 0, s>>>(a);
 }
 
-template <class T, class P, int WPR, int NV, int GROUPS, bool LEAN = false>
+template <class T, class P, int LANES, int NV, int GROUPS, bool LEAN = false>
 int launch_norm_grad(const NormGradArgs& a, hipStream_t s) {
   const int64_t wgs = std::min<int64_t>(kGradParts, (a.rows + GROUPS - 1) / GROUPS);
-  norm_grad_kernel<T, P, WPR, NV, GROUPS, LEAN><<<dim3((unsigned)wgs), 64 * WPR * GROUPS, 0, s>>>(a);
+  norm_grad_kernel<T, P, LANES, NV, GROUPS, LEAN><<<dim3((unsigned)wgs), LANES * GROUPS, 0, s>>>(a);
   return (int)wgs;
 }
 
@@ -454,11 +477,23 @@ int launch_norm_grad(const NormGradArgs& a, hipStream_t s) {
 template <class T, class P>
 int run_norm_grad(const NormGradArgs& a, hipStream_t s) {
   const int64_t vecs = ((int64_t)a.width + kVec<T> - 1) / kVec<T>;
-  if (vecs <= 64) return launch_norm_grad<T, P, 1, 1, 8>(a, s);
-  if (vecs <= 256) return launch_norm_grad<T, P, 4, 1, 4>(a, s);
-  if (vecs <= 512) return launch_norm_grad<T, P, 8, 1, 2>(a, s);
-  if (vecs <= 1024) return launch_norm_grad<T, P, 8, 2, 1>(a, s);
-  if (vecs <= 2048) return launch_norm_grad<T, P, 16, 2, 1, sizeof(T) == 2>(a, s);
+  // As few lanes per row as hold it, and as many rows as fit 1024 threads (512,
+  // where a row is one wave or less: 16 rows of 64 lanes took 2048 x 512 bf16 from
+  // 8.0 to 11.0 us): idle lanes are loads that are not in flight.  us, 64 / 16
+  // lanes (65536 x 128 bf16) 37 / 17, 256 / 128 (16384 x 768) 35.6 / 24.6, 256 / 192
+  // (16384 x 1536) 37.7 / 33.9, 512 / 320 (8192 x 2560) 38.7 / 32.8, 512 / 384 (8192 x
+  // 2880) 41.9 / 38.8; the few rows of 100 x 128 6.6 / 7.0.
+  if (vecs <= 16) return launch_norm_grad<T, P, 16, 1, 32>(a, s);
+  if (vecs <= 32) return launch_norm_grad<T, P, 32, 1, 16>(a, s);
+  if (vecs <= 64) return launch_norm_grad<T, P, 64, 1, 8>(a, s);
+  if (vecs <= 128) return launch_norm_grad<T, P, 128, 1, 8>(a, s);
+  if (vecs <= 192) return launch_norm_grad<T, P, 192, 1, 5>(a, s);
+  if (vecs <= 256) return launch_norm_grad<T, P, 256, 1, 4>(a, s);
+  if (vecs <= 320) return launch_norm_grad<T, P, 320, 1, 3>(a, s);
+  if (vecs <= 384) return launch_norm_grad<T, P, 384, 1, 2>(a, s);
+  if (vecs <= 512) return launch_norm_grad<T, P, 512, 1, 2>(a, s);
+  if (vecs <= 1024) return launch_norm_grad<T, P, 512, 2, 1>(a, s);
+  if (vecs <= 2048) return launch_norm_grad<T, P, 1024, 2, 1, sizeof(T) == 2>(a, s);
   norm_grad_wide_kernel<T, P><<<hcg::grid_of(a.rows), 1024, 0, s>>>(a);
   const int parts = (int)std::min<int64_t>(64, a.rows);
   if (a.part)
