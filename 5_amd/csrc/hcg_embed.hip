@@ -1,7 +1,9 @@
 // hcg_embed.hip -- the embedding lookup and its gradient (include/hcg_lm.h).
 //
 // Forward: out[i] = scale * table[ids[i]], a gather of whole rows; bound by
-// HBM.
+// HBM.  Every thread has four 16-byte loads in flight, whatever the row's width:
+// the rows of a workgroup are one range of vectors.  8192 of 65536 x 4096 bf16
+// 19.1 us, of which the writes (67 MB) alone are 13.
 //
 // Gradient: grad[v] = scale * sum of dy[i] over ids[i] == v.  Each workgroup
 // owns a few rows of the table.  It reads all ids (64 KB for 8192 tokens, from
@@ -13,6 +15,8 @@
 // workgroup busy long after the others, so the tokens of rows with more than
 // kLong of them are left in a list, in the order of (row, i), which a second
 // launch sums in windows of kWindow entries and a third adds up by rows.
+// Bound by the table's writes, most of them zeros: a pass over 65536 x 4096 bf16
+// with 8192 tokens 115 us for 537 MB (and 67 MB read).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -116,6 +120,10 @@ constexpr int kOneLaunch = 2048;
 constexpr int kBucketTokens = 8192;
 constexpr int kBuckets = 64;
 
+// Runs of empty rows of up to so many vectors are filled by a wave each, longer
+// ones by the workgroup.
+constexpr int kShortRun = 64 * 4;
+
 struct EmbedGradArgs {
   const void* dy;
   const void* ids;
@@ -165,6 +173,22 @@ __device__ __forceinline__ void store_grad(G* p, const float (&f)[kVec<T>], floa
         hcg::store_raw(p + h * EG, hcg::pack<G>(o), EG);
     }
   }
+}
+
+// n zeros from p on by `threads` threads (64 or more), this one number `thread`:
+// whole 128-byte lines as non-temporal vectors, the elements before and after
+// them one by one.
+template <class G>
+__device__ __forceinline__ void fill_zeros(G* p, int64_t n, int thread, int threads) {
+  constexpr int kLine = 128 / (int)sizeof(G);
+  const int64_t to_line = (kLine - (int)(reinterpret_cast<uintptr_t>(p) % 128) / (int)sizeof(G)) % kLine;
+  const int head = (int)min(n, to_line);
+  if (thread < head) p[thread] = (G)0.f;
+  p += head;
+  const int64_t vecs = (n - head) / kLine * 8, tail = n - head - vecs * kVec<G>;
+  for (int64_t i = thread; i < vecs; i += threads)
+    hcg::store_raw<true>(p + i * kVec<G>, raw4{0, 0, 0, 0}, kVec<G>);
+  if (thread < tail) p[vecs * kVec<G> + thread] = (G)0.f;
 }
 
 // A row as whole vectors and, one by one, the elements past them: items
@@ -262,7 +286,8 @@ __device__ __forceinline__ void find_ids(const I* ids, int from, int to, int64_t
 // Parts the tokens: workgroup b takes those of its bucket_rows rows of the
 // table, in order, to the places after all of lower rows.  The finds wait in
 // LDS until their place is known; where they do not fit (a hot row) the ids are
-// scanned again, from the L2.
+// scanned again, from the L2.  Bound by the latency of reading all ids once by
+// each of 64 workgroups (32768 tokens: about 10 us).
 constexpr int kPartThreads = 1024;
 constexpr int kPartWaves = kPartThreads / 64;
 constexpr int kPartList = 512;  // finds per wave
@@ -417,16 +442,36 @@ __global__ __launch_bounds__(kGradThreads, 8) void embed_grad_kernel(EmbedGradAr
     for (int j = below + total + tid; j < g.n; j += kGradThreads) g.row[j] = -1;
   __syncthreads();
 
-  // Every row that is not long, its items over the threads.
+  // The rows without tokens: neighbours together, where the gradient has no
+  // gaps, so that lines are written whole whatever the width, and past the
+  // caches.  us of a pass, row by row / so / so without non-temporal stores: 8192
+  // tokens into 65536 x 4096 bf16 151 / 115 / 148, 200 into 36696 x 3400 f32 117 /
+  // 100 / 112, 1353 into 24661 x 1367 f32 41.3 / 44.5 / 41.6, 2048 into 13384 x 128
+  // bf16 11.7 / 12.7 / 13.0.
   const T* dy = static_cast<const T*>(g.dy);
   G* grad = static_cast<G*>(g.grad);
+  uint64_t empty = __ballot(lane < rows && count[lane] == 0);
+  for (int run = 0; empty; ++run) {
+    const int first = __ffsll((unsigned long long)empty) - 1;
+    const uint64_t past = ~(empty >> first);  // (0: all 64 rows)
+    const int len = g.ldg != g.width ? 1 : past ? __ffsll((unsigned long long)past) - 1 : 64;
+    G* p = grad + (lo + first) * g.ldg;
+    const int64_t n = (int64_t)len * g.width;
+    if (n > kShortRun * kVec<G>)
+      fill_zeros<G>(p, n, tid, kGradThreads);
+    else if (run % kGradWaves == wave)
+      fill_zeros<G>(p, n, lane, 64);
+    empty &= first + len >= 64 ? 0 : ~(uint64_t)0 << (first + len);
+  }
+
+  // Every row that is neither empty nor long, its items over the threads.
   const Items it(g.width, E);
   const auto entry = [&](int j) { return ONE || fits ? grouped[j] : g.token[below + j]; };
   const int work = rows * it.items;
   for (int at = tid; at < work; at += kGradThreads) {
     const int r = at / it.items, i = at - r * it.items;
     const int n = count[r], first = start[r];
-    if (n > kLong) continue;
+    if (n == 0 || n > kLong) continue;
     const auto one_item = [&](auto whole, int c) {
       constexpr bool WHOLE = decltype(whole)::value;
       float sum[E] = {};
@@ -493,7 +538,9 @@ __device__ __forceinline__ Window window_of(const EmbedGradArgs& g, int from, in
 }
 
 // Window blockIdx.x of the lists, items blockIdx.y * 256 ...: the sum of
-// each run of one long row in it.
+// each run of one long row in it.  A run is at most 32 rows by one thread per
+// 16 bytes, eight loads in flight: bound by their latency where a few words make
+// up most of the windows (8192 tokens x 4096 bf16, a third in long rows: 14 us).
 template <class T>
 __global__ __launch_bounds__(256) void embed_window_kernel(EmbedGradArgs g) {
   constexpr int E = kVec<T>;
@@ -531,7 +578,8 @@ __global__ __launch_bounds__(256) void embed_window_kernel(EmbedGradArgs g) {
 }
 
 // The long rows that start in window blockIdx.x, columns blockIdx.y * 256 ...:
-// their windows' sums, in order.
+// their windows' sums, in order (6 us at the size above: one chain of float32
+// loads, 16 in flight, of the most frequent row's windows).
 template <class G>
 __global__ __launch_bounds__(256) void embed_long_kernel(EmbedGradArgs g) {
   const int from = blockIdx.x * kWindow, n = min(kWindow, g.n - from), lane = threadIdx.x & 63;
