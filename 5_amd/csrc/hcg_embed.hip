@@ -540,7 +540,7 @@ __device__ __forceinline__ Window window_of(const EmbedGradArgs& g, int from, in
 // Window blockIdx.x of the lists, items blockIdx.y * 256 ...: the sum of
 // each run of one long row in it.  A run is at most 32 rows by one thread per
 // 16 bytes, eight loads in flight: bound by their latency where a few words make
-// up most of the windows (8192 tokens x 4096 bf16, a third in long rows: 14 us).
+// up most of the windows (8192 tokens x 4096 bf16, a third in long rows: 8 us).
 template <class T>
 __global__ __launch_bounds__(256) void embed_window_kernel(EmbedGradArgs g) {
   constexpr int E = kVec<T>;
@@ -578,7 +578,7 @@ __global__ __launch_bounds__(256) void embed_window_kernel(EmbedGradArgs g) {
 }
 
 // The long rows that start in window blockIdx.x, columns blockIdx.y * 256 ...:
-// their windows' sums, in order (6 us at the size above: one chain of float32
+// their windows' sums, in order (7 us at the size above: one chain of float32
 // loads, 16 in flight, of the most frequent row's windows).
 template <class G>
 __global__ __launch_bounds__(256) void embed_long_kernel(EmbedGradArgs g) {
