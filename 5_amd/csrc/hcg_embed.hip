@@ -107,9 +107,13 @@ constexpr int kWindow = 32;
 // Runs of long rows in one window: those that lie inside it have more than
 // kLong entries each, and one more may enter and one leave.
 constexpr int kRuns = kWindow / (kLong + 1) + 2;
-// Up to so many tokens of rows of at most half as many items as threads, a
-// workgroup sums its long rows too, in parts that meet in LDS: then one launch
-// does it all.
+// Few tokens of narrow rows: a workgroup sums its long rows too, in parts that
+// meet in LDS, and one launch does it all.  Up to kOneLaunch tokens where a row has
+// at most half as many items as there are threads, up to twice as many, by lists
+// twice as long (54 KB of LDS: 3 workgroups per CU, not 4), where it has at most a
+// quarter.  us, one launch / three: 3160 into 5065 x 131 f32 14.2 / 24.1, 2273 into
+// 6920 x 463 f32 16.9 / 25.1, but 3720 into 731 x 1336 f16 (167 items) 28.5 / 24.0;
+// long lists / short ones: 2048 into 13384 x 128 bf16 15.4 / 12.6.
 constexpr int kOneLaunch = 2048;
 // Past so many tokens they are first parted by ranges of the table (a launch of
 // kBuckets workgroups, stable), and a workgroup scans its range's tokens only:
@@ -332,14 +336,15 @@ __global__ __launch_bounds__(kPartThreads) void embed_bucket_kernel(EmbedGradArg
   }
 }
 
-// ONE: no lists are kept (g.token is null), the workgroup sums its long rows too.
+// ONE: no lists are kept (g.token is null), the workgroup sums its long rows too;
+// the finds per wave that LDS has room for.
 // PARTED: the tokens come from the workgroup's bucket (I is int).
-template <class T, class G, class I, bool ONE, bool PARTED>
-__global__ __launch_bounds__(kGradThreads, 8) void embed_grad_kernel(EmbedGradArgs g) {
-  constexpr int E = kVec<T>;
+template <class T, class G, class I, int ONE, bool PARTED>
+__global__ __launch_bounds__(kGradThreads, ONE > kListPerWave ? 6 : 8) void embed_grad_kernel(EmbedGradArgs g) {
+  constexpr int E = kVec<T>, kList = ONE ? ONE : kListPerWave;
   __shared__ float meet[ONE ? kGradThreads * E : 1];
-  __shared__ int found[kGradWaves * kListPerWave], grouped[kGradWaves * kListPerWave];
-  __shared__ uint8_t found_row[kGradWaves * kListPerWave];
+  __shared__ int found[kGradWaves * kList], grouped[kGradWaves * kList];
+  __shared__ uint8_t found_row[kGradWaves * kList];
   __shared__ int wave_found[kGradWaves], wave_below[kGradWaves];
   __shared__ int count[kMaxRows], start[kMaxRows];
   const int tid = threadIdx.x, lane = tid & 63;
@@ -364,9 +369,9 @@ __global__ __launch_bounds__(kGradThreads, 8) void embed_grad_kernel(EmbedGradAr
     if (lane == 0) wave_found[wave] = finds, wave_below[wave] = below;
   };
   scan([&](int at, int i, int r) {
-    if (at < kListPerWave) {
-      found[wave * kListPerWave + at] = i;
-      found_row[wave * kListPerWave + at] = (uint8_t)r;
+    if (at < kList) {
+      found[wave * kList + at] = i;
+      found_row[wave * kList + at] = (uint8_t)r;
     }
   });
   __syncthreads();
@@ -377,7 +382,7 @@ __global__ __launch_bounds__(kGradThreads, 8) void embed_grad_kernel(EmbedGradAr
     if (w < wave) before += wave_found[w];
     total += wave_found[w];
     below += wave_below[w];
-    fits = fits && wave_found[w] <= kListPerWave;
+    fits = fits && wave_found[w] <= kList;
   }
   if (!ONE && !fits) {
     // (wave_found and wave_below are written again with the same values)
@@ -391,8 +396,8 @@ __global__ __launch_bounds__(kGradThreads, 8) void embed_grad_kernel(EmbedGradAr
   // Find number j of wave w.
   auto find = [&](int w, int off, int j, int& i) -> int {
     if (ONE || fits) {
-      i = found[w * kListPerWave + j];
-      return found_row[w * kListPerWave + j];
+      i = found[w * kList + j];
+      return found_row[w * kList + j];
     }
     i = g.found[below + off + j];
     return g.found_row[below + off + j];
@@ -618,7 +623,8 @@ int64_t items_of(int dtype, int64_t width) {
   return width / e + width % e;
 }
 bool one_launch(int64_t n, int64_t items) {
-  return n <= kLong || (n <= kOneLaunch && items <= kGradThreads / 2);
+  return n <= kLong || (n <= kOneLaunch && items <= kGradThreads / 2) ||
+         (n <= 2 * kOneLaunch && items <= kGradThreads / 4);
 }
 int64_t windows_of(int64_t n) { return (n + kWindow - 1) / kWindow; }
 int64_t round256(int64_t b) { return (b + 255) / 256 * 256; }
@@ -637,15 +643,18 @@ template <class T, class G, class I>
 void run_embed_grad(const EmbedGradArgs& a, hipStream_t s) {
   const dim3 grid((unsigned)((a.vocab + a.rows - 1) / a.rows));
   if (a.token == nullptr) {
-    embed_grad_kernel<T, G, I, true, false><<<grid, kGradThreads, 0, s>>>(a);
+    if (a.n <= kOneLaunch)
+      embed_grad_kernel<T, G, I, kListPerWave, false><<<grid, kGradThreads, 0, s>>>(a);
+    else
+      embed_grad_kernel<T, G, I, 2 * kListPerWave, false><<<grid, kGradThreads, 0, s>>>(a);
     return;
   }
   if (a.bucket) {
     const dim3 buckets((unsigned)((a.vocab + a.bucket_rows - 1) / a.bucket_rows));
     embed_bucket_kernel<I><<<buckets, kPartThreads, 0, s>>>(a);
-    embed_grad_kernel<T, G, int32_t, false, true><<<grid, kGradThreads, 0, s>>>(a);
+    embed_grad_kernel<T, G, int32_t, 0, true><<<grid, kGradThreads, 0, s>>>(a);
   } else {
-    embed_grad_kernel<T, G, I, false, false><<<grid, kGradThreads, 0, s>>>(a);
+    embed_grad_kernel<T, G, I, 0, false><<<grid, kGradThreads, 0, s>>>(a);
   }
   const unsigned windows = (unsigned)windows_of(a.n);
   embed_window_kernel<T><<<dim3(windows, (unsigned)((a.items + 255) / 256)), 256, 0, s>>>(a);

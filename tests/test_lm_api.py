@@ -54,7 +54,7 @@ def test_embedding_arguments(change, match):
     ({"ws": P + 8}, "workspace")])
 def test_embedding_grad_arguments(change, match):
     lib = _native.load()
-    a = dict(dtype=BF16, dy=P, lddy=8, n=3000, width=8, id_bytes=8, ids=P, vocab=5, padding=-1, scale=1.0,
+    a = dict(dtype=BF16, dy=P, lddy=8, n=5000, width=8, id_bytes=8, ids=P, vocab=5, padding=-1, scale=1.0,
              grad_dtype=BF16, grad=P, ldg=8, ws=P, ws_bytes=1 << 20, stream=None)
     a.update(change)
     _refused(lib.hcg_embedding_grad(*a.values()), match)
@@ -114,7 +114,9 @@ def test_workspace_sizes():
     assert lib.hcg_embedding_grad_workspace(BF16, 17, 1000, 1 << 20) > 0
     assert lib.hcg_embedding_grad_workspace(BF16, 2048, 1000, 2048) == 0  # one launch
     assert lib.hcg_embedding_grad_workspace(F32, 2048, 1000, 2048) > 0
-    assert lib.hcg_embedding_grad_workspace(BF16, 2049, 1000, 64) > 0
+    assert lib.hcg_embedding_grad_workspace(BF16, 4096, 1000, 1024) == 0
+    assert lib.hcg_embedding_grad_workspace(BF16, 2049, 1000, 1032) > 0
+    assert lib.hcg_embedding_grad_workspace(BF16, 4097, 1000, 64) > 0
     assert lib.hcg_embedding_grad_workspace(BF16, 0, 0, 0) == 0
     assert lib.hcg_layer_norm_grad_workspace(0, 64) == 0
     size = lib.hcg_linear_cross_entropy_workspace

@@ -153,6 +153,27 @@ def test_embedding_grad_padding_row_and_view():
     assert torch.equal(g.embedding_grad(dy, tokens, 40, padding_idx=6, out=t), got)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("n", [2047, 2048, 2049, 3001, 4095, 4096, 4097])
+@pytest.mark.parametrize("vocab,width,spread", [(1, 33, "even"), (61, 515, "zipf"), (9000, 131, "zipf"), (500, 64, "one")])
+def test_embedding_grad_at_the_lists_sizes(n, vocab, width, spread, dtype):
+    """Token counts at which the lists in LDS and the number of launches
+    change, with all tokens in one row, one row per token and between."""
+    gen = _gen(n + vocab)
+    u = torch.rand((n,), generator=gen, device=DEV, dtype=torch.float64)
+    if spread == "even":
+        tokens = (u * vocab).long().clamp_(max=vocab - 1)
+    elif spread == "one":
+        tokens = torch.where(u < 0.97, vocab // 2, (u * 31337).long() % vocab)
+    else:
+        tokens = ((torch.exp(u * math.log(vocab + 1.0)) - 1).long() * 7919 % vocab).clamp_(0, vocab - 1)
+    dy = _randn(gen, (n, width), dtype)
+    got = _twice(lambda: g.embedding_grad(dy, tokens, vocab))
+    want, mag, count = _embedding_grad_want(dy, tokens, vocab, 1.0)
+    _close(got, want, (count + 2) * E32 * mag + U[dtype] * want.abs() + TINY[dtype])
+    assert (got[(count[:, 0] == 0)] == 0).all()
+
+
 def test_embedding_grad_more_of_one_range_than_lds_lists():
     """Several rows of one workgroup's range with more tokens than its lists hold."""
     gen = _gen(9)
