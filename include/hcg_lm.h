@@ -39,7 +39,8 @@ int hcg_embedding(int dtype, const void* table, int64_t ldt, int64_t vocab, int6
  * vocab (rows without an i, and row padding_idx, are zeros; padding_idx < 0:
  * none; an id outside [0, vocab) reaches no row).  dy is n x width of dtype,
  * grad vocab x width of grad_dtype (dtype or HCG_F32).  The sum of a row is
- * float32 over ascending i, in fixed pieces where it is long. */
+ * float32 over ascending i, in fixed pieces where it is long.  n and vocab are
+ * below 2^28, width below 2^23. */
 int64_t hcg_embedding_grad_workspace(int dtype, int64_t n, int64_t vocab, int64_t width);
 int hcg_embedding_grad(int dtype, const void* dy, int64_t ldy, int64_t n, int64_t width, int id_bytes,
                        const void* ids, int64_t vocab, int64_t padding_idx, float scale, int grad_dtype,
@@ -68,7 +69,8 @@ int hcg_layer_norm_grad(int dtype, const void* dy, int64_t lddy, const void* x, 
  * both 0 where target == ignore_index (such a row may hold anything, NaN too).
  * A target outside [0, vocab) that is not ignore_index gives a NaN loss (and
  * no one-hot term in a gradient).  The workspace's size depends on the
- * weight's alignment: rows that are not 16-byte aligned are copied there. */
+ * weight's alignment: rows that are not 16-byte aligned are copied there.
+ * tokens are below 2^26, vocab and width below 4,000,000 - 8. */
 int64_t hcg_linear_cross_entropy_workspace(int64_t tokens, int64_t vocab, int64_t width, const void* weight,
                                            int64_t ldw, int grad);
 int hcg_linear_cross_entropy(int dtype, const void* x, int64_t ldx, int64_t tokens, const void* weight, int64_t ldw,
