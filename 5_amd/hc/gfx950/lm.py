@@ -295,7 +295,8 @@ def layer_norm_grad(dy: Any, x: Any, mean: Any, rstd: Any, weight: Any | None = 
     """The gradients of :func:`layer_norm`, ``(dx, dweight, dbias)``, from
     ``dy`` (x's shape and type) and what the forward call returned.  dweight
     and dbias have the type of ``weight`` (x's without one), or
-    ``param_dtype``: x's type or float32."""
+    ``param_dtype``: x's type or float32.  dx is of ``weight`` as it is,
+    whatever ``param_dtype``."""
     if param_dtype is None:
         r = _fast("layer_norm_grad", dy, x, mean, rstd, weight)
         if r is not None:
@@ -321,21 +322,26 @@ def layer_norm_grad(dy: Any, x: Any, mean: Any, rstd: Any, weight: Any | None = 
         param_dtype = x.dtype if w is None else w.dtype
     elif param_dtype is not x.dtype and param_dtype is not torch.float32:
         raise LaunchError(f"param_dtype must be {_name(x.dtype)} or float32, got {_name(param_dtype)}")
+    # The call has one type for the weight and its gradients: the wider of the
+    # two, so that the weight is never rounded, and the float32 sums are rounded
+    # to param_dtype once, below.
+    call_dtype = param_dtype
     if w is not None and w.dtype is not param_dtype:
-        w = w.to(param_dtype)
+        call_dtype = torch.float32
+        w = w.float()
     device = x.device
     dx = torch.empty(x.shape, dtype=x.dtype, device=device)
-    params = torch.empty((2, width), dtype=param_dtype, device=device)
-    dweight, dbias = params[0], params[1]
+    params = torch.empty((2, width), dtype=call_dtype, device=device)
     lib = _native.lib()
     need = lib.hcg_layer_norm_grad_workspace(n, width)
     ws = _workspace(torch, need, device)
     base = params.data_ptr()
     mean, rstd = mean.contiguous(), rstd.contiguous()
     _call(torch, index, lib.hcg_layer_norm_grad, "hcg_layer_norm_grad", code, _ptr(grads), _ld(grads), _ptr(rows),
-          _ld(rows), n, width, _ptr(mean), _ptr(rstd), _CODES[param_dtype], _ptr(w), _ptr(dx), width, base,
+          _ld(rows), n, width, _ptr(mean), _ptr(rstd), _CODES[call_dtype], _ptr(w), _ptr(dx), width, base,
           base + params.element_size() * width, _ptr(ws), need)
-    return dx, dweight, dbias
+    params = params.to(param_dtype)
+    return dx, params[0], params[1]
 
 
 # --------------------------------------------------------------------------
