@@ -264,9 +264,17 @@ __global__ __launch_bounds__(LANES * GROUPS) void norm_grad_kernel(NormGradArgs 
     for (int i = 0; i < NV; ++i) {
       float (&wi)[E] = wf[LEAN ? 0 : i];
       if constexpr (LEAN) load_weight(i, wi);
+      // Past the row's end dy is 0 and x must be the mean: -mean * rstd may
+      // overflow where no column's (x - mean) * rstd does.
+      const int left = g.width - (first + i * LANES * E);
+      if (left < E) {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (e >= left) xh[i][e] = mean;
+      }
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        xh[i][e] = (xh[i][e] - mean) * rstd;  // (past the row's end: dy = 0)
+        xh[i][e] = (xh[i][e] - mean) * rstd;
         dw[i][e] += dy[i][e] * xh[i][e];
         db[i][e] += dy[i][e];
         dy[i][e] *= wi[e];
@@ -379,7 +387,7 @@ __global__ __launch_bounds__(1024) void norm_grad_wide_kernel(NormGradArgs g) {
 #pragma unroll
         for (int e = 0; e < E; ++e) {
           s1 += df[e] * wf[e];
-          s2 += df[e] * wf[e] * ((xf[e] - mean) * rstd);
+          if (e < left) s2 += df[e] * wf[e] * ((xf[e] - mean) * rstd);  // (past the row's end: 0 * -mean * rstd)
         }
       } else {
 #pragma unroll
