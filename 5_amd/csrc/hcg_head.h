@@ -51,7 +51,7 @@ constexpr int kStep = 64;  // K per stage
 
 enum Epilogue {
   kStats,    // softmax statistics of the logits
-  kExp,      // and exp(logit - block maximum) as f16
+  kExp,      // and exp(logit - block maximum) times exp_factor as f16
   kRound,    // scaled, rounded to DT, as rows of the output
   kPartial,  // float32, into scratch
   kSplit,    // kRound, or where K is split and the tile too large to fuse kPartial
@@ -110,6 +110,12 @@ __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
                                                    0, 0);
 }
+
+// What kExp multiplies the exponentials of a block with largest exponent `top`
+// by: 2^15, so that f16 holds them to 11 bits down to 2^-29 of the largest, and
+// to 2^-40 of it below.  Past 2^20 `top` is itself rounded by more than 2^-4 and
+// the largest exponential is no longer close enough to 1 for that.
+__device__ __forceinline__ float exp_factor(float top) { return fabsf(top) < 0x1p20f ? 0x1p15f : 1.f; }
 
 template <int N>
 __device__ __forceinline__ void wait_vm() {
@@ -616,9 +622,10 @@ __device__ __forceinline__ void head_tile(Args g, int wg) {
       sum += __shfl_xor(sum, 32);
       if (half == 0 && live_n) g.stats[(int64_t)n * g.ld_stats + tm * WM + wm] = f32x2{top, sum};
       if constexpr (EPI == kExp) {
+        const float up = exp_factor(top);
 #pragma unroll
         for (int mi = 0; mi < MI; ++mi)
-          Stage::template put<HCG_F16>(rows_out, lane, mi, [&](int r) { return acc[mi][ni][r]; });
+          Stage::template put<HCG_F16>(rows_out, lane, mi, [&](int r) { return acc[mi][ni][r] * up; });
         Stage::template store<false>(rows_out, lane, mfirst, g.M, [&](int row) -> uint16_t* {
           const int to = nfirst + row;
           return to < N ? static_cast<uint16_t*>(g.out) + (int64_t)to * g.ldo : nullptr;

@@ -10,7 +10,7 @@
 // w^T keeps its logits in accumulators: it leaves, per token and block of a
 // wave's vocabulary rows, the maximum and the sum of exp(l - maximum), and for
 // the gradient the exponentials themselves as f16, relative to their block's
-// maximum (so within 2^-12 of the value wherever they matter).  One pass over
+// maximum (within 2^-11 of the value, or 2^-40 of that maximum).  One pass over
 // those makes the row's lse and the probabilities (minus the one-hot) in the
 // operands' type, from which dx and dw are two more products: three in all,
 // where recomputing the logits would take four.  Exponentials and
@@ -35,9 +35,10 @@ constexpr int64_t kPieceBytes = (int64_t)1 << 30;
 constexpr int64_t kPieceTokens = (int64_t)1 << 22, kPieceLogits = (int64_t)1 << 32;
 constexpr int64_t kMaxTokens = (int64_t)1 << 26;
 constexpr int64_t kMaxExtent = 4000000;  // of vocabulary and width: a tile's offsets stay in 31 bits
-// f16 probabilities are held times 2^12 (a uniform one over a vocabulary past
-// 2^14 would be subnormal), undone in the products' float32 factor.
-constexpr float kF16Scale = 4096.f;
+// f16 probabilities are held times 2^15 (a uniform one over a vocabulary past
+// 2^14 would be subnormal; so they are normal down to 2^-29, and held to 2^-40
+// below), undone in the products' float32 factor.
+constexpr float kF16Scale = 32768.f;
 
 // ---------------------------------------------------------------------------
 // Packing
@@ -224,9 +225,9 @@ struct SoftmaxArgs {
 // One row by one workgroup: lse from the blocks' statistics, the loss, and
 // (GRAD) the probabilities in place of the exponentials.  With block maxima m_b
 // and sums s_b, lse = ref + log2 sum_b s_b 2^(m_b - ref) in powers of two, and a
-// probability is its exponential times 2^(m_b - ref) / sum: one multiply-add per
-// element.  Bound by HBM, 2 bytes read and written per probability: 8192 x 65536
-// 447 us (4.8 TB/s), 8192 x 32768 215 (5.0).
+// probability is its exponential times 2^(m_b - ref) / (sum exp_factor): one
+// multiply-add per element.  Bound by HBM, 2 bytes read and written per
+// probability: 8192 x 65536 447 us (4.8 TB/s), 8192 x 32768 215 (5.0).
 template <int DT, bool GRAD>
 __global__ __launch_bounds__(256) void softmax_kernel(SoftmaxArgs g) {
   constexpr double kLn2 = 0.693147180559945309;
@@ -265,7 +266,8 @@ __global__ __launch_bounds__(256) void softmax_kernel(SoftmaxArgs g) {
     const float rest = scale / sum;
     for (int c = tid * 8; c < g.vocab; c += 256 * 8) {
       const float m = stats[c / g.block].x;
-      const float f = rest * __builtin_amdgcn_exp2f(m == -__builtin_inff() ? -1e30f : m - ref);
+      const float down = 1.f / head::exp_factor(m);
+      const float f = rest * __builtin_amdgcn_exp2f(m == -__builtin_inff() ? -1e30f : m - ref) * down;
       float v[8];
       hcg::unpack<_Float16>(*reinterpret_cast<const raw4*>(row + c), v);
 #pragma unroll
