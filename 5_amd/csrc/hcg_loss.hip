@@ -726,8 +726,9 @@ int check_call(int dtype, const Call& c, int64_t tokens, int64_t vocab, int64_t 
                      (vocab <= 1 || (c.ldw >= width && (!grad || c.lddw >= width))),
                  "row stride below the width %lld", (long long)width);
   HCG_LM_REQUIRE(hcg::elem_aligned(c.x, 2) && hcg::elem_aligned(c.weight, 2) && hcg::elem_aligned(c.dx, 2) &&
-                     hcg::elem_aligned(c.dw, 2) && hcg::elem_aligned(c.targets, c.id_bytes),
-                 "rows and targets must be aligned to their elements");
+                     hcg::elem_aligned(c.dw, 2) && hcg::elem_aligned(c.targets, c.id_bytes) &&
+                     hcg::elem_aligned(c.loss, 4) && hcg::elem_aligned(c.lse, 4),
+                 "rows, targets and losses must be aligned to their elements");
   if (tokens == 0 || vocab == 0 || width == 0) return HCG_OK;
   *plan = make_plan(tokens, vocab, width, !weight_in_place(c.weight, c.ldw, vocab, width), grad);
   const int64_t most = ((int64_t)1 << 31) - 1;

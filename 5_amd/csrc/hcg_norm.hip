@@ -547,6 +547,10 @@ int hcg_layer_norm(int dtype, const void* x, int64_t ldx, int64_t rows, int64_t 
   HCG_LM_REQUIRE(rows == 1 || (ldx >= width && ldy >= width), "row stride below the width %lld", (long long)width);
   HCG_LM_REQUIRE(hcg::elem_aligned(x, hcg::elem_bytes(dtype)) && hcg::elem_aligned(y, hcg::elem_bytes(dtype)),
                  "rows must be aligned to their elements");
+  const int pb = hcg::elem_bytes(param_dtype);
+  HCG_LM_REQUIRE(hcg::elem_aligned(weight, pb) && hcg::elem_aligned(bias, pb) && hcg::elem_aligned(mean, 4) &&
+                     hcg::elem_aligned(rstd, 4),
+                 "parameters and statistics must be aligned to their elements");
   const NormArgs a{x, weight, bias, y, mean, rstd, ldx, ldy, rows, (int)width, eps};
   with_types(dtype, param_dtype, [&](auto t, auto p) {
     if constexpr (std::is_same_v<decltype(p), float> || std::is_same_v<decltype(p), decltype(t)>)
@@ -579,6 +583,10 @@ int hcg_layer_norm_grad(int dtype, const void* dy, int64_t lddy, const void* x, 
   const int eb = hcg::elem_bytes(dtype);
   HCG_LM_REQUIRE(hcg::elem_aligned(dy, eb) && hcg::elem_aligned(x, eb) && hcg::elem_aligned(dx, eb),
                  "rows must be aligned to their elements");
+  const int pb = hcg::elem_bytes(param_dtype);
+  HCG_LM_REQUIRE(hcg::elem_aligned(weight, pb) && hcg::elem_aligned(dweight, pb) && hcg::elem_aligned(dbias, pb) &&
+                     hcg::elem_aligned(mean, 4) && hcg::elem_aligned(rstd, 4),
+                 "parameters and statistics must be aligned to their elements");
   const bool params = dweight || dbias;
   if (params && rows > 0) {
     HCG_LM_REQUIRE(workspace && workspace_bytes >= hcg_layer_norm_grad_workspace(rows, width) &&

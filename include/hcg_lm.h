@@ -6,8 +6,8 @@
  * have no counterpart in the reference, whose only data-parallel path is the
  * tiled product.
  *
- * Matrices are row-major, with the row stride in elements; rows need no
- * alignment beyond their elements'.  Element types are HCG_F16, HCG_BF16
+ * Matrices are row-major, with the row stride in elements; nothing but scratch
+ * needs an alignment beyond its elements'.  Element types are HCG_F16, HCG_BF16
  * (hcg_gemm.h) or HCG_F32.  Sums and statistics are float32; a 16-bit output
  * is rounded once (to nearest, ties to even).  Every result is bit-reproducible.
  *
