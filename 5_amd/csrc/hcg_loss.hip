@@ -762,6 +762,25 @@ int64_t hcg_linear_cross_entropy_workspace(int64_t tokens, int64_t vocab, int64_
   return make_plan(tokens, vocab, width, !weight_in_place(weight, ldw, vocab, width), grad != 0).total;
 }
 
+int hcg_linear_cross_entropy_plan(int64_t tokens, int64_t vocab, int64_t width, int grad, int* plan) {
+  HCG_LM_REQUIRE(plan, "null pointer");
+  HCG_LM_REQUIRE(tokens > 0 && tokens < kMaxTokens && vocab > 0 && vocab < kMaxExtent - 8 && width > 0 &&
+                     width < kMaxExtent - 8,
+                 "%lld tokens, %lld rows of %lld elements are out of range", (long long)tokens, (long long)vocab,
+                 (long long)width);
+  const Plan p = make_plan(tokens, vocab, width, false, grad != 0);
+  *plan++ = p.pieces;
+  const auto put = [&](bool made, const Product& q, int64_t m, int64_t n) {
+    *plan++ = made ? kShapes[q.shape].tm : 0;
+    *plan++ = made ? kShapes[q.shape].tn : 0;
+    *plan++ = made ? (int)std::max<int64_t>(1, std::min<int64_t>(q.max_splits, q.units / tiles(q.shape, m, n))) : 0;
+  };
+  put(true, p.logits, vocab, p.piece);
+  put(grad != 0, p.dx, width, p.piece);
+  put(grad != 0, p.dw, width, vocab);
+  return HCG_OK;
+}
+
 int hcg_linear_cross_entropy(int dtype, const void* x, int64_t ldx, int64_t tokens, const void* weight, int64_t ldw,
                              int64_t vocab, int64_t width, int id_bytes, const void* targets, int64_t ignore_index,
                              float* loss, float* lse, void* workspace, int64_t workspace_bytes, void* stream) {

@@ -61,7 +61,7 @@ EXPORTS = ("hcg_init", "hcg_gemm", "hcg_gemm_algo", "hcg_gemm_noalloc", "hcg_gem
 # Every symbol include/hcg_lm.h declares.
 LM_EXPORTS = ("hcg_embedding", "hcg_embedding_grad", "hcg_embedding_grad_workspace", "hcg_layer_norm",
               "hcg_layer_norm_grad", "hcg_layer_norm_grad_workspace", "hcg_linear_cross_entropy",
-              "hcg_linear_cross_entropy_grad", "hcg_linear_cross_entropy_workspace")
+              "hcg_linear_cross_entropy_grad", "hcg_linear_cross_entropy_plan", "hcg_linear_cross_entropy_workspace")
 
 NOALLOC_SCRATCH_BYTES = 32 << 20  # HCG_NOALLOC_SCRATCH_BYTES
 
@@ -105,6 +105,7 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.hcg_layer_norm_grad.argtypes = [c_int, vp, i64, vp, i64, i64, i64, vp, vp, c_int, vp, vp, i64, vp, vp, vp,
                                         i64, vp]
     lib.hcg_linear_cross_entropy_workspace.argtypes = [i64, i64, i64, vp, i64, c_int]
+    lib.hcg_linear_cross_entropy_plan.argtypes = [i64, i64, i64, c_int, ctypes.POINTER(c_int)]
     lib.hcg_linear_cross_entropy.argtypes = [c_int, vp, i64, i64, vp, i64, i64, i64, c_int, vp, i64, vp, vp, vp, i64,
                                              vp]
     lib.hcg_linear_cross_entropy_grad.argtypes = [c_int, vp, i64, i64, vp, i64, i64, i64, c_int, vp, i64, c_int, f32,

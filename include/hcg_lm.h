@@ -86,6 +86,13 @@ int hcg_linear_cross_entropy_grad(int dtype, const void* x, int64_t ldx, int64_t
                                   int64_t lddx, void* dweight, int64_t lddw, void* workspace,
                                   int64_t workspace_bytes, void* stream);
 
+/* How calls of these sizes run (no device is asked): plan[0] is the number of
+ * pieces that the tokens are taken in; then, for the logits (vocab x tokens)
+ * and, where grad is not 0, dx (width x tokens) and dweight (width x vocab),
+ * three values each: a tile's rows, its columns, and the parts that the sums
+ * are split into if every token of a piece counts.  plan has room for 10. */
+int hcg_linear_cross_entropy_plan(int64_t tokens, int64_t vocab, int64_t width, int grad, int* plan);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,5 +1,6 @@
 """hc.gfx950.linear_cross_entropy and its gradient: probabilities far below
-the largest."""
+the largest, and sizes that reach every tile shape of the three products (on
+the host test_lm_plan.py asks the library that they do)."""
 
 from __future__ import annotations
 
@@ -9,7 +10,8 @@ torch = pytest.importorskip("torch")
 
 import hc.gfx950 as g  # noqa: E402
 
-from .test_lm_gpu import BF16, DEV, E32, F16, TINY, U, _close, _head_want  # noqa: E402
+from .test_lm_gpu import (BF16, DEV, E32, F16, F32, TINY, U, _close, _gen, _grad_tols, _head, _head_want,  # noqa: E402
+                          _loss_tol, _twice)
 
 pytestmark = pytest.mark.gpu
 
@@ -37,3 +39,43 @@ def test_small_probabilities_keep_their_gradient(t, v, base, dtype):
     eps = rel * p + U[dtype] * gz.abs() * (1 + rel) + (2.0**-39 if base < 2**20 else 2.0**-24)
     want, tol = gz.sum(0) * scale, eps.sum(0) * scale
     _close(dw[:, 0], want, tol + U[dtype] * (want.abs() + tol) + TINY[dtype])
+
+
+# Tokens, vocabulary, width: with those of test_lm_gpu.py every tile shape of
+# logits, dx and dweight, with and without split sums; ragged on all sides, and
+# in whole tiles; the last one in two pieces of large tiles.
+HEADS = [(432, 31059, 200), (2707, 413, 3416), (3861, 27862, 133), (3000, 3000, 3000), (1999, 50021, 1027),
+         (2048, 32768, 1024), (3138, 20, 1922), (36, 5794, 4089), (618, 16, 19), (3450, 17, 1159), (68, 39280, 19),
+         (4500, 131072, 264)]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("t,v,d", HEADS)
+def test_loss_by_every_tile_shape(t, v, d, dtype):
+    x, w, y = _head(t, v, d, dtype, t + v + d)
+    keep = torch.rand((t,), generator=_gen(t), device=DEV) < 0.9
+    x[~keep] = float("nan")  # ignored rows may hold anything
+    lse, loss, slack, _, _ = _head_want(x, w, y, keep)
+    got = _twice(lambda: g.linear_cross_entropy(x, w, torch.where(keep, y, -100)))
+    tol = _loss_tol(slack, lse)
+    for a, b in zip(got, (loss, lse)):
+        assert a.shape == (t,) and a.dtype == F32 and (a[~keep] == 0).all()
+        _close(a[keep], b[keep], tol[keep])
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("share", [0.8, 0.1])  # (few that count: the device splits sums into more parts than the host planned)
+@pytest.mark.parametrize("t,v,d", HEADS)
+def test_gradient_by_every_tile_shape(t, v, d, share, dtype):
+    x, w, y = _head(t, v, d, dtype, 2 * t + v + d)
+    keep = torch.rand((t,), generator=_gen(t), device=DEV) < share
+    x[~keep] = float("nan")
+    lse, loss, slack, gz, p = _head_want(x, w, y, keep)
+    got = _twice(lambda: g.linear_cross_entropy_grad(x, w, torch.where(keep, y, -100), reduction="sum"))
+    assert got[0].shape == () and got[1].dtype == got[2].dtype == dtype
+    tol = _loss_tol(slack, lse)[keep].sum() + (t / 1024 + 30) * E32 * loss[keep].abs().sum()
+    assert abs(float(got[0]) - float(loss[keep].sum())) <= float(tol)
+    (dx, tx), (dw, tw) = _grad_tols(x, w, gz, p, slack, keep, 1.0, dtype)
+    _close(got[1], dx, tx)
+    _close(got[2], dw, tw)
+    assert (got[1][~keep] == 0).all()
