@@ -141,6 +141,16 @@ def _ids(torch: Any, t: Any, what: str, index: int) -> tuple[Any, int]:
     return (t if t.is_contiguous() else t.contiguous()), size
 
 
+def _whole(value: Any, what: str) -> int:
+    try:
+        n = int(value)
+    except (TypeError, ValueError, OverflowError):
+        n = None
+    if n is None or n != value or not -(1 << 63) <= n < 1 << 63:
+        raise LaunchError(f"{what} must be a whole number of 64 bits, got {value!r}")
+    return n
+
+
 def _workspace(torch: Any, size: int, device: Any) -> Any:
     # From torch's allocator, which hands memory freed on a stream to later
     # work on that stream only.
@@ -204,11 +214,13 @@ def embedding_grad(dy: Any, tokens: Any, vocab: int, *, scale: float = 1.0, padd
     ids, size = _ids(torch, tokens, "tokens", index)
     if dy.ndim != tokens.ndim + 1 or dy.shape[:-1] != tokens.shape:
         raise LaunchError(f"dy shape {tuple(dy.shape)} does not match tokens {tuple(tokens.shape)}")
-    vocab = int(vocab)
+    vocab = _whole(vocab, "vocab")
     if vocab < 0:
         raise LaunchError(f"vocab must not be negative, got {vocab}")
-    if padding_idx is not None and not 0 <= padding_idx < vocab:
-        raise LaunchError(f"padding_idx {padding_idx} is outside the vocabulary of {vocab}")
+    if padding_idx is not None:
+        padding_idx = _whole(padding_idx, "padding_idx")
+        if not 0 <= padding_idx < vocab:
+            raise LaunchError(f"padding_idx {padding_idx} is outside the vocabulary of {vocab}")
     rows = _rows(dy, "dy")
     n, width = rows.shape
     if out is not None:

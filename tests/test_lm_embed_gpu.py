@@ -10,6 +10,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 import hc.gfx950 as g  # noqa: E402
+from hc._errors import LaunchError  # noqa: E402
 
 from .test_lm_gpu import (BF16, DEV, E32, F16, F32, TINY, U, _close, _embedding_grad_want, _gen, _randn,  # noqa: E402
                           _twice)
@@ -74,3 +75,16 @@ def test_gradient_of_unknown_tokens_only(n, vocab):
     assert (g.embedding_grad(dy, tokens, vocab) == 0).all()
     tokens[:] = 5
     assert (g.embedding_grad(dy, tokens, vocab, padding_idx=5) == 0).all()
+
+
+def test_gradient_refuses_counts_that_are_no_whole_numbers():
+    dy, tokens = torch.ones((3, 8), device=DEV), torch.tensor([0, 1, 4], device=DEV)
+    for bad in (4.5, "5", None, float("inf"), float("nan")):
+        with pytest.raises(LaunchError, match="vocab must be a whole number"):
+            g.embedding_grad(dy, tokens, bad)
+        if bad is not None:
+            with pytest.raises(LaunchError, match="padding_idx must be a whole number"):
+                g.embedding_grad(dy, tokens, 5, padding_idx=bad)
+    want = g.embedding_grad(dy, tokens, 5)
+    assert torch.equal(g.embedding_grad(dy, tokens, 5.0), want)
+    assert torch.equal(g.embedding_grad(dy, tokens, torch.tensor(5), padding_idx=torch.tensor(2)), want)
