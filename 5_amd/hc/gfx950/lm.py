@@ -361,7 +361,7 @@ def layer_norm_grad(dy: Any, x: Any, mean: Any, rstd: Any, weight: Any | None = 
 # --------------------------------------------------------------------------
 
 
-def _head_args(torch: Any, x: Any, weight: Any, targets: Any) -> tuple[Any, ...]:
+def _head_args(torch: Any, x: Any, weight: Any, targets: Any, ignore_index: Any) -> tuple[Any, ...]:
     index = _check_tensor(torch, x, "x")
     code = _code(x, "x", _HALF)
     _check_tensor(torch, weight, "weight", index)
@@ -376,7 +376,7 @@ def _head_args(torch: Any, x: Any, weight: Any, targets: Any) -> tuple[Any, ...]
         raise LaunchError("a softmax over no vocabulary")
     if weight.shape[1] == 0 and targets.numel():
         raise LaunchError("hidden states without elements")
-    return index, code, _rows(x, "x"), _rows(weight, "weight"), ids, size
+    return index, code, _rows(x, "x"), _rows(weight, "weight"), ids, size, _whole(ignore_index, "ignore_index")
 
 
 def linear_cross_entropy(x: Any, weight: Any, targets: Any, *, ignore_index: int = -100) -> tuple[Any, Any]:
@@ -392,7 +392,7 @@ def linear_cross_entropy(x: Any, weight: Any, targets: Any, *, ignore_index: int
     if r is not None:
         return r
     torch = _torch()
-    index, code, rows, w, ids, size = _head_args(torch, x, weight, targets)
+    index, code, rows, w, ids, size, ignore = _head_args(torch, x, weight, targets, ignore_index)
     n, width = rows.shape
     vocab = w.shape[0]
     out = torch.empty((2, *targets.shape), dtype=torch.float32, device=x.device)
@@ -402,7 +402,7 @@ def linear_cross_entropy(x: Any, weight: Any, targets: Any, *, ignore_index: int
     if n:
         base = out.data_ptr()
         _call(torch, index, lib.hcg_linear_cross_entropy, "hcg_linear_cross_entropy", code, _ptr(rows), _ld(rows), n,
-              _ptr(w), _ld(w), vocab, width, size, _ptr(ids), ignore_index, base, base + 4 * n, _ptr(ws), need)
+              _ptr(w), _ld(w), vocab, width, size, _ptr(ids), ignore, base, base + 4 * n, _ptr(ws), need)
     return out[0], out[1]
 
 
@@ -424,7 +424,7 @@ def linear_cross_entropy_grad(x: Any, weight: Any, targets: Any, *, ignore_index
     torch = _torch()
     if reduction not in ("mean", "sum"):
         raise LaunchError(f"unknown reduction {reduction!r}; expected 'mean' or 'sum'")
-    index, code, rows, w, ids, size = _head_args(torch, x, weight, targets)
+    index, code, rows, w, ids, size, ignore = _head_args(torch, x, weight, targets, ignore_index)
     n, width = rows.shape
     vocab = w.shape[0]
     device = x.device
@@ -435,6 +435,6 @@ def linear_cross_entropy_grad(x: Any, weight: Any, targets: Any, *, ignore_index
     need = lib.hcg_linear_cross_entropy_workspace(n, vocab, width, _ptr(w), _ld(w), 1)
     ws = _workspace(torch, need, device)
     _call(torch, index, lib.hcg_linear_cross_entropy_grad, "hcg_linear_cross_entropy_grad", code, _ptr(rows),
-          _ld(rows), n, _ptr(w), _ld(w), vocab, width, size, _ptr(ids), ignore_index, reduction == "mean", grad_scale,
+          _ld(rows), n, _ptr(w), _ld(w), vocab, width, size, _ptr(ids), ignore, reduction == "mean", grad_scale,
           _ptr(loss), _ptr(dx), width, _ptr(dweight), width, _ptr(ws), need)
     return loss, dx, dweight

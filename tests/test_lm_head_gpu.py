@@ -9,6 +9,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 import hc.gfx950 as g  # noqa: E402
+from hc._errors import LaunchError  # noqa: E402
 
 from .test_lm_gpu import (BF16, DEV, E32, F16, F32, TINY, U, _close, _gen, _grad_tols, _head, _head_want,  # noqa: E402
                           _loss_tol, _twice)
@@ -79,3 +80,11 @@ def test_gradient_by_every_tile_shape(t, v, d, share, dtype):
     _close(got[1], dx, tx)
     _close(got[2], dw, tw)
     assert (got[1][~keep] == 0).all()
+
+
+def test_refuses_an_ignored_target_that_no_target_can_be():
+    x, w, y = _head(4, 9, 8, BF16, 0)
+    for bad in (1.5, "-100", None, 2**63, 2**64 - 100):
+        for call in (g.linear_cross_entropy, g.linear_cross_entropy_grad):
+            with pytest.raises(LaunchError, match="ignore_index must be a whole number"):
+                call(x, w, y, ignore_index=bad)
