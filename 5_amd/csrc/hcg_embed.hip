@@ -137,7 +137,6 @@ struct EmbedGradArgs {
   int width, items;  // items: dy's whole 16-byte vectors in a row, and the elements past them
   int rows;         // table rows per workgroup
   float scale;
-  bool lines;       // the gradient's rows are whole 128-byte lines
   // Lists over the tokens in the order of (row, i).
   int* token;     // i (null: one launch)
   int* row;       // the long row it belongs to, or -1
@@ -158,10 +157,8 @@ __device__ __forceinline__ int lanes_below(uint64_t mask) {
 }
 
 // f[0..E) of dy scaled, as the sum's rounding to G and one 16- or 32-byte store.
-// nt: the rows are whole 128-byte lines, so non-temporal stores leave no partial
-// ones (65536 x 4096 bf16: 170 us without, 135 with).
 template <bool WHOLE, class T, class G>
-__device__ __forceinline__ void store_grad(G* p, const float (&f)[kVec<T>], float scale, bool nt) {
+__device__ __forceinline__ void store_grad(G* p, const float (&f)[kVec<T>], float scale) {
   constexpr int E = kVec<T>, EG = kVec<G>;
   if constexpr (!WHOLE) {
     *p = (G)(f[0] * scale);
@@ -171,10 +168,7 @@ __device__ __forceinline__ void store_grad(G* p, const float (&f)[kVec<T>], floa
       float o[EG];
 #pragma unroll
       for (int e = 0; e < EG; ++e) o[e] = f[h * EG + e] * scale;
-      if (nt)
-        hcg::store_raw<true>(p + h * EG, hcg::pack<G>(o), EG);
-      else
-        hcg::store_raw(p + h * EG, hcg::pack<G>(o), EG);
+      hcg::store_raw(p + h * EG, hcg::pack<G>(o), EG);
     }
   }
 }
@@ -481,7 +475,7 @@ __global__ __launch_bounds__(kGradThreads, ONE > kListPerWave ? 6 : 8) void embe
       constexpr bool WHOLE = decltype(whole)::value;
       float sum[E] = {};
       sum_rows<WHOLE, T>(sum, dy + c, g.lddy, n, [&](int j) { return entry(first + j); });
-      store_grad<WHOLE, T, G>(grad + (lo + r) * g.ldg + c, sum, g.scale, g.lines);
+      store_grad<WHOLE, T, G>(grad + (lo + r) * g.ldg + c, sum, g.scale);
     };
     if (i < it.whole)
       one_item(std::true_type{}, i * E);
@@ -522,9 +516,9 @@ __global__ __launch_bounds__(kGradThreads, ONE > kListPerWave ? 6 : 8) void embe
         for (int e = 0; e < E; ++e) sum[e] += meet[e * kGradThreads + q * it.items + tid];
       G* p = grad + (lo + r) * g.ldg + c;
       if (whole)
-        store_grad<true, T, G>(p, sum, g.scale, g.lines);
+        store_grad<true, T, G>(p, sum, g.scale);
       else
-        store_grad<false, T, G>(p, sum, g.scale, g.lines);
+        store_grad<false, T, G>(p, sum, g.scale);
     }
     __syncthreads();
   }
@@ -739,8 +733,6 @@ int hcg_embedding_grad(int dtype, const void* dy, int64_t lddy, int64_t n, int64
   const int64_t quick = std::min((vocab + 1023) / 1024, std::max<int64_t>(1, (128 << 10) / (width * eb)));
   a.rows = (int)std::min<int64_t>(kMaxRows, std::max((vocab + 4095) / 4096, quick));
   a.scale = scale;
-  const int gb = hcg::elem_bytes(grad_dtype);
-  a.lines = hcg::elem_aligned(grad, 128) && (vocab == 1 || ldg * gb % 128 == 0);
   if (need > 0) {
     char* p = static_cast<char*>(workspace);
     a.token = reinterpret_cast<int*>(p);
