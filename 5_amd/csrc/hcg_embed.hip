@@ -16,7 +16,8 @@
 // kLong of them are left in a list, in the order of (row, i), which a second
 // launch sums in windows of kWindow entries and a third adds up by rows.
 // Bound by the table's writes, most of them zeros: a pass over 65536 x 4096 bf16
-// with 8192 tokens 115 us for 537 MB (and 67 MB read).
+// with 8192 tokens 115 us on the same inputs and 125 on new ones, for 537 MB (and
+// 67 MB read); its first launch 105.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -99,8 +100,8 @@ constexpr int kScan = 4;           // pairs of ids in flight per lane
 constexpr int kMaxRows = 64;       // table rows per workgroup
 constexpr int kListPerWave = 256;  // ids of a workgroup's rows kept in LDS, per wave that scans
 // Rows of dy in flight per thread.  (16 take registers that leave two workgroups
-// per CU instead of four: 999 tokens of 515 f32 into 5003 rows 10.9 us with 8,
-// 12.7 with 16.)
+// per CU instead of four: 999 tokens of 515 f32 into 5003 rows 13.6 us with 8,
+// 18.7 with 16.)
 constexpr int kSumLoads = 8;
 constexpr int kLong = 16;
 constexpr int kWindow = 32;
@@ -111,16 +112,16 @@ constexpr int kRuns = kWindow / (kLong + 1) + 2;
 // meet in LDS, and one launch does it all.  Up to kOneLaunch tokens where a row has
 // at most half as many items as there are threads, up to twice as many, by lists
 // twice as long (54 KB of LDS: 3 workgroups per CU, not 4), where it has at most a
-// quarter.  us, one launch / three: 3160 into 5065 x 131 f32 14.2 / 24.1, 2273 into
-// 6920 x 463 f32 16.9 / 25.1, but 3720 into 731 x 1336 f16 (167 items) 28.5 / 24.0;
-// long lists / short ones: 2048 into 13384 x 128 bf16 15.4 / 12.6.
+// quarter.  us, one launch / three: 3160 into 5065 x 131 f32 14.6 / 24.9, 2273 into
+// 6920 x 463 f32 17.0 / 24.8, but 3720 into 731 x 1336 f16 (167 items) 28.6 / 23.7;
+// long lists / short ones: 2048 into 13384 x 128 bf16 15.0 / 12.1.
 constexpr int kOneLaunch = 2048;
 // Past so many tokens they are first parted by ranges of the table (a launch of
 // kBuckets workgroups, stable), and a workgroup scans its range's tokens only:
 // 4096 workgroups that scan them all read 1 GB from the L2s at 32768 tokens.
-// us, all scanned / parted: 32768 into 108888 x 512 f16 86 / 70, 65536 into 32768
-// x 1024 bf16 185 / 140, 8192 into 65536 x 4096 150 / 149, 5000 into 5000 x 512
-// f32 26.2 / 27.1.
+// us, all scanned / parted: 32768 into 108888 x 512 f16 80 / 71, 65536 into 32768
+// x 1024 bf16 181 / 141, 8192 into 65536 x 4096 117 / 119, 5000 into 5000 x 512
+// f32 25.8 / 26.4.
 constexpr int kBucketTokens = 8192;
 constexpr int kBuckets = 64;
 
@@ -444,9 +445,9 @@ __global__ __launch_bounds__(kGradThreads, ONE > kListPerWave ? 6 : 8) void embe
   // The rows without tokens: neighbours together, where the gradient has no
   // gaps, so that lines are written whole whatever the width, and past the
   // caches.  us of a pass, row by row / so / so without non-temporal stores: 8192
-  // tokens into 65536 x 4096 bf16 151 / 115 / 148, 200 into 36696 x 3400 f32 117 /
-  // 100 / 112, 1353 into 24661 x 1367 f32 41.3 / 44.5 / 41.6, 2048 into 13384 x 128
-  // bf16 11.7 / 12.7 / 13.0.
+  // tokens into 65536 x 4096 bf16 117 / 115 / 146, 200 into 36696 x 3400 f32 102 /
+  // 102 / 110, 1353 into 24661 x 1367 f32 49 / 45 / 44, 2048 into 13384 x 128 bf16
+  // 15.3 / 11.8 / 11.8.
   const T* dy = static_cast<const T*>(g.dy);
   G* grad = static_cast<G*>(g.grad);
   uint64_t empty = __ballot(lane < rows && count[lane] == 0);
@@ -729,7 +730,7 @@ int hcg_embedding_grad(int dtype, const void* dy, int64_t lddy, int64_t n, int64
   a.items = (int)items_of(dtype, width);
   // A small table in one round of workgroups (1024), a large one in up to four,
   // so that some scan the ids while others write (65536 x 4096 bf16: 1024
-  // workgroups 135 us, 4096 123).
+  // workgroups 130 us, 4096 115).
   const int64_t quick = std::min((vocab + 1023) / 1024, std::max<int64_t>(1, (128 << 10) / (width * eb)));
   a.rows = (int)std::min<int64_t>(kMaxRows, std::max((vocab + 4095) / 4096, quick));
   a.scale = scale;

@@ -17,12 +17,13 @@
 // stage before, whose two units are refilled UNITS units ahead.  Operand
 // layouts, swizzles and fragment reads are those of hcg_wg8.h.
 //
-// Large products are bound by the board's power: MFMAs issue in 92% of the cycles
-// of dX, 86% of dW's and 82% of the logits' at 1.5 GHz (8192 x 65536 x 4096 bf16:
-// 2.9, 3.0 and 3.2 ms, 1.51, 1.46 and 1.36 PFLOP/s; the logits' epilogue takes the
+// Large products are bound by the board's power: MFMAs issue in 90% of the cycles
+// of dX, 85% of dW's and 80% of the logits' at 1.6 GHz (8192 x 65536 x 4096 bf16:
+// 2.9, 3.0 and 3.2 ms, 1.52, 1.46 and 1.37 PFLOP/s; the logits' epilogue takes the
 // exponentials and writes 1 GB), without LDS bank conflicts.  The 5-unit ring of 160
-// KB carries them: with four units (128 KB) 49 to 54 M cycles instead of 37 to 41.
-// Products of few tokens are bound by HBM (16 x 65536 x 4096: 90 us, 5.96 TB/s) or,
+// KB carries them: with four units (128 KB) 3355, 3544 and 3654 us on a card that
+// takes 2938, 3082 and 3333 with five.
+// Products of few tokens are bound by HBM (16 x 65536 x 4096: 90.5 us, 5.9 TB/s) or,
 // the smallest, by a launch and a tile's start and end.
 #pragma once
 
@@ -59,8 +60,8 @@ enum Epilogue {
 
 // Tiles whose K splits the tile's last workgroup sums itself (hcg_splitsum.h);
 // larger ones are added up by a launch of their own (dx of 256 x 4096 x 512 in
-// 128x128 tiles and 8 parts: 16.0 us by the last workgroup, 12.6 by a launch; in
-// 128x32 tiles of 128 x 6000 x 700 11.2 by the last one).
+// 128x128 tiles and 8 parts: 21.7 us by the last workgroup, 14.6 with a launch; in
+// 128x32 tiles and 4 parts 11 by the last one).
 constexpr bool can_fuse(int tm, int tn) { return tm * tn <= 128 * 64; }
 
 struct Args {
@@ -323,7 +324,7 @@ struct RowStage {
 // workgroup starts at a stage of its own (a golden-ratio sequence) and wraps.
 // With all of them at one k, rows a power of two apart put every piece that is
 // read at one offset, and the reads pile onto a few HBM channels: logits of 16 x
-// 65536 x 4096 bf16 110 us, rotated 90 (5.96 TB/s).
+// 65536 x 4096 bf16 109 us, rotated 94 (on another card 90.5, 5.9 TB/s).
 template <int DT, int TM, int TN, int WM, int WN, int UNITS, bool AKC, bool BKC, int EPI, bool COUNT_K, bool ROTATE>
 __device__ __forceinline__ void head_tile(Args g, int wg) {
   constexpr int NW = WM * WN;

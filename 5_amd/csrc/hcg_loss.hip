@@ -29,6 +29,8 @@ using hcg::raw4;
 namespace head = hcg::head;
 typedef head::f32x2 f32x2;
 
+// (16-bit values, without the rows' padding; at least 256 tokens, however large the
+// vocabulary)
 constexpr int64_t kPieceBytes = (int64_t)1 << 30;
 // ... and no more than so many tokens, whose launches stay below 2^32 threads
 // (a loss alone holds no probabilities, and its pieces kPieceLogits logits).
@@ -72,8 +74,8 @@ constexpr int kPackThreads = 256;
 constexpr int kPackRun = 128;  // tokens per workgroup at most: their places are in LDS
 
 // Past so many tokens, a launch counts them by runs of that many first.  us of
-// hcg_linear_cross_entropy over 64 x 16, counted first / not: 98304 tokens 161 /
-// 182, 262144 319 / 470, 1048576 1092 / 4624.
+// hcg_linear_cross_entropy over 64 x 16, counted first / not: 98304 tokens 159 /
+// 181, 262144 316 / 468, 1048576 1092 / 4734.
 constexpr int kCountRun = 1 << 16;
 constexpr int kCountThreads = 1024;
 template <class I>
@@ -280,7 +282,7 @@ __global__ __launch_bounds__(256) void softmax_kernel(SoftmaxArgs g) {
 // Rows of dx from the K splits' sums (where head_kernel split K in large tiles).
 // The parts come from the L2s and the Infinity Cache: 1300 x 1027 in 8 parts 11
 // us; a launch with nothing to add (few splits on the host's count of tokens, none
-// on the device's) 3.
+// on the device's) 3 to 5.
 struct JoinArgs {
   const float* part;  // [splits][live tokens][ld]
   int64_t ld;
@@ -335,11 +337,12 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // stage of K on an idle and on a busy chip, per round of workgroups
 // (per_cu of which share a CU).  Fitted to 10 sizes with every shape and 1 to 8
 // K splits: its choice is the fastest, or within 8% of it, at nine of them.  Both
-// sides, us: dx of 1300 x 50000 x 1032 large in 8 parts 150, medium in 4 189; of
-// 256 x 4096 x 512 large in 8 parts 28, few in 4 10; of 1000 x 30000 x 1000
-// large in 8 parts 87, medium in 4 73; logits of 128 x 6000 x 700 large 20, few
-// 7; of 1024 x 32768 x 2048 large 117, medium 147; dw of 64 x 32768 x 4096 large
-// 111, medium 78, small 125; of 4096 x 32768 x 512 109, 140, 190.
+// sides, us (a launch that adds up parts included): dx of 1300 x 50000 x 1032
+// large in 8 parts 158, medium in 4 196; of 256 x 4096 x 512 large in 8 parts 28,
+// few in 4 11; of 1000 x 30000 x 1000 large in 8 parts 88, medium in 4 77; logits
+// of 128 x 6000 x 700 large 18, few 7; of 1024 x 32768 x 2048 large 121, medium
+// 159; dw of 64 x 32768 x 4096 large 110, medium 80, small 127; of 4096 x 32768 x
+// 512 113, 142, 188.
 enum Shape { kLarge, kMedium, kSmall, kFew };
 struct ShapeInfo {
   int tm, tn, wm, per_cu;
@@ -451,7 +454,7 @@ Plan make_plan(int64_t tokens, int64_t vocab, int64_t width, bool copy_weight, b
   p.ldx = round_up(width, 8);
   // Whole 128-byte lines, and not a multiple of 1 KB: rows a power of two apart
   // put the pieces that are read at one k on a few HBM channels (dx of 4096 x
-  // 32768 x 512 bf16 145 us, so 118).
+  // 32768 x 512 bf16 167 us, so 126).
   p.lde = round_up(vocab, 64) + (round_up(vocab, 64) % 512 ? 0 : 64);
   const int64_t fit = (grad ? kPieceBytes / 2 : kPieceLogits) / vocab / 256 * 256;
   p.piece = std::min({tokens, std::max<int64_t>(256, fit), kPieceTokens});
@@ -507,7 +510,7 @@ void launch_head(const Product& p, head::Args a, hipStream_t s, int extra = 0) {
   // Large tiles: four waves read the least LDS (128 KB per stage against 192 KB
   // by eight), and the board runs at its power limit; the softmax's epilogue is
   // faster by eight.  8192 x 65536 x 4096 bf16, us, four / eight waves: logits
-  // 3598 / 3513, dx 3096 / 3150, dw 3243 / 3259.
+  // 3464 / 3333, dx 2938 / 2964, dw 3082 / 3116.
   constexpr bool kSoftmax = EPI == head::kStats || EPI == head::kExp;
   if (shape == kLarge) {
     head::head_kernel<DT, 256, 256, 2, kSoftmax ? 4 : 2, 5, AKC, BKC, EPI, COUNT_K, false>
@@ -515,8 +518,8 @@ void launch_head(const Product& p, head::Args a, hipStream_t s, int extra = 0) {
   } else if (shape == kMedium) {
     // A ring of 5 units, 80 KB: two workgroups share a CU, and one computes while
     // the other starts or ends.  Eight units at one per CU / five, us: logits of
-    // 4096 x 32768 x 512 251 / 198, dw of 64 x 32768 x 4096 130 / 78, dx of 1024 x
-    // 32768 x 2048 134 / 133.
+    // 4096 x 32768 x 512 233 / 201, dw of 64 x 32768 x 4096 127 / 80, dx of 1024 x
+    // 32768 x 2048 156 / 151.
     head::head_kernel<DT, 128, 128, 2, 4, 5, AKC, BKC, EPI, COUNT_K, false><<<grid, 512, 0, s>>>(a);
   } else if (shape == kSmall) {
     // (one tile of tokens: bound by reading the weights)

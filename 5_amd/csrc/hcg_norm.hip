@@ -8,8 +8,8 @@
 // Both are bound by HBM: a row is read once (the gradient reads two) and held in
 // registers, so the variance is the sum of squares about the mean, without the
 // cancellation of E[x^2] - mean^2 and without a second read.  A row takes as
-// few lanes as hold it with 16 bytes each.  8192 x 4096 bf16: forward 24.8 us
-// (5.4 TB/s), gradient 43.3 + 4.6 (4.2 TB/s); the sums' divisions are true
+// few lanes as hold it with 16 bytes each.  8192 x 4096 bf16: forward 24.4 us
+// (5.5 TB/s), gradient 43.7 + 4.7 (4.2 TB/s); the sums' divisions are true
 // ones, so that a row of equal values gives exactly 0.
 #include <hip/hip_runtime.h>
 
@@ -466,8 +466,8 @@ void run_norm(const NormArgs& a, hipStream_t s) {
   if (vecs <= 16) return launch_norm<T, P, 16, 1>(a, s);
   if (vecs <= 32) return launch_norm<T, P, 32, 1>(a, s);
   if (vecs <= 64) return launch_norm<T, P, 64, 1>(a, s);
-  // As few lanes as hold the row.  us, 64 / 16 lanes (65536 x 128 bf16) 23.9 / 9.5,
-  // 64 / 32 (16384 x 256) 8.9 / 6.6, 256 / 128 (16384 x 1024) 23.4 / 16.4.
+  // As few lanes as hold the row.  us, 64 / 16 lanes (65536 x 128 bf16) 23.6 / 9.1,
+  // 64 / 32 (16384 x 256) 7.8 / 5.5, 256 / 128 (16384 x 1024) 22.0 / 16.1.
   if (vecs <= 128) return launch_norm<T, P, 128, 1>(a, s);
   if (vecs <= 256) return launch_norm<T, P, 256, 1>(a, s);
   if (vecs <= 512) return launch_norm<T, P, 256, 2>(a, s);
@@ -489,10 +489,10 @@ int run_norm_grad(const NormGradArgs& a, hipStream_t s) {
   const int64_t vecs = ((int64_t)a.width + kVec<T> - 1) / kVec<T>;
   // As few lanes per row as hold it, and as many rows as fit 1024 threads (512,
   // where a row is one wave or less: 16 rows of 64 lanes took 2048 x 512 bf16 from
-  // 8.0 to 11.0 us): idle lanes are loads that are not in flight.  us, 64 / 16
-  // lanes (65536 x 128 bf16) 37 / 17, 256 / 128 (16384 x 768) 35.6 / 24.6, 256 / 192
-  // (16384 x 1536) 37.7 / 33.9, 512 / 320 (8192 x 2560) 38.7 / 32.8, 512 / 384 (8192 x
-  // 2880) 41.9 / 38.8; the few rows of 100 x 128 6.6 / 7.0.
+  // 8.0 to 13.0 us): idle lanes are loads that are not in flight.  us, 64 / 16
+  // lanes (65536 x 128 bf16) 37.0 / 16.4, 256 / 128 (16384 x 768) 33.1 / 23.1, 256 /
+  // 192 (16384 x 1536) 36.2 / 33.0, 512 / 320 (8192 x 2560) 35.5 / 30.2, 512 / 384
+  // (8192 x 2880) 37.2 / 35.9; the few rows of 100 x 128 8.0 / 8.0.
   if (vecs <= 16) return launch_norm_grad<T, P, 16, 1, 32>(a, s);
   if (vecs <= 32) return launch_norm_grad<T, P, 32, 1, 16>(a, s);
   if (vecs <= 64) return launch_norm_grad<T, P, 64, 1, 8>(a, s);
@@ -596,7 +596,7 @@ int hcg_layer_norm_grad(int dtype, const void* dy, int64_t lddy, const void* x, 
   }
   const NormGradArgs a{dy,   x,   mean, rstd, weight,     dx, params ? static_cast<float*>(workspace) : nullptr,
                        lddy, ldx, lddx, rows, (int)width,
-                       // (past the L2s' 32 MB, where rows are whole lines: 8192 x 4096 bf16 47.6 -> 46.2 us)
+                       // (past the L2s' 32 MB, where rows are whole lines: 8192 x 4096 bf16 45.1 -> 44.8 us)
                        rows * width * eb > (32 << 20) && hcg::elem_aligned(dx, 128) && lddx * eb % 128 == 0};
   const hipStream_t s = static_cast<hipStream_t>(stream);
   with_types(dtype, param_dtype, [&](auto t, auto p) {

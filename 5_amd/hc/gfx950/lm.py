@@ -7,7 +7,11 @@ the tensors' device and current stream, asynchronously; arguments are checked
 before anything is launched and raise ``LaunchError``.  Leading dimensions are
 rows: an activation is ``(..., width)``.  Rows may be strided views; other
 layouts are copied.  Sums and statistics are float32, a 16-bit result is
-rounded once, and every result is the same from run to run.
+rounded once (the head's gradient holds two intermediates in 16 bits, see
+there), and every result is the same from run to run.
+
+The gradients are calls of their own: outputs carry no autograd graph, also
+where inputs require gradients.
 """
 
 from __future__ import annotations
@@ -413,9 +417,13 @@ def linear_cross_entropy_grad(x: Any, weight: Any, targets: Any, *, ignore_index
     count (``"mean"``; 0 when none does), a 0-dimensional float32 tensor, and
     the gradients of ``grad_scale`` times it, of x's type.
 
-    The probabilities are held for up to 1 GiB of tokens at a time, in the
-    operands' type.  float16 gradients of a mean over many tokens reach the
-    type's subnormals: scale them (``grad_scale``) as loss scaling does."""
+    Between the products, exponentials are held as float16 (within 2^-11 of the
+    value, or 2^-40 of the largest among some neighbouring words) and
+    probabilities minus the one-hot in the operands' type, each before the
+    gradients' own rounding.  They take up to 1 GiB (and the rows' padding; more
+    where 256 tokens do), and more tokens run in pieces.  float16 gradients of a
+    mean over many tokens reach the type's subnormals: scale them
+    (``grad_scale``) as loss scaling does."""
     if reduction in ("mean", "sum"):
         r = _fast("linear_cross_entropy_grad", x, weight, targets, ignore_index, reduction == "mean",
                   grad_scale)

@@ -9,7 +9,9 @@
  * Matrices are row-major, with the row stride in elements; nothing but scratch
  * needs an alignment beyond its elements'.  Element types are HCG_F16, HCG_BF16
  * (hcg_gemm.h) or HCG_F32.  Sums and statistics are float32; a 16-bit output
- * is rounded once (to nearest, ties to even).  Every result is bit-reproducible.
+ * is rounded once (to nearest, ties to even); hcg_linear_cross_entropy_grad
+ * holds two intermediates in 16 bits, see there.  Every result is
+ * bit-reproducible.
  *
  * Scratch is the caller's: a call that needs some has a ..._workspace
  * function for its size in bytes, takes 256-byte aligned device memory of at
@@ -79,7 +81,14 @@ int hcg_linear_cross_entropy(int dtype, const void* x, int64_t ldx, int64_t toke
 
 /* The sum of the losses (mean = 0) or their mean over the rows that count
  * (mean = 1; 0 when none does) into *loss, and the gradients of grad_scale
- * times it: dx (tokens x width) and dweight (vocab x width), of dtype. */
+ * times it: dx (tokens x width) and dweight (vocab x width), of dtype.  Between
+ * the products, exponentials are held as f16 (within 2^-11 of the value, or
+ * 2^-40 of the largest among the 32 to 128 words they are computed with; 2^-25
+ * where logits pass 7e5) and
+ * probabilities minus the one-hot in dtype (HCG_F16: times 2^15, so 2^-40 near
+ * zero): beside the result's own rounding, as much again where few tokens or
+ * words enter a sum.  They take scratch of 2 bytes per word for up to 2^29 words
+ * (1 GiB, and the rows' padding), or 256 tokens if those have more. */
 int hcg_linear_cross_entropy_grad(int dtype, const void* x, int64_t ldx, int64_t tokens, const void* weight,
                                   int64_t ldw, int64_t vocab, int64_t width, int id_bytes, const void* targets,
                                   int64_t ignore_index, int mean, float grad_scale, float* loss, void* dx,
