@@ -29,7 +29,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 PKG = os.path.dirname(HERE)
 ROOT = os.path.dirname(PKG)
 STAMPED_SRCS = [os.path.join(HERE, f) for f in ("hcg_gemm.hip", "hcg_tile.hip", "hcg_mfma.hip")]
-SRCS = STAMPED_SRCS + [os.path.join(HERE, f) for f in ("hcg_embed.hip", "hcg_norm.hip", "hcg_loss.hip")]
+SRCS = STAMPED_SRCS + [os.path.join(HERE, f) for f in ("hcg_embed.hip", "hcg_norm.hip", "hcg_loss.hip", "hcg_rms.hip",
+                                                       "hcg_quantize.hip", "hcg_linear8.hip")]
 INCLUDE = os.path.join(ROOT, "include")
 OUT = os.path.join(PKG, "hc", "gfx950", "libhcg_gfx950.so")
 # The products' sources with -DHCG_STAMPS: the tiled and streaming kernels record

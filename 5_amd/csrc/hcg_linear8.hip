@@ -1,0 +1,450 @@
+// hcg_linear8.hip -- the product of two quantised matrices, y = x w^T
+// (include/hcg_fp8.h):
+//
+//   y[t][v] = sum_b sx[t][b] sw[v][b] sum_{k in b} x[t][k] w[v][k]
+//
+// over blocks b of 128 inputs (sw per row v or per 128 of them).  One
+// v_mfma_f32_16x16x128 takes a block: w's rows on its M side (a lane's four
+// registers, consecutive outputs of a token), tokens on its N side (lanes), so
+// that a token's scale is one value per lane.  Both operands' lanes hold the
+// same 32 of a block's inputs, l / 16 of them; which, makes no difference.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "hcg_scale8.h"
+#include "hcg_tile8.h"
+#include "hcg_vec.h"
+
+namespace {
+
+using hcg::ElemOf;
+using hcg::u32x4;
+using hcg::fp8::Args;
+using hcg::fp8::f32x4;
+using hcg::fp8::Halves;
+using hcg::fp8::halves;
+using hcg::fp8::i32x8;
+using hcg::fp8::join;
+using hcg::fp8::kBlock;
+using hcg::fp8::kPower;
+using hcg::fp8::kRow;
+using hcg::fp8::kTile;
+using hcg::fp8::mfma;
+using hcg::fp8::Scaling;
+
+typedef uint32_t u32x4b __attribute__((ext_vector_type(4), aligned(1)));
+
+// 16 bytes at p, of which the first `left` are in the row (the rest zero, not read).
+__device__ __forceinline__ u32x4 load16(const unsigned char* p, int left) {
+  if (left >= 16) return *reinterpret_cast<const u32x4b*>(p);
+  u32x4 r{0, 0, 0, 0};
+#pragma unroll
+  for (int b = 0; b < 16; ++b)
+    if (b < left) r[b >> 2] |= (uint32_t)p[b] << (8 * (b & 3));
+  return r;
+}
+// Four consecutive outputs of a token, the first `valid` of them in the row.
+__device__ __forceinline__ void store4(const Args& g, int64_t t, int v, f32x4 f) {
+  const int valid = g.V - v;
+  if (valid <= 0) return;
+  if (g.y_dtype == HCG_F32) {
+    float* p = static_cast<float*>(g.y) + t * g.ldy + v;
+    typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+    if (valid >= 4) {
+      *reinterpret_cast<f32x4u*>(p) = f;
+    } else {
+      for (int e = 0; e < valid; ++e) p[e] = f[e];
+    }
+    return;
+  }
+  uint16_t h[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    h[e] = g.y_dtype == HCG_F16 ? __builtin_bit_cast(uint16_t, (_Float16)f[e])
+                                : __builtin_bit_cast(uint16_t, (__bf16)f[e]);
+  uint16_t* p = static_cast<uint16_t*>(g.y) + t * g.ldy + v;
+  typedef uint32_t u32x2h __attribute__((ext_vector_type(2), aligned(2)));
+  if (valid >= 4) {
+    *reinterpret_cast<u32x2h*>(p) = u32x2h{(uint32_t)h[0] | (uint32_t)h[1] << 16, (uint32_t)h[2] | (uint32_t)h[3] << 16};
+  } else {
+    for (int e = 0; e < valid; ++e) p[e] = h[e];
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Operands straight into registers
+// ---------------------------------------------------------------------------
+
+// A scale as a float.
+__device__ __forceinline__ float power(uint32_t byte) {
+  return __builtin_bit_cast(float, byte == 0 ? 0x00400000u : byte == 255 ? 0x7fc00000u : byte << 23);
+}
+template <Scaling SC>
+__device__ __forceinline__ float scale_at(const void* p, int64_t at) {
+  if constexpr (SC == kPower) return power(static_cast<const unsigned char*>(p)[at]);
+  return static_cast<const float*>(p)[at];
+}
+
+// A workgroup takes 16 rows of the weight and 16 NI tokens; its waves take the
+// blocks of K in turn and their sums meet in LDS, in the order of the waves.
+constexpr int kStreamWaves = 4;
+
+template <bool X5, Scaling SC, bool EXACT, int NI>
+__global__ __launch_bounds__(64 * kStreamWaves) void stream_kernel(Args g) {
+  __shared__ f32x4 meet[kStreamWaves][NI][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int tiles_v = (g.V + 15) / 16;
+  const int64_t wg = hcg::workgroup();
+  const int v0 = (int)(wg % tiles_v) * 16;
+  const int64_t t0 = wg / tiles_v * (16 * NI);
+  if (t0 >= g.T) return;
+  // (Rows past the ends read the last one; their results go nowhere.)
+  const int v = min(v0 + (lane & 15), g.V - 1);
+  const unsigned char* w = g.w + v * g.ldw;
+  const unsigned char* x[NI];
+  int64_t sx[NI];
+#pragma unroll
+  for (int j = 0; j < NI; ++j) {
+    const int64_t t = min(t0 + j * 16 + (lane & 15), (int64_t)g.T - 1);
+    x[j] = g.x + t * g.ldx;
+    sx[j] = t * g.sx_row;
+  }
+  f32x4 acc[NI];
+#pragma unroll
+  for (int j = 0; j < NI; ++j) acc[j] = f32x4{};
+  const int blocks = (g.K + kBlock - 1) / kBlock;
+  for (int b = wave; b < blocks; b += kStreamWaves) {
+    const int k = b * kBlock + (lane >> 4) * 32, left = g.K - k;
+    const i32x8 fw = join(load16(w + k, left), load16(w + k + 16, left - 16));
+#pragma unroll
+    for (int j = 0; j < NI; ++j) {
+      const i32x8 fx = join(load16(x[j] + k, left), load16(x[j] + k + 16, left - 16));
+      if constexpr (SC == kPower && !EXACT) {
+        const int ew = static_cast<const unsigned char*>(g.sw)[(g.w_tile ? v / kBlock : v) * g.sw_row + b * g.sw_block];
+        const int ex = static_cast<const unsigned char*>(g.sx)[sx[j] + b * g.sx_block];
+        acc[j] = mfma<X5>(fw, fx, acc[j], ew, ex);
+      } else {
+        f32x4 part;
+        if constexpr (EXACT)
+          part = mfma(halves<false>(fw), halves<X5>(fx));
+        else
+          part = mfma<X5>(fw, fx, f32x4{});
+        const float fx_scale = scale_at<SC>(g.sx, sx[j] + b * g.sx_block);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int vr = min(v0 + 4 * (lane >> 4) + r, g.V - 1);
+          const int64_t row = SC == kTile || (SC == kPower && g.w_tile) ? vr / kBlock : vr;
+          acc[j][r] = __builtin_fmaf(part[r], fx_scale * scale_at<SC>(g.sw, row * g.sw_row + b * g.sw_block), acc[j][r]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < NI; ++j) meet[wave][j][lane] = acc[j];
+  __syncthreads();
+  for (int j = wave; j < NI; j += kStreamWaves) {
+    f32x4 sum = meet[0][j][lane];
+#pragma unroll
+    for (int q = 1; q < kStreamWaves; ++q) sum += meet[q][j][lane];
+    const int64_t t = t0 + j * 16 + (lane & 15);
+    if (t < g.T) store4(g, t, v0 + 4 * (lane >> 4), sum);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// What the tiled kernel does not take as it is
+// ---------------------------------------------------------------------------
+
+// Rows of `width` bytes at any address into rows of whole 16 bytes (zeros past
+// the width).
+__global__ __launch_bounds__(256) void copy_rows_kernel(const unsigned char* from, int64_t ld, int64_t rows, int width,
+                                                        unsigned char* to, int64_t ldt) {
+  const int64_t vecs = ldt / 16, total = rows * vecs;
+  for (int64_t at = hcg::workgroup() * 256 + threadIdx.x; at < total; at += (int64_t)gridDim.x * gridDim.y * 256) {
+    const int64_t row = at / vecs;
+    const int c = (int)(at - row * vecs) * 16;
+    *reinterpret_cast<u32x4*>(to + row * ldt + c) = load16(from + row * ld + c, width - c);
+  }
+}
+
+// Scales in any strides to rows next to each other, block by block, as floats or
+// (e8m0 to e8m0) bytes; zeros in rows past `rows`.
+__global__ __launch_bounds__(256) void copy_scales_kernel(const void* from, int64_t row_stride, int64_t block_stride,
+                                                          int64_t rows, int64_t blocks, void* to, int64_t ldt,
+                                                          bool from_e8m0, bool to_e8m0) {
+  const int64_t total = blocks * ldt;
+  for (int64_t at = hcg::workgroup() * 256 + threadIdx.x; at < total; at += (int64_t)gridDim.x * gridDim.y * 256) {
+    const int64_t block = at / ldt, row = at - block * ldt;
+    const int64_t src = row * row_stride + block * block_stride;
+    if (to_e8m0)
+      static_cast<unsigned char*>(to)[at] = row < rows ? static_cast<const unsigned char*>(from)[src] : 0;
+    else
+      static_cast<float*>(to)[at] = row >= rows  ? 0.f
+                                    : from_e8m0 ? power(static_cast<const unsigned char*>(from)[src])
+                                                : static_cast<const float*>(from)[src];
+  }
+}
+
+// The splits' sums, added in order, rounded.
+template <class T>
+__global__ __launch_bounds__(256) void join_kernel(const float* part, int64_t ld_part, int splits, int64_t tokens, int V,
+                                                   T* y, int64_t ldy) {
+  const int64_t vecs = ld_part / 4, total = tokens * vecs;
+  for (int64_t at = hcg::workgroup() * 256 + threadIdx.x; at < total; at += (int64_t)gridDim.x * gridDim.y * 256) {
+    const int64_t t = at / vecs;
+    const int v = (int)(at - t * vecs) * 4;
+    const float* p = part + t * ld_part + v;
+    f32x4 sum{};
+#pragma unroll 4
+    for (int s = 0; s < splits; ++s) sum += *reinterpret_cast<const f32x4*>(p + s * tokens * ld_part);
+    T* row = y + t * ldy;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (v + e < V) row[v + e] = (T)sum[e];
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host
+// ---------------------------------------------------------------------------
+
+constexpr int64_t kMaxInputs = 4000000;  // and row strides: a tile's offsets stay in 31 bits
+constexpr int64_t kMaxRows = (int64_t)1 << 26;
+
+int64_t round_up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Tile shapes: rows of outputs and tokens.
+enum Shape { kStream, kLarge, kMedium, kNumShapes };
+struct ShapeInfo {
+  int tm, tn;
+};
+constexpr ShapeInfo kShapes[kNumShapes] = {{0, 0}, {256, 256}, {128, 128}};
+
+struct Plan {
+  Shape shape;
+  int splits, chunk;
+  bool copy_x, copy_w, copy_sx, copy_sw;
+  int64_t ldx, ldw, lds_x, lds_w, ld_part;                // of the copies
+  int64_t x, w, sx, sw, part, total;                      // offsets into the workspace
+};
+
+struct Problem {
+  int algo;
+  int64_t tokens, outputs, inputs;
+  const void* x;
+  int64_t ldx;
+  const void* w;
+  int64_t ldw;
+  bool w_tile, e8m0, exact;
+  int64_t sx_row, sw_row, sw_block;
+  const void* sw;
+};
+
+bool in_place(const void* p, int64_t ld, int64_t rows) {
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (rows == 1 || ld % 16 == 0);
+}
+
+Plan make_plan(const Problem& q) {
+  Plan p{};
+  if (q.algo == HCG_FP8_AUTO)
+    p.shape = q.tokens <= 64 ? kStream : kMedium;
+  else
+    p.shape = (Shape)(q.algo - HCG_FP8_STREAM);
+  if (p.shape == kLarge && (q.exact || (!q.w_tile && !q.e8m0))) p.shape = kMedium;
+  p.splits = 1;
+  p.chunk = (int)round_up(q.inputs, kBlock);
+  if (p.shape == kStream) return p;
+  const int64_t blocks = ceil_div(q.inputs, kBlock);
+  const bool floats = q.exact || !q.e8m0;  // scales that the kernel takes
+  p.copy_x = !in_place(q.x, q.ldx, q.tokens);
+  p.copy_w = !in_place(q.w, q.ldw, q.outputs);
+  p.ldx = p.ldw = round_up(q.inputs, 16);
+  p.copy_sx = (q.tokens > 1 && q.sx_row != 1) || (q.e8m0 && floats);
+  p.lds_x = q.tokens;
+  // The weight's rows are read in whole, aligned fours.
+  const int64_t rows = q.w_tile ? ceil_div(q.outputs, kBlock) : q.outputs;
+  p.copy_sw = (rows > 1 && q.sw_row != 1) || (q.e8m0 && floats) ||
+              (floats && !q.w_tile && (rows % 4 || (blocks > 1 && q.sw_block % 4) || (reinterpret_cast<uintptr_t>(q.sw) & 15)));
+  p.lds_w = round_up(rows, 4);
+  p.ld_part = round_up(q.outputs, 4);
+  int64_t at = 0;
+  const auto take = [&](bool wanted, int64_t bytes) {
+    const int64_t here = at;
+    if (wanted) at += round_up(bytes, 256);
+    return here;
+  };
+  p.x = take(p.copy_x, q.tokens * p.ldx);
+  p.w = take(p.copy_w, q.outputs * p.ldw);
+  p.sx = take(p.copy_sx, blocks * p.lds_x * 4);
+  p.sw = take(p.copy_sw, blocks * p.lds_w * 4);
+  p.part = take(p.splits > 1, p.splits * q.tokens * p.ld_part * 4);
+  p.total = at;
+  return p;
+}
+
+template <bool X5, Scaling SC, bool EXACT>
+void run_stream(const Args& a, hipStream_t s) {
+  const int64_t tiles_v = (a.V + 15) / 16;
+  if (a.T <= 16)
+    stream_kernel<X5, SC, EXACT, 1><<<hcg::grid_of(tiles_v), 64 * kStreamWaves, 0, s>>>(a);
+  else
+    stream_kernel<X5, SC, EXACT, 4><<<hcg::grid_of(tiles_v * ((a.T + 63) / 64)), 64 * kStreamWaves, 0, s>>>(a);
+}
+
+template <bool X5, Scaling SC, bool EXACT>
+void run_tiles(Shape shape, const Args& a, hipStream_t s) {
+  const dim3 grid((unsigned)(ceil_div(a.V, kShapes[shape].tm) * ceil_div(a.T, kShapes[shape].tn) * a.splits));
+  if constexpr (SC != kRow && !EXACT) {
+    if (shape == kLarge)
+      return hcg::fp8::tile_kernel<X5, SC, EXACT, 256, 256, 2, 4, 5><<<grid, 512, 0, s>>>(a);
+  }
+  if constexpr (SC == kRow || EXACT)
+    hcg::fp8::tile_kernel<X5, SC, EXACT, 128, 128, 2, 2, 5><<<grid, 256, 0, s>>>(a);
+  else
+    hcg::fp8::tile_kernel<X5, SC, EXACT, 128, 128, 2, 4, 5><<<grid, 512, 0, s>>>(a);
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t hcg_linear_fp8_workspace(int algo, int64_t tokens, int64_t outputs, int64_t inputs, const void* x, int64_t ldx,
+                                 const void* weight, int64_t ldw, int scale_dtype, int64_t xs_row, int w_tile,
+                                 const void* w_scale, int64_t ws_row, int64_t ws_block, int out_dtype) {
+  if (tokens <= 0 || outputs <= 0 || inputs <= 0) return 0;
+  return make_plan(Problem{algo, tokens, outputs, inputs, x, ldx, weight, ldw, w_tile != 0, scale_dtype == HCG_E8M0,
+                           out_dtype == HCG_F32, xs_row, ws_row, ws_block, w_scale})
+      .total;
+}
+
+int hcg_linear_fp8(int algo, int x_dtype, const void* x, int64_t ldx, int64_t tokens, const void* weight, int64_t ldw,
+                   int64_t outputs, int64_t inputs, int scale_dtype, const void* x_scale, int64_t xs_row,
+                   int64_t xs_block, int w_tile, const void* w_scale, int64_t ws_row, int64_t ws_block, int out_dtype,
+                   void* y, int64_t ldy, void* workspace, int64_t workspace_bytes, void* stream) {
+  HCG_LM_REQUIRE(algo >= HCG_FP8_AUTO && algo <= HCG_FP8_128x128, "unknown algo %d", algo);
+  HCG_LM_REQUIRE(hcg::fp8::type_ok(x_dtype), "x's type %d is not HCG_E4M3 or HCG_E5M2", x_dtype);
+  HCG_LM_REQUIRE(hcg::fp8::scale_ok(scale_dtype), "scales of type %d are not HCG_F32 or HCG_E8M0", scale_dtype);
+  HCG_LM_REQUIRE(hcg::elem_ok(out_dtype), "the output's type %d is not HCG_F16, HCG_BF16 or HCG_F32", out_dtype);
+  HCG_LM_REQUIRE(tokens >= 0 && tokens < kMaxRows && outputs >= 0 && outputs < kMaxRows && inputs >= 0 &&
+                     inputs < kMaxInputs,
+                 "%lld tokens, %lld outputs and %lld inputs are out of range", (long long)tokens, (long long)outputs,
+                 (long long)inputs);
+  if (tokens == 0 || outputs == 0) return HCG_OK;
+  HCG_LM_REQUIRE(inputs > 0, "a product over no inputs");
+  HCG_LM_REQUIRE(x && weight && x_scale && w_scale && y, "null pointer");
+  HCG_LM_REQUIRE((tokens == 1 || (ldx >= inputs && ldy >= outputs)) && (outputs == 1 || ldw >= inputs),
+                 "row stride below the width");
+  HCG_LM_REQUIRE((tokens == 1 || ldx < kMaxInputs) && (outputs == 1 || ldw < kMaxInputs),
+                 "row strides of %lld and %lld are out of range", (long long)ldx, (long long)ldw);
+  HCG_LM_REQUIRE(hcg::elem_aligned(y, hcg::elem_bytes(out_dtype)), "rows must be aligned to their elements");
+  const int sb = hcg::fp8::scale_bytes(scale_dtype);
+  HCG_LM_REQUIRE(hcg::elem_aligned(x_scale, sb) && hcg::elem_aligned(w_scale, sb), "scales must be aligned");
+  const bool e8m0 = scale_dtype == HCG_E8M0, exact = out_dtype == HCG_F32;
+  const Plan p = make_plan(Problem{algo, tokens, outputs, inputs, x, ldx, weight, ldw, w_tile != 0, e8m0, exact, xs_row,
+                                   ws_row, ws_block, w_scale});
+  HCG_LM_REQUIRE(p.total == 0 || (workspace && workspace_bytes >= p.total && hcg::elem_aligned(workspace, 256)),
+                 "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)p.total);
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  char* const ws = static_cast<char*>(workspace);
+  Args a{static_cast<const unsigned char*>(x),
+         static_cast<const unsigned char*>(weight),
+         tokens == 1 ? 0 : ldx,
+         outputs == 1 ? 0 : ldw,
+         x_scale,
+         w_scale,
+         xs_row,
+         xs_block,
+         ws_row,
+         ws_block,
+         w_tile != 0,
+         (int)tokens,
+         (int)outputs,
+         (int)inputs,
+         y,
+         ldy,
+         out_dtype,
+         p.splits,
+         p.chunk,
+         reinterpret_cast<float*>(ws + p.part),
+         p.ld_part};
+  const auto grid = [](int64_t items) { return dim3((unsigned)std::min<int64_t>(ceil_div(items, 256), 1 << 14)); };
+  const int64_t blocks = ceil_div(inputs, kBlock), w_rows = w_tile ? ceil_div(outputs, kBlock) : outputs;
+  if (p.copy_x) {
+    unsigned char* to = reinterpret_cast<unsigned char*>(ws + p.x);
+    copy_rows_kernel<<<grid(tokens * p.ldx / 16), 256, 0, s>>>(a.x, a.ldx, tokens, a.K, to, p.ldx);
+    a.x = to;
+    a.ldx = p.ldx;
+  }
+  if (p.copy_w) {
+    unsigned char* to = reinterpret_cast<unsigned char*>(ws + p.w);
+    copy_rows_kernel<<<grid(outputs * p.ldw / 16), 256, 0, s>>>(a.w, a.ldw, outputs, a.K, to, p.ldw);
+    a.w = to;
+    a.ldw = p.ldw;
+  }
+  const bool bytes = e8m0 && !exact;
+  if (p.copy_sx) {
+    void* to = ws + p.sx;
+    copy_scales_kernel<<<grid(blocks * p.lds_x), 256, 0, s>>>(x_scale, xs_row, xs_block, tokens, blocks, to, p.lds_x, e8m0,
+                                                              bytes);
+    a.sx = to;
+    a.sx_block = p.lds_x;
+  }
+  if (p.copy_sw) {
+    void* to = ws + p.sw;
+    copy_scales_kernel<<<grid(blocks * p.lds_w), 256, 0, s>>>(w_scale, ws_row, ws_block, w_rows, blocks, to, p.lds_w, e8m0,
+                                                              bytes);
+    a.sw = to;
+    a.sw_block = p.lds_w;
+  }
+  const auto with = [&](auto x5, auto scaling, auto exactly) {
+    constexpr bool X5 = decltype(x5)::value, EXACT = decltype(exactly)::value;
+    constexpr Scaling SC = decltype(scaling)::value;
+    if (p.shape == kStream) {
+      run_stream<X5, SC, EXACT>(a, s);
+    } else if constexpr (SC == kPower && EXACT) {
+      if (w_tile)
+        run_tiles<X5, kTile, true>(p.shape, a, s);
+      else
+        run_tiles<X5, kRow, true>(p.shape, a, s);
+    } else {
+      run_tiles<X5, SC, EXACT>(p.shape, a, s);
+    }
+  };
+  const auto with_scales = [&](auto x5, auto exactly) {
+    if (e8m0)
+      with(x5, std::integral_constant<Scaling, kPower>{}, exactly);
+    else if (w_tile)
+      with(x5, std::integral_constant<Scaling, kTile>{}, exactly);
+    else
+      with(x5, std::integral_constant<Scaling, kRow>{}, exactly);
+  };
+  const auto with_x = [&](auto exactly) {
+    if (x_dtype == HCG_E5M2)
+      with_scales(std::true_type{}, exactly);
+    else
+      with_scales(std::false_type{}, exactly);
+  };
+  if (exact)
+    with_x(std::true_type{});
+  else
+    with_x(std::false_type{});
+  if (p.splits > 1) {
+    const dim3 all = grid(tokens * p.ld_part / 4);
+    switch (out_dtype) {
+      case HCG_F16:
+        join_kernel<<<all, 256, 0, s>>>(a.part, p.ld_part, p.splits, tokens, a.V, static_cast<_Float16*>(y), ldy);
+        break;
+      case HCG_BF16:
+        join_kernel<<<all, 256, 0, s>>>(a.part, p.ld_part, p.splits, tokens, a.V, static_cast<__bf16*>(y), ldy);
+        break;
+      default: join_kernel<<<all, 256, 0, s>>>(a.part, p.ld_part, p.splits, tokens, a.V, static_cast<float*>(y), ldy);
+    }
+  }
+  HCG_LM_HIP_CHECK(hipGetLastError());
+  return HCG_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,190 @@
+// hcg_quantize.hip -- quantises a matrix to 8-bit floating point with a scale
+// for each 128 columns of a row or each 128 x 128 tile, also transposed
+// (include/hcg_fp8.h).
+//
+//   a = max |x| over the block, s = a / F, q = rne(x F / a).
+//
+// Bound by HBM: a workgroup reads a 128 x 128 tile of x once, whole 16-byte
+// vectors, all of them in flight, and holds it in registers (8 x 8 values per
+// thread) between the maximum and the result.  Transposed, the bytes pass
+// through LDS, so that both sides are whole lines.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "hcg_scale8.h"
+#include "hcg_vec.h"
+
+namespace {
+
+using hcg::ElemOf;
+using hcg::fp8::kBlock;
+
+struct QuantArgs {
+  const void* x;
+  int64_t ldx, rows, cols;
+  int64_t tiles_c;  // tiles along x's columns
+  hcg::fp8::Out out;
+};
+
+constexpr int kThreads = 256;
+constexpr int kSide = 8;                     // a thread's rows and columns
+constexpr int kAcross = kBlock / kSide;      // threads along either side of a tile
+constexpr int kPitch = kBlock + 16;          // bytes between rows in LDS
+
+__device__ __forceinline__ uint32_t shfl_max(uint32_t v, int mask) {
+  return max(v, (uint32_t)__shfl_xor((int)v, mask));
+}
+
+// Thread (i, j) = (tid / 16, tid % 16) holds rows 8 i ... and columns 8 j ... of
+// the workgroup's tile.
+template <class T, bool TRANS, bool TILE>
+__global__ __launch_bounds__(kThreads) void quantize_kernel(QuantArgs g) {
+  __shared__ uint32_t meet[4 * kBlock];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int i = tid / kAcross, j = tid % kAcross;
+  const int64_t tile = hcg::workgroup();
+  const int64_t tr = tile / g.tiles_c, tc = tile - tr * g.tiles_c;
+  const int64_t row0 = tr * kBlock + i * kSide, col0 = tc * kBlock + j * kSide;
+  const int rows = (int)min((int64_t)kSide, g.rows - row0), cols = (int)min((int64_t)kSide, g.cols - col0);
+  if (tr * kBlock >= g.rows) return;  // (a whole workgroup past the grid's last tile)
+
+  float v[kSide][kSide];
+#pragma unroll
+  for (int r = 0; r < kSide; ++r) {
+    const int valid = r < rows ? cols : 0;
+#pragma unroll
+    for (int e = 0; e < kSide; ++e) v[r][e] = 0.f;
+    if (valid > 0) hcg::load_floats<T, kSide>(static_cast<const T*>(g.x) + (row0 + r) * g.ldx + col0, valid, v[r]);
+  }
+
+  hcg::fp8::Scale s[kSide];  // per row of q that the thread holds (TILE: the first alone)
+  if constexpr (TILE) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int r = 0; r < kSide; ++r)
+#pragma unroll
+      for (int e = 0; e < kSide; ++e) top = max(top, hcg::fp8::magnitude(v[r][e]));
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) top = shfl_max(top, m);
+    if (lane == 0) meet[wave] = top;
+    __syncthreads();
+    top = max(max(meet[0], meet[1]), max(meet[2], meet[3]));
+    s[0] = hcg::fp8::scale_of(top, g.out.e5m2, g.out.e8m0);
+    if (tid == 0) hcg::fp8::put_scale(g.out, TRANS ? tc : tr, TRANS ? tr : tc, s[0].held);
+  } else if constexpr (TRANS) {
+    // A row of q is a column of x.
+#pragma unroll
+    for (int e = 0; e < kSide; ++e) {
+      uint32_t top = 0;
+#pragma unroll
+      for (int r = 0; r < kSide; ++r) top = max(top, hcg::fp8::magnitude(v[r][e]));
+      top = shfl_max(shfl_max(top, 16), 32);
+      if (lane < kAcross) meet[wave * kBlock + j * kSide + e] = top;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < kSide; ++e) {
+      const int c = j * kSide + e;
+      const uint32_t top = max(max(meet[c], meet[kBlock + c]), max(meet[2 * kBlock + c], meet[3 * kBlock + c]));
+      s[e] = hcg::fp8::scale_of(top, g.out.e5m2, g.out.e8m0);
+      if (i == 0 && e < cols) hcg::fp8::put_scale(g.out, col0 + e, tr, s[e].held);
+    }
+  } else {
+#pragma unroll
+    for (int r = 0; r < kSide; ++r) {
+      uint32_t top = 0;
+#pragma unroll
+      for (int e = 0; e < kSide; ++e) top = max(top, hcg::fp8::magnitude(v[r][e]));
+#pragma unroll
+      for (int m = kAcross / 2; m >= 1; m >>= 1) top = shfl_max(top, m);
+      s[r] = hcg::fp8::scale_of(top, g.out.e5m2, g.out.e8m0);
+      if (j == 0 && r < rows) hcg::fp8::put_scale(g.out, row0 + r, tc, s[r].held);
+    }
+  }
+
+  if constexpr (!TRANS) {
+    if (cols <= 0) return;
+#pragma unroll
+    for (int r = 0; r < kSide; ++r)
+      if (r < rows)
+        hcg::fp8::store_q<kSide>(g.out.q + (row0 + r) * g.out.ldq + col0, v[r], s[TILE ? 0 : r].inverse, cols,
+                                 g.out.e5m2);
+  } else {
+    __shared__ __attribute__((aligned(16))) unsigned char turned[kBlock * kPitch];
+#pragma unroll
+    for (int e = 0; e < kSide; ++e) {
+      float f[kSide];
+#pragma unroll
+      for (int r = 0; r < kSide; ++r) f[r] = v[r][e];
+      hcg::fp8::store_q<kSide>(turned + (j * kSide + e) * kPitch + i * kSide, f, s[TILE ? 0 : e].inverse, kSide,
+                               g.out.e5m2);
+    }
+    __syncthreads();
+    // Rows of q by 8 lanes each, 16 bytes a lane.
+    const int part = tid & 7;
+    const int left = (int)min((int64_t)16, g.rows - (tr * kBlock + part * 16));
+    typedef uint32_t u32x4a __attribute__((ext_vector_type(4), aligned(1)));
+#pragma unroll
+    for (int c = tid >> 3; c < kBlock; c += kThreads / 8) {
+      if (tc * kBlock + c >= g.cols || left <= 0) continue;
+      const unsigned char* from = turned + c * kPitch + part * 16;
+      unsigned char* to = g.out.q + (tc * kBlock + c) * g.out.ldq + tr * kBlock + part * 16;
+      if (left == 16) {
+        *reinterpret_cast<u32x4a*>(to) = *reinterpret_cast<const hcg::raw4*>(from);
+      } else {
+        for (int b = 0; b < left; ++b) to[b] = from[b];
+      }
+    }
+  }
+}
+
+template <class T>
+void launch(const QuantArgs& a, bool transpose, bool tile, hipStream_t s) {
+  const dim3 grid = hcg::grid_of(a.tiles_c * ((a.rows + kBlock - 1) / kBlock));
+  if (transpose && tile)
+    quantize_kernel<T, true, true><<<grid, kThreads, 0, s>>>(a);
+  else if (transpose)
+    quantize_kernel<T, true, false><<<grid, kThreads, 0, s>>>(a);
+  else if (tile)
+    quantize_kernel<T, false, true><<<grid, kThreads, 0, s>>>(a);
+  else
+    quantize_kernel<T, false, false><<<grid, kThreads, 0, s>>>(a);
+}
+
+}  // namespace
+
+extern "C" int hcg_quantize_fp8(int dtype, const void* x, int64_t ldx, int64_t rows, int64_t cols, int transpose,
+                                int tile, int q_dtype, void* q, int64_t ldq, int scale_dtype, void* scale,
+                                int64_t scale_row, int64_t scale_block, void* stream) {
+  HCG_LM_REQUIRE(hcg::elem_ok(dtype), "dtype %d is not HCG_F16, HCG_BF16 or HCG_F32", dtype);
+  HCG_LM_REQUIRE(hcg::fp8::type_ok(q_dtype), "q's type %d is not HCG_E4M3 or HCG_E5M2", q_dtype);
+  HCG_LM_REQUIRE(hcg::fp8::scale_ok(scale_dtype), "scales of type %d are not HCG_F32 or HCG_E8M0", scale_dtype);
+  constexpr int64_t kMost = (int64_t)1 << 31;
+  HCG_LM_REQUIRE(rows >= 0 && rows < kMost && cols >= 0 && cols < kMost, "a matrix of %lld x %lld is out of range",
+                 (long long)rows, (long long)cols);
+  if (rows == 0 || cols == 0) return HCG_OK;
+  HCG_LM_REQUIRE(x && q && scale, "null pointer");
+  const int64_t qrows = transpose ? cols : rows, qcols = transpose ? rows : cols;
+  HCG_LM_REQUIRE((rows == 1 || ldx >= cols) && (qrows == 1 || ldq >= qcols), "row stride below the width");
+  HCG_LM_REQUIRE(hcg::elem_aligned(x, hcg::elem_bytes(dtype)), "rows must be aligned to their elements");
+  HCG_LM_REQUIRE(hcg::elem_aligned(scale, hcg::fp8::scale_bytes(scale_dtype)), "scales must be aligned");
+  const int64_t tiles_c = (cols + kBlock - 1) / kBlock, tiles_r = (rows + kBlock - 1) / kBlock;
+  HCG_LM_REQUIRE(tiles_c * tiles_r < (int64_t)1 << 36, "a matrix of %lld x %lld is out of range", (long long)rows,
+                 (long long)cols);
+  const QuantArgs a{x,
+                    ldx,
+                    rows,
+                    cols,
+                    tiles_c,
+                    {static_cast<unsigned char*>(q), scale, ldq, scale_row, scale_block, q_dtype == HCG_E5M2,
+                     scale_dtype == HCG_E8M0}};
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  switch (dtype) {
+    case HCG_F16: launch<ElemOf<HCG_F16>::type>(a, transpose, tile, s); break;
+    case HCG_BF16: launch<ElemOf<HCG_BF16>::type>(a, transpose, tile, s); break;
+    default: launch<float>(a, transpose, tile, s);
+  }
+  HCG_LM_HIP_CHECK(hipGetLastError());
+  return HCG_OK;
+}

@@ -1,0 +1,584 @@
+// hcg_tile8.h -- the tiled product of two quantised matrices on gfx950 (device
+// code).
+//
+// A TM x TN tile of outputs x tokens by WM x WN waves; K advances one block of 128
+// (a scale each) per stage.  A stage is two units, the weight's rows and x's, of
+// 128 bytes a row; a ring of UNITS LDS units is filled by global-to-LDS DMA.  One
+// barrier per stage: past it every wave has read the stage before, whose two
+// units are refilled UNITS units ahead.  The 16-byte chunks of an LDS row are
+// XOR-swizzled so that the 16 lanes that read a fragment's column of chunks
+// cover all banks.
+//
+// A 16-bit result takes v_mfma_f32_16x16x128 on the bytes as they are: a block's
+// products in one instruction, whose sum is multiplied by both scales into the
+// accumulators, or whose scales are the instruction's own (e8m0), which then
+// adds up all of K.  The instruction cuts each product of 8 neighbours to
+// multiples of 2^-13 of the largest exponent among them (measured: beside 448 *
+// 448 the bits below 2^3 are lost), 1.5e-5 of a sum of 128 random products: less
+// than a 16-bit result's rounding, but not float32.  So a float32 result (EXACT)
+// takes the bytes as f16, which holds both formats, in v_mfma_f32_16x16x32,
+// whose sums are within 2^-22 of the magnitudes.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <type_traits>
+
+#include "hcg_scale8.h"
+#include "hcg_tile.h"
+
+namespace hcg {
+namespace fp8 {
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+// How scales are held and used.
+enum Scaling {
+  kTile,  // float32, the weight's by tiles
+  kRow,   // float32, the weight's by rows
+  kPower  // exponent bytes, which the MFMA takes itself
+};
+
+struct Args {
+  const unsigned char* x;
+  const unsigned char* w;
+  int64_t ldx, ldw;
+  const void* sx;
+  const void* sw;
+  int64_t sx_row, sx_block, sw_row, sw_block;  // (tiled: the rows' strides are 1)
+  bool w_tile;                                 // kPower: the weight's scales are by tiles
+  int T, V, K;
+  void* y;
+  int64_t ldy;
+  int y_dtype;
+  // Tiled: K in splits of `chunk` (a multiple of kBlock); where there are more than
+  // one, float32 sums go to part[split][T][ld_part].
+  int splits, chunk;
+  float* part;
+  int64_t ld_part;
+};
+
+// c + w-block . x-block, 128 deep.  X5: x is e5m2.
+template <bool X5>
+__device__ __forceinline__ f32x4 mfma(i32x8 w, i32x8 x, f32x4 c) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, c, 0, X5 ? 1 : 0, 0, 0, 0, 0);
+}
+template <bool X5>
+__device__ __forceinline__ f32x4 mfma(i32x8 w, i32x8 x, f32x4 c, int sw, int sx) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, c, 0, X5 ? 1 : 0, 0, sw, 0, sx);
+}
+
+// 8 bytes as f16, exactly (a byte of e5m2 is an f16's upper one).
+template <bool E5>
+__device__ __forceinline__ f16x8 halves(int lo, int hi) {
+  uint32_t r[4];
+  if constexpr (E5) {
+    r[0] = __builtin_amdgcn_perm(0u, (uint32_t)lo, 0x010c000cu);
+    r[1] = __builtin_amdgcn_perm(0u, (uint32_t)lo, 0x030c020cu);
+    r[2] = __builtin_amdgcn_perm(0u, (uint32_t)hi, 0x010c000cu);
+    r[3] = __builtin_amdgcn_perm(0u, (uint32_t)hi, 0x030c020cu);
+  } else {
+    r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((uint32_t)lo, 1.f, false));
+    r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((uint32_t)lo, 1.f, true));
+    r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((uint32_t)hi, 1.f, false));
+    r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((uint32_t)hi, 1.f, true));
+  }
+  return __builtin_bit_cast(f16x8, u32x4{r[0], r[1], r[2], r[3]});
+}
+struct Halves {
+  f16x8 v[4];
+};
+template <bool E5>
+__device__ __forceinline__ Halves halves(i32x8 b) {
+  Halves h;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) h.v[q] = halves<E5>(b[2 * q], b[2 * q + 1]);
+  return h;
+}
+// The same sum of 128 products, exactly.
+__device__ __forceinline__ f32x4 mfma(const Halves& w, const Halves& x) {
+  f32x4 c{};
+#pragma unroll
+  for (int q = 0; q < 4; ++q) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(w.v[q], x.v[q], c, 0, 0, 0);
+  return c;
+}
+
+__device__ __forceinline__ i32x8 join(u32x4 a, u32x4 b) {
+  return i32x8{(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)b[0], (int)b[1], (int)b[2], (int)b[3]};
+}
+
+__device__ __forceinline__ uint32_t pack_out(float a, float b, int dtype) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  if (dtype == HCG_F16) return __builtin_bit_cast(uint32_t, f16x2{(_Float16)a, (_Float16)b});
+  return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)a, (__bf16)b});
+}
+
+template <int N>
+__device__ __forceinline__ void wait_vm() {
+  static_assert(N >= 0 && N < 64, "vmcnt range");
+  __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | ((N >> 4) << 14));
+}
+__device__ __forceinline__ void wait_lgkm() { __builtin_amdgcn_s_waitcnt(0xc07f); }
+
+// Each unit is an LDS object of its own, named at compile time, so that the
+// compiler does not serialize a DMA into one with reads of another.
+template <int BYTES, int S>
+__device__ __forceinline__ unsigned char* ring_unit() {
+  __shared__ __attribute__((aligned(1024))) unsigned char buf[BYTES];
+  return buf;
+}
+
+// blockIdx -> (K split, tile): each XCD (id % 8) takes a contiguous run of
+// units, within a split in groups of 4 tile rows, so that the workgroups
+// sharing an L2 share operand rows.
+__device__ __forceinline__ void unit_of(int tiles_m, int tiles_n, int splits, int wg, int& split, int& tm, int& tn) {
+  const int nt = tiles_m * tiles_n, n = nt * splits;
+  const int per = n >> 3, rem = n & 7, xcd = wg & 7, idx = wg >> 3;
+  const int unit = xcd < rem ? xcd * (per + 1) + idx : rem * (per + 1) + (xcd - rem) * per + idx;
+  split = unit / nt;
+  const int logical = unit - split * nt;
+  const int span = 4 * tiles_n;
+  const int group = logical / span, first = group * 4;
+  const int size = min(tiles_m - first, 4);
+  const int in_group = logical - group * span;
+  tm = first + in_group % size;
+  tn = in_group / size;
+}
+
+// One operand's unit: ROWS rows of a block's 128 bytes, loaded by NW waves.
+template <int ROWS, int NW>
+struct Side {
+  static constexpr int kBytes = ROWS * kBlock;
+  static constexpr int kInst = kBytes / 1024 / NW;  // DMA instructions per wave per unit
+  static_assert(kInst >= 1 && kInst * NW * 1024 == kBytes, "a unit is whole DMA instructions of every wave");
+  static __device__ __forceinline__ int swz(int row, int c) { return c ^ ((row >> 1) & 7); }
+
+  int off[kInst];  // byte offset of the lane's chunk from the unit's first byte, or kOobOffset
+  int key[kInst];  // the chunk's first byte in its row
+
+  // extent: rows from the tile's first on.
+  __device__ __forceinline__ void init(int wave, int lane, int extent, int64_t ld) {
+#pragma unroll
+    for (int i = 0; i < kInst; ++i) {
+      const int row = (wave * kInst + i) * 8 + (lane >> 3);
+      key[i] = swz(row, lane & 7) * 16;
+      off[i] = row < extent ? row * (int)ld + key[i] : kOobOffset;
+    }
+  }
+  // Instructions FROM to TO - 1 of the wave's, of the unit whose first byte is at p
+  // and whose rows have `left` bytes from there on (FULL: all of them).  The
+  // resource starts at the unit, so offsets stay in 31 bits whatever the
+  // matrix's size; chunks out of range are redirected past its extent and load
+  // zeros.  The chunk with a row's last byte is loaded whole, from within its
+  // own 16-byte granule.
+  template <bool FULL, int FROM, int TO>
+  __device__ __forceinline__ void issue(const unsigned char* p, unsigned char* st, int wave, int left) const {
+    const __amdgpu_buffer_rsrc_t r = make_rsrc(p, 0x7fffffe0);
+#pragma unroll
+    for (int i = FROM; i < TO; ++i) {
+      lds_void* dst = (lds_void*)(st + (wave * kInst + i) * 1024);
+      if constexpr (FULL)
+        dma16(r, dst, off[i]);
+      else
+        dma16(r, dst, dma_offset(key[i] < left, off[i]));
+    }
+  }
+  // Zeros in place of what lies past `left` bytes in the chunk that holds them.
+  static __device__ __forceinline__ void cut(unsigned char* st, int tid, int left) {
+    for (int row = tid; row < ROWS; row += 64 * NW) {
+      u32x4* chunk = reinterpret_cast<u32x4*>(st + row * kBlock + swz(row, left >> 4) * 16);
+      u32x4 v = *chunk;
+      const int valid = left & 15;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int bytes = min(max(valid - 4 * e, 0), 4);
+        v[e] &= bytes == 4 ? 0xffffffffu : (1u << (8 * bytes)) - 1;
+      }
+      *chunk = v;
+    }
+  }
+  // The lane's fragment of rows 16 i ... past `base` (made from the wave's first).
+  static __device__ __forceinline__ int base_of(int lane, int first) {
+    const int row = lane & 15;
+    return (first + row) * kBlock + swz(row, 2 * (lane >> 4)) * 16;
+  }
+  static __device__ __forceinline__ i32x8 frag(const unsigned char* st, int base, int i) {
+    return join(*reinterpret_cast<const u32x4*>(st + base + i * 16 * kBlock),
+                *reinterpret_cast<const u32x4*>(st + (base ^ 16) + i * 16 * kBlock));
+  }
+};
+
+template <int I>
+using Int = std::integral_constant<int, I>;
+
+// Waves per SIMD: two workgroups per CU where the ring takes at most half its LDS.
+constexpr int waves_per_simd(int tm, int tn, int waves, int units) {
+  return waves / 4 * ((tm + tn) * kBlock * units / 2 <= 80 * 1024 ? 2 : 1);
+}
+
+template <bool X5, Scaling SC, bool EXACT, int TM, int TN, int WM, int WN, int UNITS>
+__global__ __launch_bounds__(64 * WM * WN, waves_per_simd(TM, TN, WM* WN, UNITS)) void tile_kernel(Args g) {
+  constexpr int NW = WM * WN;
+  constexpr int MI = TM / WM / 16, NI = TN / WN / 16;
+  static_assert(MI >= 2 && NI >= 1 && MI * WM * 16 == TM && NI * WN * 16 == TN, "wave tile");
+  static_assert(kBlock % (TM / WM) == 0, "a wave's outputs share a tile's scale");
+  static_assert(!EXACT || SC != kPower, "exact products take float32 scales");
+  using OpA = Side<TM, NW>;
+  using OpB = Side<TN, NW>;
+  // (In a ring of an even number of units a place holds units of one operand.)
+  constexpr int kUnitA = UNITS % 2 && OpB::kBytes > OpA::kBytes ? OpB::kBytes : OpA::kBytes;
+  constexpr int kUnitB = UNITS % 2 && OpA::kBytes > OpB::kBytes ? OpA::kBytes : OpB::kBytes;
+  static_assert(UNITS >= 4 && kUnitA * ((UNITS + 1) / 2) + kUnitB * (UNITS / 2) <= 160 * 1024, "ring");
+  auto place = [](auto uc) {
+    constexpr int P = decltype(uc)::value % UNITS;
+    return ring_unit<P % 2 ? kUnitB : kUnitA, P>();
+  };
+  constexpr int kPeriod = UNITS % 2 ? UNITS : UNITS / 2;  // stages until the units' places repeat
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+  const int tiles_m = (g.V + TM - 1) / TM, tiles_n = (g.T + TN - 1) / TN;
+  int split, tm, tn;
+  unit_of(tiles_m, tiles_n, g.splits, blockIdx.x, split, tm, tn);
+  const int m0 = tm * TM, n0 = tn * TN;
+  const int mfirst = m0 + wm * (TM / WM), nfirst = n0 + wn * (TN / WN);
+  const int kbeg = split * g.chunk;
+  const int K = min(g.K - kbeg, g.chunk);
+  const int nk = (K + kBlock - 1) / kBlock;
+
+  const unsigned char* pa = g.w + (int64_t)m0 * g.ldw + kbeg;
+  const unsigned char* pb = g.x + (int64_t)n0 * g.ldx + kbeg;
+  OpA a;
+  OpB b;
+  a.init(wave, lane, g.V - m0, g.ldw);
+  b.init(wave, lane, g.T - n0, g.ldx);
+  const int base_a = OpA::base_of(lane, wm * (TM / WM)), base_b = OpB::base_of(lane, wn * (TN / WN));
+
+  // Scales: a stage's are loaded a stage ahead.
+  const int quad = lane >> 4;
+  int at_x[NI];
+#pragma unroll
+  for (int j = 0; j < NI; ++j) at_x[j] = min(nfirst + 16 * j + (lane & 15), g.T - 1);
+  int at_w[SC == kPower ? MI : 1];
+  if constexpr (SC == kPower) {
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+      const int v = min(mfirst + 16 * i + (lane & 15), g.V - 1);
+      at_w[i] = g.w_tile ? v / kBlock : v;
+    }
+  }
+  const int tile_w = min(mfirst / kBlock, (g.V - 1) / kBlock);
+  const int last_v = (g.V - 1) & ~3;
+  int block = kbeg / kBlock;  // of the scales that are loaded next
+  const int last_block = block + nk - 1;
+  struct Scales {
+    float x[NI];
+    f32x4 w[SC == kRow ? MI : 1];
+    int ex[NI], ew[SC == kPower ? MI : 1];
+  };
+  auto load_scales = [&](Scales& s) {
+    if constexpr (SC == kPower) {
+      const unsigned char* px = static_cast<const unsigned char*>(g.sx) + block * g.sx_block;
+      const unsigned char* pw = static_cast<const unsigned char*>(g.sw) + block * g.sw_block;
+#pragma unroll
+      for (int j = 0; j < NI; ++j) s.ex[j] = px[at_x[j]];
+#pragma unroll
+      for (int i = 0; i < MI; ++i) s.ew[i] = pw[at_w[i]];
+    } else {
+      const float* px = static_cast<const float*>(g.sx) + block * g.sx_block;
+      const float* pw = static_cast<const float*>(g.sw) + block * g.sw_block;
+#pragma unroll
+      for (int j = 0; j < NI; ++j) s.x[j] = px[at_x[j]];
+      if constexpr (SC == kTile) {
+        s.w[0][0] = pw[tile_w];
+      } else {
+        // (rows of whole fours)
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+          s.w[i] = *reinterpret_cast<const f32x4*>(pw + min(mfirst + 16 * i + 4 * quad, last_v));
+      }
+    }
+    block = min(block + 1, last_block);
+  };
+
+  f32x4 acc[MI][NI];
+#pragma unroll
+  for (int i = 0; i < MI; ++i)
+#pragma unroll
+    for (int j = 0; j < NI; ++j) acc[i][j] = f32x4{};
+
+  int left_a = K, left_b = K;
+  auto issue = [&](auto uc, auto full, auto from, auto to) {
+    constexpr int U = decltype(uc)::value, F = decltype(from)::value, T = decltype(to)::value;
+    constexpr bool kFull = decltype(full)::value;
+    unsigned char* st = place(uc);
+    if constexpr (U % 2 == 0) {
+      a.template issue<kFull, F, T>(pa, st, wave, left_a);
+      if constexpr (T == OpA::kInst) pa += kBlock, left_a -= kBlock;
+    } else {
+      b.template issue<kFull, F, T>(pb, st, wave, left_b);
+      if constexpr (T == OpB::kInst) pb += kBlock, left_b -= kBlock;
+    }
+  };
+  constexpr auto parts_of = [](int u) { return u % 2 ? OpB::kInst : OpA::kInst; };
+  constexpr auto dmas = [](int u, int n) {
+    int c = 0;
+    for (int i = 0; i < n; ++i) c += (u + i) % 2 ? OpB::kInst : OpA::kInst;
+    return c;
+  };
+
+  using FragA = std::conditional_t<EXACT, Halves, i32x8>;
+  using FragB = std::conditional_t<EXACT, Halves, i32x8>;
+  i32x8 ra, rb[NI];  // fragments as read
+  Scales next;
+  // Sums of a block that are not yet in the accumulators: the scaling of a sum runs
+  // kLag products behind, so that it does not wait for its own.  Everything is
+  // issued in the order written here: left to itself the compiler starts all
+  // products of a stage and spills.
+  constexpr int kLag = EXACT ? NI : NI / 2;
+  f32x4 parts[EXACT ? 2 * NI : NI];
+  auto scale = [&](auto nc, const Scales& s) {  // product number n of the stage
+    constexpr int n = decltype(nc)::value, i = n / NI, j = n % NI;
+    const f32x4 part = parts[EXACT ? (i & 1) * NI + j : j];
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      acc[i][j][r] = __builtin_fmaf(part[r], SC == kTile ? s.x[j] : s.x[j] * s.w[i][r], acc[i][j][r]);
+  };
+  // One group of 16 outputs times the wave's tokens.
+  auto multiply = [&](auto ic, const FragA& fa, const FragB (&fb)[NI], const Scales& s) {
+    constexpr int i = decltype(ic)::value;
+    auto product = [&](auto jc) {
+      constexpr int j = decltype(jc)::value, n = i * NI + j;
+      if constexpr (SC == kPower) {
+        acc[i][j] = mfma<X5>(fa, fb[j], acc[i][j], s.ew[i], s.ex[j]);
+      } else {
+        if constexpr (EXACT)
+          parts[(i & 1) * NI + j] = mfma(fa, fb[j]);
+        else
+          parts[j] = mfma<X5>(fa, fb[j], f32x4{});
+        if constexpr (n >= kLag) scale(Int<n - kLag>{}, s);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    product(Int<0>{});
+    if constexpr (NI > 1) product(Int<1>{});
+    if constexpr (NI > 2) product(Int<2>{});
+    if constexpr (NI > 3) product(Int<3>{});
+    static_assert(NI <= 4, "products");
+  };
+  auto finish = [&](const Scales& s) {
+    if constexpr (SC != kPower) {
+      constexpr int n = MI * NI;
+      if constexpr (kLag > 3) scale(Int<n - 4>{}, s);
+      if constexpr (kLag > 2) scale(Int<n - 3>{}, s);
+      if constexpr (kLag > 1) scale(Int<n - 2>{}, s);
+      scale(Int<n - 1>{}, s);
+    }
+  };
+  auto as_a = [](i32x8 v) -> FragA {
+    if constexpr (EXACT)
+      return halves<false>(v);
+    else
+      return v;
+  };
+  auto as_b = [](i32x8 v) -> FragB {
+    if constexpr (EXACT)
+      return halves<X5>(v);
+    else
+      return v;
+  };
+  using Full = std::true_type;
+  using Checked = std::false_type;
+  // Where K ends inside a chunk, the last stage's bytes past it are cleared once
+  // they have landed (in both operands: they may be NaNs).
+  const bool ragged = (K & 15) != 0;
+  auto cut = [&](auto kc) {
+    constexpr int k = decltype(kc)::value;
+    OpA::cut(place(Int<2 * k>{}), tid, K & (kBlock - 1));
+    OpB::cut(place(Int<2 * k + 1>{}), tid, K & (kBlock - 1));
+    wait_lgkm();
+    __builtin_amdgcn_s_barrier();
+  };
+  // Stage k (known modulo kPeriod): on entry its scales, its tokens' fragments and
+  // the first of its outputs' are in registers or on their way, on exit the next
+  // stage's.  The DMA of unit 2 k + UNITS goes out behind the barrier, that of
+  // the unit after it over the next stage's steps.
+  auto iteration = [&](auto kc, auto full, int kt) {
+    constexpr int k = decltype(kc)::value;
+    constexpr int kLast = 2 * k + UNITS - 1;  // the unit that the stage before left to issue
+    constexpr int kParts = parts_of(kLast);
+    constexpr int kNext = 2 * k + UNITS;
+    const unsigned char* sa = place(Int<2 * k>{});
+    Scales s = next;
+    if constexpr (SC == kTile) {
+#pragma unroll
+      for (int j = 0; j < NI; ++j) s.x[j] *= s.w[0][0];
+    }
+    load_scales(next);
+    FragB fb[NI];
+#pragma unroll
+    for (int j = 0; j < NI; ++j) fb[j] = as_b(rb[j]);
+    auto step = [&](auto ic) {
+      constexpr int i = decltype(ic)::value;
+      constexpr int from = kParts * i / (MI - 1), to = kParts * (i + 1) / (MI - 1);
+      const FragA fa = as_a(ra);
+      ra = OpA::frag(sa, base_a, i + 1);
+      if constexpr (to > from) issue(Int<kLast>{}, full, Int<from>{}, Int<to>{});
+      multiply(ic, fa, fb, s);
+    };
+    step(Int<0>{});
+    if constexpr (MI > 2) step(Int<1>{});
+    if constexpr (MI > 3) step(Int<2>{});
+    if constexpr (MI > 4) step(Int<3>{});
+    if constexpr (MI > 5) step(Int<4>{});
+    if constexpr (MI > 6) step(Int<5>{});
+    if constexpr (MI > 7) step(Int<6>{});
+    static_assert(MI <= 8, "steps");
+    wait_vm<dmas(2 * k + 4, UNITS - 4)>();  // the next stage's two units have landed
+    wait_lgkm();
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (!decltype(full)::value) {
+      if (ragged && kt + 2 == nk) cut(Int<k + 1>{});
+    }
+    const FragA fa = as_a(ra);
+    const unsigned char* na = place(Int<2 * k + 2>{});
+    const unsigned char* nb = place(Int<2 * k + 3>{});
+    ra = OpA::frag(na, base_a, 0);
+    multiply(Int<MI - 1>{}, fa, fb, s);
+#pragma unroll
+    for (int j = 0; j < NI; ++j) rb[j] = OpB::frag(nb, base_b, j);
+    issue(Int<kNext>{}, full, Int<0>{}, Int<parts_of(kNext)>{});
+    finish(s);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+
+  auto first = [&](auto uc) {
+    constexpr int U = decltype(uc)::value;
+    if constexpr (U < UNITS - 1) issue(uc, Checked{}, Int<0>{}, Int<parts_of(U)>{});
+  };
+  load_scales(next);
+  first(Int<0>{});
+  first(Int<1>{});
+  first(Int<2>{});
+  first(Int<3>{});
+  first(Int<4>{});
+  first(Int<5>{});
+  first(Int<6>{});
+  static_assert(UNITS <= 8, "ring");
+  wait_vm<dmas(2, UNITS - 3)>();
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+  if (ragged && nk == 1) cut(Int<0>{});
+  ra = OpA::frag(place(Int<0>{}), base_a, 0);
+#pragma unroll
+  for (int j = 0; j < NI; ++j) rb[j] = OpB::frag(place(Int<1>{}), base_b, j);
+
+  int kt = 0;
+  const int nfull = K / kBlock;
+  for (; kt + kPeriod + UNITS / 2 <= nfull; kt += kPeriod) {
+    iteration(Int<0>{}, Full{}, 0);
+    iteration(Int<1>{}, Full{}, 0);
+    if constexpr (kPeriod > 2) iteration(Int<2>{}, Full{}, 0);
+    if constexpr (kPeriod > 3) iteration(Int<3>{}, Full{}, 0);
+    if constexpr (kPeriod > 4) iteration(Int<4>{}, Full{}, 0);
+  }
+  static_assert(kPeriod <= 5, "ring");
+  while (kt < nk) {
+    iteration(Int<0>{}, Checked{}, kt);
+    if (++kt >= nk) break;
+    iteration(Int<1>{}, Checked{}, kt);
+    if (++kt >= nk) break;
+    if constexpr (kPeriod > 2) {
+      iteration(Int<2>{}, Checked{}, kt);
+      if (++kt >= nk) break;
+    }
+    if constexpr (kPeriod > 3) {
+      iteration(Int<3>{}, Checked{}, kt);
+      if (++kt >= nk) break;
+    }
+    if constexpr (kPeriod > 4) {
+      iteration(Int<4>{}, Checked{}, kt);
+      ++kt;
+    }
+  }
+  wait_vm<0>();  // no DMA may still be writing LDS
+  wait_lgkm();
+  __builtin_amdgcn_s_barrier();  // every wave has read its last fragments: the units are free
+
+  // Block (i, j) of a lane: token nfirst + 16 j + lane % 16, outputs mfirst + 16 i +
+  // 4 (lane / 16) + r.
+  if (g.splits > 1) {
+#pragma unroll
+    for (int j = 0; j < NI; ++j) {
+      const int t = nfirst + 16 * j + (lane & 15);
+      if (t >= g.T) continue;
+      float* row = g.part + ((int64_t)split * g.T + t) * g.ld_part;  // (rows of whole fours)
+#pragma unroll
+      for (int i = 0; i < MI; ++i) {
+        const int v = mfirst + 16 * i + 4 * quad;
+        if (v < g.V) *reinterpret_cast<f32x4*>(row + v) = acc[i][j];
+      }
+    }
+    return;
+  }
+  // A wave's 16 tokens at a time pass through LDS, so that rows leave in pieces of
+  // 16 bytes that are neighbours.
+  constexpr int kSize = EXACT ? 4 : 2;
+  constexpr int kRow = MI * 16 * kSize, kChunks = kRow / 16, kStage = 16 * kRow;
+  constexpr int kLeast = kUnitA < kUnitB ? kUnitA : kUnitB;
+  constexpr int kPerUnit = kLeast / kStage;
+  static_assert(kPerUnit * 4 >= NW && kChunks <= 64, "staging");
+  unsigned char* const out = (wave < kPerUnit       ? place(Int<0>{})
+                              : wave < 2 * kPerUnit ? place(Int<1>{})
+                              : wave < 3 * kPerUnit ? place(Int<2>{})
+                                                    : place(Int<3>{})) +
+                             wave % kPerUnit * kStage;
+  // (Chunk c of row t lies at c ^ t, within the row's chunks.)
+  auto chunk_at = [](int t, int c) { return t * kRow + (c ^ (t & (kChunks - 1))) * 16; };
+  typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+  typedef uint32_t u32x4w __attribute__((ext_vector_type(4), aligned(4)));
+  typedef uint32_t u32x4h __attribute__((ext_vector_type(4), aligned(2)));
+  using u32x4u = std::conditional_t<EXACT, u32x4w, u32x4h>;
+#pragma unroll
+  for (int j = 0; j < NI; ++j) {
+    const int t = lane & 15;
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+      const f32x4 v = acc[i][j];
+      if constexpr (EXACT)
+        *reinterpret_cast<f32x4*>(out + chunk_at(t, 4 * i + quad)) = v;
+      else
+        *reinterpret_cast<u32x2*>(out + chunk_at(t, 2 * i + (quad >> 1)) + 8 * (quad & 1)) =
+            u32x2{pack_out(v[0], v[1], g.y_dtype), pack_out(v[2], v[3], g.y_dtype)};
+    }
+    constexpr int kRows = 64 / kChunks;  // per instruction
+    const int c = lane % kChunks, v0 = mfirst + c * (16 / kSize);
+#pragma unroll
+    for (int q = 0; q < 16 / kRows; ++q) {
+      const int row = q * kRows + lane / kChunks, to = nfirst + 16 * j + row;
+      const u32x4 v = *reinterpret_cast<const u32x4*>(out + chunk_at(row, c));
+      if (to >= g.T || v0 >= g.V) continue;
+      unsigned char* p = static_cast<unsigned char*>(g.y) + ((int64_t)to * g.ldy + v0) * kSize;
+      if (v0 + 16 / kSize <= g.V) {
+        *reinterpret_cast<u32x4u*>(p) = v;
+      } else if constexpr (EXACT) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (v0 + e < g.V) reinterpret_cast<uint32_t*>(p)[e] = v[e];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (v0 + e < g.V) reinterpret_cast<uint16_t*>(p)[e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
+      }
+    }
+  }
+}
+
+}  // namespace fp8
+}  // namespace hcg

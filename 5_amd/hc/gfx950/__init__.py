@@ -383,14 +383,17 @@ def _gemm_torch(torch: Any, a: Any, b: Any, out: Any | None, algo: int) -> Any:
     return out
 
 
-from .lm import (  # noqa: E402  (a language model's ends and norm, with their gradients)
+from .lm import (  # noqa: E402  (a language model's ends and norms, with their gradients)
     embedding,
     embedding_grad,
     layer_norm,
     layer_norm_grad,
     linear_cross_entropy,
     linear_cross_entropy_grad,
+    rms_norm,
+    rms_norm_grad,
 )
+from .fp8 import linear_fp8, quantize_fp8, rms_norm_fp8  # noqa: E402  (8-bit linear layers)
 from .tiles import tile_load, tile_store  # noqa: E402  (masked tile gather / scatter)
 
 
@@ -417,7 +420,12 @@ __all__ = [
     "library_path",
     "linear_cross_entropy",
     "linear_cross_entropy_grad",
+    "linear_fp8",
+    "quantize_fp8",
     "register_kernel",
+    "rms_norm",
+    "rms_norm_fp8",
+    "rms_norm_grad",
     "run",
     "tile_load",
     "tile_store",

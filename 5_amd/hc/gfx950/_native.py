@@ -29,6 +29,12 @@ HCG_EDECLINED = 3
 HCG_F16 = 0
 HCG_BF16 = 1
 HCG_F32 = 2  # include/hcg_lm.h
+HCG_E4M3 = 3  # include/hcg_fp8.h
+HCG_E5M2 = 4
+HCG_E8M0 = 5
+
+FP8_BLOCK = 128  # HCG_FP8_BLOCK
+FP8_ALGOS = {"auto": 0, "stream": 1, "256x256": 2, "128x128": 3}  # HCG_FP8_*
 
 HCG_ALGO_AUTO = 0
 HCG_ALGO_TILED = 1
@@ -61,7 +67,11 @@ EXPORTS = ("hcg_init", "hcg_gemm", "hcg_gemm_algo", "hcg_gemm_noalloc", "hcg_gem
 # Every symbol include/hcg_lm.h declares.
 LM_EXPORTS = ("hcg_embedding", "hcg_embedding_grad", "hcg_embedding_grad_workspace", "hcg_layer_norm",
               "hcg_layer_norm_grad", "hcg_layer_norm_grad_workspace", "hcg_linear_cross_entropy",
-              "hcg_linear_cross_entropy_grad", "hcg_linear_cross_entropy_plan", "hcg_linear_cross_entropy_workspace")
+              "hcg_linear_cross_entropy_grad", "hcg_linear_cross_entropy_plan", "hcg_linear_cross_entropy_workspace",
+              "hcg_rms_norm", "hcg_rms_norm_grad", "hcg_rms_norm_grad_workspace")
+
+# Every symbol include/hcg_fp8.h declares.
+FP8_EXPORTS = ("hcg_linear_fp8", "hcg_linear_fp8_workspace", "hcg_quantize_fp8", "hcg_rms_norm_fp8")
 
 NOALLOC_SCRATCH_BYTES = 32 << 20  # HCG_NOALLOC_SCRATCH_BYTES
 
@@ -110,7 +120,17 @@ def _declare(lib: ctypes.CDLL) -> None:
                                              vp]
     lib.hcg_linear_cross_entropy_grad.argtypes = [c_int, vp, i64, i64, vp, i64, i64, i64, c_int, vp, i64, c_int, f32,
                                                   vp, vp, i64, vp, i64, vp, i64, vp]
-    for name in LM_EXPORTS:
+    lib.hcg_rms_norm.argtypes = [c_int, vp, i64, i64, i64, c_int, vp, i64, c_int, vp, f32, vp, i64, vp, i64, vp, vp]
+    lib.hcg_rms_norm_grad_workspace.argtypes = [i64, i64]
+    lib.hcg_rms_norm_grad.argtypes = [c_int, vp, i64, c_int, vp, i64, i64, i64, vp, c_int, vp, vp, i64, vp, i64, vp, vp,
+                                      i64, vp]
+    lib.hcg_rms_norm_fp8.argtypes = [c_int, vp, i64, i64, i64, c_int, vp, i64, c_int, vp, f32, c_int, vp, i64, c_int, vp,
+                                     i64, i64, vp, i64, vp, vp]
+    lib.hcg_quantize_fp8.argtypes = [c_int, vp, i64, i64, i64, c_int, c_int, c_int, vp, i64, c_int, vp, i64, i64, vp]
+    lib.hcg_linear_fp8_workspace.argtypes = [c_int, i64, i64, i64, vp, i64, vp, i64, c_int, i64, c_int, vp, i64, i64, c_int]
+    lib.hcg_linear_fp8.argtypes = [c_int, c_int, vp, i64, i64, vp, i64, i64, i64, c_int, vp, i64, i64, c_int, vp, i64,
+                                   i64, c_int, vp, i64, vp, i64, vp]
+    for name in LM_EXPORTS + FP8_EXPORTS:
         getattr(lib, name).restype = i64 if name.endswith("_workspace") else c_int
 
 

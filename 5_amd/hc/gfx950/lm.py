@@ -1,7 +1,7 @@
-"""The two ends of a language model on gfx950, and the norm between them.
+"""The two ends of a language model on gfx950, and the norms between them.
 
-``embedding``, ``layer_norm`` and ``linear_cross_entropy`` with their
-gradients, for training beside the products of :func:`hc.gfx950.gemm`.  They
+``embedding``, ``layer_norm``, ``rms_norm`` and ``linear_cross_entropy`` with
+their gradients, for training beside the products of :func:`hc.gfx950.gemm`.  They
 take torch tensors on a GPU and run in libhcg_gfx950.so (include/hcg_lm.h) on
 the tensors' device and current stream, asynchronously; arguments are checked
 before anything is launched and raise ``LaunchError``.  Leading dimensions are
@@ -358,6 +358,109 @@ def layer_norm_grad(dy: Any, x: Any, mean: Any, rstd: Any, weight: Any | None = 
           base + params.element_size() * width, _ptr(ws), need)
     params = params.to(param_dtype)
     return dx, params[0], params[1]
+
+
+# --------------------------------------------------------------------------
+# Root-mean-square norm
+# --------------------------------------------------------------------------
+
+
+def _rms_args(torch: Any, x: Any, weight: Any, residual: Any) -> tuple[Any, ...]:
+    """What both forms of the norm take: (device index, x's code, x's rows,
+    weight, its code, residual's rows, its code, h, h's rows, rstd).  h and
+    its rows are x and None without a residual."""
+    index = _check_tensor(torch, x, "x")
+    code = _code(x, "x", _ANY)
+    rows = _rows(x, "x")
+    if rows.shape[1] == 0:
+        raise LaunchError("norm of rows without elements")
+    w = _param(torch, weight, "weight", x, index)
+    h, hrows, res, rcode = x, None, None, code
+    if residual is not None:
+        _check_tensor(torch, residual, "residual", index)
+        if residual.shape != x.shape:
+            raise LaunchError(f"residual shape {tuple(residual.shape)} does not match x {tuple(x.shape)}")
+        if residual.dtype is not x.dtype and residual.dtype is not torch.float32:
+            raise LaunchError(f"residual must be {_name(x.dtype)} or float32, got {_name(residual.dtype)}")
+        res, rcode = _rows(residual, "residual"), _CODES[residual.dtype]
+        h = torch.empty(x.shape, dtype=residual.dtype, device=x.device)
+        hrows = h.view(rows.shape)
+    rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    return index, code, rows, w, code if w is None else _CODES[w.dtype], res, rcode, h, hrows, rstd
+
+
+def rms_norm(x: Any, weight: Any | None = None, residual: Any | None = None, *, eps: float = 1e-6,
+             out: Any | None = None) -> tuple[Any, Any, Any]:
+    """Root-mean-square norm over the last dimension of ``x + residual``:
+    ``(y, h, rstd)`` with ``h = x + residual`` rounded to the residual's type
+    (x itself without one), ``rstd = 1 / sqrt(mean(h * h) + eps)`` as float32
+    and ``y = h * rstd * weight`` of x's type (float16, bfloat16 or float32).
+    ``residual``: x's shape, its type or float32; ``weight``: a vector of x's
+    type or float32, or None.  h and rstd are what :func:`rms_norm_grad`
+    takes, and h is the next residual."""
+    torch = _torch()
+    index, code, rows, w, wcode, res, rcode, h, hrows, rstd = _rms_args(torch, x, weight, residual)
+    n, width = rows.shape
+    if out is None:
+        out = m = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        ldo = width
+    else:
+        out, m = _out_rows(torch, out, tuple(x.shape), x.dtype, "out", index)
+        ldo = _ld(m)
+    _call(torch, index, _native.lib().hcg_rms_norm, "hcg_rms_norm", code, _ptr(rows), _ld(rows), n, width, rcode,
+          _ptr(res), 0 if res is None else _ld(res), wcode, _ptr(w), eps, _ptr(m), ldo, _ptr(hrows), width, _ptr(rstd))
+    return (out if m is out else _finish(out, m)), h, rstd
+
+
+def rms_norm_grad(dy: Any, h: Any, rstd: Any, weight: Any | None = None, *, dresidual: Any | None = None,
+                  param_dtype: Any | None = None) -> tuple[Any, Any]:
+    """The gradients of :func:`rms_norm`, ``(dh, dweight)``, from ``dy`` and
+    what the forward call returned.  dh, of h's type, is the gradient for x and
+    for the residual; ``dresidual`` (h's shape and type), the gradient that
+    reaches h past the norm, is added to it.  dweight has the type of
+    ``weight`` (dy's without one), or ``param_dtype``: dy's type or float32."""
+    torch = _torch()
+    index = _check_tensor(torch, dy, "dy")
+    code = _code(dy, "dy", _ANY)
+    _check_tensor(torch, h, "h", index)
+    if h.shape != dy.shape:
+        raise LaunchError(f"dy shape {tuple(dy.shape)} does not match h {tuple(h.shape)}")
+    if h.dtype is not dy.dtype and h.dtype is not torch.float32:
+        raise LaunchError(f"h must be {_name(dy.dtype)} as dy or float32, got {_name(h.dtype)}")
+    grads, rows = _rows(dy, "dy"), _rows(h, "h")
+    n, width = rows.shape
+    if width == 0:
+        raise LaunchError("norm of rows without elements")
+    _check_tensor(torch, rstd, "rstd", index)
+    if rstd.numel() != n or rstd.dtype is not torch.float32:
+        raise LaunchError(f"rstd must be {n} float32 values, got {tuple(rstd.shape)} {_name(rstd.dtype)}")
+    w = _param(torch, weight, "weight", dy, index)
+    past = None
+    if dresidual is not None:
+        _check_tensor(torch, dresidual, "dresidual", index)
+        if dresidual.shape != h.shape or dresidual.dtype is not h.dtype:
+            raise LaunchError(f"dresidual must be {tuple(h.shape)} {_name(h.dtype)} as h, "
+                              f"got {tuple(dresidual.shape)} {_name(dresidual.dtype)}")
+        past = _rows(dresidual, "dresidual")
+    if param_dtype is None:
+        param_dtype = dy.dtype if w is None else w.dtype
+    elif param_dtype is not dy.dtype and param_dtype is not torch.float32:
+        raise LaunchError(f"param_dtype must be {_name(dy.dtype)} or float32, got {_name(param_dtype)}")
+    # One type for the weight and its gradient, the wider of the two, as in layer_norm_grad.
+    call_dtype = param_dtype
+    if w is not None and w.dtype is not param_dtype:
+        call_dtype = torch.float32
+        w = w.float()
+    dh = torch.empty(h.shape, dtype=h.dtype, device=h.device)
+    dweight = torch.empty((width,), dtype=call_dtype, device=h.device)
+    lib = _native.lib()
+    need = lib.hcg_rms_norm_grad_workspace(n, width)
+    ws = _workspace(torch, need, h.device)
+    rstd = rstd.contiguous()
+    _call(torch, index, lib.hcg_rms_norm_grad, "hcg_rms_norm_grad", code, _ptr(grads), _ld(grads), _CODES[h.dtype],
+          _ptr(rows), _ld(rows), n, width, _ptr(rstd), _CODES[call_dtype], _ptr(w), _ptr(past),
+          0 if past is None else _ld(past), _ptr(dh), width, _ptr(dweight), _ptr(ws), need)
+    return dh, dweight.to(param_dtype)
 
 
 # --------------------------------------------------------------------------

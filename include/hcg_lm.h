@@ -1,7 +1,7 @@
 /*
  * hcg_lm.h -- C ABI of the language-model operators of the gfx950 backend:
- * the embedding lookup, layer norm and the softmax cross entropy of a linear
- * head, each with its gradient.  They stand next to the products of
+ * the embedding lookup, layer norm, root-mean-square norm and the softmax cross
+ * entropy of a linear head, each with its gradient.  They stand next to the products of
  * hcg_gemm.h (same library, status codes, error text and stream rules) and
  * have no counterpart in the reference, whose only data-parallel path is the
  * tiled product.
@@ -63,6 +63,26 @@ int hcg_layer_norm_grad(int dtype, const void* dy, int64_t lddy, const void* x, 
                         int64_t width, const float* mean, const float* rstd, int param_dtype, const void* weight,
                         void* dx, int64_t lddx, void* dweight, void* dbias, void* workspace, int64_t workspace_bytes,
                         void* stream);
+
+/* y = h * rstd * weight by rows, rstd = 1 / sqrt(mean of h^2 + eps).  h = x +
+ * residual, rounded to residual_dtype (dtype or HCG_F32) and written to h, which
+ * may be the residual itself; without one (null) h is x and is not written.
+ * weight (param_dtype: dtype or HCG_F32, width elements) and rstd (float32, one
+ * per row) may be null. */
+int hcg_rms_norm(int dtype, const void* x, int64_t ldx, int64_t rows, int64_t width, int residual_dtype,
+                 const void* residual, int64_t ldr, int param_dtype, const void* weight, float eps, void* y,
+                 int64_t ldy, void* h, int64_t ldh, float* rstd, void* stream);
+
+/* The gradients of hcg_rms_norm for x and the residual, which are one: dh =
+ * rstd * (dy * weight - h * rstd * mean of (dy * weight * h * rstd)) + dresidual
+ * (h_dtype: dtype or HCG_F32, as h and dresidual, the gradient that reaches h
+ * past the norm; may be null), and dweight = sum over rows of dy * h * rstd
+ * (param_dtype; may be null, and so may weight).  dh may be dresidual itself. */
+int64_t hcg_rms_norm_grad_workspace(int64_t rows, int64_t width);
+int hcg_rms_norm_grad(int dtype, const void* dy, int64_t lddy, int h_dtype, const void* h, int64_t ldh, int64_t rows,
+                      int64_t width, const float* rstd, int param_dtype, const void* weight, const void* dresidual,
+                      int64_t lddr, void* dh, int64_t lddh, void* dweight, void* workspace, int64_t workspace_bytes,
+                      void* stream);
 
 /* Softmax cross entropy of the logits x @ weight^T against one target per
  * row, without the logits in memory.  x: tokens x width, weight: vocab x

@@ -1,0 +1,424 @@
+"""The 8-bit linear layers of hc.gfx950 on the GPU: the quantiser bit for bit
+against its definition, the norm's 8-bit form, and the product.
+
+Products are held to two kinds of test.  With small whole numbers and powers of
+two as scales every partial sum is a float32 number, so results are compared bit
+for bit.  With arbitrary values the tolerance is a forward error bound, of the sum
+of magnitudes: a block's 128 products and its sum with the others are at most
+(130 + blocks) additions deep, each within 2^-23 (a matrix instruction may cut
+instead of round).  For a 16-bit result each of 8 neighbouring products is cut
+towards zero below 2^-13 of the largest's power of two, so the 7 that are not the
+largest lose at most 7 * 2^-13 of it together.  And an output's rounding u of the
+result."""
+
+from __future__ import annotations
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+import hc.gfx950 as g  # noqa: E402
+from hc._errors import LaunchError  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
+E4M3, E5M2, E8M0 = torch.float8_e4m3fn, torch.float8_e5m2, torch.float8_e8m0fnu
+U = {F16: 2.0**-11, BF16: 2.0**-8, F32: 2.0**-24}
+LARGEST = {E4M3: 448.0, E5M2: 57344.0}
+ALGOS = ["auto", "stream", "256x256", "128x128"]
+
+
+def _gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def _randn(gen, shape, dtype, std=1.0):
+    return (torch.randn(shape, generator=gen, device=DEV) * std).to(dtype)
+
+
+def _bits(t):
+    return t.contiguous().view(torch.uint8 if t.element_size() == 1 else torch.int32)
+
+
+def _blocks(n):
+    return -(-n // 128)
+
+
+def _spread(scale, rows, cols, tile):
+    """The scale of every element."""
+    r = torch.arange(rows, device=scale.device)
+    c = torch.arange(cols, device=scale.device) // 128
+    return scale[(r // 128 if tile else r)][:, c]
+
+
+def _quantize_want(x, tile, dtype, scale_dtype):
+    """The definition, in float32 on the CPU."""
+    x = x.float().cpu()
+    rows, cols = x.shape
+    high = 128 if tile else 1
+    pad = torch.zeros((-(-rows // high) * high, _blocks(cols) * 128))
+    pad[:rows, :cols] = x
+    parts = pad.view(-1, high, _blocks(cols), 128)
+    top = parts.abs().amax((1, 3)).clamp(min=2.0**-100)
+    large = torch.tensor(LARGEST[dtype])
+    if scale_dtype is F32:
+        scale, inverse = top / large, large / top
+        scale_held = scale
+    else:
+        d = top.double() / LARGEST[dtype]
+        power = torch.ceil(torch.log2(d))
+        power = torch.where(torch.exp2(power - 1) >= d, power - 1, power)
+        power = torch.where(torch.exp2(power) < d, power + 1, power)
+        finite = top.isfinite()
+        byte = torch.where(finite, power + 127, 255.0).nan_to_num(255.0).to(torch.uint8)
+        scale_held = byte.view(E8M0)
+        inverse = torch.where(finite, torch.exp2(-power), float("nan")).float()
+    q = (parts * inverse[:, None, :, None]).flatten(2).flatten(0, 1)[:rows, :cols].to(dtype)
+    return q, scale_held
+
+
+def _same(got, want):
+    got, want = got.float().cpu(), want.float().cpu()
+    assert got.shape == want.shape
+    assert torch.equal(got.isnan(), want.isnan())
+    assert torch.equal(got.nan_to_num(), want.nan_to_num())
+
+
+@pytest.mark.parametrize("tile", [False, True])
+@pytest.mark.parametrize("transpose", [False, True])
+@pytest.mark.parametrize("dtype,scale_dtype", [(E4M3, F32), (E5M2, F32), (E4M3, E8M0), (E5M2, E8M0)])
+@pytest.mark.parametrize("rows,cols,src", [(1, 1, F32), (1, 4096, BF16), (5, 127, F16), (128, 128, BF16), (129, 130, F32),
+                                           (300, 515, BF16), (64, 1000, F32), (257, 96, F16), (1000, 8, BF16)])
+def test_quantize(rows, cols, src, dtype, scale_dtype, transpose, tile):
+    gen = _gen(rows * 7 + cols)
+    x = _randn(gen, (rows, cols), F32)
+    x *= torch.exp2(torch.randint(-12, 13, (rows, 1), generator=gen, device=DEV).float())  # rows of different sizes
+    buf = torch.full((rows, cols + 5), float("nan"), dtype=src, device=DEV)
+    x = buf[:, 3 : 3 + cols].copy_(x.clamp(-6e4, 6e4))  # (unaligned rows, NaN around them)
+    q, scale = g.quantize_fp8(x, block="tile" if tile else "row", transpose=transpose, dtype=dtype, scale_dtype=scale_dtype)
+    want_q, want_scale = _quantize_want(x.t() if transpose else x, tile, dtype, scale_dtype)
+    assert q.dtype == dtype and scale.dtype == scale_dtype
+    assert q.stride(0) % 16 == 0 and q.data_ptr() % 16 == 0
+    _same(scale, want_scale)
+    _same(q, want_q)
+
+
+@pytest.mark.parametrize("dtype,scale_dtype", [(E4M3, F32), (E5M2, F32), (E4M3, E8M0), (E5M2, E8M0)])
+def test_quantize_special_values(dtype, scale_dtype):
+    """Zeros, subnormals, the largest floats, powers of two and their
+    neighbours, infinities and NaNs, a block each."""
+    big, small = 3.4028234663852886e38, 1e-45
+    firsts = [0.0, -0.0, small, 1e-39, 2.0**-100, 2.0**-99, big, -big, 1.75, 1.7500001, 1.7499999, 448.0, 57344.0, 2.0**-120,
+              float("inf"), float("-inf"), float("nan"), 1.0]
+    x = torch.zeros((len(firsts), 128), device=DEV)
+    x[:, 0] = torch.tensor(firsts, device=DEV)
+    x[:, 64] = x[:, 0] / 3
+    x[:, 127] = -x[:, 0] / 1000
+    q, scale = g.quantize_fp8(x, dtype=dtype, scale_dtype=scale_dtype)
+    want_q, want_scale = _quantize_want(x, False, dtype, scale_dtype)
+    _same(scale, want_scale)
+    _same(q, want_q)
+    stands = q.float() * scale.float()
+    assert stands[14:17].isnan().all() and not stands[:14].isnan().any() and not stands[17].isnan().any()
+
+
+def test_quantize_every_rounding():
+    """Every 16-bit float of one binade and its neighbours, against torch's
+    conversion."""
+    values = torch.arange(1 << 16, dtype=torch.int32).to(torch.int16).view(F16).float()
+    values = values[values.isfinite()].to(DEV)
+    for dtype, large in ((E4M3, 448.0), (E5M2, 57344.0)):
+        inside = values[values.abs() <= large]
+        pad = torch.full((-inside.numel() % 127,), 0.0, device=DEV)
+        x = torch.cat([inside, pad]).view(-1, 127)
+        x = torch.cat([x, torch.full((x.shape[0], 1), large, device=DEV)], 1)  # (scale 1 in every block)
+        q, scale = g.quantize_fp8(x, dtype=dtype)
+        assert (scale == 1).all()
+        assert torch.equal(_bits(q), _bits(x.to(dtype)))
+
+
+def test_quantize_shapes():
+    gen = _gen(4)
+    x = _randn(gen, (2, 3, 200), BF16)
+    q, s = g.quantize_fp8(x)
+    assert q.shape == (2, 3, 200) and s.shape == (2, 3, 2)
+    fq, fs = g.quantize_fp8(x.view(6, 200))
+    assert torch.equal(_bits(q).view(6, 200), _bits(fq)) and torch.equal(s.reshape(6, 2), fs)
+    tq, ts = g.quantize_fp8(x, transpose=True)
+    assert tq.shape == (200, 6) and ts.shape == (200, 1)
+    assert g.quantize_fp8(x, block="tile")[1].shape == (1, 2)
+    vq, vs = g.quantize_fp8(x[0, 0])
+    assert vq.shape == (200,) and vs.shape == (2,)
+    for t in (x.transpose(0, 1), x[..., ::2]):
+        a, b = g.quantize_fp8(t), g.quantize_fp8(t.contiguous())
+        assert torch.equal(_bits(a[0]), _bits(b[0])) and torch.equal(a[1], b[1])
+    eq, es = g.quantize_fp8(x[:, :0])
+    assert eq.shape == (2, 0, 200) and es.shape == (2, 0, 2)
+    eq, es = g.quantize_fp8(x[:, :0], transpose=True)
+    assert eq.shape == (200, 0) and es.shape == (200, 0)
+
+
+@pytest.mark.parametrize("dtype,wide", [(F16, F16), (BF16, BF16), (F32, F32), (BF16, F32), (F16, F32)])
+@pytest.mark.parametrize("rows,width", [(1, 1), (1, 4096), (3, 60), (33, 127), (7, 128), (9, 129), (300, 256), (31, 515),
+                                        (64, 1024), (17, 2048), (6, 4100), (3, 8192), (5, 16384), (2, 40001)])
+@pytest.mark.parametrize("to,scale_dtype", [(E4M3, F32), (E5M2, E8M0)])
+def test_norm(rows, width, dtype, wide, to, scale_dtype):
+    gen = _gen(rows * 3 + width)
+    x = _randn(gen, (rows, width), dtype)
+    res = _randn(gen, (rows, width), wide, 2.0)
+    weight = (_randn(gen, (width,), F32, 0.1) + 1).to(dtype)
+    q, scale, h, rstd = g.rms_norm_fp8(x, weight, res, dtype=to, scale_dtype=scale_dtype)
+    y, h16, rstd16 = g.rms_norm(x, weight, res)
+    assert torch.equal(h, h16) and torch.equal(rstd, rstd16)
+    assert q.dtype == to and scale.dtype == scale_dtype and q.shape == x.shape and scale.shape == (rows, _blocks(width))
+    # h rstd weight in the kernel's own float32 products, quantised by the definition
+    f = h.float() * rstd[:, None] * weight.float()
+    want_q, want_scale = _quantize_want(f, False, to, scale_dtype)
+    _same(scale, want_scale)
+    _same(q, want_q)
+
+
+def test_norm_shapes():
+    gen = _gen(6)
+    x = _randn(gen, (2, 3, 200), BF16)
+    q, s, h, rstd = g.rms_norm_fp8(x)
+    assert h is x and q.shape == (2, 3, 200) and s.shape == (2, 3, 2) and rstd.shape == (2, 3)
+    q, s, h, rstd = g.rms_norm_fp8(x[:, :0], None, x[:, :0])
+    assert q.shape == (2, 0, 200) and s.shape == (2, 0, 2) and h.shape == (2, 0, 200)
+
+
+# --------------------------------------------------------------------------
+# The product
+# --------------------------------------------------------------------------
+
+
+def _strided(t, pad, offset):
+    """t's values as a view with rows `pad` bytes longer, NaN around it."""
+    rows, cols = t.shape
+    buf = torch.full((rows * (cols + pad) + offset + 16,), 0x7F, dtype=torch.uint8, device=DEV)
+    view = buf[offset : offset + rows * (cols + pad)].view(rows, cols + pad)[:, :cols]
+    view.copy_(_bits(t))
+    return view.view(t.dtype)
+
+
+def _whole(gen, tokens, outputs, inputs, x_dtype, tile, scale_dtype):
+    """Operands of whole numbers up to 4 and scales from 1/2 to 2: every sum of
+    products below 2^24 quarters is a float32 number."""
+    x = torch.randint(-4, 5, (tokens, inputs), generator=gen, device=DEV).float().to(x_dtype)
+    w = torch.randint(-4, 5, (outputs, inputs), generator=gen, device=DEV).float().to(E4M3)
+    assert inputs * 16 * 4 * 4 < 1 << 24
+    down = _blocks(outputs) if tile else outputs
+    sx = torch.exp2(torch.randint(-1, 2, (tokens, _blocks(inputs)), generator=gen, device=DEV).float()).to(scale_dtype)
+    sw = torch.exp2(torch.randint(-1, 2, (down, _blocks(inputs)), generator=gen, device=DEV).float()).to(scale_dtype)
+    return x, sx, w, sw
+
+
+def _want(x, sx, w, sw, tile):
+    a = x.double() * _spread(sx.double(), *x.shape, False)
+    b = w.double() * _spread(sw.double(), *w.shape, tile)
+    return a @ b.t().contiguous(), a.abs() @ b.abs().t().contiguous()
+
+
+SIZES = [(1, 1, 1), (1, 16, 128), (3, 5, 7), (2, 130, 129), (16, 64, 256), (17, 33, 144), (64, 128, 512), (65, 130, 1000),
+         (129, 257, 1027), (300, 515, 640), (1, 1000, 4100), (257, 256, 128), (256, 512, 2048), (520, 300, 96)]
+
+
+@pytest.mark.parametrize("algo", ALGOS)
+@pytest.mark.parametrize("x_dtype,tile,scale_dtype", [(E4M3, True, F32), (E5M2, True, F32), (E4M3, False, F32),
+                                                      (E5M2, False, F32), (E4M3, True, E8M0), (E5M2, False, E8M0)])
+@pytest.mark.parametrize("tokens,outputs,inputs", SIZES)
+def test_linear_bit_for_bit(tokens, outputs, inputs, x_dtype, tile, scale_dtype, algo):
+    gen = _gen(tokens * 5 + outputs * 3 + inputs)
+    x, sx, w, sw = _whole(gen, tokens, outputs, inputs, x_dtype, tile, scale_dtype)
+    want, _ = _want(x, sx, w, sw, tile)
+    got = g.linear_fp8(x, sx, w, sw, out_dtype=F32, algo=algo)
+    assert got.dtype == F32 and torch.equal(got.double(), want)
+    for dtype in (F16, BF16):
+        assert torch.equal(g.linear_fp8(x, sx, w, sw, out_dtype=dtype, algo=algo), want.float().to(dtype))
+    # rows where they lie, scales block by block, a strided result
+    xs, ws = _strided(x, 16 - inputs % 16 + 32, 16), _strided(w, 16 - inputs % 16, 32)
+    buf = torch.full((tokens, outputs + 5), 7.0, device=DEV)
+    out = buf[:, 2 : 2 + outputs]
+    got = g.linear_fp8(xs, sx.t().contiguous().t(), ws, sw.t().contiguous().t(), out=out, algo=algo)
+    assert got is out and torch.equal(got.double(), want) and (buf[:, :2] == 7).all() and (buf[:, 2 + outputs :] == 7).all()
+    # rows at any address, NaN past their ends
+    xs, ws = _strided(x, 5, 3), _strided(w, 7, 1)
+    assert torch.equal(g.linear_fp8(xs, sx, ws, sw, out_dtype=F32, algo=algo).double(), want)
+
+
+@pytest.mark.parametrize("algo", ALGOS)
+@pytest.mark.parametrize("x_dtype,tile,scale_dtype", [(E4M3, True, F32), (E5M2, False, F32), (E4M3, False, E8M0),
+                                                      (E5M2, True, E8M0)])
+@pytest.mark.parametrize("tokens,outputs,inputs", [(1, 515, 4096), (33, 200, 1027), (700, 900, 1500)])
+def test_linear_values(tokens, outputs, inputs, x_dtype, tile, scale_dtype, algo):
+    gen = _gen(tokens + outputs + inputs)
+    x = _randn(gen, (tokens, inputs), F32) * torch.exp(_randn(gen, (tokens, 1), F32) * 2)
+    w = _randn(gen, (outputs, inputs), F32, 0.02)
+    xq, sx = g.quantize_fp8(x, dtype=x_dtype, scale_dtype=scale_dtype)
+    wq, sw = g.quantize_fp8(w, block="tile" if tile else "row", scale_dtype=scale_dtype)
+    want, mag = _want(xq, sx, wq, sw, tile)
+    for dtype in (F32, F16, BF16):
+        rel = (130 + _blocks(inputs)) * 2.0**-23 + (0 if dtype is F32 else 7 * 2.0**-13)
+        got = g.linear_fp8(xq, sx, wq, sw, out_dtype=dtype, algo=algo)
+        again = g.linear_fp8(xq, sx, wq, sw, out_dtype=dtype, algo=algo)
+        assert torch.equal(got, again)
+        tiny = 2.0**-25 if dtype is F16 else 0.0
+        bad = ~((got.double() - want).abs() <= rel * mag + U[dtype] * want.abs() + tiny)
+        assert not bad.any(), (int(bad.sum()), float((got.double() - want).abs().max()))
+    # and the layer's error against the operands before quantising: each within
+    # half a step of its block's largest value's binade
+    full = x.double() @ w.double().t()
+    step = {E4M3: 2.0**-4, E5M2: 2.0**-3}
+    err = (step[x_dtype] + step[E4M3] + 2.0**-7) * (x.double().abs() @ w.double().abs().t())
+    floor = 2.0**-9 * 2 * (x.abs().amax(1, keepdim=True).double() * w.abs().amax(1)) * inputs  # subnormal q
+    assert ((got.double() - full).abs() <= err + floor + U[BF16] * full.abs()).all()
+
+
+@pytest.mark.parametrize("algo", ALGOS)
+@pytest.mark.parametrize("scale_dtype", [F32, E8M0])
+def test_linear_keeps_nan_where_it_is(scale_dtype, algo):
+    """A NaN in a token's row, a weight's row or a scale reaches the outputs of
+    that row and no other; infinities of e5m2 as well."""
+    gen = _gen(9)
+    tokens, outputs, inputs = 70, 150, 300
+    x, sx, w, sw = _whole(gen, tokens, outputs, inputs, E5M2, False, scale_dtype)
+    want, _ = _want(x, sx, w, sw, False)
+    x = _bits(x).clone()
+    x[3, 299] = 0x7F   # NaN
+    x[68, 0] = 0x7C    # infinity
+    w = _bits(w).clone()
+    w[149, 131] = 0x7F
+    sx, sw = sx.clone(), sw.clone()
+    sx[11, 1] = float("nan")
+    sw[7, 2] = float("nan")
+    got = g.linear_fp8(x.view(E5M2), sx, w.view(E4M3), sw, out_dtype=F32, algo=algo)
+    bad = torch.zeros((tokens, outputs), dtype=torch.bool, device=DEV)
+    bad[[3, 11]] = True
+    bad[:, [7, 149]] = True
+    assert got[bad].isnan().all()
+    assert not got[68].isfinite().any()
+    bad[68] = True
+    assert torch.equal(got[~bad].double(), want[~bad])
+
+
+def test_linear_shapes_and_empty():
+    gen = _gen(10)
+    x, sx, w, sw = _whole(gen, 6, 40, 200, E4M3, True, F32)
+    flat = g.linear_fp8(x, sx, w, sw)
+    assert flat.dtype == BF16
+    deep = g.linear_fp8(x.view(2, 3, 200), sx.view(2, 3, 2), w, sw)
+    assert torch.equal(deep.view(6, 40), flat)
+    assert torch.equal(g.linear_fp8(x[0], sx[0], w, sw), flat[0])
+    assert g.linear_fp8(x[:0], sx[:0], w, sw).shape == (0, 40)
+    assert g.linear_fp8(x, sx, w[:0], sw[:0]).shape == (6, 0)
+    assert torch.equal(g.linear_fp8(x[::2], sx[::2], w, sw), flat[::2])
+    # one scale for all, spread by strides of zero
+    one = torch.full((1, 1), 0.5, device=DEV)
+    got = g.linear_fp8(x, one.expand(6, 2), w, one.expand(1, 2), out_dtype=F32)
+    assert torch.equal(got.double(), x.double() @ w.double().t().contiguous() / 4)
+    # columns that are not neighbours, and a transposed result
+    spread = torch.zeros((6, 400), dtype=torch.uint8, device=DEV)
+    spread[:, ::2] = _bits(x)
+    assert torch.equal(g.linear_fp8(spread.view(E4M3)[:, ::2], sx, w, sw), flat)
+    turned = torch.empty((40, 6), dtype=BF16, device=DEV)
+    assert torch.equal(g.linear_fp8(x, sx, w, sw, out=turned.t()), flat) and torch.equal(turned.t(), flat)
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(x="half"), "x must be"), (dict(weight="e5m2"), "weight must be float8_e4m3fn"), (dict(x="short"), "do not match"),
+    (dict(x_scale="half"), "x_scale must be"), (dict(x_scale="e8m0"), "one type"), (dict(x_scale="short"), "x_scale shape"),
+    (dict(weight_scale="short"), "weight_scale shape"), (dict(algo="best"), "unknown algo"),
+    (dict(out_dtype=torch.float64), "output must be"), (dict(out="half"), "out must be"), (dict(weight="cpu"), "GPU")])
+def test_linear_refusals(change, match):
+    a = dict(x=torch.zeros((4, 300), dtype=E4M3, device=DEV), x_scale=torch.ones((4, 3), device=DEV),
+             weight=torch.zeros((500, 300), dtype=E4M3, device=DEV), weight_scale=torch.ones((4, 3), device=DEV))
+    for k, v in change.items():
+        t = a.get(k, torch.zeros((4, 500), device=DEV))
+        a[k] = (t.float().half() if v == "half" else t.float().to(E5M2) if v == "e5m2" else t.to(E8M0) if v == "e8m0" else
+                t[:, :2] if v == "short" else t.cpu() if v == "cpu" else v)
+    if "out" in change:
+        a["out_dtype"] = BF16
+    with pytest.raises(LaunchError, match=match):
+        g.linear_fp8(**a)
+
+
+@pytest.mark.parametrize("call,match", [
+    (lambda x: g.quantize_fp8(x, block="column"), "unknown block"), (lambda x: g.quantize_fp8(x.double()), "x must be"),
+    (lambda x: g.quantize_fp8(x, dtype=F16), "dtype must be"), (lambda x: g.quantize_fp8(x, scale_dtype=F16), "scale_dtype"),
+    (lambda x: g.quantize_fp8(x.cpu()), "GPU"), (lambda x: g.rms_norm_fp8(x, dtype=BF16), "dtype must be"),
+    (lambda x: g.rms_norm_fp8(x, None, x[:3]), "residual shape"), (lambda x: g.rms_norm_fp8(x[:, :0]), "without elements")])
+def test_quantize_refusals(call, match):
+    with pytest.raises(LaunchError, match=match):
+        call(torch.ones((4, 16), dtype=BF16, device=DEV))
+
+
+@pytest.mark.parametrize("tokens", [1, 40, 600])
+def test_layer_and_its_gradients(tokens):
+    """Norm, product and their gradients as a layer uses them, against the same
+    layer in 64 bits, by norms.  A value's rounding error is spread evenly over
+    half a step to either side, u = 2^-4 (e4m3) or 2^-3 (e5m2) of the lower end
+    of its binade, so its root mean square is at most u / sqrt(3) of the value:
+    0.0361 and 0.0722.  A product's two operands err independently, so its
+    norm's error is expected below the root of the sum of their squares, and is
+    held to their sum (1.34 to 1.41 times that; the errors of 384 and more
+    roundings enter every output).  That is 0.0722 for y and 0.1083 for the
+    gradients, which take e5m2."""
+    two, three = (2 * 2.0**-4) / 3**0.5, (2.0**-4 + 2.0**-3) / 3**0.5
+    gen = _gen(tokens)
+    width, outputs = 384, 520
+    x, res = _randn(gen, (tokens, width), BF16), _randn(gen, (tokens, width), BF16, 2.0)
+    weight = (_randn(gen, (width,), F32, 0.1) + 1).to(BF16)
+    w = _randn(gen, (outputs, width), F32, 0.05)
+    dy = _randn(gen, (tokens, outputs), BF16, 1e-3)
+    q, s, h, rstd = g.rms_norm_fp8(x, weight, res)
+    y = g.linear_fp8(q, s, *g.quantize_fp8(w, block="tile"))
+    dn = g.linear_fp8(*g.quantize_fp8(dy, dtype=E5M2), *g.quantize_fp8(w, block="tile", transpose=True))
+    n = g.rms_norm(x, weight, res)[0]
+    dw = g.linear_fp8(*g.quantize_fp8(dy, transpose=True, dtype=E5M2), *g.quantize_fp8(n, transpose=True), out_dtype=F32)
+    dh, dweight = g.rms_norm_grad(dn, h, rstd, weight, dresidual=res)
+
+    hd = h.double().requires_grad_()
+    wt, wd = weight.double().requires_grad_(), w.double().requires_grad_()
+    nd = hd * (hd.square().mean(1, keepdim=True) + 1e-6).rsqrt() * wt
+    yd = nd @ wd.t()
+    ((yd * dy.double()).sum() + (hd * res.double()).sum()).backward()
+
+    def off(got, want):
+        return float((got.double() - want).norm() / want.norm())
+
+    assert off(y, yd.detach()) < two
+    assert off(dw, wd.grad) < three
+    assert off(dh - res, hd.grad - res.double()) < three + float(
+        2.0**-8 * res.double().norm() / (hd.grad - res.double()).norm())
+    assert off(dweight, wt.grad) < three + 2.0**-7
+
+
+def test_graph_and_streams():
+    """Captured once and replayed over new inputs, against eager calls on
+    another stream."""
+    gen = _gen(11)
+    x = _randn(gen, (200, 640), BF16)
+    w = _randn(gen, (300, 640), BF16, 0.05)
+    wq, sw = g.quantize_fp8(w, block="tile")
+
+    def call():
+        q, s, h, rstd = g.rms_norm_fp8(x)
+        qt, st = g.quantize_fp8(x, transpose=True)
+        return g.linear_fp8(q, s, wq, sw), g.linear_fp8(qt, st, qt, st, out_dtype=F32), rstd
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = call()
+    for i in range(3):
+        x.copy_(_randn(gen, (200, 640), BF16))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in held]
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            want = call()
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
