@@ -22,13 +22,16 @@ namespace {
 using hcg::ElemOf;
 using hcg::u32x4;
 using hcg::fp8::Args;
+using hcg::fp8::by_power;
+using hcg::fp8::by_tile;
 using hcg::fp8::f32x4;
 using hcg::fp8::Halves;
 using hcg::fp8::halves;
 using hcg::fp8::i32x8;
 using hcg::fp8::join;
 using hcg::fp8::kBlock;
-using hcg::fp8::kPower;
+using hcg::fp8::kPowerRow;
+using hcg::fp8::kPowerTile;
 using hcg::fp8::kRow;
 using hcg::fp8::kTile;
 using hcg::fp8::mfma;
@@ -83,7 +86,7 @@ __device__ __forceinline__ float power(uint32_t byte) {
 }
 template <Scaling SC>
 __device__ __forceinline__ float scale_at(const void* p, int64_t at) {
-  if constexpr (SC == kPower) return power(static_cast<const unsigned char*>(p)[at]);
+  if constexpr (by_power(SC)) return power(static_cast<const unsigned char*>(p)[at]);
   return static_cast<const float*>(p)[at];
 }
 
@@ -121,8 +124,8 @@ __global__ __launch_bounds__(64 * kStreamWaves) void stream_kernel(Args g) {
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
       const i32x8 fx = join(load16(x[j] + k, left), load16(x[j] + k + 16, left - 16));
-      if constexpr (SC == kPower && !EXACT) {
-        const int ew = static_cast<const unsigned char*>(g.sw)[(g.w_tile ? v / kBlock : v) * g.sw_row + b * g.sw_block];
+      if constexpr (by_power(SC) && !EXACT) {
+        const int ew = static_cast<const unsigned char*>(g.sw)[(by_tile(SC) ? v / kBlock : v) * g.sw_row + b * g.sw_block];
         const int ex = static_cast<const unsigned char*>(g.sx)[sx[j] + b * g.sx_block];
         acc[j] = mfma<X5>(fw, fx, acc[j], ew, ex);
       } else {
@@ -135,7 +138,7 @@ __global__ __launch_bounds__(64 * kStreamWaves) void stream_kernel(Args g) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int vr = min(v0 + 4 * (lane >> 4) + r, g.V - 1);
-          const int64_t row = SC == kTile || (SC == kPower && g.w_tile) ? vr / kBlock : vr;
+          const int64_t row = by_tile(SC) ? vr / kBlock : vr;
           acc[j][r] = __builtin_fmaf(part[r], fx_scale * scale_at<SC>(g.sw, row * g.sw_row + b * g.sw_block), acc[j][r]);
         }
       }
@@ -359,7 +362,6 @@ int hcg_linear_fp8(int algo, int x_dtype, const void* x, int64_t ldx, int64_t to
          xs_block,
          ws_row,
          ws_block,
-         w_tile != 0,
          (int)tokens,
          (int)outputs,
          (int)inputs,
@@ -404,18 +406,17 @@ int hcg_linear_fp8(int algo, int x_dtype, const void* x, int64_t ldx, int64_t to
     constexpr Scaling SC = decltype(scaling)::value;
     if (p.shape == kStream) {
       run_stream<X5, SC, EXACT>(a, s);
-    } else if constexpr (SC == kPower && EXACT) {
-      if (w_tile)
-        run_tiles<X5, kTile, true>(p.shape, a, s);
-      else
-        run_tiles<X5, kRow, true>(p.shape, a, s);
+    } else if constexpr (by_power(SC) && EXACT) {
+      run_tiles<X5, by_tile(SC) ? kTile : kRow, true>(p.shape, a, s);  // (scales copied to floats)
     } else {
       run_tiles<X5, SC, EXACT>(p.shape, a, s);
     }
   };
   const auto with_scales = [&](auto x5, auto exactly) {
-    if (e8m0)
-      with(x5, std::integral_constant<Scaling, kPower>{}, exactly);
+    if (e8m0 && w_tile)
+      with(x5, std::integral_constant<Scaling, kPowerTile>{}, exactly);
+    else if (e8m0)
+      with(x5, std::integral_constant<Scaling, kPowerRow>{}, exactly);
     else if (w_tile)
       with(x5, std::integral_constant<Scaling, kTile>{}, exactly);
     else

@@ -38,10 +38,13 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 // How scales are held and used.
 enum Scaling {
-  kTile,  // float32, the weight's by tiles
-  kRow,   // float32, the weight's by rows
-  kPower  // exponent bytes, which the MFMA takes itself
+  kTile,       // float32, the weight's by tiles
+  kRow,        // float32, the weight's by rows
+  kPowerTile,  // exponent bytes, which the MFMA takes itself
+  kPowerRow
 };
+constexpr bool by_power(Scaling s) { return s == kPowerTile || s == kPowerRow; }
+constexpr bool by_tile(Scaling s) { return s == kTile || s == kPowerTile; }
 
 struct Args {
   const unsigned char* x;
@@ -50,7 +53,6 @@ struct Args {
   const void* sx;
   const void* sw;
   int64_t sx_row, sx_block, sw_row, sw_block;  // (tiled: the rows' strides are 1)
-  bool w_tile;                                 // kPower: the weight's scales are by tiles
   int T, V, K;
   void* y;
   int64_t ldy;
@@ -157,34 +159,36 @@ struct Side {
   static_assert(kInst >= 1 && kInst * NW * 1024 == kBytes, "a unit is whole DMA instructions of every wave");
   static __device__ __forceinline__ int swz(int row, int c) { return c ^ ((row >> 1) & 7); }
 
-  int off[kInst];  // byte offset of the lane's chunk from the unit's first byte, or kOobOffset
-  int key[kInst];  // the chunk's first byte in its row
+  int64_t ld;
+  int rows;       // of the matrix, from the tile's first on
+  int key;        // the lane's first byte in an even instruction's rows; in an odd one's key ^ 64
+  int at[2];      // and its place from the wave's first row in either
 
-  // extent: rows from the tile's first on.
-  __device__ __forceinline__ void init(int wave, int lane, int extent, int64_t ld) {
-#pragma unroll
-    for (int i = 0; i < kInst; ++i) {
-      const int row = (wave * kInst + i) * 8 + (lane >> 3);
-      key[i] = swz(row, lane & 7) * 16;
-      off[i] = row < extent ? row * (int)ld + key[i] : kOobOffset;
-    }
+  __device__ __forceinline__ void init(int lane, int extent, int64_t stride) {
+    ld = stride;
+    rows = min(extent, ROWS);
+    key = swz(lane >> 3, lane & 7) * 16;  // (8 rows on the swizzle differs by 4 chunks)
+    at[0] = (lane >> 3) * (int)ld + key;
+    at[1] = (lane >> 3) * (int)ld + (key ^ 64);
   }
   // Instructions FROM to TO - 1 of the wave's, of the unit whose first byte is at p
   // and whose rows have `left` bytes from there on (FULL: all of them).  The
-  // resource starts at the unit, so offsets stay in 31 bits whatever the
-  // matrix's size; chunks out of range are redirected past its extent and load
-  // zeros.  The chunk with a row's last byte is loaded whole, from within its
-  // own 16-byte granule.
+  // resource starts at the unit and ends with the matrix's last row, so that
+  // offsets stay in 31 bits whatever the matrix's size and rows past it load
+  // zeros; chunks past a row's end are redirected past it.  The chunk with a
+  // row's last byte is loaded whole, from within its own 16-byte granule.
   template <bool FULL, int FROM, int TO>
   __device__ __forceinline__ void issue(const unsigned char* p, unsigned char* st, int wave, int left) const {
-    const __amdgpu_buffer_rsrc_t r = make_rsrc(p, 0x7fffffe0);
+    const int end = (int)((rows - 1) * ld) + (FULL ? kBlock : min((left + 15) & ~15, kBlock));
+    const __amdgpu_buffer_rsrc_t r = make_rsrc(p, max(end, 0));
 #pragma unroll
     for (int i = FROM; i < TO; ++i) {
       lds_void* dst = (lds_void*)(st + (wave * kInst + i) * 1024);
+      const int row = (wave * kInst + i) * 8 * (int)ld;
       if constexpr (FULL)
-        dma16(r, dst, off[i]);
+        dma16(r, dst, at[i & 1], row);
       else
-        dma16(r, dst, dma_offset(key[i] < left, off[i]));
+        dma16(r, dst, dma_offset((i & 1 ? key ^ 64 : key) < left, at[i & 1]), row);
     }
   }
   // Zeros in place of what lies past `left` bytes in the chunk that holds them.
@@ -226,7 +230,7 @@ __global__ __launch_bounds__(64 * WM * WN, waves_per_simd(TM, TN, WM* WN, UNITS)
   constexpr int MI = TM / WM / 16, NI = TN / WN / 16;
   static_assert(MI >= 2 && NI >= 1 && MI * WM * 16 == TM && NI * WN * 16 == TN, "wave tile");
   static_assert(kBlock % (TM / WM) == 0, "a wave's outputs share a tile's scale");
-  static_assert(!EXACT || SC != kPower, "exact products take float32 scales");
+  static_assert(!EXACT || !by_power(SC), "exact products take float32 scales");
   using OpA = Side<TM, NW>;
   using OpB = Side<TN, NW>;
   // (In a ring of an even number of units a place holds units of one operand.)
@@ -255,52 +259,45 @@ __global__ __launch_bounds__(64 * WM * WN, waves_per_simd(TM, TN, WM* WN, UNITS)
   const unsigned char* pb = g.x + (int64_t)n0 * g.ldx + kbeg;
   OpA a;
   OpB b;
-  a.init(wave, lane, g.V - m0, g.ldw);
-  b.init(wave, lane, g.T - n0, g.ldx);
+  a.init(lane, g.V - m0, g.ldw);
+  b.init(lane, g.T - n0, g.ldx);
   const int base_a = OpA::base_of(lane, wm * (TM / WM)), base_b = OpB::base_of(lane, wn * (TN / WN));
 
-  // Scales: a stage's are loaded a stage ahead.
+  // Scales: a stage's are loaded a stage ahead, those of rows past the last as
+  // zeros.
+  constexpr int kHeld = by_power(SC) ? 1 : 4;
   const int quad = lane >> 4;
-  int at_x[NI];
-#pragma unroll
-  for (int j = 0; j < NI; ++j) at_x[j] = min(nfirst + 16 * j + (lane & 15), g.T - 1);
-  int at_w[SC == kPower ? MI : 1];
-  if constexpr (SC == kPower) {
-#pragma unroll
-    for (int i = 0; i < MI; ++i) {
-      const int v = min(mfirst + 16 * i + (lane & 15), g.V - 1);
-      at_w[i] = g.w_tile ? v / kBlock : v;
-    }
-  }
-  const int tile_w = min(mfirst / kBlock, (g.V - 1) / kBlock);
-  const int last_v = (g.V - 1) & ~3;
+  const int at_x = (nfirst + (lane & 15)) * kHeld;
+  const int at_w = by_tile(SC) ? mfirst / kBlock * kHeld : by_power(SC) ? mfirst + (lane & 15) : (mfirst + 4 * quad) * kHeld;
+  const int rows_w = by_tile(SC) ? (g.V + kBlock - 1) / kBlock : SC == kRow ? (g.V + 3) & ~3 : g.V;
   int block = kbeg / kBlock;  // of the scales that are loaded next
   const int last_block = block + nk - 1;
+  constexpr int kWs = by_tile(SC) ? 1 : MI;
   struct Scales {
     float x[NI];
     f32x4 w[SC == kRow ? MI : 1];
-    int ex[NI], ew[SC == kPower ? MI : 1];
+    int ex[NI], ew[kWs];
   };
   auto load_scales = [&](Scales& s) {
-    if constexpr (SC == kPower) {
-      const unsigned char* px = static_cast<const unsigned char*>(g.sx) + block * g.sx_block;
-      const unsigned char* pw = static_cast<const unsigned char*>(g.sw) + block * g.sw_block;
+    const __amdgpu_buffer_rsrc_t rx =
+        make_rsrc(static_cast<const unsigned char*>(g.sx) + block * g.sx_block * kHeld, g.T * kHeld);
+    const __amdgpu_buffer_rsrc_t rw =
+        make_rsrc(static_cast<const unsigned char*>(g.sw) + block * g.sw_block * kHeld, rows_w * kHeld);
+    if constexpr (by_power(SC)) {
 #pragma unroll
-      for (int j = 0; j < NI; ++j) s.ex[j] = px[at_x[j]];
+      for (int j = 0; j < NI; ++j) s.ex[j] = __builtin_amdgcn_raw_buffer_load_b8(rx, at_x + 16 * j, 0, 0);
 #pragma unroll
-      for (int i = 0; i < MI; ++i) s.ew[i] = pw[at_w[i]];
+      for (int i = 0; i < kWs; ++i) s.ew[i] = __builtin_amdgcn_raw_buffer_load_b8(rw, at_w + 16 * i, 0, 0);
     } else {
-      const float* px = static_cast<const float*>(g.sx) + block * g.sx_block;
-      const float* pw = static_cast<const float*>(g.sw) + block * g.sw_block;
 #pragma unroll
-      for (int j = 0; j < NI; ++j) s.x[j] = px[at_x[j]];
+      for (int j = 0; j < NI; ++j)
+        s.x[j] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rx, at_x + 64 * j, 0, 0));
       if constexpr (SC == kTile) {
-        s.w[0][0] = pw[tile_w];
+        s.w[0][0] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rw, at_w, 0, 0));
       } else {
-        // (rows of whole fours)
 #pragma unroll
         for (int i = 0; i < MI; ++i)
-          s.w[i] = *reinterpret_cast<const f32x4*>(pw + min(mfirst + 16 * i + 4 * quad, last_v));
+          s.w[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rw, at_w + 64 * i, 0, 0));
       }
     }
     block = min(block + 1, last_block);
@@ -348,14 +345,16 @@ __global__ __launch_bounds__(64 * WM * WN, waves_per_simd(TM, TN, WM* WN, UNITS)
 #pragma unroll
     for (int r = 0; r < 4; ++r)
       acc[i][j][r] = __builtin_fmaf(part[r], SC == kTile ? s.x[j] : s.x[j] * s.w[i][r], acc[i][j][r]);
+    asm volatile("" : "+v"(acc[i][j]));  // (here and not where the sums are used next)
   };
   // One group of 16 outputs times the wave's tokens.
   auto multiply = [&](auto ic, const FragA& fa, const FragB (&fb)[NI], const Scales& s) {
     constexpr int i = decltype(ic)::value;
     auto product = [&](auto jc) {
       constexpr int j = decltype(jc)::value, n = i * NI + j;
-      if constexpr (SC == kPower) {
-        acc[i][j] = mfma<X5>(fa, fb[j], acc[i][j], s.ew[i], s.ex[j]);
+      if constexpr (by_power(SC)) {
+        acc[i][j] = mfma<X5>(fa, fb[j], acc[i][j], s.ew[SC == kPowerRow ? i : 0], s.ex[j]);
+        asm volatile("" : "+v"(acc[i][j]));
       } else {
         if constexpr (EXACT)
           parts[(i & 1) * NI + j] = mfma(fa, fb[j]);
@@ -372,7 +371,7 @@ __global__ __launch_bounds__(64 * WM * WN, waves_per_simd(TM, TN, WM* WN, UNITS)
     static_assert(NI <= 4, "products");
   };
   auto finish = [&](const Scales& s) {
-    if constexpr (SC != kPower) {
+    if constexpr (!by_power(SC)) {
       constexpr int n = MI * NI;
       if constexpr (kLag > 3) scale(Int<n - 4>{}, s);
       if constexpr (kLag > 2) scale(Int<n - 3>{}, s);
@@ -524,6 +523,7 @@ __global__ __launch_bounds__(64 * WM * WN, waves_per_simd(TM, TN, WM* WN, UNITS)
         const int v = mfirst + 16 * i + 4 * quad;
         if (v < g.V) *reinterpret_cast<f32x4*>(row + v) = acc[i][j];
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
     return;
   }
@@ -557,6 +557,7 @@ __global__ __launch_bounds__(64 * WM * WN, waves_per_simd(TM, TN, WM* WN, UNITS)
         *reinterpret_cast<u32x2*>(out + chunk_at(t, 2 * i + (quad >> 1)) + 8 * (quad & 1)) =
             u32x2{pack_out(v[0], v[1], g.y_dtype), pack_out(v[2], v[3], g.y_dtype)};
     }
+    __builtin_amdgcn_sched_barrier(0);
     constexpr int kRows = 64 / kChunks;  // per instruction
     const int c = lane % kChunks, v0 = mfirst + c * (16 / kSize);
 #pragma unroll
