@@ -205,14 +205,18 @@ struct Side {
       *chunk = v;
     }
   }
-  // The lane's fragment of rows 16 i ... past `base` (made from the wave's first).
+  // The lane's fragment of rows 16 i ... past `base` (made from the wave's first):
+  // chunks l / 16 and l / 16 + 4.  An LDS cycle serves lanes 0 - 3, 12 - 15 and 20 -
+  // 27 together, or 4 - 11, 16 - 19 and 28 - 31 (and so on): with neighbouring
+  // chunks in lanes 16 apart those are 16 places in different banks (with chunks
+  // 2 (l / 16) half of all LDS cycles were conflicts; 8192^3 436 -> XX us).
   static __device__ __forceinline__ int base_of(int lane, int first) {
     const int row = lane & 15;
-    return (first + row) * kBlock + swz(row, 2 * (lane >> 4)) * 16;
+    return (first + row) * kBlock + swz(row, lane >> 4) * 16;
   }
   static __device__ __forceinline__ i32x8 frag(const unsigned char* st, int base, int i) {
     return join(*reinterpret_cast<const u32x4*>(st + base + i * 16 * kBlock),
-                *reinterpret_cast<const u32x4*>(st + (base ^ 16) + i * 16 * kBlock));
+                *reinterpret_cast<const u32x4*>(st + (base ^ 64) + i * 16 * kBlock));
   }
 };
 
@@ -267,31 +271,61 @@ __global__ __launch_bounds__(64 * WM * WN, waves_per_simd(TM, TN, WM* WN, UNITS)
   // zeros.
   constexpr int kHeld = by_power(SC) ? 1 : 4;
   const int quad = lane >> 4;
-  const int at_x = (nfirst + (lane & 15)) * kHeld;
+  static_assert(NI == 2 || NI == 4, "tokens' scales");
+  const int at_x = (nfirst + (lane & (16 * NI - 1))) * kHeld;
   const int at_w = by_tile(SC) ? mfirst / kBlock * kHeld : by_power(SC) ? mfirst + (lane & 15) : (mfirst + 4 * quad) * kHeld;
   const int rows_w = by_tile(SC) ? (g.V + kBlock - 1) / kBlock : SC == kRow ? (g.V + 3) & ~3 : g.V;
   int block = kbeg / kBlock;  // of the scales that are loaded next
   const int last_block = block + nk - 1;
   constexpr int kWs = by_tile(SC) ? 1 : MI;
+  // As loaded: of the wave's tokens, one a lane (a load for each group of 16 would
+  // take as many of the CU's address cycles as a third of the operands' DMA).
+  struct Loaded {
+    uint32_t x;
+    f32x4 w[SC == kRow ? MI : 1];
+    int ew[kWs];
+  };
+  // As used: x[j] in every lane that holds a sum of token 16 j + lane % 16.
   struct Scales {
     float x[NI];
     f32x4 w[SC == kRow ? MI : 1];
     int ex[NI], ew[kWs];
   };
-  auto load_scales = [&](Scales& s) {
+  auto spread = [&](const Loaded& l) {
+    Scales s;
+    uint32_t x[NI];
+    const auto rows = __builtin_amdgcn_permlane16_swap(l.x, l.x, false, false);
+    if constexpr (NI == 2) {
+      x[0] = rows[0], x[1] = rows[1];
+    } else {
+      const auto even = __builtin_amdgcn_permlane32_swap(rows[0], rows[0], false, false);
+      const auto odd = __builtin_amdgcn_permlane32_swap(rows[1], rows[1], false, false);
+      x[0] = even[0], x[1] = odd[0], x[2] = even[1], x[3] = odd[1];
+    }
+#pragma unroll
+    for (int j = 0; j < NI; ++j) {
+      if constexpr (by_power(SC))
+        s.ex[j] = (int)x[j];
+      else
+        s.x[j] = SC == kTile ? __builtin_bit_cast(float, x[j]) * l.w[0][0] : __builtin_bit_cast(float, x[j]);
+    }
+#pragma unroll
+    for (int i = 0; i < (SC == kRow ? MI : 1); ++i) s.w[i] = l.w[i];
+#pragma unroll
+    for (int i = 0; i < kWs; ++i) s.ew[i] = l.ew[i];
+    return s;
+  };
+  auto load_scales = [&](Loaded& s) {
     const __amdgpu_buffer_rsrc_t rx =
         make_rsrc(static_cast<const unsigned char*>(g.sx) + block * g.sx_block * kHeld, g.T * kHeld);
     const __amdgpu_buffer_rsrc_t rw =
         make_rsrc(static_cast<const unsigned char*>(g.sw) + block * g.sw_block * kHeld, rows_w * kHeld);
     if constexpr (by_power(SC)) {
-#pragma unroll
-      for (int j = 0; j < NI; ++j) s.ex[j] = __builtin_amdgcn_raw_buffer_load_b8(rx, at_x + 16 * j, 0, 0);
+      s.x = __builtin_amdgcn_raw_buffer_load_b8(rx, at_x, 0, 0);
 #pragma unroll
       for (int i = 0; i < kWs; ++i) s.ew[i] = __builtin_amdgcn_raw_buffer_load_b8(rw, at_w + 16 * i, 0, 0);
     } else {
-#pragma unroll
-      for (int j = 0; j < NI; ++j)
-        s.x[j] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rx, at_x + 64 * j, 0, 0));
+      s.x = __builtin_amdgcn_raw_buffer_load_b32(rx, at_x, 0, 0);
       if constexpr (SC == kTile) {
         s.w[0][0] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rw, at_w, 0, 0));
       } else {
@@ -332,7 +366,7 @@ __global__ __launch_bounds__(64 * WM * WN, waves_per_simd(TM, TN, WM* WN, UNITS)
   using FragA = std::conditional_t<EXACT, Halves, i32x8>;
   using FragB = std::conditional_t<EXACT, Halves, i32x8>;
   i32x8 ra, rb[NI];  // fragments as read
-  Scales next;
+  Loaded next;
   // Sums of a block that are not yet in the accumulators: the scaling of a sum runs
   // kLag products behind, so that it does not wait for its own.  Everything is
   // issued in the order written here: left to itself the compiler starts all
@@ -413,11 +447,7 @@ __global__ __launch_bounds__(64 * WM * WN, waves_per_simd(TM, TN, WM* WN, UNITS)
     constexpr int kParts = parts_of(kLast);
     constexpr int kNext = 2 * k + UNITS;
     const unsigned char* sa = place(Int<2 * k>{});
-    Scales s = next;
-    if constexpr (SC == kTile) {
-#pragma unroll
-      for (int j = 0; j < NI; ++j) s.x[j] *= s.w[0][0];
-    }
+    const Scales s = spread(next);
     load_scales(next);
     FragB fb[NI];
 #pragma unroll
