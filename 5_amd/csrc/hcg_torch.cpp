@@ -10,8 +10,9 @@
 // its general path; otherwise it returns hcg_gemm_algo's status (the message
 // is hcg_last_error's).
 //
-// The language-model operators handle contiguous device tensors on the current
-// device with new outputs.  They return those, None for anything else (the
+// The language-model operators handle contiguous device tensors (an 8-bit
+// product's operands: any rows that one stride reaches) on the current device
+// with new outputs.  They return those, None for anything else (the
 // Python wrapper's general path, which also names what is wrong with it), or
 // the call's status where it is not HCG_OK.
 
@@ -23,6 +24,7 @@
 
 #include <optional>
 
+#include "hcg_fp8.h"
 #include "hcg_gemm.h"
 #include "hcg_lm.h"
 
@@ -215,6 +217,190 @@ py::object linear_cross_entropy_grad(const at::Tensor& x, const at::Tensor& weig
   return rc ? py::cast(rc) : py::object(py::make_tuple(loss, dx, dw));
 }
 
+// What both forms of the root-mean-square norm make of their arguments.
+struct Rms {
+  int dtype, rdtype, pdtype;
+  int64_t rows, width;
+  at::Tensor h, rstd;
+  const void* residual;
+  void* sum;
+};
+bool rms_fits(const at::Tensor& x, const std::optional<at::Tensor>& weight, const std::optional<at::Tensor>& residual,
+              c10::DeviceIndex& dev, Rms& r) {
+  r.dtype = r.rdtype = r.pdtype = dtype_of(x);
+  if (r.dtype < 0 || x.dim() < 1 || x.size(-1) == 0 || !here(x, dev)) return false;
+  if (weight) {
+    if (!param_fits(*weight, x, dev)) return false;
+    r.pdtype = dtype_of(*weight);
+  }
+  if (residual) {
+    if (!here(*residual, dev) || residual->sizes() != x.sizes() ||
+        (residual->scalar_type() != x.scalar_type() && residual->scalar_type() != at::kFloat))
+      return false;
+    r.rdtype = dtype_of(*residual);
+  }
+  r.width = x.size(-1);
+  r.rows = x.numel() / r.width;
+  r.h = residual ? at::empty(x.sizes(), residual->options()) : x;
+  r.residual = residual ? residual->data_ptr() : nullptr;
+  r.sum = residual ? r.h.data_ptr() : nullptr;
+  r.rstd = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+  return true;
+}
+
+py::object rms_norm(const at::Tensor& x, const std::optional<at::Tensor>& weight,
+                    const std::optional<at::Tensor>& residual, double eps) {
+  c10::DeviceIndex dev = -1;
+  Rms r;
+  if (!rms_fits(x, weight, residual, dev, r)) return py::none();
+  at::Tensor y = at::empty(x.sizes(), x.options());
+  const int rc = hcg_rms_norm(r.dtype, x.data_ptr(), r.width, r.rows, r.width, r.rdtype, r.residual, r.width, r.pdtype,
+                              weight ? weight->data_ptr() : nullptr, (float)eps, y.data_ptr(), r.width, r.sum, r.width,
+                              static_cast<float*>(r.rstd.data_ptr()), stream_of(dev));
+  return rc ? py::cast(rc) : py::object(py::make_tuple(y, r.h, r.rstd));
+}
+
+py::object rms_norm_grad(const at::Tensor& dy, const at::Tensor& h, const at::Tensor& rstd,
+                         const std::optional<at::Tensor>& weight, const std::optional<at::Tensor>& dresidual) {
+  c10::DeviceIndex dev = -1;
+  const int dtype = dtype_of(dy), hdtype = dtype_of(h);
+  if (dtype < 0 || dy.dim() < 1 || dy.size(-1) == 0 || !here(dy, dev) || !here(h, dev) || !here(rstd, dev) ||
+      h.sizes() != dy.sizes() || (hdtype != dtype && hdtype != HCG_F32) || rstd.scalar_type() != at::kFloat)
+    return py::none();
+  const int64_t width = dy.size(-1), rows = dy.numel() / width;
+  if (rstd.numel() != rows || (weight && !param_fits(*weight, dy, dev))) return py::none();
+  if (dresidual && (!here(*dresidual, dev) || dresidual->sizes() != h.sizes() ||
+                    dresidual->scalar_type() != h.scalar_type()))
+    return py::none();
+  const int pdtype = weight ? dtype_of(*weight) : dtype;
+  at::Tensor dh = at::empty(h.sizes(), h.options()), dw = at::empty({width}, weight ? weight->options() : dy.options()),
+             ws;
+  const int64_t need = hcg_rms_norm_grad_workspace(rows, width);
+  if (need > 0) ws = workspace(need, dy);
+  const int rc = hcg_rms_norm_grad(dtype, dy.data_ptr(), width, hdtype, h.data_ptr(), width, rows, width,
+                                   static_cast<const float*>(rstd.data_ptr()), pdtype,
+                                   weight ? weight->data_ptr() : nullptr, dresidual ? dresidual->data_ptr() : nullptr,
+                                   width, dh.data_ptr(), width, dw.data_ptr(), need > 0 ? ws.data_ptr() : nullptr, need,
+                                   stream_of(dev));
+  return rc ? py::cast(rc) : py::object(py::make_tuple(dh, dw));
+}
+
+// New q (rows of whole 16 bytes) and scale (block by block in memory), as
+// hc.gfx950.fp8 lays them out.
+struct Quantized {
+  at::Tensor q, scale;
+  int64_t ldq, step;
+};
+Quantized new_quantized(const at::Tensor& like, c10::IntArrayRef lead, int64_t cols, c10::IntArrayRef down, int q_dtype,
+                        int scale_dtype) {
+  const auto strided = [](c10::IntArrayRef dims, int64_t last, int64_t first, at::ScalarType type, const at::Tensor& t,
+                          int64_t last_stride) {
+    auto shape = dims.vec();
+    std::vector<int64_t> strides(shape.size() + 1, last_stride);
+    int64_t step = first;
+    for (size_t i = shape.size(); i-- > 0; step *= std::max<int64_t>(shape[i], 1)) strides[i] = step;
+    shape.push_back(last);
+    return at::empty_strided(shape, strides, t.options().dtype(type));
+  };
+  Quantized r;
+  r.ldq = std::max<int64_t>((cols + 15) / 16 * 16, 1);
+  r.step = 1;
+  for (const int64_t n : down) r.step *= n;
+  r.step = std::max<int64_t>(r.step, 1);
+  r.q = strided(lead, cols, r.ldq, q_dtype == HCG_E5M2 ? at::kFloat8_e5m2 : at::kFloat8_e4m3fn, like, 1);
+  r.scale = strided(down, (cols + HCG_FP8_BLOCK - 1) / HCG_FP8_BLOCK, 1,
+                    scale_dtype == HCG_E8M0 ? at::kFloat8_e8m0fnu : at::kFloat, like, r.step);
+  return r;
+}
+
+py::object rms_norm_fp8(const at::Tensor& x, const std::optional<at::Tensor>& weight,
+                        const std::optional<at::Tensor>& residual, double eps, int q_dtype, int scale_dtype) {
+  c10::DeviceIndex dev = -1;
+  Rms r;
+  if (!rms_fits(x, weight, residual, dev, r)) return py::none();
+  const auto lead = x.sizes().slice(0, x.dim() - 1);
+  const Quantized o = new_quantized(x, lead, r.width, lead, q_dtype, scale_dtype);
+  const int rc = hcg_rms_norm_fp8(r.dtype, x.data_ptr(), r.width, r.rows, r.width, r.rdtype, r.residual, r.width,
+                                  r.pdtype, weight ? weight->data_ptr() : nullptr, (float)eps, q_dtype, o.q.data_ptr(),
+                                  o.ldq, scale_dtype, o.scale.data_ptr(), 1, o.step, r.sum, r.width,
+                                  static_cast<float*>(r.rstd.data_ptr()), stream_of(dev));
+  return rc ? py::cast(rc) : py::object(py::make_tuple(o.q, o.scale, r.h, r.rstd));
+}
+
+py::object quantize_fp8(const at::Tensor& x, bool tile, bool transpose, int q_dtype, int scale_dtype) {
+  c10::DeviceIndex dev = -1;
+  const int dtype = dtype_of(x);
+  if (dtype < 0 || x.dim() < 1 || x.numel() == 0 || !here(x, dev)) return py::none();
+  const int64_t cols = x.size(-1), rows = x.numel() / cols;
+  const int64_t turned[] = {cols}, tiles[] = {((transpose ? cols : rows) + HCG_FP8_BLOCK - 1) / HCG_FP8_BLOCK};
+  const auto lead = transpose ? c10::IntArrayRef(turned, 1) : x.sizes().slice(0, x.dim() - 1);
+  const Quantized o =
+      new_quantized(x, lead, transpose ? rows : cols, tile ? c10::IntArrayRef(tiles, 1) : lead, q_dtype, scale_dtype);
+  const int rc = hcg_quantize_fp8(dtype, x.data_ptr(), cols, rows, cols, transpose, tile, q_dtype, o.q.data_ptr(), o.ldq,
+                                  scale_dtype, o.scale.data_ptr(), 1, o.step, stream_of(dev));
+  return rc ? py::cast(rc) : py::object(py::make_tuple(o.q, o.scale));
+}
+
+// Whether the leading dimensions are rows that one stride reaches, which it gives.
+bool rows_of(const at::Tensor& t, int64_t& stride) {
+  stride = 1;
+  int64_t next = -1;
+  for (int64_t d = t.dim() - 2; d >= 0; --d) {
+    if (t.size(d) == 1) continue;
+    if (next < 0)
+      stride = t.stride(d);
+    else if (t.stride(d) != next)
+      return false;
+    next = t.stride(d) * t.size(d);
+  }
+  return true;
+}
+
+py::object linear_fp8(const at::Tensor& x, const at::Tensor& x_scale, const at::Tensor& weight,
+                      const at::Tensor& weight_scale, int out_dtype) {
+  if (!x.is_cuda() || !x_scale.is_cuda() || !weight.is_cuda() || !weight_scale.is_cuda()) return py::none();
+  const c10::DeviceIndex dev = x.get_device();
+  if (x_scale.get_device() != dev || weight.get_device() != dev || weight_scale.get_device() != dev ||
+      c10::hip::current_device() != dev)
+    return py::none();
+  const auto xt = x.scalar_type(), st = x_scale.scalar_type();
+  if ((xt != at::kFloat8_e4m3fn && xt != at::kFloat8_e5m2) || weight.scalar_type() != at::kFloat8_e4m3fn ||
+      (st != at::kFloat && st != at::kFloat8_e8m0fnu) || weight_scale.scalar_type() != st || x.dim() < 1 ||
+      weight.dim() != 2 || weight_scale.dim() != 2 || x_scale.dim() != x.dim() || x.numel() == 0 || weight.numel() == 0)
+    return py::none();
+  const int64_t inputs = x.size(-1), outputs = weight.size(0), tokens = x.numel() / inputs;
+  const int64_t blocks = (inputs + HCG_FP8_BLOCK - 1) / HCG_FP8_BLOCK;
+  const int64_t tiles = (outputs + HCG_FP8_BLOCK - 1) / HCG_FP8_BLOCK;
+  const bool tile = weight_scale.size(0) == tiles;
+  int64_t ldx, xs_row;
+  if (weight.size(1) != inputs || x_scale.size(-1) != blocks || weight_scale.size(1) != blocks ||
+      (!tile && weight_scale.size(0) != outputs) ||
+      x_scale.sizes().slice(0, x.dim() - 1) != x.sizes().slice(0, x.dim() - 1) || !rows_of(x, ldx) ||
+      !rows_of(x_scale, xs_row) || (inputs > 1 && (x.stride(-1) != 1 || weight.stride(1) != 1)) ||
+      (tokens > 1 && ldx < inputs) || (outputs > 1 && weight.stride(0) < inputs))
+    return py::none();
+  auto shape = x.sizes().vec();
+  shape.back() = outputs;
+  at::Tensor y = at::empty(shape, x.options().dtype(out_dtype == HCG_F16    ? at::kHalf
+                                                    : out_dtype == HCG_BF16 ? at::kBFloat16
+                                                                            : at::kFloat));
+  at::Tensor ws;
+  const int sdtype = st == at::kFloat ? HCG_F32 : HCG_E8M0;
+  if (tokens == 1) ldx = inputs;
+  const int64_t ldw = outputs == 1 ? inputs : weight.stride(0);
+  const int64_t need =
+      hcg_linear_fp8_workspace(HCG_FP8_AUTO, tokens, outputs, inputs, x.data_ptr(), ldx, weight.data_ptr(), ldw, sdtype,
+                               xs_row, tile, weight_scale.data_ptr(), weight_scale.stride(0), weight_scale.stride(1),
+                               out_dtype);
+  if (need > 0) ws = workspace(need, x);
+  const int rc =
+      hcg_linear_fp8(HCG_FP8_AUTO, xt == at::kFloat8_e5m2 ? HCG_E5M2 : HCG_E4M3, x.data_ptr(), ldx, tokens,
+                     weight.data_ptr(), ldw, outputs, inputs, sdtype, x_scale.data_ptr(), xs_row, x_scale.stride(-1), tile,
+                     weight_scale.data_ptr(), weight_scale.stride(0), weight_scale.stride(1), out_dtype, y.data_ptr(),
+                     outputs, need > 0 ? ws.data_ptr() : nullptr, need, stream_of(dev));
+  return rc ? py::cast(rc) : py::cast(y);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_hcg_torch, mod) {
@@ -225,4 +411,9 @@ PYBIND11_MODULE(_hcg_torch, mod) {
   mod.def("layer_norm_grad", &layer_norm_grad);
   mod.def("linear_cross_entropy", &linear_cross_entropy);
   mod.def("linear_cross_entropy_grad", &linear_cross_entropy_grad);
+  mod.def("rms_norm", &rms_norm);
+  mod.def("rms_norm_grad", &rms_norm_grad);
+  mod.def("rms_norm_fp8", &rms_norm_fp8);
+  mod.def("quantize_fp8", &quantize_fp8);
+  mod.def("linear_fp8", &linear_fp8);
 }

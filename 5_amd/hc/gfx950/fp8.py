@@ -27,11 +27,13 @@ autograd graph.
 
 from __future__ import annotations
 
+import math
 from typing import Any
 
 from .._errors import LaunchError
 from . import _native, lm
-from .lm import _ANY, _CODES, _call, _check_tensor, _code, _finish, _ld, _name, _out_rows, _ptr, _rms_args, _rows
+from .lm import (_ANY, _CODES, _call, _check_tensor, _code, _fast, _finish, _ld, _name, _out_rows, _ptr, _rms_args,
+                 _rows)
 
 _Q_CODES: dict[Any, int] = {}      # torch dtype -> HCG_E4M3, HCG_E5M2
 _SCALE_CODES: dict[Any, int] = {}  # torch dtype -> HCG_F32, HCG_E8M0
@@ -59,18 +61,27 @@ def _types(torch: Any, dtype: Any, scale_dtype: Any) -> tuple[Any, Any]:
     return dtype, scale_dtype
 
 
+def _new(torch: Any, lead: tuple[int, ...], last: int, first: int, step: int, dtype: Any, device: Any) -> Any:
+    """A tensor of shape lead + (last,): rows `first` apart, their elements `step`."""
+    strides = [step]
+    for n in reversed(lead):
+        strides.insert(0, first)
+        first *= max(n, 1)
+    return torch.empty_strided((*lead, last), strides, dtype=dtype, device=device)
+
+
 def _new_q(torch: Any, lead: tuple[int, ...], cols: int, dtype: Any, device: Any) -> tuple[Any, int]:
     """(q of shape lead + (cols,), its row stride): rows start at multiples of
     16 bytes, as the product reads them in place."""
-    ld = -(-cols // 16) * 16
-    return torch.empty((*lead, ld), dtype=dtype, device=device)[..., :cols], max(ld, 1)
+    ld = max(-(-cols // 16) * 16, 1)
+    return _new(torch, lead, cols, ld, 1, dtype, device), ld
 
 
 def _new_scale(torch: Any, lead: tuple[int, ...], blocks: int, dtype: Any, device: Any) -> tuple[Any, int]:
     """(scale of shape lead + (blocks,), the stride between its blocks): block
     by block in memory, so that neighbouring rows' lie next to each other."""
-    held = torch.empty((blocks, *lead), dtype=dtype, device=device)
-    return held.permute(*range(1, held.ndim), 0), max(held.numel() // max(blocks, 1), 1)
+    step = max(math.prod(lead), 1)
+    return _new(torch, lead, blocks, 1, step, dtype, device), step
 
 
 def quantize_fp8(x: Any, *, block: str = "row", transpose: bool = False, dtype: Any | None = None,
@@ -90,7 +101,6 @@ def quantize_fp8(x: Any, *, block: str = "row", transpose: bool = False, dtype: 
     code = _code(x, "x", _ANY)
     if block not in ("row", "tile"):
         raise LaunchError(f"unknown block {block!r}; expected 'row' or 'tile'")
-    dtype, scale_dtype = _types(torch, dtype, scale_dtype)
     rows = _rows(x, "x")
     n, cols = rows.shape
     lead, across = ((cols,), n) if transpose else (tuple(x.shape[:-1]), cols)
@@ -110,6 +120,9 @@ def rms_norm_fp8(x: Any, weight: Any | None = None, residual: Any | None = None,
     rstd)``, where q and scale stand for ``h * rstd * weight``."""
     torch = _torch()
     dtype, scale_dtype = _types(torch, dtype, scale_dtype)
+    r = _fast("rms_norm_fp8", x, weight, residual, eps, _Q_CODES[dtype], _SCALE_CODES[scale_dtype])
+    if r is not None:
+        return r if residual is not None else (r[0], r[1], x, r[3])
     index, code, rows, w, wcode, res, rcode, h, hrows, rstd = _rms_args(torch, x, weight, residual)
     n, width = rows.shape
     lead = tuple(x.shape[:-1])
@@ -145,6 +158,12 @@ def linear_fp8(x: Any, x_scale: Any, weight: Any, weight_scale: Any, *, out_dtyp
     result's own rounding.  Rows that start at multiples of 16 bytes, as
     :func:`quantize_fp8` makes them, are read where they lie."""
     torch = _torch()
+    if out is None and algo == "auto":
+        code = _CODES.get(torch.bfloat16 if out_dtype is None else out_dtype)
+        if code is not None:
+            r = _fast("linear_fp8", x, x_scale, weight, weight_scale, code)
+            if r is not None:
+                return r
     index = _check_tensor(torch, x, "x")
     if x.dtype not in _Q_CODES:
         raise LaunchError(f"x must be float8_e4m3fn or float8_e5m2, got {_name(x.dtype)}")

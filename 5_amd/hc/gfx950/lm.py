@@ -398,6 +398,10 @@ def rms_norm(x: Any, weight: Any | None = None, residual: Any | None = None, *, 
     ``residual``: x's shape, its type or float32; ``weight``: a vector of x's
     type or float32, or None.  h and rstd are what :func:`rms_norm_grad`
     takes, and h is the next residual."""
+    if out is None:
+        r = _fast("rms_norm", x, weight, residual, eps)
+        if r is not None:
+            return r if residual is not None else (r[0], x, r[2])
     torch = _torch()
     index, code, rows, w, wcode, res, rcode, h, hrows, rstd = _rms_args(torch, x, weight, residual)
     n, width = rows.shape
@@ -419,6 +423,10 @@ def rms_norm_grad(dy: Any, h: Any, rstd: Any, weight: Any | None = None, *, dres
     for the residual; ``dresidual`` (h's shape and type), the gradient that
     reaches h past the norm, is added to it.  dweight has the type of
     ``weight`` (dy's without one), or ``param_dtype``: dy's type or float32."""
+    if param_dtype is None:
+        r = _fast("rms_norm_grad", dy, h, rstd, weight, dresidual)
+        if r is not None:
+            return r
     torch = _torch()
     index = _check_tensor(torch, dy, "dy")
     code = _code(dy, "dy", _ANY)
