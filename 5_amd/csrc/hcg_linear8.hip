@@ -90,69 +90,156 @@ __device__ __forceinline__ float scale_at(const void* p, int64_t at) {
   return static_cast<const float*>(p)[at];
 }
 
-// A workgroup takes 16 rows of the weight and 16 NI tokens; its waves take the
-// blocks of K in turn and their sums meet in LDS, in the order of the waves.
-constexpr int kStreamWaves = 4;
+// For few tokens, bound by reading the weight (8192 x 8192: one token XX us, XX
+// TB/s).  A workgroup takes 16 R rows of the weight and 16 NI tokens; its waves
+// take the blocks of K in turn, each an own load of both operands, a block ahead,
+// and their sums meet in LDS, in the order of the waves.  Workgroups start at
+// blocks of their own (a golden-ratio sequence) and wrap: rows a power of two
+// apart put what is read at one k on a few HBM channels (4096 x 4096, one token:
+// 5.9 -> 4.7 us).
+constexpr int kStreamWaves = 8;
 
-template <bool X5, Scaling SC, bool EXACT, int NI>
+template <bool X5, Scaling SC, bool EXACT, int NI, int R>
 __global__ __launch_bounds__(64 * kStreamWaves) void stream_kernel(Args g) {
-  __shared__ f32x4 meet[kStreamWaves][NI][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int tiles_v = (g.V + 15) / 16;
+  __shared__ f32x4 meet[kStreamWaves][R * NI][64];
+  const int lane = threadIdx.x & 63, quad = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t tiles_v = (g.V + 16 * R - 1) / (16 * R), tiles = tiles_v * ((g.T + 16 * NI - 1) / (16 * NI));
   const int64_t wg = hcg::workgroup();
-  const int v0 = (int)(wg % tiles_v) * 16;
-  const int64_t t0 = wg / tiles_v * (16 * NI);
-  if (t0 >= g.T) return;
+  const int split = (int)(wg / tiles);
+  if (split >= g.splits) return;
+  const int64_t tile = wg - split * tiles;
+  const int v0 = (int)(tile % tiles_v) * 16 * R;
+  const int64_t t0 = tile / tiles_v * (16 * NI);
   // (Rows past the ends read the last one; their results go nowhere.)
-  const int v = min(v0 + (lane & 15), g.V - 1);
-  const unsigned char* w = g.w + v * g.ldw;
+  const unsigned char* w[R];
+  int64_t sw[R][by_power(SC) && !EXACT ? 1 : 4];
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int v = min(v0 + 16 * i + (lane & 15), g.V - 1);
+    w[i] = g.w + v * g.ldw + quad * 16;
+    if constexpr (by_power(SC) && !EXACT) {
+      sw[i][0] = (by_tile(SC) ? v / kBlock : v) * g.sw_row;
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int vr = min(v0 + 16 * i + 4 * quad + r, g.V - 1);
+        sw[i][r] = (by_tile(SC) ? vr / kBlock : vr) * g.sw_row;
+      }
+    }
+  }
   const unsigned char* x[NI];
   int64_t sx[NI];
 #pragma unroll
   for (int j = 0; j < NI; ++j) {
     const int64_t t = min(t0 + j * 16 + (lane & 15), (int64_t)g.T - 1);
-    x[j] = g.x + t * g.ldx;
+    x[j] = g.x + t * g.ldx + quad * 16;
     sx[j] = t * g.sx_row;
   }
-  f32x4 acc[NI];
+  f32x4 acc[R][NI];
 #pragma unroll
-  for (int j = 0; j < NI; ++j) acc[j] = f32x4{};
-  const int blocks = (g.K + kBlock - 1) / kBlock;
-  for (int b = wave; b < blocks; b += kStreamWaves) {
-    const int k = b * kBlock + (lane >> 4) * 32, left = g.K - k;
-    const i32x8 fw = join(load16(w + k, left), load16(w + k + 16, left - 16));
+  for (int i = 0; i < R; ++i)
 #pragma unroll
-    for (int j = 0; j < NI; ++j) {
-      const i32x8 fx = join(load16(x[j] + k, left), load16(x[j] + k + 16, left - 16));
-      if constexpr (by_power(SC) && !EXACT) {
-        const int ew = static_cast<const unsigned char*>(g.sw)[(by_tile(SC) ? v / kBlock : v) * g.sw_row + b * g.sw_block];
-        const int ex = static_cast<const unsigned char*>(g.sx)[sx[j] + b * g.sx_block];
-        acc[j] = mfma<X5>(fw, fx, acc[j], ew, ex);
-      } else {
-        f32x4 part;
-        if constexpr (EXACT)
-          part = mfma(halves<false>(fw), halves<X5>(fx));
-        else
-          part = mfma<X5>(fw, fx, f32x4{});
-        const float fx_scale = scale_at<SC>(g.sx, sx[j] + b * g.sx_block);
+    for (int j = 0; j < NI; ++j) acc[i][j] = f32x4{};
+
+  // Blocks of this split: `first` on, `whole` of them of kBlock inputs.
+  const int first = split * (g.chunk / kBlock), K = min(g.K - split * g.chunk, g.chunk), whole = K / kBlock;
+  const int start = (int)(((uint64_t)((uint32_t)wg * 2654435769u) * (uint32_t)whole) >> 32);
+  struct Block {
+    u32x4 w[R][2], x[NI][2];
+    float sx[NI], sw[R][by_tile(SC) ? 1 : 4];
+    int ex[NI], ew[R];
+  };
+  // A lane's bytes of a block are chunks l / 16 and l / 16 + 4: 64 neighbouring bytes
+  // of a row per load.
+  auto load = [&](Block& q, int b, auto full) {
+    const int64_t k = (int64_t)b * kBlock;
+    const int left = decltype(full)::value ? kBlock : g.K - (int)k - quad * 16;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int vr = min(v0 + 4 * (lane >> 4) + r, g.V - 1);
-          const int64_t row = by_tile(SC) ? vr / kBlock : vr;
-          acc[j][r] = __builtin_fmaf(part[r], fx_scale * scale_at<SC>(g.sw, row * g.sw_row + b * g.sw_block), acc[j][r]);
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int i = 0; i < R; ++i)
+        q.w[i][h] = decltype(full)::value ? *reinterpret_cast<const u32x4b*>(w[i] + k + 64 * h)
+                                          : load16(w[i] + k + 64 * h, left - 64 * h);
+#pragma unroll
+      for (int j = 0; j < NI; ++j)
+        q.x[j][h] = decltype(full)::value ? *reinterpret_cast<const u32x4b*>(x[j] + k + 64 * h)
+                                          : load16(x[j] + k + 64 * h, left - 64 * h);
+    }
+    if constexpr (by_power(SC) && !EXACT) {
+#pragma unroll
+      for (int j = 0; j < NI; ++j) q.ex[j] = static_cast<const unsigned char*>(g.sx)[sx[j] + b * g.sx_block];
+#pragma unroll
+      for (int i = 0; i < R; ++i) q.ew[i] = static_cast<const unsigned char*>(g.sw)[sw[i][0] + b * g.sw_block];
+    } else {
+#pragma unroll
+      for (int j = 0; j < NI; ++j) q.sx[j] = scale_at<SC>(g.sx, sx[j] + b * g.sx_block);
+#pragma unroll
+      for (int i = 0; i < R; ++i)
+#pragma unroll
+        for (int r = 0; r < (by_tile(SC) ? 1 : 4); ++r) q.sw[i][r] = scale_at<SC>(g.sw, sw[i][r] + b * g.sw_block);
+    }
+  };
+  auto add = [&](const Block& q) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const i32x8 fw = join(q.w[i][0], q.w[i][1]);
+#pragma unroll
+      for (int j = 0; j < NI; ++j) {
+        const i32x8 fx = join(q.x[j][0], q.x[j][1]);
+        if constexpr (by_power(SC) && !EXACT) {
+          acc[i][j] = mfma<X5>(fw, fx, acc[i][j], q.ew[i], q.ex[j]);
+        } else {
+          f32x4 part;
+          if constexpr (EXACT)
+            part = mfma(halves<false>(fw), halves<X5>(fx));
+          else
+            part = mfma<X5>(fw, fx, f32x4{});
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            acc[i][j][r] = __builtin_fmaf(part[r], q.sx[j] * q.sw[i][by_tile(SC) ? 0 : r], acc[i][j][r]);
         }
       }
     }
+  };
+  auto place = [&](int n) {  // of a wave's n-th block
+    const int b = n + start;
+    return first + (b >= whole ? b - whole : b);
+  };
+  Block now;
+  int n = wave;
+  if (n < whole) {
+    load(now, place(n), std::true_type{});
+    for (n += kStreamWaves; n < whole; n += kStreamWaves) {
+      Block next;
+      load(next, place(n), std::true_type{});
+      add(now);
+      now = next;
+    }
+    add(now);
   }
+  if (K % kBlock && wave == whole % kStreamWaves) {
+    load(now, first + whole, std::false_type{});
+    add(now);
+  }
+
 #pragma unroll
-  for (int j = 0; j < NI; ++j) meet[wave][j][lane] = acc[j];
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int j = 0; j < NI; ++j) meet[wave][i * NI + j][lane] = acc[i][j];
   __syncthreads();
-  for (int j = wave; j < NI; j += kStreamWaves) {
-    f32x4 sum = meet[0][j][lane];
+  for (int u = wave; u < R * NI; u += kStreamWaves) {
+    f32x4 sum = meet[0][u][lane];
 #pragma unroll
-    for (int q = 1; q < kStreamWaves; ++q) sum += meet[q][j][lane];
-    const int64_t t = t0 + j * 16 + (lane & 15);
-    if (t < g.T) store4(g, t, v0 + 4 * (lane >> 4), sum);
+    for (int q = 1; q < kStreamWaves; ++q) sum += meet[q][u][lane];
+    const int64_t t = t0 + u % NI * 16 + (lane & 15);
+    const int v = v0 + u / NI * 16 + 4 * quad;
+    if (t >= g.T) continue;
+    if (g.splits > 1) {
+      if (v < g.V) *reinterpret_cast<f32x4*>(g.part + ((int64_t)split * g.T + t) * g.ld_part + v) = sum;
+    } else {
+      store4(g, t, v, sum);
+    }
   }
 }
 
@@ -220,11 +307,12 @@ int64_t round_up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Tile shapes: rows of outputs and tokens.
-enum Shape { kStream, kLarge, kMedium, kNumShapes };
+enum Shape { kStream, kLarge, kMedium, kSmall, kNumShapes };
 struct ShapeInfo {
   int tm, tn;
 };
-constexpr ShapeInfo kShapes[kNumShapes] = {{0, 0}, {256, 256}, {128, 128}};
+constexpr ShapeInfo kShapes[kNumShapes] = {{0, 0}, {256, 256}, {128, 128}, {128, 64}};
+constexpr int kMaxSplits = 16;
 
 struct Plan {
   Shape shape;
@@ -252,25 +340,27 @@ bool in_place(const void* p, int64_t ld, int64_t rows) {
 
 Plan make_plan(const Problem& q) {
   Plan p{};
-  if (q.algo == HCG_FP8_AUTO)
+  const int64_t blocks = ceil_div(q.inputs, kBlock);
+  int splits = q.algo / HCG_FP8_SPLITS;
+  if (q.algo % HCG_FP8_SPLITS == HCG_FP8_AUTO)
     p.shape = q.tokens <= 64 ? kStream : kMedium;
   else
-    p.shape = (Shape)(q.algo - HCG_FP8_STREAM);
+    p.shape = (Shape)(q.algo % HCG_FP8_SPLITS - HCG_FP8_STREAM);
   if (p.shape == kLarge && (q.exact || (!q.w_tile && !q.e8m0))) p.shape = kMedium;
-  p.splits = 1;
-  p.chunk = (int)round_up(q.inputs, kBlock);
-  if (p.shape == kStream) return p;
-  const int64_t blocks = ceil_div(q.inputs, kBlock);
+  p.chunk = (int)ceil_div(blocks, std::max(1, splits)) * kBlock;
+  p.splits = (int)ceil_div(q.inputs, p.chunk);
+  const bool stream = p.shape == kStream;
   const bool floats = q.exact || !q.e8m0;  // scales that the kernel takes
-  p.copy_x = !in_place(q.x, q.ldx, q.tokens);
-  p.copy_w = !in_place(q.w, q.ldw, q.outputs);
+  p.copy_x = !stream && !in_place(q.x, q.ldx, q.tokens);
+  p.copy_w = !stream && !in_place(q.w, q.ldw, q.outputs);
   p.ldx = p.ldw = round_up(q.inputs, 16);
-  p.copy_sx = (q.tokens > 1 && q.sx_row != 1) || (q.e8m0 && floats);
+  p.copy_sx = !stream && ((q.tokens > 1 && q.sx_row != 1) || (q.e8m0 && floats));
   p.lds_x = q.tokens;
   // The weight's rows are read in whole, aligned fours.
   const int64_t rows = q.w_tile ? ceil_div(q.outputs, kBlock) : q.outputs;
-  p.copy_sw = (rows > 1 && q.sw_row != 1) || (q.e8m0 && floats) ||
-              (floats && !q.w_tile && (rows % 4 || (blocks > 1 && q.sw_block % 4) || (reinterpret_cast<uintptr_t>(q.sw) & 15)));
+  p.copy_sw = !stream && ((rows > 1 && q.sw_row != 1) || (q.e8m0 && floats) ||
+                          (floats && !q.w_tile &&
+                           (rows % 4 || (blocks > 1 && q.sw_block % 4) || (reinterpret_cast<uintptr_t>(q.sw) & 15))));
   p.lds_w = round_up(rows, 4);
   p.ld_part = round_up(q.outputs, 4);
   int64_t at = 0;
@@ -288,13 +378,24 @@ Plan make_plan(const Problem& q) {
   return p;
 }
 
+template <bool X5, Scaling SC, bool EXACT, int NI, int R>
+void launch_stream(const Args& a, hipStream_t s) {
+  const int64_t wgs = ceil_div(a.V, 16 * R) * ceil_div(a.T, 16 * NI) * a.splits;
+  stream_kernel<X5, SC, EXACT, NI, R><<<hcg::grid_of(wgs), 64 * kStreamWaves, 0, s>>>(a);
+}
+
 template <bool X5, Scaling SC, bool EXACT>
 void run_stream(const Args& a, hipStream_t s) {
-  const int64_t tiles_v = (a.V + 15) / 16;
+  // 32 rows per workgroup read x half as often, where that leaves a workgroup per
+  // CU: us, 16 / 32 rows, 16 tokens by 8192 x 8192 16.7 / 12.8, 64 tokens 37.9 /
+  // 24.3; 16 by 4096 x 4096 5.8 / 7.4; one token by 8192 x 8192 12.2 / 13.3.
+  const bool two = a.T > 1 && ceil_div(a.V, 32) * a.splits >= 256;
   if (a.T <= 16)
-    stream_kernel<X5, SC, EXACT, 1><<<hcg::grid_of(tiles_v), 64 * kStreamWaves, 0, s>>>(a);
+    two ? launch_stream<X5, SC, EXACT, 1, 2>(a, s) : launch_stream<X5, SC, EXACT, 1, 1>(a, s);
+  else if (a.T <= 32)
+    two ? launch_stream<X5, SC, EXACT, 2, 2>(a, s) : launch_stream<X5, SC, EXACT, 2, 1>(a, s);
   else
-    stream_kernel<X5, SC, EXACT, 4><<<hcg::grid_of(tiles_v * ((a.T + 63) / 64)), 64 * kStreamWaves, 0, s>>>(a);
+    two ? launch_stream<X5, SC, EXACT, 4, 2>(a, s) : launch_stream<X5, SC, EXACT, 4, 1>(a, s);
 }
 
 template <bool X5, Scaling SC, bool EXACT>
@@ -304,6 +405,8 @@ void run_tiles(Shape shape, const Args& a, hipStream_t s) {
     if (shape == kLarge)
       return hcg::fp8::tile_kernel<X5, SC, EXACT, 256, 256, 2, 4, 5><<<grid, 512, 0, s>>>(a);
   }
+  if (shape == kSmall)
+    return hcg::fp8::tile_kernel<X5, SC, EXACT, 128, 64, 4, 2, 6><<<grid, 512, 0, s>>>(a);
   if constexpr (SC == kRow || EXACT)
     hcg::fp8::tile_kernel<X5, SC, EXACT, 128, 128, 2, 2, 5><<<grid, 256, 0, s>>>(a);
   else
@@ -327,7 +430,8 @@ int hcg_linear_fp8(int algo, int x_dtype, const void* x, int64_t ldx, int64_t to
                    int64_t outputs, int64_t inputs, int scale_dtype, const void* x_scale, int64_t xs_row,
                    int64_t xs_block, int w_tile, const void* w_scale, int64_t ws_row, int64_t ws_block, int out_dtype,
                    void* y, int64_t ldy, void* workspace, int64_t workspace_bytes, void* stream) {
-  HCG_LM_REQUIRE(algo >= HCG_FP8_AUTO && algo <= HCG_FP8_128x128, "unknown algo %d", algo);
+  HCG_LM_REQUIRE(algo >= 0 && algo % HCG_FP8_SPLITS <= HCG_FP8_128x64 && algo / HCG_FP8_SPLITS <= kMaxSplits,
+                 "unknown algo %d", algo);
   HCG_LM_REQUIRE(hcg::fp8::type_ok(x_dtype), "x's type %d is not HCG_E4M3 or HCG_E5M2", x_dtype);
   HCG_LM_REQUIRE(hcg::fp8::scale_ok(scale_dtype), "scales of type %d are not HCG_F32 or HCG_E8M0", scale_dtype);
   HCG_LM_REQUIRE(hcg::elem_ok(out_dtype), "the output's type %d is not HCG_F16, HCG_BF16 or HCG_F32", out_dtype);

@@ -161,13 +161,13 @@ struct Side {
 
   int64_t ld;
   int rows;       // of the matrix, from the tile's first on
-  int key;        // the lane's first byte in an even instruction's rows; in an odd one's key ^ 64
-  int at[2];      // and its place from the wave's first row in either
+  int key;        // the lane's first byte in the rows of the wave's even instructions; in an odd one's key ^ 64
+  int at[2];      // and its place from the instruction's first row in either
 
-  __device__ __forceinline__ void init(int lane, int extent, int64_t stride) {
+  __device__ __forceinline__ void init(int wave, int lane, int extent, int64_t stride) {
     ld = stride;
     rows = min(extent, ROWS);
-    key = swz(lane >> 3, lane & 7) * 16;  // (8 rows on the swizzle differs by 4 chunks)
+    key = swz(wave * kInst * 8 + (lane >> 3), lane & 7) * 16;  // (8 rows on the swizzle differs by 4 chunks)
     at[0] = (lane >> 3) * (int)ld + key;
     at[1] = (lane >> 3) * (int)ld + (key ^ 64);
   }
@@ -263,11 +263,11 @@ __global__ __launch_bounds__(64 * WM * WN, waves_per_simd(TM, TN, WM* WN, UNITS)
   const unsigned char* pb = g.x + (int64_t)n0 * g.ldx + kbeg;
   OpA a;
   OpB b;
-  a.init(lane, g.V - m0, g.ldw);
-  b.init(lane, g.T - n0, g.ldx);
+  a.init(wave, lane, g.V - m0, g.ldw);
+  b.init(wave, lane, g.T - n0, g.ldx);
   const int base_a = OpA::base_of(lane, wm * (TM / WM)), base_b = OpB::base_of(lane, wn * (TN / WN));
 
-  // Scales: a stage's are loaded a stage ahead, those of rows past the last as
+  // Scales: a stage's are loaded two stages ahead, those of rows past the last as
   // zeros.
   constexpr int kHeld = by_power(SC) ? 1 : 4;
   const int quad = lane >> 4;
@@ -366,7 +366,8 @@ __global__ __launch_bounds__(64 * WM * WN, waves_per_simd(TM, TN, WM* WN, UNITS)
   using FragA = std::conditional_t<EXACT, Halves, i32x8>;
   using FragB = std::conditional_t<EXACT, Halves, i32x8>;
   i32x8 ra, rb[NI];  // fragments as read
-  Loaded next;
+  Loaded next;  // of the stage after the next one
+  Scales now;
   // Sums of a block that are not yet in the accumulators: the scaling of a sum runs
   // kLag products behind, so that it does not wait for its own.  Everything is
   // issued in the order written here: left to itself the compiler starts all
@@ -447,8 +448,7 @@ __global__ __launch_bounds__(64 * WM * WN, waves_per_simd(TM, TN, WM* WN, UNITS)
     constexpr int kParts = parts_of(kLast);
     constexpr int kNext = 2 * k + UNITS;
     const unsigned char* sa = place(Int<2 * k>{});
-    const Scales s = spread(next);
-    load_scales(next);
+    const Scales s = now;
     FragB fb[NI];
 #pragma unroll
     for (int j = 0; j < NI; ++j) fb[j] = as_b(rb[j]);
@@ -479,10 +479,13 @@ __global__ __launch_bounds__(64 * WM * WN, waves_per_simd(TM, TN, WM* WN, UNITS)
     const unsigned char* na = place(Int<2 * k + 2>{});
     const unsigned char* nb = place(Int<2 * k + 3>{});
     ra = OpA::frag(na, base_a, 0);
+    now = spread(next);
+    load_scales(next);  // (before the DMA that the next stage's wait may leave in flight)
+    __builtin_amdgcn_sched_barrier(0);
+    issue(Int<kNext>{}, full, Int<0>{}, Int<parts_of(kNext)>{});
     multiply(Int<MI - 1>{}, fa, fb, s);
 #pragma unroll
     for (int j = 0; j < NI; ++j) rb[j] = OpB::frag(nb, base_b, j);
-    issue(Int<kNext>{}, full, Int<0>{}, Int<parts_of(kNext)>{});
     finish(s);
     __builtin_amdgcn_sched_barrier(0);
   };
@@ -502,6 +505,9 @@ __global__ __launch_bounds__(64 * WM * WN, waves_per_simd(TM, TN, WM* WN, UNITS)
   static_assert(UNITS <= 8, "ring");
   wait_vm<dmas(2, UNITS - 3)>();
   __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+  now = spread(next);
+  load_scales(next);
   __builtin_amdgcn_sched_barrier(0);
   if (ragged && nk == 1) cut(Int<0>{});
   ra = OpA::frag(place(Int<0>{}), base_a, 0);

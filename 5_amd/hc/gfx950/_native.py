@@ -34,7 +34,8 @@ HCG_E5M2 = 4
 HCG_E8M0 = 5
 
 FP8_BLOCK = 128  # HCG_FP8_BLOCK
-FP8_ALGOS = {"auto": 0, "stream": 1, "256x256": 2, "128x128": 3}  # HCG_FP8_*
+FP8_ALGOS = {"auto": 0, "stream": 1, "256x256": 2, "128x128": 3, "128x64": 4}  # HCG_FP8_*
+FP8_SPLITS = 256
 
 HCG_ALGO_AUTO = 0
 HCG_ALGO_TILED = 1

@@ -97,10 +97,14 @@ def quantize_fp8(x: Any, *, block: str = "row", transpose: bool = False, dtype: 
     a), rounded to nearest; a float8_e8m0fnu scale is the least power of two not
     below a / F.  A block that holds an infinity or a NaN stands for NaN."""
     torch = _torch()
-    index = _check_tensor(torch, x, "x")
-    code = _code(x, "x", _ANY)
     if block not in ("row", "tile"):
         raise LaunchError(f"unknown block {block!r}; expected 'row' or 'tile'")
+    dtype, scale_dtype = _types(torch, dtype, scale_dtype)
+    r = _fast("quantize_fp8", x, block == "tile", bool(transpose), _Q_CODES[dtype], _SCALE_CODES[scale_dtype])
+    if r is not None:
+        return r
+    index = _check_tensor(torch, x, "x")
+    code = _code(x, "x", _ANY)
     rows = _rows(x, "x")
     n, cols = rows.shape
     lead, across = ((cols,), n) if transpose else (tuple(x.shape[:-1]), cols)
@@ -184,9 +188,11 @@ def linear_fp8(x: Any, x_scale: Any, weight: Any, weight_scale: Any, *, out_dtyp
     if not tile and tuple(weight_scale.shape) != (outputs, blocks):
         raise LaunchError(f"weight_scale shape {tuple(weight_scale.shape)} is neither {(outputs, blocks)} (rows) nor "
                           f"{(_blocks(outputs), blocks)} (tiles)")
-    number = _native.FP8_ALGOS.get(algo)
-    if number is None:
+    name, _, splits = str(algo).partition("/")  # "128x128/4": K in four parts
+    number = _native.FP8_ALGOS.get(name)
+    if number is None or (splits and not splits.isdigit()):
         raise LaunchError(f"unknown algo {algo!r}; expected one of {', '.join(_native.FP8_ALGOS)}")
+    number += _native.FP8_SPLITS * int(splits or 0)
     if out is not None:
         out_dtype = out.dtype if out_dtype is None and isinstance(out, torch.Tensor) else out_dtype
     out_dtype = torch.bfloat16 if out_dtype is None else out_dtype

@@ -27,7 +27,7 @@ F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
 E4M3, E5M2, E8M0 = torch.float8_e4m3fn, torch.float8_e5m2, torch.float8_e8m0fnu
 U = {F16: 2.0**-11, BF16: 2.0**-8, F32: 2.0**-24}
 LARGEST = {E4M3: 448.0, E5M2: 57344.0}
-ALGOS = ["auto", "stream", "256x256", "128x128"]
+ALGOS = ["auto", "stream", "stream/3", "256x256", "256x256/3", "128x128", "128x128/2", "128x64", "128x64/16"]
 
 
 def _gen(seed):
