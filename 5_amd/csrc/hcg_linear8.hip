@@ -403,14 +403,14 @@ void run_tiles(Shape shape, const Args& a, hipStream_t s) {
   const dim3 grid((unsigned)(ceil_div(a.V, kShapes[shape].tm) * ceil_div(a.T, kShapes[shape].tn) * a.splits));
   if constexpr (SC != kRow && !EXACT) {
     if (shape == kLarge)
-      return hcg::fp8::tile_kernel<X5, SC, EXACT, 256, 256, 2, 4, 5><<<grid, 512, 0, s>>>(a);
+      return hcg::fp8::tile_kernel<X5, SC, EXACT, 256, 256, 2, 4><<<grid, 512, 0, s>>>(a);
   }
   if (shape == kSmall)
-    return hcg::fp8::tile_kernel<X5, SC, EXACT, 128, 64, 4, 2, 6><<<grid, 512, 0, s>>>(a);
+    return hcg::fp8::tile_kernel<X5, SC, EXACT, 128, 64, 4, 2><<<grid, 512, 0, s>>>(a);
   if constexpr (SC == kRow || EXACT)
-    hcg::fp8::tile_kernel<X5, SC, EXACT, 128, 128, 2, 2, 5><<<grid, 256, 0, s>>>(a);
+    hcg::fp8::tile_kernel<X5, SC, EXACT, 128, 128, 2, 2><<<grid, 256, 0, s>>>(a);
   else
-    hcg::fp8::tile_kernel<X5, SC, EXACT, 128, 128, 2, 4, 5><<<grid, 512, 0, s>>>(a);
+    hcg::fp8::tile_kernel<X5, SC, EXACT, 128, 128, 2, 4><<<grid, 512, 0, s>>>(a);
 }
 
 }  // namespace

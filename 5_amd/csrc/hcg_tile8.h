@@ -3,9 +3,8 @@
 //
 // A TM x TN tile of outputs x tokens by WM x WN waves; K advances one block of 128
 // (a scale each) per stage.  A stage is two units, the weight's rows and x's, of
-// 128 bytes a row; a ring of UNITS LDS units is filled by global-to-LDS DMA.  One
-// barrier per stage: past it every wave has read the stage before, whose two
-// units are refilled UNITS units ahead.  The 16-byte chunks of an LDS row are
+// 128 bytes a row, filled by global-to-LDS DMA two stages ahead: three places for
+// the weight's, two for x's (160 KB for 256 x 256).  The 16-byte chunks of an LDS row are
 // XOR-swizzled so that the 16 lanes that read a fragment's column of chunks
 // cover all banks.
 //
@@ -223,13 +222,16 @@ struct Side {
 template <int I>
 using Int = std::integral_constant<int, I>;
 
-// Waves per SIMD: two workgroups per CU where the ring takes at most half its LDS.
-constexpr int waves_per_simd(int tm, int tn, int waves, int units) {
-  return waves / 4 * ((tm + tn) * kBlock * units / 2 <= 80 * 1024 ? 2 : 1);
+// Places in LDS for units of the weight and of x.
+constexpr int kPlacesA = 3, kPlacesB = 2;
+
+// Waves per SIMD: two workgroups per CU where the rings take at most half its LDS.
+constexpr int waves_per_simd(int tm, int tn, int waves) {
+  return waves / 4 * ((tm * kPlacesA + tn * kPlacesB) * kBlock <= 80 * 1024 ? 2 : 1);
 }
 
-template <bool X5, Scaling SC, bool EXACT, int TM, int TN, int WM, int WN, int UNITS>
-__global__ __launch_bounds__(64 * WM * WN, waves_per_simd(TM, TN, WM* WN, UNITS)) void tile_kernel(Args g) {
+template <bool X5, Scaling SC, bool EXACT, int TM, int TN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN, waves_per_simd(TM, TN, WM* WN)) void tile_kernel(Args g) {
   constexpr int NW = WM * WN;
   constexpr int MI = TM / WM / 16, NI = TN / WN / 16;
   static_assert(MI >= 2 && NI >= 1 && MI * WM * 16 == TM && NI * WN * 16 == TN, "wave tile");
@@ -237,15 +239,10 @@ __global__ __launch_bounds__(64 * WM * WN, waves_per_simd(TM, TN, WM* WN, UNITS)
   static_assert(!EXACT || !by_power(SC), "exact products take float32 scales");
   using OpA = Side<TM, NW>;
   using OpB = Side<TN, NW>;
-  // (In a ring of an even number of units a place holds units of one operand.)
-  constexpr int kUnitA = UNITS % 2 && OpB::kBytes > OpA::kBytes ? OpB::kBytes : OpA::kBytes;
-  constexpr int kUnitB = UNITS % 2 && OpA::kBytes > OpB::kBytes ? OpA::kBytes : OpB::kBytes;
-  static_assert(UNITS >= 4 && kUnitA * ((UNITS + 1) / 2) + kUnitB * (UNITS / 2) <= 160 * 1024, "ring");
-  auto place = [](auto uc) {
-    constexpr int P = decltype(uc)::value % UNITS;
-    return ring_unit<P % 2 ? kUnitB : kUnitA, P>();
-  };
-  constexpr int kPeriod = UNITS % 2 ? UNITS : UNITS / 2;  // stages until the units' places repeat
+  static_assert(OpA::kBytes * kPlacesA + OpB::kBytes * kPlacesB <= 160 * 1024, "rings");
+  auto place_a = [](auto kc) { return ring_unit<OpA::kBytes, decltype(kc)::value % kPlacesA>(); };
+  auto place_b = [](auto kc) { return ring_unit<OpB::kBytes, kPlacesA + decltype(kc)::value % kPlacesB>(); };
+  constexpr int kPeriod = 6;  // stages until the places repeat
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -344,23 +341,17 @@ __global__ __launch_bounds__(64 * WM * WN, waves_per_simd(TM, TN, WM* WN, UNITS)
     for (int j = 0; j < NI; ++j) acc[i][j] = f32x4{};
 
   int left_a = K, left_b = K;
-  auto issue = [&](auto uc, auto full, auto from, auto to) {
-    constexpr int U = decltype(uc)::value, F = decltype(from)::value, T = decltype(to)::value;
-    constexpr bool kFull = decltype(full)::value;
-    unsigned char* st = place(uc);
-    if constexpr (U % 2 == 0) {
-      a.template issue<kFull, F, T>(pa, st, wave, left_a);
-      if constexpr (T == OpA::kInst) pa += kBlock, left_a -= kBlock;
-    } else {
-      b.template issue<kFull, F, T>(pb, st, wave, left_b);
-      if constexpr (T == OpB::kInst) pb += kBlock, left_b -= kBlock;
-    }
+  // DMA instructions FROM to TO - 1 of the next unit of the weight, or of x, which is
+  // stage kc's.
+  auto issue_a = [&](auto kc, auto full, auto from, auto to) {
+    constexpr int F = decltype(from)::value, T = decltype(to)::value;
+    if constexpr (T > F) a.template issue<decltype(full)::value, F, T>(pa, place_a(kc), wave, left_a);
+    if constexpr (T > F && T == OpA::kInst) pa += kBlock, left_a -= kBlock;
   };
-  constexpr auto parts_of = [](int u) { return u % 2 ? OpB::kInst : OpA::kInst; };
-  constexpr auto dmas = [](int u, int n) {
-    int c = 0;
-    for (int i = 0; i < n; ++i) c += (u + i) % 2 ? OpB::kInst : OpA::kInst;
-    return c;
+  auto issue_b = [&](auto kc, auto full, auto from, auto to) {
+    constexpr int F = decltype(from)::value, T = decltype(to)::value;
+    if constexpr (T > F) b.template issue<decltype(full)::value, F, T>(pb, place_b(kc), wave, left_b);
+    if constexpr (T > F && T == OpB::kInst) pb += kBlock, left_b -= kBlock;
   };
 
   using FragA = std::conditional_t<EXACT, Halves, i32x8>;
@@ -432,33 +423,43 @@ __global__ __launch_bounds__(64 * WM * WN, waves_per_simd(TM, TN, WM* WN, UNITS)
   // they have landed (in both operands: they may be NaNs).
   const bool ragged = (K & 15) != 0;
   auto cut = [&](auto kc) {
-    constexpr int k = decltype(kc)::value;
-    OpA::cut(place(Int<2 * k>{}), tid, K & (kBlock - 1));
-    OpB::cut(place(Int<2 * k + 1>{}), tid, K & (kBlock - 1));
+    OpA::cut(place_a(kc), tid, K & (kBlock - 1));
+    OpB::cut(place_b(kc), tid, K & (kBlock - 1));
     wait_lgkm();
     __builtin_amdgcn_s_barrier();
   };
   // Stage k (known modulo kPeriod): on entry its scales, its tokens' fragments and
   // the first of its outputs' are in registers or on their way, on exit the next
-  // stage's.  The DMA of unit 2 k + UNITS goes out behind the barrier, that of
-  // the unit after it over the next stage's steps.
+  // stage's.  Its steps take 16 outputs each.  The weight's unit of stage k + 2
+  // goes out over the first half of them (its place held stage k - 1's); x's over
+  // the second half: its place held this stage's, whose fragments every wave has
+  // read once all have met in the middle.  So DMA instructions, each 16 cycles of
+  // the CU's address unit, never queue up in front of a wave's products.
+  constexpr int kHalf = MI / 2;
   auto iteration = [&](auto kc, auto full, int kt) {
     constexpr int k = decltype(kc)::value;
-    constexpr int kLast = 2 * k + UNITS - 1;  // the unit that the stage before left to issue
-    constexpr int kParts = parts_of(kLast);
-    constexpr int kNext = 2 * k + UNITS;
-    const unsigned char* sa = place(Int<2 * k>{});
+    const unsigned char* sa = place_a(kc);
     const Scales s = now;
     FragB fb[NI];
 #pragma unroll
     for (int j = 0; j < NI; ++j) fb[j] = as_b(rb[j]);
+    auto dma = [&](auto ic) {
+      constexpr int i = decltype(ic)::value;
+      if constexpr (i < kHalf)
+        issue_a(Int<k + 2>{}, full, Int<OpA::kInst * i / kHalf>{}, Int<OpA::kInst*(i + 1) / kHalf>{});
+      else
+        issue_b(Int<k + 2>{}, full, Int<OpB::kInst*(i - kHalf) / kHalf>{}, Int<OpB::kInst*(i - kHalf + 1) / kHalf>{});
+    };
     auto step = [&](auto ic) {
       constexpr int i = decltype(ic)::value;
-      constexpr int from = kParts * i / (MI - 1), to = kParts * (i + 1) / (MI - 1);
       const FragA fa = as_a(ra);
       ra = OpA::frag(sa, base_a, i + 1);
-      if constexpr (to > from) issue(Int<kLast>{}, full, Int<from>{}, Int<to>{});
+      dma(ic);
       multiply(ic, fa, fb, s);
+      if constexpr (i == kHalf - 1 && i < MI - 2) {
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+      }
     };
     step(Int<0>{});
     if constexpr (MI > 2) step(Int<1>{});
@@ -467,8 +468,10 @@ __global__ __launch_bounds__(64 * WM * WN, waves_per_simd(TM, TN, WM* WN, UNITS)
     if constexpr (MI > 5) step(Int<4>{});
     if constexpr (MI > 6) step(Int<5>{});
     if constexpr (MI > 7) step(Int<6>{});
-    static_assert(MI <= 8, "steps");
-    wait_vm<dmas(2 * k + 4, UNITS - 4)>();  // the next stage's two units have landed
+    static_assert(MI == 2 || MI == 4 || MI == 8, "steps");
+    // The next stage's two units have landed; what this stage has issued may be on
+    // its way.
+    wait_vm<OpA::kInst + OpB::kInst*(kHalf - 1) / kHalf>();
     wait_lgkm();
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
@@ -476,71 +479,57 @@ __global__ __launch_bounds__(64 * WM * WN, waves_per_simd(TM, TN, WM* WN, UNITS)
       if (ragged && kt + 2 == nk) cut(Int<k + 1>{});
     }
     const FragA fa = as_a(ra);
-    const unsigned char* na = place(Int<2 * k + 2>{});
-    const unsigned char* nb = place(Int<2 * k + 3>{});
-    ra = OpA::frag(na, base_a, 0);
-    now = spread(next);
-    load_scales(next);  // (before the DMA that the next stage's wait may leave in flight)
-    __builtin_amdgcn_sched_barrier(0);
-    issue(Int<kNext>{}, full, Int<0>{}, Int<parts_of(kNext)>{});
+    const unsigned char* nb = place_b(Int<k + 1>{});
+    ra = OpA::frag(place_a(Int<k + 1>{}), base_a, 0);
+    dma(Int<MI - 1>{});
     multiply(Int<MI - 1>{}, fa, fb, s);
+    now = spread(next);
+    load_scales(next);
 #pragma unroll
     for (int j = 0; j < NI; ++j) rb[j] = OpB::frag(nb, base_b, j);
     finish(s);
     __builtin_amdgcn_sched_barrier(0);
   };
 
-  auto first = [&](auto uc) {
-    constexpr int U = decltype(uc)::value;
-    if constexpr (U < UNITS - 1) issue(uc, Checked{}, Int<0>{}, Int<parts_of(U)>{});
-  };
   load_scales(next);
-  first(Int<0>{});
-  first(Int<1>{});
-  first(Int<2>{});
-  first(Int<3>{});
-  first(Int<4>{});
-  first(Int<5>{});
-  first(Int<6>{});
-  static_assert(UNITS <= 8, "ring");
-  wait_vm<dmas(2, UNITS - 3)>();
+  issue_a(Int<0>{}, Checked{}, Int<0>{}, Int<OpA::kInst>{});
+  issue_b(Int<0>{}, Checked{}, Int<0>{}, Int<OpB::kInst>{});
+  issue_a(Int<1>{}, Checked{}, Int<0>{}, Int<OpA::kInst>{});
+  issue_b(Int<1>{}, Checked{}, Int<0>{}, Int<OpB::kInst>{});
+  wait_vm<OpA::kInst + OpB::kInst>();
   __builtin_amdgcn_s_barrier();
   __builtin_amdgcn_sched_barrier(0);
   now = spread(next);
   load_scales(next);
   __builtin_amdgcn_sched_barrier(0);
   if (ragged && nk == 1) cut(Int<0>{});
-  ra = OpA::frag(place(Int<0>{}), base_a, 0);
+  ra = OpA::frag(place_a(Int<0>{}), base_a, 0);
 #pragma unroll
-  for (int j = 0; j < NI; ++j) rb[j] = OpB::frag(place(Int<1>{}), base_b, j);
+  for (int j = 0; j < NI; ++j) rb[j] = OpB::frag(place_b(Int<0>{}), base_b, j);
 
   int kt = 0;
   const int nfull = K / kBlock;
-  for (; kt + kPeriod + UNITS / 2 <= nfull; kt += kPeriod) {
+  for (; kt + kPeriod + 2 <= nfull; kt += kPeriod) {
     iteration(Int<0>{}, Full{}, 0);
     iteration(Int<1>{}, Full{}, 0);
-    if constexpr (kPeriod > 2) iteration(Int<2>{}, Full{}, 0);
-    if constexpr (kPeriod > 3) iteration(Int<3>{}, Full{}, 0);
-    if constexpr (kPeriod > 4) iteration(Int<4>{}, Full{}, 0);
+    iteration(Int<2>{}, Full{}, 0);
+    iteration(Int<3>{}, Full{}, 0);
+    iteration(Int<4>{}, Full{}, 0);
+    iteration(Int<5>{}, Full{}, 0);
   }
-  static_assert(kPeriod <= 5, "ring");
   while (kt < nk) {
     iteration(Int<0>{}, Checked{}, kt);
     if (++kt >= nk) break;
     iteration(Int<1>{}, Checked{}, kt);
     if (++kt >= nk) break;
-    if constexpr (kPeriod > 2) {
-      iteration(Int<2>{}, Checked{}, kt);
-      if (++kt >= nk) break;
-    }
-    if constexpr (kPeriod > 3) {
-      iteration(Int<3>{}, Checked{}, kt);
-      if (++kt >= nk) break;
-    }
-    if constexpr (kPeriod > 4) {
-      iteration(Int<4>{}, Checked{}, kt);
-      ++kt;
-    }
+    iteration(Int<2>{}, Checked{}, kt);
+    if (++kt >= nk) break;
+    iteration(Int<3>{}, Checked{}, kt);
+    if (++kt >= nk) break;
+    iteration(Int<4>{}, Checked{}, kt);
+    if (++kt >= nk) break;
+    iteration(Int<5>{}, Checked{}, kt);
+    ++kt;
   }
   wait_vm<0>();  // no DMA may still be writing LDS
   wait_lgkm();
@@ -567,13 +556,11 @@ __global__ __launch_bounds__(64 * WM * WN, waves_per_simd(TM, TN, WM* WN, UNITS)
   // 16 bytes that are neighbours.
   constexpr int kSize = EXACT ? 4 : 2;
   constexpr int kRow = MI * 16 * kSize, kChunks = kRow / 16, kStage = 16 * kRow;
-  constexpr int kLeast = kUnitA < kUnitB ? kUnitA : kUnitB;
-  constexpr int kPerUnit = kLeast / kStage;
-  static_assert(kPerUnit * 4 >= NW && kChunks <= 64, "staging");
-  unsigned char* const out = (wave < kPerUnit       ? place(Int<0>{})
-                              : wave < 2 * kPerUnit ? place(Int<1>{})
-                              : wave < 3 * kPerUnit ? place(Int<2>{})
-                                                    : place(Int<3>{})) +
+  constexpr int kPerUnit = OpA::kBytes / kStage;
+  static_assert(kPerUnit * kPlacesA >= NW && kChunks <= 64, "staging");
+  unsigned char* const out = (wave < kPerUnit       ? place_a(Int<0>{})
+                              : wave < 2 * kPerUnit ? place_a(Int<1>{})
+                                                    : place_a(Int<2>{})) +
                              wave % kPerUnit * kStage;
   // (Chunk c of row t lies at c ^ t, within the row's chunks.)
   auto chunk_at = [](int t, int c) { return t * kRow + (c ^ (t & (kChunks - 1))) * 16; };
