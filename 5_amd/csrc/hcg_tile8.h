@@ -262,25 +262,26 @@ __global__ __launch_bounds__(64 * WM * WN, waves_per_simd(TM, TN, WM* WN)) void 
   OpB b;
   a.init(wave, lane, g.V - m0, g.ldw);
   b.init(wave, lane, g.T - n0, g.ldx);
-  const int base_a = OpA::base_of(lane, wm * (TM / WM)), base_b = OpB::base_of(lane, wn * (TN / WN));
+  const int first_a = OpA::base_of(lane, wm * (TM / WM)), first_b = OpB::base_of(lane, wn * (TN / WN));
 
   // Scales: a stage's are loaded two stages ahead, those of rows past the last as
   // zeros.
   constexpr int kHeld = by_power(SC) ? 1 : 4;
   const int quad = lane >> 4;
-  static_assert(NI == 2 || NI == 4, "tokens' scales");
-  const int at_x = (nfirst + (lane & (16 * NI - 1))) * kHeld;
-  const int at_w = by_tile(SC) ? mfirst / kBlock * kHeld : by_power(SC) ? mfirst + (lane & 15) : (mfirst + 4 * quad) * kHeld;
+  static_assert(NI == 2 || NI == 4 || NI == 8, "tokens' scales");
+  const int at_x = (nfirst + (lane & (16 * NI - 1) & 63)) * kHeld;
+  const int at_w = by_tile(SC) ? mfirst / kBlock * kHeld : by_power(SC) ? mfirst + (lane & (16 * MI - 1) & 63) : (mfirst + 4 * quad) * kHeld;
   const int rows_w = by_tile(SC) ? (g.V + kBlock - 1) / kBlock : SC == kRow ? (g.V + 3) & ~3 : g.V;
   int block = kbeg / kBlock;  // of the scales that are loaded next
   const int last_block = block + nk - 1;
-  constexpr int kWs = by_tile(SC) ? 1 : MI;
-  // As loaded: of the wave's tokens, one a lane (a load for each group of 16 would
-  // take as many of the CU's address cycles as a third of the operands' DMA).
+  constexpr int kWs = SC == kPowerRow ? MI : 1;
+  // As loaded: of 64 of the wave's tokens or outputs, one a lane (a load for each
+  // group of 16 would take as many of the CU's address cycles as a third of the
+  // operands' DMA).
+  constexpr int kXs = NI > 4 ? NI / 4 : 1, kEws = SC == kPowerRow && MI > 4 ? MI / 4 : 1;
   struct Loaded {
-    uint32_t x;
+    uint32_t x[kXs], ew[kEws];
     f32x4 w[SC == kRow ? MI : 1];
-    int ew[kWs];
   };
   // As used: x[j] in every lane that holds a sum of token 16 j + lane % 16.
   struct Scales {
@@ -288,17 +289,26 @@ __global__ __launch_bounds__(64 * WM * WN, waves_per_simd(TM, TN, WM* WN)) void 
     f32x4 w[SC == kRow ? MI : 1];
     int ex[NI], ew[kWs];
   };
+  // v[j] = lane % 16 of each 16 lanes' values, j of `groups`.
+  auto fan = [](auto groups, const uint32_t* l, uint32_t* v) {
+    constexpr int G = decltype(groups)::value;
+    static_assert(G == 2 || G % 4 == 0, "groups");
+#pragma unroll
+    for (int q = 0; q < (G + 3) / 4; ++q) {
+      const auto rows = __builtin_amdgcn_permlane16_swap(l[q], l[q], false, false);
+      if constexpr (G == 2) {
+        v[0] = rows[0], v[1] = rows[1];
+      } else {
+        const auto even = __builtin_amdgcn_permlane32_swap(rows[0], rows[0], false, false);
+        const auto odd = __builtin_amdgcn_permlane32_swap(rows[1], rows[1], false, false);
+        v[4 * q] = even[0], v[4 * q + 1] = odd[0], v[4 * q + 2] = even[1], v[4 * q + 3] = odd[1];
+      }
+    }
+  };
   auto spread = [&](const Loaded& l) {
     Scales s;
     uint32_t x[NI];
-    const auto rows = __builtin_amdgcn_permlane16_swap(l.x, l.x, false, false);
-    if constexpr (NI == 2) {
-      x[0] = rows[0], x[1] = rows[1];
-    } else {
-      const auto even = __builtin_amdgcn_permlane32_swap(rows[0], rows[0], false, false);
-      const auto odd = __builtin_amdgcn_permlane32_swap(rows[1], rows[1], false, false);
-      x[0] = even[0], x[1] = odd[0], x[2] = even[1], x[3] = odd[1];
-    }
+    fan(Int<NI>{}, l.x, x);
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
       if constexpr (by_power(SC))
@@ -308,8 +318,14 @@ __global__ __launch_bounds__(64 * WM * WN, waves_per_simd(TM, TN, WM* WN)) void 
     }
 #pragma unroll
     for (int i = 0; i < (SC == kRow ? MI : 1); ++i) s.w[i] = l.w[i];
+    if constexpr (SC == kPowerRow) {
+      uint32_t w[MI];
+      fan(Int<MI>{}, l.ew, w);
 #pragma unroll
-    for (int i = 0; i < kWs; ++i) s.ew[i] = l.ew[i];
+      for (int i = 0; i < MI; ++i) s.ew[i] = (int)w[i];
+    } else {
+      s.ew[0] = (int)l.ew[0];
+    }
     return s;
   };
   auto load_scales = [&](Loaded& s) {
@@ -317,19 +333,23 @@ __global__ __launch_bounds__(64 * WM * WN, waves_per_simd(TM, TN, WM* WN)) void 
         make_rsrc(static_cast<const unsigned char*>(g.sx) + block * g.sx_block * kHeld, g.T * kHeld);
     const __amdgpu_buffer_rsrc_t rw =
         make_rsrc(static_cast<const unsigned char*>(g.sw) + block * g.sw_block * kHeld, rows_w * kHeld);
+#pragma unroll
+    for (int q = 0; q < kXs; ++q) {
+      if constexpr (by_power(SC))
+        s.x[q] = __builtin_amdgcn_raw_buffer_load_b8(rx, at_x + 64 * q, 0, 0);
+      else
+        s.x[q] = __builtin_amdgcn_raw_buffer_load_b32(rx, at_x + 256 * q, 0, 0);
+    }
     if constexpr (by_power(SC)) {
-      s.x = __builtin_amdgcn_raw_buffer_load_b8(rx, at_x, 0, 0);
 #pragma unroll
-      for (int i = 0; i < kWs; ++i) s.ew[i] = __builtin_amdgcn_raw_buffer_load_b8(rw, at_w + 16 * i, 0, 0);
+      for (int q = 0; q < kEws; ++q)
+        s.ew[q] = __builtin_amdgcn_raw_buffer_load_b8(rw, at_w + 64 * q, 0, 0);
+    } else if constexpr (SC == kTile) {
+      s.w[0][0] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rw, at_w, 0, 0));
     } else {
-      s.x = __builtin_amdgcn_raw_buffer_load_b32(rx, at_x, 0, 0);
-      if constexpr (SC == kTile) {
-        s.w[0][0] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rw, at_w, 0, 0));
-      } else {
 #pragma unroll
-        for (int i = 0; i < MI; ++i)
-          s.w[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rw, at_w + 64 * i, 0, 0));
-      }
+      for (int i = 0; i < MI; ++i)
+        s.w[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rw, at_w + 64 * i, 0, 0));
     }
     block = min(block + 1, last_block);
   };
@@ -363,38 +383,34 @@ __global__ __launch_bounds__(64 * WM * WN, waves_per_simd(TM, TN, WM* WN)) void 
   // kLag products behind, so that it does not wait for its own.  Everything is
   // issued in the order written here: left to itself the compiler starts all
   // products of a stage and spills.
-  constexpr int kLag = EXACT ? NI : NI / 2;
-  f32x4 parts[EXACT ? 2 * NI : NI];
-  auto scale = [&](auto nc, const Scales& s) {  // product number n of the stage
-    constexpr int n = decltype(nc)::value, i = n / NI, j = n % NI;
-    const f32x4 part = parts[EXACT ? (i & 1) * NI + j : j];
+  constexpr int kLag = EXACT ? NI : NI / 2, kSums = EXACT ? 2 * NI : NI;
+  f32x4 parts[kSums];
+  // The stage's products in their order: the last kLate groups of outputs are taken
+  // token group by token group, so that x's fragments come free one by one.
+  constexpr int kLate = MI > 2 ? 2 : 1, kEarly = MI - kLate;
+  constexpr auto group_of = [](int n) { return n < kEarly * NI ? n / NI : kEarly + n % kLate; };
+  constexpr auto tokens_of = [](int n) { return n < kEarly * NI ? n % NI : (n - kEarly * NI) / kLate; };
+  auto scale = [&](auto nc, const Scales& s) {
+    constexpr int n = decltype(nc)::value, i = group_of(n), j = tokens_of(n);
+    const f32x4 part = parts[n % kSums];
 #pragma unroll
     for (int r = 0; r < 4; ++r)
       acc[i][j][r] = __builtin_fmaf(part[r], SC == kTile ? s.x[j] : s.x[j] * s.w[i][r], acc[i][j][r]);
     asm volatile("" : "+v"(acc[i][j]));  // (here and not where the sums are used next)
   };
-  // One group of 16 outputs times the wave's tokens.
-  auto multiply = [&](auto ic, const FragA& fa, const FragB (&fb)[NI], const Scales& s) {
-    constexpr int i = decltype(ic)::value;
-    auto product = [&](auto jc) {
-      constexpr int j = decltype(jc)::value, n = i * NI + j;
-      if constexpr (by_power(SC)) {
-        acc[i][j] = mfma<X5>(fa, fb[j], acc[i][j], s.ew[SC == kPowerRow ? i : 0], s.ex[j]);
-        asm volatile("" : "+v"(acc[i][j]));
-      } else {
-        if constexpr (EXACT)
-          parts[(i & 1) * NI + j] = mfma(fa, fb[j]);
-        else
-          parts[j] = mfma<X5>(fa, fb[j], f32x4{});
-        if constexpr (n >= kLag) scale(Int<n - kLag>{}, s);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-    };
-    product(Int<0>{});
-    if constexpr (NI > 1) product(Int<1>{});
-    if constexpr (NI > 2) product(Int<2>{});
-    if constexpr (NI > 3) product(Int<3>{});
-    static_assert(NI <= 4, "products");
+  auto product = [&](auto nc, const FragA& fa, const FragB& fb, const Scales& s) {
+    constexpr int n = decltype(nc)::value, i = group_of(n), j = tokens_of(n);
+    if constexpr (by_power(SC)) {
+      acc[i][j] = mfma<X5>(fa, fb, acc[i][j], s.ew[SC == kPowerRow ? i : 0], s.ex[j]);
+      asm volatile("" : "+v"(acc[i][j]));
+    } else {
+      if constexpr (EXACT)
+        parts[n % kSums] = mfma(fa, fb);
+      else
+        parts[n % kSums] = mfma<X5>(fa, fb, f32x4{});
+      if constexpr (n >= kLag) scale(Int<n - kLag>{}, s);
+    }
+    __builtin_amdgcn_sched_barrier(0);
   };
   auto finish = [&](const Scales& s) {
     if constexpr (!by_power(SC)) {
@@ -430,19 +446,26 @@ __global__ __launch_bounds__(64 * WM * WN, waves_per_simd(TM, TN, WM* WN)) void 
   };
   // Stage k (known modulo kPeriod): on entry its scales, its tokens' fragments and
   // the first of its outputs' are in registers or on their way, on exit the next
-  // stage's.  Its steps take 16 outputs each.  The weight's unit of stage k + 2
-  // goes out over the first half of them (its place held stage k - 1's); x's over
-  // the second half: its place held this stage's, whose fragments every wave has
-  // read once all have met in the middle.  So DMA instructions, each 16 cycles of
-  // the CU's address unit, never queue up in front of a wave's products.
+  // stage's.  Its steps take 16 outputs each, the last kLate of them as one.  The
+  // weight's unit of stage k + 2 goes out over the first half (its place held stage
+  // k - 1's); x's over the second half: its place held this stage's, whose
+  // fragments every wave has read once all have met in the middle.  So DMA
+  // instructions, each 16 cycles of the CU's address unit, never queue up in front
+  // of a wave's products.  Before the last step all have read this stage's
+  // fragments and the next one's have landed: they are read between its products.
   constexpr int kHalf = MI / 2;
   auto iteration = [&](auto kc, auto full, int kt) {
     constexpr int k = decltype(kc)::value;
     const unsigned char* sa = place_a(kc);
     const Scales s = now;
+    // (Fresh every stage: the compiler would hold an address for each read whose
+    // place lies past the 64 KB that an LDS instruction's offset reaches.)
+    int base_a = first_a, base_b = first_b;
+    asm volatile("" : "+v"(base_a), "+v"(base_b));
     FragB fb[NI];
 #pragma unroll
     for (int j = 0; j < NI; ++j) fb[j] = as_b(rb[j]);
+    i32x8 rz = ra;  // of the last group of outputs
     auto dma = [&](auto ic) {
       constexpr int i = decltype(ic)::value;
       if constexpr (i < kHalf)
@@ -454,39 +477,64 @@ __global__ __launch_bounds__(64 * WM * WN, waves_per_simd(TM, TN, WM* WN)) void 
       constexpr int i = decltype(ic)::value;
       const FragA fa = as_a(ra);
       ra = OpA::frag(sa, base_a, i + 1);
+      if constexpr (kLate > 1 && i == kEarly - 1) rz = OpA::frag(sa, base_a, i + 2);
       dma(ic);
-      multiply(ic, fa, fb, s);
-      if constexpr (i == kHalf - 1 && i < MI - 2) {
-        __builtin_amdgcn_s_barrier();
-        __builtin_amdgcn_sched_barrier(0);
+      product(Int<i * NI>{}, fa, fb[0], s);
+      if constexpr (NI > 1) product(Int<i * NI + 1>{}, fa, fb[1], s);
+      if constexpr (NI > 2) product(Int<i * NI + 2>{}, fa, fb[2], s);
+      if constexpr (NI > 3) product(Int<i * NI + 3>{}, fa, fb[3], s);
+      if constexpr (NI > 4) {
+        product(Int<i * NI + 4>{}, fa, fb[4], s);
+        product(Int<i * NI + 5>{}, fa, fb[5], s);
+        product(Int<i * NI + 6>{}, fa, fb[6], s);
+        product(Int<i * NI + 7>{}, fa, fb[7], s);
+      }
+      if constexpr (i == kHalf - 1) {
+        wait_vm<OpA::kInst>();  // the next stage's two units have landed
+        if constexpr (i < kEarly - 1) {
+          __builtin_amdgcn_s_barrier();
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
     };
     step(Int<0>{});
-    if constexpr (MI > 2) step(Int<1>{});
-    if constexpr (MI > 3) step(Int<2>{});
-    if constexpr (MI > 4) step(Int<3>{});
-    if constexpr (MI > 5) step(Int<4>{});
-    if constexpr (MI > 6) step(Int<5>{});
-    if constexpr (MI > 7) step(Int<6>{});
+    if constexpr (kEarly > 1) step(Int<1>{});
+    if constexpr (kEarly > 2) step(Int<2>{});
+    if constexpr (kEarly > 3) step(Int<3>{});
+    if constexpr (kEarly > 4) step(Int<4>{});
+    if constexpr (kEarly > 5) step(Int<5>{});
+    if constexpr (kEarly > 6) step(Int<6>{});
     static_assert(MI == 2 || MI == 4 || MI == 8, "steps");
-    // The next stage's two units have landed; what this stage has issued may be on
-    // its way.
-    wait_vm<OpA::kInst + OpB::kInst*(kHalf - 1) / kHalf>();
     wait_lgkm();
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
     if constexpr (!decltype(full)::value) {
       if (ragged && kt + 2 == nk) cut(Int<k + 1>{});
     }
-    const FragA fa = as_a(ra);
+    const FragA fa = as_a(ra), fz = as_a(rz);
     const unsigned char* nb = place_b(Int<k + 1>{});
     ra = OpA::frag(place_a(Int<k + 1>{}), base_a, 0);
-    dma(Int<MI - 1>{});
-    multiply(Int<MI - 1>{}, fa, fb, s);
+    if constexpr (kLate > 1) dma(Int<kEarly>{});
+    auto late = [&](auto jc) {
+      constexpr int j = decltype(jc)::value, n = kEarly * NI + j * kLate;
+      if constexpr (j == NI / 2) dma(Int<MI - 1>{});
+      if constexpr (kLate > 1) product(Int<n>{}, fa, fb[j], s);
+      product(Int<n + kLate - 1>{}, kLate > 1 ? fz : fa, fb[j], s);
+      rb[j] = OpB::frag(nb, base_b, j);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    late(Int<0>{});
+    if constexpr (NI > 1) late(Int<1>{});
+    if constexpr (NI > 2) late(Int<2>{});
+    if constexpr (NI > 3) late(Int<3>{});
+    if constexpr (NI > 4) {
+      late(Int<4>{});
+      late(Int<5>{});
+      late(Int<6>{});
+      late(Int<7>{});
+    }
     now = spread(next);
     load_scales(next);
-#pragma unroll
-    for (int j = 0; j < NI; ++j) rb[j] = OpB::frag(nb, base_b, j);
     finish(s);
     __builtin_amdgcn_sched_barrier(0);
   };
@@ -503,9 +551,9 @@ __global__ __launch_bounds__(64 * WM * WN, waves_per_simd(TM, TN, WM* WN)) void 
   load_scales(next);
   __builtin_amdgcn_sched_barrier(0);
   if (ragged && nk == 1) cut(Int<0>{});
-  ra = OpA::frag(place_a(Int<0>{}), base_a, 0);
+  ra = OpA::frag(place_a(Int<0>{}), first_a, 0);
 #pragma unroll
-  for (int j = 0; j < NI; ++j) rb[j] = OpB::frag(place_b(Int<0>{}), base_b, j);
+  for (int j = 0; j < NI; ++j) rb[j] = OpB::frag(place_b(Int<0>{}), first_b, j);
 
   int kt = 0;
   const int nfull = K / kBlock;
