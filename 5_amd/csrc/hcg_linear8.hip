@@ -39,15 +39,34 @@ using hcg::fp8::Scaling;
 
 typedef uint32_t u32x4b __attribute__((ext_vector_type(4), aligned(1)));
 
-// 16 bytes at p, of which the first `left` are in the row (the rest zero, not read).
-__device__ __forceinline__ u32x4 load16(const unsigned char* p, int left) {
+// 16 bytes at p, of which the first `left` are in the row (the rest zero, not
+// read).  before: the row has bytes in front of p (at least 16 in all): a part is
+// then one load of the row's last 16, shifted.
+__device__ __forceinline__ u32x4 load16(const unsigned char* p, int left, bool before) {
   if (left >= 16) return *reinterpret_cast<const u32x4b*>(p);
   u32x4 r{0, 0, 0, 0};
+  if (left <= 0) return r;
+  if (before) {
+    const u32x4 v = *reinterpret_cast<const u32x4b*>(p + left - 16);
+    const int gone = 16 - left, words = gone >> 2;
+    uint32_t w[5];
+#pragma unroll
+    for (int i = 0; i < 5; ++i) {
+      w[i] = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (i + words == e) w[i] = v[e];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = __builtin_amdgcn_alignbyte(w[i + 1], w[i], gone & 3);
+    return r;
+  }
 #pragma unroll
   for (int b = 0; b < 16; ++b)
     if (b < left) r[b >> 2] |= (uint32_t)p[b] << (8 * (b & 3));
   return r;
 }
+
 // Four consecutive outputs of a token, the first `valid` of them in the row.
 __device__ __forceinline__ void store4(const Args& g, int64_t t, int v, f32x4 f) {
   const int valid = g.V - v;
@@ -160,11 +179,11 @@ __global__ __launch_bounds__(64 * kStreamWaves) void stream_kernel(Args g) {
 #pragma unroll
       for (int i = 0; i < R; ++i)
         q.w[i][h] = decltype(full)::value ? *reinterpret_cast<const u32x4b*>(w[i] + k + 64 * h)
-                                          : load16(w[i] + k + 64 * h, left - 64 * h);
+                                          : load16(w[i] + k + 64 * h, left - 64 * h, g.K >= 16);
 #pragma unroll
       for (int j = 0; j < NI; ++j)
         q.x[j][h] = decltype(full)::value ? *reinterpret_cast<const u32x4b*>(x[j] + k + 64 * h)
-                                          : load16(x[j] + k + 64 * h, left - 64 * h);
+                                          : load16(x[j] + k + 64 * h, left - 64 * h, g.K >= 16);
     }
     if constexpr (by_power(SC) && !EXACT) {
 #pragma unroll
@@ -255,7 +274,7 @@ __global__ __launch_bounds__(256) void copy_rows_kernel(const unsigned char* fro
   for (int64_t at = hcg::workgroup() * 256 + threadIdx.x; at < total; at += (int64_t)gridDim.x * gridDim.y * 256) {
     const int64_t row = at / vecs;
     const int c = (int)(at - row * vecs) * 16;
-    *reinterpret_cast<u32x4*>(to + row * ldt + c) = load16(from + row * ld + c, width - c);
+    *reinterpret_cast<u32x4*>(to + row * ldt + c) = load16(from + row * ld + c, width - c, width >= 16);
   }
 }
 
@@ -306,21 +325,41 @@ constexpr int64_t kMaxRows = (int64_t)1 << 26;
 int64_t round_up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Tile shapes: rows of outputs and tokens.
+// Forms of the product: tiles of outputs and tokens, and the workgroups that share
+// a CU.
 enum Shape { kStream, kLarge, kMedium, kSmall, kNumShapes };
 struct ShapeInfo {
-  int tm, tn;
+  int tm, tn, per_cu;
 };
-constexpr ShapeInfo kShapes[kNumShapes] = {{0, 0}, {256, 256}, {128, 128}, {128, 64}};
+constexpr ShapeInfo kShapes[kNumShapes] = {{0, 0, 2}, {256, 256, 1}, {128, 128, 2}, {128, 64, 2}};
 constexpr int kMaxSplits = 16;
+constexpr int kCus = 256;
+constexpr int64_t kMaxTiles = (int64_t)1 << 22;  // of a launch: its threads are fewer than 2^32
 
-struct Plan {
-  Shape shape;
-  int splits, chunk;
-  bool copy_x, copy_w, copy_sx, copy_sw;
-  int64_t ldx, ldw, lds_x, lds_w, ld_part;                // of the copies
-  int64_t x, w, sx, sw, part, total;                      // offsets into the workspace
+// A model of a form's time in us.  Tiles: a launch, and per round of workgroups a
+// tile's start and end and its stages, one of which takes `lo` on an idle chip and
+// `hi` on a busy one.  Stream: a launch, reading (16 or 32 rows of the weight and
+// x's) by a CU, per block, and the weight from HBM, in MB per us.  Split sums: a
+// launch, and their MB per us.  Fitted to 95000 times of 10000 random sizes of up
+// to 16384, every form and 1 to 16 splits; the pick is within 2.5% of the fastest in
+// the mean, and within 11% at 90% of the sizes.
+struct Cost {
+  double launch, fixed, lo, hi, join, join_rate;
 };
+enum Kind { kEightBit, kByRows, kExact };  // 16-bit results, those of weights scaled by rows in float32, float32 results
+constexpr Cost kCosts[3][kNumShapes] = {
+    {{3.343, 0, 0.04469, 26.64, 2.116, 1},
+     {2.864, 4.401, 1.084, 1.522, 1.01, 2.877},
+     {1.647, 2.906, 0.5214, 1.133, 2.254, 2.485},
+     {1.319, 2.742, 0.4667, 0.7993, 2.269, 2.223}},
+    {{3.378, 0, 0.04665, 16.02, 2.08, 0.837},
+     {},
+     {3.152, 2.545, 0.6693, 1.365, 1.75, 2.568},
+     {1.942, 2.631, 0.5516, 0.9689, 2.526, 2.431}},
+    {{3.463, 0, 0.04588, 16.01, 2.068, 0.7364},
+     {},
+     {2.088, 3.47, 1.069, 2.147, 1.994, 2.534},
+     {1.707, 3.495, 0.709, 1.333, 2.536, 2.255}}};
 
 struct Problem {
   int algo;
@@ -334,6 +373,72 @@ struct Problem {
   const void* sw;
 };
 
+// 32 rows per workgroup of the streaming form read x half as often, where that
+// leaves a workgroup per CU: us, 16 / 32 rows, 16 tokens by 8192 x 8192 16.7 / 12.8,
+// 64 tokens 37.9 / 24.3; 16 by 4096 x 4096 5.8 / 7.4; one token by 8192 x 8192 12.2 /
+// 13.3.
+int stream_rows(int64_t tokens, int64_t outputs, int splits) {
+  return tokens > 1 && ceil_div(outputs, 32) * splits >= kCus ? 2 : 1;
+}
+int stream_groups(int64_t tokens) { return tokens <= 16 ? 1 : tokens <= 32 ? 2 : 4; }
+
+// us; `chunk` blocks of K per split.
+double cost_of(Shape shape, Kind kind, const Problem& q, int chunk, int splits) {
+  const Cost& c = kCosts[kind][shape];
+  const uint32_t T = (uint32_t)q.tokens, V = (uint32_t)q.outputs;
+  double us = c.launch;
+  if (shape == kStream) {
+    const uint32_t r = stream_rows(T, V, splits), n = stream_groups(T);
+    const uint32_t wgs = (V + 16 * r - 1) / (16 * r) * ((T + 16 * n - 1) / (16 * n)) * splits;
+    us += (double)((wgs + kCus - 1) / kCus) * chunk * (r + n) * c.lo + (double)V * q.inputs * 1e-6 / c.hi;
+  } else {
+    const ShapeInfo& s = kShapes[shape];
+    const uint32_t units = ((V + s.tm - 1) / s.tm) * ((T + s.tn - 1) / s.tn) * splits, room = kCus * s.per_cu;
+    const uint32_t rest = units % room;
+    us += (double)(units / room) * (c.fixed + chunk * c.hi);
+    if (rest) {
+      const double busy = s.per_cu == 1 ? (double)rest / room : std::max(0.0, ((double)rest - kCus) / kCus);
+      us += c.fixed + chunk * (c.lo + (c.hi - c.lo) * busy);
+    }
+  }
+  if (splits > 1) us += c.join + (splits + 0.5) * T * V * 4e-6 / c.join_rate;
+  return us;
+}
+
+int64_t tiles_of(Shape s, const Problem& q) {
+  return ceil_div(q.outputs, kShapes[s].tm) * ceil_div(q.tokens, kShapes[s].tn);
+}
+
+void pick(const Problem& q, Shape& shape, int& splits) {
+  const Kind kind = q.exact ? kExact : !q.w_tile && !q.e8m0 ? kByRows : kEightBit;
+  const int blocks = (int)ceil_div(q.inputs, kBlock);
+  double best = -1;
+  for (int i = 0; i < kNumShapes; ++i) {
+    const Shape s = (Shape)i;
+    if (s == kStream && q.tokens > 64) continue;  // (past that a weight is read too often)
+    if (s == kLarge && kind != kEightBit) continue;
+    const int64_t tiles = s == kStream ? 1 : tiles_of(s, q);
+    if (tiles >= kMaxTiles) continue;
+    for (const int n : {1, 2, 3, 4, 6, 8, 12, 16}) {
+      if (n > 1 && (blocks / n < 2 || tiles * n > 5 * kCus)) break;
+      const int chunk = (blocks + n - 1) / n;
+      const double us = cost_of(s, kind, q, chunk, (blocks + chunk - 1) / chunk);
+      if (best >= 0 && us >= best) continue;
+      best = us;
+      shape = s;
+      splits = n;
+    }
+  }
+}
+
+struct Plan {
+  Shape shape;
+  int splits, chunk;
+  bool copy_x, copy_w, copy_sx, copy_sw;
+  int64_t ldx, ldw, lds_x, lds_w, ld_part;                // of the copies
+  int64_t x, w, sx, sw, part, total;                      // offsets into the workspace
+};
+
 bool in_place(const void* p, int64_t ld, int64_t rows) {
   return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (rows == 1 || ld % 16 == 0);
 }
@@ -342,10 +447,12 @@ Plan make_plan(const Problem& q) {
   Plan p{};
   const int64_t blocks = ceil_div(q.inputs, kBlock);
   int splits = q.algo / HCG_FP8_SPLITS;
-  if (q.algo % HCG_FP8_SPLITS == HCG_FP8_AUTO)
-    p.shape = q.tokens <= 64 ? kStream : kMedium;
-  else
+  if (q.algo % HCG_FP8_SPLITS == HCG_FP8_AUTO) {
+    p.shape = kMedium;
+    pick(q, p.shape, splits);
+  } else {
     p.shape = (Shape)(q.algo % HCG_FP8_SPLITS - HCG_FP8_STREAM);
+  }
   if (p.shape == kLarge && (q.exact || (!q.w_tile && !q.e8m0))) p.shape = kMedium;
   p.chunk = (int)ceil_div(blocks, std::max(1, splits)) * kBlock;
   p.splits = (int)ceil_div(q.inputs, p.chunk);
@@ -386,13 +493,11 @@ void launch_stream(const Args& a, hipStream_t s) {
 
 template <bool X5, Scaling SC, bool EXACT>
 void run_stream(const Args& a, hipStream_t s) {
-  // 32 rows per workgroup read x half as often, where that leaves a workgroup per
-  // CU: us, 16 / 32 rows, 16 tokens by 8192 x 8192 16.7 / 12.8, 64 tokens 37.9 /
-  // 24.3; 16 by 4096 x 4096 5.8 / 7.4; one token by 8192 x 8192 12.2 / 13.3.
-  const bool two = a.T > 1 && ceil_div(a.V, 32) * a.splits >= 256;
-  if (a.T <= 16)
+  const bool two = stream_rows(a.T, a.V, a.splits) == 2;
+  const int groups = stream_groups(a.T);
+  if (groups == 1)
     two ? launch_stream<X5, SC, EXACT, 1, 2>(a, s) : launch_stream<X5, SC, EXACT, 1, 1>(a, s);
-  else if (a.T <= 32)
+  else if (groups == 2)
     two ? launch_stream<X5, SC, EXACT, 2, 2>(a, s) : launch_stream<X5, SC, EXACT, 2, 1>(a, s);
   else
     two ? launch_stream<X5, SC, EXACT, 4, 2>(a, s) : launch_stream<X5, SC, EXACT, 4, 1>(a, s);
@@ -450,8 +555,12 @@ int hcg_linear_fp8(int algo, int x_dtype, const void* x, int64_t ldx, int64_t to
   const int sb = hcg::fp8::scale_bytes(scale_dtype);
   HCG_LM_REQUIRE(hcg::elem_aligned(x_scale, sb) && hcg::elem_aligned(w_scale, sb), "scales must be aligned");
   const bool e8m0 = scale_dtype == HCG_E8M0, exact = out_dtype == HCG_F32;
-  const Plan p = make_plan(Problem{algo, tokens, outputs, inputs, x, ldx, weight, ldw, w_tile != 0, e8m0, exact, xs_row,
-                                   ws_row, ws_block, w_scale});
+  const Problem q{algo, tokens, outputs, inputs, x,      ldx,    weight,   ldw,
+                  w_tile != 0, e8m0, exact, xs_row, ws_row, ws_block, w_scale};
+  const Plan p = make_plan(q);
+  HCG_LM_REQUIRE(p.shape == kStream ? ceil_div(tokens, 16) * ceil_div(outputs, 16) < (int64_t)1 << 32
+                                    : tiles_of(p.shape, q) * p.splits < kMaxTiles,
+                 "%lld tokens by %lld outputs are out of range", (long long)tokens, (long long)outputs);
   HCG_LM_REQUIRE(p.total == 0 || (workspace && workspace_bytes >= p.total && hcg::elem_aligned(workspace, 256)),
                  "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)p.total);
   const hipStream_t s = static_cast<hipStream_t>(stream);
