@@ -116,10 +116,12 @@ __device__ __forceinline__ float scale_at(const void* p, int64_t at) {
 // blocks of their own (a golden-ratio sequence) and wrap: rows a power of two
 // apart put what is read at one k on a few HBM channels (4096 x 4096, one token:
 // 5.9 -> 4.7 us).
-constexpr int kStreamWaves = 8;
+// Waves, that is, parts of K: as many again where a workgroup has 16 rows.
+constexpr int stream_waves(int r) { return r == 1 ? 8 : 4; }
 
 template <bool X5, Scaling SC, bool EXACT, int NI, int R>
-__global__ __launch_bounds__(64 * kStreamWaves) void stream_kernel(Args g) {
+__global__ __launch_bounds__(64 * stream_waves(R)) void stream_kernel(Args g) {
+  constexpr int kStreamWaves = stream_waves(R);
   __shared__ f32x4 meet[kStreamWaves][R * NI][64];
   const int lane = threadIdx.x & 63, quad = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -225,17 +227,22 @@ __global__ __launch_bounds__(64 * kStreamWaves) void stream_kernel(Args g) {
     const int b = n + start;
     return first + (b >= whole ? b - whole : b);
   };
-  Block now;
-  int n = wave;
-  if (n < whole) {
-    load(now, place(n), std::true_type{});
-    for (n += kStreamWaves; n < whole; n += kStreamWaves) {
-      Block next;
-      load(next, place(n), std::true_type{});
+  // Two blocks in turn, so that a block's loads never wait for a move of the one
+  // before; a load past the end reads the last block again.
+  Block now, next;
+  const int last = (whole - 1 - wave) / kStreamWaves * kStreamWaves + wave;
+  if (wave < whole) {
+    load(now, place(wave), std::true_type{});
+    for (int n = wave; n < whole; n += 2 * kStreamWaves) {
+      load(next, place(min(n + kStreamWaves, last)), std::true_type{});
+      __builtin_amdgcn_sched_barrier(0);
       add(now);
-      now = next;
+      __builtin_amdgcn_sched_barrier(0);
+      load(now, place(min(n + 2 * kStreamWaves, last)), std::true_type{});
+      __builtin_amdgcn_sched_barrier(0);
+      if (n + kStreamWaves < whole) add(next);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    add(now);
   }
   if (K % kBlock && wave == whole % kStreamWaves) {
     load(now, first + whole, std::false_type{});
@@ -373,12 +380,12 @@ struct Problem {
   const void* sw;
 };
 
-// 32 rows per workgroup of the streaming form read x half as often, where that
-// leaves a workgroup per CU: us, 16 / 32 rows, 16 tokens by 8192 x 8192 16.7 / 12.8,
-// 64 tokens 37.9 / 24.3; 16 by 4096 x 4096 5.8 / 7.4; one token by 8192 x 8192 12.2 /
-// 13.3.
+// 32 rows per workgroup (and four waves) of the streaming form read x half as
+// often, where that leaves a workgroup per CU: us, 16 rows and eight waves / 32 and
+// four, one token by 8192 x 8192 12.2 / 11.4, 16 tokens 16.7 / 12.9, 64 tokens 37.9 /
+// 24.3; one by 4096 x 4096 4.6 / 6.1, 16 by it 5.8 / 7.4.
 int stream_rows(int64_t tokens, int64_t outputs, int splits) {
-  return tokens > 1 && ceil_div(outputs, 32) * splits >= kCus ? 2 : 1;
+  return ceil_div(outputs, 32) * splits >= kCus ? 2 : 1;
 }
 int stream_groups(int64_t tokens) { return tokens <= 16 ? 1 : tokens <= 32 ? 2 : 4; }
 
@@ -488,7 +495,7 @@ Plan make_plan(const Problem& q) {
 template <bool X5, Scaling SC, bool EXACT, int NI, int R>
 void launch_stream(const Args& a, hipStream_t s) {
   const int64_t wgs = ceil_div(a.V, 16 * R) * ceil_div(a.T, 16 * NI) * a.splits;
-  stream_kernel<X5, SC, EXACT, NI, R><<<hcg::grid_of(wgs), 64 * kStreamWaves, 0, s>>>(a);
+  stream_kernel<X5, SC, EXACT, NI, R><<<hcg::grid_of(wgs), 64 * stream_waves(R), 0, s>>>(a);
 }
 
 template <bool X5, Scaling SC, bool EXACT>
