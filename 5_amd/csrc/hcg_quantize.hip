@@ -30,7 +30,10 @@ struct QuantArgs {
 constexpr int kThreads = 256;
 constexpr int kSide = 8;                     // a thread's rows and columns
 constexpr int kAcross = kBlock / kSide;      // threads along either side of a tile
-constexpr int kPitch = kBlock + 16;          // bytes between rows in LDS
+
+// Where row c of a turned tile has its 8 bytes i in LDS: the 16 threads that write
+// one i of rows 8 apart cover 32 banks (side by side they would share two).
+__device__ __forceinline__ int turned_at(int c, int i) { return c * kBlock + (i ^ (c / kSide)) * kSide; }
 
 __device__ __forceinline__ uint32_t shfl_max(uint32_t v, int mask) {
   return max(v, (uint32_t)__shfl_xor((int)v, mask));
@@ -111,13 +114,13 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(QuantArgs g) {
         hcg::fp8::store_q<kSide>(g.out.q + (row0 + r) * g.out.ldq + col0, v[r], s[TILE ? 0 : r].inverse, cols,
                                  g.out.e5m2);
   } else {
-    __shared__ __attribute__((aligned(16))) unsigned char turned[kBlock * kPitch];
+    __shared__ __attribute__((aligned(16))) unsigned char turned[kBlock * kBlock];
 #pragma unroll
     for (int e = 0; e < kSide; ++e) {
       float f[kSide];
 #pragma unroll
       for (int r = 0; r < kSide; ++r) f[r] = v[r][e];
-      hcg::fp8::store_q<kSide>(turned + (j * kSide + e) * kPitch + i * kSide, f, s[TILE ? 0 : e].inverse, kSide,
+      hcg::fp8::store_q<kSide>(turned + turned_at(j * kSide + e, i), f, s[TILE ? 0 : e].inverse, kSide,
                                g.out.e5m2);
     }
     __syncthreads();
@@ -128,12 +131,17 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(QuantArgs g) {
 #pragma unroll
     for (int c = tid >> 3; c < kBlock; c += kThreads / 8) {
       if (tc * kBlock + c >= g.cols || left <= 0) continue;
-      const unsigned char* from = turned + c * kPitch + part * 16;
+      // (Two neighbouring pieces of 8 bytes, in either order.)
+      const hcg::raw4 v = *reinterpret_cast<const hcg::raw4*>(turned + (turned_at(c, 2 * part) & ~15));
+      const bool swapped = c / kSide & 1;
+      const hcg::raw4 q = swapped ? hcg::raw4{v[2], v[3], v[0], v[1]} : v;
       unsigned char* to = g.out.q + (tc * kBlock + c) * g.out.ldq + tr * kBlock + part * 16;
       if (left == 16) {
-        *reinterpret_cast<u32x4a*>(to) = *reinterpret_cast<const hcg::raw4*>(from);
+        *reinterpret_cast<u32x4a*>(to) = q;
       } else {
-        for (int b = 0; b < left; ++b) to[b] = from[b];
+#pragma unroll
+        for (int b = 0; b < 16; ++b)
+          if (b < left) to[b] = (unsigned char)(q[b >> 2] >> (8 * (b & 3)));
       }
     }
   }

@@ -276,7 +276,7 @@ struct RmsGradArgs {
 // GROUPS row groups of LANES lanes; group q of workgroup b takes rows b * GROUPS +
 // q, + gridDim.x * GROUPS, ... and keeps its columns' sums of dy xh in registers;
 // the groups' sums meet in LDS once, at the end.
-template <class T, class H, int LANES, int NV, int GROUPS>
+template <class T, class H, int LANES, int NV, int GROUPS, bool AHEAD>
 __global__ __launch_bounds__(LANES * GROUPS) void rms_grad_kernel(RmsGradArgs g) {
   constexpr int E = kVec<T>, kWaves = LANES / 64;
   __shared__ float slots[2][kWaves > 1 ? GROUPS * kWaves : 1];
@@ -295,28 +295,45 @@ __global__ __launch_bounds__(LANES * GROUPS) void rms_grad_kernel(RmsGradArgs g)
   }
   const int64_t step = (int64_t)gridDim.x * GROUPS;
   int parity = 0;
+  // Loads run a row ahead of the work, where registers allow.
+  struct Row {
+    float rstd;
+    Raws<T, E> dy[NV];
+    Raws<H, E> h[NV], dres[NV];
+  };
+  auto load = [&](Row& r, int64_t row) {
+    const bool live = row < g.rows;
+    const int64_t at = live ? row : 0;
+    r.rstd = live ? g.rstd[at] : 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = first + i * LANES * E, left = live ? g.width - c : 0;
+      r.dy[i].load(static_cast<const T*>(g.dy) + at * g.lddy + c, left);
+      r.h[i].load(static_cast<const H*>(g.h) + at * g.ldh + c, left);
+      if (g.dres)
+        r.dres[i].load(static_cast<const H*>(g.dres) + at * g.lddr + c, left);
+      else
+        r.dres[i].clear();
+    }
+  };
+  Row next;
+  if constexpr (AHEAD) load(next, (int64_t)blockIdx.x * GROUPS + group);
   // (Every group runs as many turns as the workgroup's first: barriers.)
   for (int64_t row0 = (int64_t)blockIdx.x * GROUPS; row0 < g.rows; row0 += step) {
     const int64_t row = row0 + group;
     const bool live = row < g.rows;
-    const float rstd = live ? g.rstd[row] : 0.f;
+    if constexpr (!AHEAD) load(next, row);
+    const float rstd = next.rstd;
     float dy[NV][E], xh[NV][E];
     Raws<H, E> dres[NV];
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = first + i * LANES * E, left = live ? g.width - c : 0;
-      Raws<T, E> a;
-      Raws<H, E> b;
-      a.load(static_cast<const T*>(g.dy) + (live ? row : 0) * g.lddy + c, left);
-      b.load(static_cast<const H*>(g.h) + (live ? row : 0) * g.ldh + c, left);
-      if (g.dres)
-        dres[i].load(static_cast<const H*>(g.dres) + (live ? row : 0) * g.lddr + c, left);
-      else
-        dres[i].clear();
-      a.floats(dy[i]);
-      b.floats(xh[i]);
+      next.dy[i].floats(dy[i]);
+      next.h[i].floats(xh[i]);
+      dres[i] = next.dres[i];
     }
+    if constexpr (AHEAD) load(next, row + step);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
 #pragma unroll
@@ -496,10 +513,10 @@ void run_rms(const RmsArgs& a, hipStream_t s) {
   rms_wide_kernel<T, H, Q><<<hcg::grid_of(a.rows), 1024, 0, s>>>(a);
 }
 
-template <class T, class H, int LANES, int NV, int GROUPS>
+template <class T, class H, int LANES, int NV, int GROUPS, bool AHEAD = true>
 int launch_rms_grad(const RmsGradArgs& a, hipStream_t s) {
   const int64_t wgs = std::min<int64_t>(kGradParts, (a.rows + GROUPS - 1) / GROUPS);
-  rms_grad_kernel<T, H, LANES, NV, GROUPS><<<dim3((unsigned)wgs), LANES * GROUPS, 0, s>>>(a);
+  rms_grad_kernel<T, H, LANES, NV, GROUPS, AHEAD><<<dim3((unsigned)wgs), LANES * GROUPS, 0, s>>>(a);
   return (int)wgs;
 }
 
@@ -511,10 +528,13 @@ int run_rms_grad(const RmsGradArgs& a, hipStream_t s) {
   if (vecs <= 32) return launch_rms_grad<T, H, 32, 1, 16>(a, s);
   if (vecs <= 64) return launch_rms_grad<T, H, 64, 1, 8>(a, s);
   if (vecs <= 128) return launch_rms_grad<T, H, 128, 1, 8>(a, s);
+  if (vecs <= 192) return launch_rms_grad<T, H, 192, 1, 5>(a, s);
   if (vecs <= 256) return launch_rms_grad<T, H, 256, 1, 4>(a, s);
+  if (vecs <= 320) return launch_rms_grad<T, H, 320, 1, 3>(a, s);
+  if (vecs <= 384) return launch_rms_grad<T, H, 384, 1, 2>(a, s);
   if (vecs <= 512) return launch_rms_grad<T, H, 512, 1, 2>(a, s);
   if (vecs <= 1024) return launch_rms_grad<T, H, 512, 2, 1>(a, s);
-  if (vecs <= 2048) return launch_rms_grad<T, H, 1024, 2, 1>(a, s);
+  if (vecs <= 2048) return launch_rms_grad<T, H, 1024, 2, 1, false>(a, s);
   rms_grad_wide_kernel<T, H><<<hcg::grid_of(a.rows), 1024, 0, s>>>(a);
   const int parts = (int)std::min<int64_t>(64, a.rows);
   if (a.part) rms_columns_kernel<T, H><<<dim3((unsigned)((a.width + 255) / 256), parts), 256, 0, s>>>(a);
