@@ -109,8 +109,8 @@ __device__ __forceinline__ float scale_at(const void* p, int64_t at) {
   return static_cast<const float*>(p)[at];
 }
 
-// For few tokens, bound by reading the weight (8192 x 8192: one token XX us, XX
-// TB/s).  A workgroup takes 16 R rows of the weight and 16 NI tokens; its waves
+// For few tokens, bound by reading the weight (8192 x 8192: one token 12.9 us, 5.2
+// TB/s, 16 tokens 14.7).  A workgroup takes 16 R rows of the weight and 16 NI tokens; its waves
 // take the blocks of K in turn, each an own load of both operands, a block ahead,
 // and their sums meet in LDS, in the order of the waves.  Workgroups start at
 // blocks of their own (a golden-ratio sequence) and wrap: rows a power of two
@@ -345,28 +345,29 @@ constexpr int64_t kMaxTiles = (int64_t)1 << 22;  // of a launch: its threads are
 
 // A model of a form's time in us.  Tiles: a launch, and per round of workgroups a
 // tile's start and end and its stages, one of which takes `lo` on an idle chip and
-// `hi` on a busy one.  Stream: a launch, reading (16 or 32 rows of the weight and
-// x's) by a CU, per block, and the weight from HBM, in MB per us.  Split sums: a
-// launch, and their MB per us.  Fitted to 95000 times of 10000 random sizes of up
-// to 16384, every form and 1 to 16 splits; the pick is within 2.5% of the fastest in
-// the mean, and within 11% at 90% of the sizes.
+// `hi` on a busy one.  Stream: a launch, a CU's reading of 16 rows (of the weight
+// and of x), per block, by eight waves (`fixed`) or by four (`lo`), and the weight
+// from HBM, in MB per us.  Split sums: a launch, and their MB per us.  Fitted to
+// 100000 times of 9000 random sizes of up to 16384, every form and 1 to 16 splits;
+// the pick is within 2.5% of the fastest in the mean, and within 10% at 90% of the
+// sizes.
 struct Cost {
   double launch, fixed, lo, hi, join, join_rate;
 };
 enum Kind { kEightBit, kByRows, kExact };  // 16-bit results, those of weights scaled by rows in float32, float32 results
 constexpr Cost kCosts[3][kNumShapes] = {
-    {{3.343, 0, 0.04469, 26.64, 2.116, 1},
-     {2.864, 4.401, 1.084, 1.522, 1.01, 2.877},
-     {1.647, 2.906, 0.5214, 1.133, 2.254, 2.485},
-     {1.319, 2.742, 0.4667, 0.7993, 2.269, 2.223}},
-    {{3.378, 0, 0.04665, 16.02, 2.08, 0.837},
+    {{3.486, 0.04653, 0.05115, 20.52, 2.469, 0.7162},
+     {2.446, 4.91, 1.041, 1.471, 1.096, 2.883},
+     {1.618, 2.978, 0.5232, 1.128, 2.222, 2.526},
+     {1.026, 3.015, 0.467, 0.7949, 2.312, 2.276}},
+    {{3.504, 0.04981, 0.05003, 11.75, 2.475, 0.6476},
      {},
-     {3.152, 2.545, 0.6693, 1.365, 1.75, 2.568},
-     {1.942, 2.631, 0.5516, 0.9689, 2.526, 2.431}},
-    {{3.463, 0, 0.04588, 16.01, 2.068, 0.7364},
+     {3.208, 2.44, 0.6607, 1.355, 1.786, 2.613},
+     {1.988, 2.661, 0.5501, 0.9477, 2.407, 2.34}},
+    {{3.573, 0.0528, 0.06427, 29.02, 2.45, 0.4975},
      {},
-     {2.088, 3.47, 1.069, 2.147, 1.994, 2.534},
-     {1.707, 3.495, 0.709, 1.333, 2.536, 2.255}}};
+     {1.984, 3.684, 1.068, 2.101, 1.97, 2.505},
+     {1.843, 3.401, 0.7088, 1.331, 2.542, 2.282}}};
 
 struct Problem {
   int algo;
@@ -397,7 +398,7 @@ double cost_of(Shape shape, Kind kind, const Problem& q, int chunk, int splits) 
   if (shape == kStream) {
     const uint32_t r = stream_rows(T, V, splits), n = stream_groups(T);
     const uint32_t wgs = (V + 16 * r - 1) / (16 * r) * ((T + 16 * n - 1) / (16 * n)) * splits;
-    us += (double)((wgs + kCus - 1) / kCus) * chunk * (r + n) * c.lo + (double)V * q.inputs * 1e-6 / c.hi;
+    us += (double)((wgs + kCus - 1) / kCus) * chunk * (r + n) * (r == 1 ? c.fixed : c.lo) + (double)V * q.inputs * 1e-6 / c.hi;
   } else {
     const ShapeInfo& s = kShapes[shape];
     const uint32_t units = ((V + s.tm - 1) / s.tm) * ((T + s.tn - 1) / s.tn) * splits, room = kCus * s.per_cu;

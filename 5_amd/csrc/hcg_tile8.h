@@ -208,7 +208,7 @@ struct Side {
   // chunks l / 16 and l / 16 + 4.  An LDS cycle serves lanes 0 - 3, 12 - 15 and 20 -
   // 27 together, or 4 - 11, 16 - 19 and 28 - 31 (and so on): with neighbouring
   // chunks in lanes 16 apart those are 16 places in different banks (with chunks
-  // 2 (l / 16) half of all LDS cycles were conflicts; 8192^3 436 -> XX us).
+  // 2 (l / 16) half of all LDS cycles were conflicts).
   static __device__ __forceinline__ int base_of(int lane, int first) {
     const int row = lane & 15;
     return (first + row) * kBlock + swz(row, lane >> 4) * 16;
@@ -383,7 +383,7 @@ __global__ __launch_bounds__(64 * WM * WN, waves_per_simd(TM, TN, WM* WN)) void 
   // kLag products behind, so that it does not wait for its own.  Everything is
   // issued in the order written here: left to itself the compiler starts all
   // products of a stage and spills.
-  constexpr int kLag = EXACT ? NI : NI / 2, kSums = EXACT ? 2 * NI : NI;
+  constexpr int kLag = EXACT ? NI : NI - 1, kSums = EXACT ? 2 * NI : NI;
   f32x4 parts[kSums];
   // The stage's products in their order: the last kLate groups of outputs are taken
   // token group by token group, so that x's fragments come free one by one.
