@@ -345,29 +345,29 @@ constexpr int64_t kMaxTiles = (int64_t)1 << 22;  // of a launch: its threads are
 
 // A model of a form's time in us.  Tiles: a launch, and per round of workgroups a
 // tile's start and end and its stages, one of which takes `lo` on an idle chip and
-// `hi` on a busy one.  Stream: a launch, a CU's reading of 16 rows (of the weight
-// and of x), per block, by eight waves (`fixed`) or by four (`lo`), and the weight
-// from HBM, in MB per us.  Split sums: a launch, and their MB per us.  Fitted to
-// 100000 times of 9000 random sizes of up to 16384, every form and 1 to 16 splits;
-// the pick is within 2.5% of the fastest in the mean, and within 10% at 90% of the
-// sizes.
+// `hi` on a busy one, or a start and the weight from HBM (`rate`, MB per us).  Stream:
+// a launch, and a CU's reading of 16 rows (of the weight and of x's), per block, by
+// eight waves (`fixed`) or by four (`lo`), or the weight from HBM.  Split sums: a
+// launch, and their MB per us.  Fitted to 100000 times of 9000 random sizes of up to
+// 16384, every form and 1 to 16 splits; the pick is within 2.1% of the fastest in the
+// mean, and within 10% at 90% of the sizes.
 struct Cost {
-  double launch, fixed, lo, hi, join, join_rate;
+  double launch, fixed, lo, hi, join, join_rate, rate;
 };
 enum Kind { kEightBit, kByRows, kExact };  // 16-bit results, those of weights scaled by rows in float32, float32 results
 constexpr Cost kCosts[3][kNumShapes] = {
-    {{3.486, 0.04653, 0.05115, 20.52, 2.469, 0.7162},
-     {2.446, 4.91, 1.041, 1.471, 1.096, 2.883},
-     {1.618, 2.978, 0.5232, 1.128, 2.222, 2.526},
-     {1.026, 3.015, 0.467, 0.7949, 2.312, 2.276}},
-    {{3.504, 0.04981, 0.05003, 11.75, 2.475, 0.6476},
+    {{3.501, 0.06312, 0.06408, 0, 2.493, 0.7264, 4.346},
+     {2.441, 4.915, 1.041, 1.47, 1.095, 2.883, 5.371},
+     {1.471, 3.126, 0.5236, 1.092, 2.125, 2.53, 5.047},
+     {0.8981, 3.142, 0.4686, 0.7523, 2.162, 2.272, 5.164}},
+    {{3.533, 0.06905, 0.06739, 0, 2.522, 0.6559, 3.862},
      {},
-     {3.208, 2.44, 0.6607, 1.355, 1.786, 2.613},
-     {1.988, 2.661, 0.5501, 0.9477, 2.407, 2.34}},
-    {{3.573, 0.0528, 0.06427, 29.02, 2.45, 0.4975},
+     {2.985, 2.664, 0.6613, 1.294, 1.688, 2.596, 4.44},
+     {1.861, 2.786, 0.552, 0.9062, 2.285, 2.311, 4.965}},
+    {{3.57, 0.07146, 0.08228, 0, 2.481, 0.5148, 4.034},
      {},
-     {1.984, 3.684, 1.068, 2.101, 1.97, 2.505},
-     {1.843, 3.401, 0.7088, 1.331, 2.542, 2.282}}};
+     {1.761, 3.908, 1.068, 2.036, 1.858, 2.495, 2.848},
+     {1.722, 3.517, 0.7111, 1.298, 2.425, 2.274, 3.875}}};
 
 struct Problem {
   int algo;
@@ -381,12 +381,15 @@ struct Problem {
   const void* sw;
 };
 
-// 32 rows per workgroup (and four waves) of the streaming form read x half as
-// often, where that leaves a workgroup per CU: us, 16 rows and eight waves / 32 and
-// four, one token by 8192 x 8192 12.2 / 11.4, 16 tokens 16.7 / 12.9, 64 tokens 37.9 /
-// 24.3; one by 4096 x 4096 4.6 / 6.1, 16 by it 5.8 / 7.4.
+// 16 rows per workgroup of the streaming form (by eight waves), or 32 (by four),
+// which read x half as often: what gives a CU less to read.  us, 16 / 32 rows, one
+// token by 8192 x 8192 12.2 / 11.4, 16 tokens 16.7 / 12.9, 64 tokens 37.9 / 24.3; one
+// by 4096 x 4096 4.6 / 6.1, 16 by it 5.8 / 7.4.
 int stream_rows(int64_t tokens, int64_t outputs, int splits) {
-  return ceil_div(outputs, 32) * splits >= kCus ? 2 : 1;
+  const int64_t tiles = ceil_div(tokens, 64) * splits, n = std::min<int64_t>(tokens, 64);
+  const int64_t one = ceil_div(ceil_div(outputs, 16) * tiles, kCus) * (16 + n);
+  const int64_t two = ceil_div(ceil_div(outputs, 32) * tiles, kCus) * (32 + n);
+  return two < one ? 2 : 1;
 }
 int stream_groups(int64_t tokens) { return tokens <= 16 ? 1 : tokens <= 32 ? 2 : 4; }
 
@@ -394,21 +397,23 @@ int stream_groups(int64_t tokens) { return tokens <= 16 ? 1 : tokens <= 32 ? 2 :
 double cost_of(Shape shape, Kind kind, const Problem& q, int chunk, int splits) {
   const Cost& c = kCosts[kind][shape];
   const uint32_t T = (uint32_t)q.tokens, V = (uint32_t)q.outputs;
-  double us = c.launch;
+  const double from_hbm = (double)V * q.inputs * 1e-6 / c.rate;
+  double us = 0;
   if (shape == kStream) {
-    const uint32_t r = stream_rows(T, V, splits), n = stream_groups(T);
-    const uint32_t wgs = (V + 16 * r - 1) / (16 * r) * ((T + 16 * n - 1) / (16 * n)) * splits;
-    us += (double)((wgs + kCus - 1) / kCus) * chunk * (r + n) * (r == 1 ? c.fixed : c.lo) + (double)V * q.inputs * 1e-6 / c.hi;
+    const uint32_t r = stream_rows(T, V, splits), wgs = (V + 16 * r - 1) / (16 * r) * splits;  // (up to 64 tokens)
+    us = std::max((double)((wgs + kCus - 1) / kCus) * chunk * (r + T / 16.0) * (r == 1 ? c.fixed : c.lo), from_hbm);
   } else {
     const ShapeInfo& s = kShapes[shape];
     const uint32_t units = ((V + s.tm - 1) / s.tm) * ((T + s.tn - 1) / s.tn) * splits, room = kCus * s.per_cu;
     const uint32_t rest = units % room;
-    us += (double)(units / room) * (c.fixed + chunk * c.hi);
+    us = (double)(units / room) * (c.fixed + chunk * c.hi);
     if (rest) {
       const double busy = s.per_cu == 1 ? (double)rest / room : std::max(0.0, ((double)rest - kCus) / kCus);
       us += c.fixed + chunk * (c.lo + (c.hi - c.lo) * busy);
     }
+    us = std::max(us, c.fixed + from_hbm);
   }
+  us += c.launch;
   if (splits > 1) us += c.join + (splits + 0.5) * T * V * 4e-6 / c.join_rate;
   return us;
 }
