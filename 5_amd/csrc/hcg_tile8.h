@@ -183,11 +183,12 @@ struct Side {
 #pragma unroll
     for (int i = FROM; i < TO; ++i) {
       lds_void* dst = (lds_void*)(st + (wave * kInst + i) * 1024);
-      const int row = (wave * kInst + i) * 8 * (int)ld;
+      // (All of the offset is the lane's: what is checked against the extent.)
+      const int off = at[i & 1] + (wave * kInst + i) * 8 * (int)ld;
       if constexpr (FULL)
-        dma16(r, dst, at[i & 1], row);
+        dma16(r, dst, off);
       else
-        dma16(r, dst, dma_offset((i & 1 ? key ^ 64 : key) < left, at[i & 1]), row);
+        dma16(r, dst, dma_offset((i & 1 ? key ^ 64 : key) < left, off));
     }
   }
   // Zeros in place of what lies past `left` bytes in the chunk that holds them.

@@ -422,3 +422,99 @@ def test_graph_and_streams():
         torch.cuda.synchronize()
         for a, b in zip(got, want):
             assert torch.equal(a, b)
+
+
+# --------------------------------------------------------------------------
+# Past 31 bits, beside other work, on other streams
+# --------------------------------------------------------------------------
+
+
+def test_quantize_past_31_bits():
+    """More than 2^31 elements in, more than 2^31 bytes out, compared by some
+    of the rows."""
+    rows, cols = 70001, 32768
+    x = torch.empty((rows, cols), dtype=BF16, device=DEV)
+    gen = _gen(12)
+    picks = [0, 1, 65535, 65536, 65537, rows - 1]
+    x.zero_()
+    for r in picks:
+        x[r] = _randn(gen, (cols,), BF16)
+    q, s = g.quantize_fp8(x)
+    for r in picks:
+        want_q, want_s = _quantize_want(x[r : r + 1], False, E4M3, F32)
+        _same(q[r : r + 1], want_q)
+        _same(s[r : r + 1], want_s)
+    del q, s
+    q, s = g.quantize_fp8(x, transpose=True)
+    cols_at = [0, 32767, 12345]
+    want_q, want_s = _quantize_want(x[:, cols_at].t().contiguous(), False, E4M3, F32)
+    _same(q[cols_at], want_q)
+    _same(s[cols_at], want_s)
+
+
+@pytest.mark.parametrize("algo", ["auto", "128x64"])
+def test_linear_past_31_bits(algo):
+    """More than 2^31 bytes of x, and more than 2^31 bytes of results."""
+    gen = _gen(13)
+    tokens, outputs, inputs = 140000, 9000, 16384
+    x, sx, w, sw = _whole(gen, 1000, outputs, inputs, E4M3, True, F32)
+    q = torch.zeros((tokens, inputs), dtype=torch.uint8, device=DEV)
+    s = torch.ones((tokens, _blocks(inputs)), device=DEV)
+    at = torch.cat([torch.arange(500, device=DEV), torch.arange(tokens - 500, tokens, device=DEV)])
+    q[at] = _bits(x)
+    s[at] = sx
+    y = g.linear_fp8(q.view(E4M3), s, w, sw, algo=algo)
+    want, _ = _want(x, sx, w, sw, True)
+    assert torch.equal(y[at], want.float().to(BF16))
+    assert (y[500 : tokens - 500 : 1000] == 0).all()
+
+
+def test_linear_on_two_streams_at_once():
+    """Calls that overlap, with workspaces (split sums and copied operands) of
+    their own."""
+    gen = _gen(14)
+    sets = [_whole(gen, 100, 1024, 8200 if i else 8192, E4M3, True, F32) for i in range(2)]
+    wants = [_want(*t, True)[0].float() for t in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i].append(g.linear_fp8(*sets[i], out_dtype=F32))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for y in got[i]:
+            assert torch.equal(y, wants[i])
+
+
+def test_linear_writes_only_its_rows():
+    """Neither rows behind the last token nor what lies around a result change,
+    for every form, split or not."""
+    gen = _gen(15)
+    x, sx, w, sw = _whole(gen, 37, 133, 1000, E4M3, True, F32)
+    want, _ = _want(x, sx, w, sw, True)
+    for algo in ALGOS:
+        for dtype in (F32, BF16):
+            buf = torch.full((64, 160), 7.0, dtype=dtype, device=DEV)
+            g.linear_fp8(x, sx, w, sw, out=buf[:37, 9:142], algo=algo)
+            assert torch.equal(buf[:37, 9:142], want.float().to(dtype))
+            buf[:37, 9:142] = 7.0
+            assert (buf == 7).all()
+
+
+def test_norm_past_31_bits():
+    rows, width = 70001, 32768
+    x = torch.zeros((rows, width), dtype=BF16, device=DEV)
+    gen = _gen(16)
+    picks = [0, 65535, 65536, rows - 1]
+    for r in picks:
+        x[r] = _randn(gen, (width,), BF16)
+    q, s, _, rstd = g.rms_norm_fp8(x)
+    part = torch.stack([x[r] for r in picks])
+    pq, ps, _, prstd = g.rms_norm_fp8(part)
+    for i, r in enumerate(picks):
+        assert torch.equal(_bits(q[r]), _bits(pq[i])) and torch.equal(s[r], ps[i]) and torch.equal(rstd[r], prstd[i])
+    y, _, _ = g.rms_norm(x)
+    py, _, _ = g.rms_norm(part)
+    assert all(torch.equal(y[r], py[i]) for i, r in enumerate(picks))
