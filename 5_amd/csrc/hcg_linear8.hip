@@ -89,7 +89,8 @@ __device__ __forceinline__ void store4(const Args& g, int64_t t, int v, f32x4 f)
   uint16_t* p = static_cast<uint16_t*>(g.y) + t * g.ldy + v;
   typedef uint32_t u32x2h __attribute__((ext_vector_type(2), aligned(2)));
   if (valid >= 4) {
-    *reinterpret_cast<u32x2h*>(p) = u32x2h{(uint32_t)h[0] | (uint32_t)h[1] << 16, (uint32_t)h[2] | (uint32_t)h[3] << 16};
+    *reinterpret_cast<u32x2h*>(p) =
+        u32x2h{(uint32_t)h[0] | (uint32_t)h[1] << 16, (uint32_t)h[2] | (uint32_t)h[3] << 16};
   } else {
     for (int e = 0; e < valid; ++e) p[e] = h[e];
   }
@@ -110,12 +111,12 @@ __device__ __forceinline__ float scale_at(const void* p, int64_t at) {
 }
 
 // For few tokens, bound by reading the weight (8192 x 8192: one token 12.9 us, 5.2
-// TB/s, 16 tokens 14.7).  A workgroup takes 16 R rows of the weight and 16 NI tokens; its waves
-// take the blocks of K in turn, each an own load of both operands, a block ahead,
-// and their sums meet in LDS, in the order of the waves.  Workgroups start at
-// blocks of their own (a golden-ratio sequence) and wrap: rows a power of two
-// apart put what is read at one k on a few HBM channels (4096 x 4096, one token:
-// 5.9 -> 4.7 us).
+// TB/s, 16 tokens 14.7).  A workgroup takes 16 R rows of the weight and 16 NI tokens;
+// its waves take the blocks of K in turn, each an own load of both operands, a block
+// ahead, and their sums meet in LDS, in the order of the waves.  Workgroups start at
+// blocks of their own (a golden-ratio sequence) and wrap: rows a power of two apart
+// put what is read at one k on a few HBM channels (4096 x 4096, one token: 5.9 -> 4.7
+// us).
 // Waves, that is, parts of K: as many again where a workgroup has 16 rows.
 constexpr int stream_waves(int r) { return r == 1 ? 8 : 4; }
 
@@ -125,13 +126,14 @@ __global__ __launch_bounds__(64 * stream_waves(R)) void stream_kernel(Args g) {
   __shared__ f32x4 meet[kStreamWaves][R * NI][64];
   const int lane = threadIdx.x & 63, quad = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t tiles_v = (g.V + 16 * R - 1) / (16 * R), tiles = tiles_v * ((g.T + 16 * NI - 1) / (16 * NI));
-  const int64_t wg = hcg::workgroup();
+  // (Fewer than 2^32 workgroups.)
+  const uint32_t tiles_v = (g.V + 16 * R - 1) / (16 * R), tiles = tiles_v * ((g.T + 16 * NI - 1) / (16 * NI));
+  const int64_t number = hcg::workgroup();
+  if (number >= (int64_t)tiles * g.splits) return;
+  const uint32_t wg = (uint32_t)number, tile = wg % tiles;
   const int split = (int)(wg / tiles);
-  if (split >= g.splits) return;
-  const int64_t tile = wg - split * tiles;
   const int v0 = (int)(tile % tiles_v) * 16 * R;
-  const int64_t t0 = tile / tiles_v * (16 * NI);
+  const int64_t t0 = (int64_t)(tile / tiles_v) * (16 * NI);
   // (Rows past the ends read the last one; their results go nowhere.)
   const unsigned char* w[R];
   int64_t sw[R][by_power(SC) && !EXACT ? 1 : 4];
@@ -165,7 +167,7 @@ __global__ __launch_bounds__(64 * stream_waves(R)) void stream_kernel(Args g) {
 
   // Blocks of this split: `first` on, `whole` of them of kBlock inputs.
   const int first = split * (g.chunk / kBlock), K = min(g.K - split * g.chunk, g.chunk), whole = K / kBlock;
-  const int start = (int)(((uint64_t)((uint32_t)wg * 2654435769u) * (uint32_t)whole) >> 32);
+  const int start = (int)(((uint64_t)(wg * 2654435769u) * (uint32_t)whole) >> 32);
   struct Block {
     u32x4 w[R][2], x[NI][2];
     float sx[NI], sw[R][by_tile(SC) ? 1 : 4];
@@ -354,7 +356,8 @@ constexpr int64_t kMaxTiles = (int64_t)1 << 22;  // of a launch: its threads are
 struct Cost {
   double launch, fixed, lo, hi, join, join_rate, rate;
 };
-enum Kind { kEightBit, kByRows, kExact };  // 16-bit results, those of weights scaled by rows in float32, float32 results
+// 16-bit results, those of weights scaled by rows in float32, float32 results.
+enum Kind { kEightBit, kByRows, kExact };
 constexpr Cost kCosts[3][kNumShapes] = {
     {{3.501, 0.06312, 0.06408, 0, 2.493, 0.7264, 4.346},
      {2.441, 4.915, 1.041, 1.47, 1.095, 2.883, 5.371},
@@ -548,7 +551,8 @@ int hcg_linear_fp8(int algo, int x_dtype, const void* x, int64_t ldx, int64_t to
                    int64_t outputs, int64_t inputs, int scale_dtype, const void* x_scale, int64_t xs_row,
                    int64_t xs_block, int w_tile, const void* w_scale, int64_t ws_row, int64_t ws_block, int out_dtype,
                    void* y, int64_t ldy, void* workspace, int64_t workspace_bytes, void* stream) {
-  HCG_LM_REQUIRE(algo >= 0 && algo % HCG_FP8_SPLITS <= HCG_FP8_128x64 && algo / HCG_FP8_SPLITS <= kMaxSplits,
+  HCG_LM_REQUIRE(algo >= 0 && algo % HCG_FP8_SPLITS <= HCG_FP8_128x64 && algo / HCG_FP8_SPLITS <= kMaxSplits &&
+                     (algo % HCG_FP8_SPLITS != HCG_FP8_AUTO || algo == HCG_FP8_AUTO),
                  "unknown algo %d", algo);
   HCG_LM_REQUIRE(hcg::fp8::type_ok(x_dtype), "x's type %d is not HCG_E4M3 or HCG_E5M2", x_dtype);
   HCG_LM_REQUIRE(hcg::fp8::scale_ok(scale_dtype), "scales of type %d are not HCG_F32 or HCG_E8M0", scale_dtype);
@@ -571,7 +575,7 @@ int hcg_linear_fp8(int algo, int x_dtype, const void* x, int64_t ldx, int64_t to
   const Problem q{algo, tokens, outputs, inputs, x,      ldx,    weight,   ldw,
                   w_tile != 0, e8m0, exact, xs_row, ws_row, ws_block, w_scale};
   const Plan p = make_plan(q);
-  HCG_LM_REQUIRE(p.shape == kStream ? ceil_div(tokens, 16) * ceil_div(outputs, 16) < (int64_t)1 << 32
+  HCG_LM_REQUIRE(p.shape == kStream ? ceil_div(tokens, 16) * ceil_div(outputs, 16) * p.splits < (int64_t)1 << 32
                                     : tiles_of(p.shape, q) * p.splits < kMaxTiles,
                  "%lld tokens by %lld outputs are out of range", (long long)tokens, (long long)outputs);
   HCG_LM_REQUIRE(p.total == 0 || (workspace && workspace_bytes >= p.total && hcg::elem_aligned(workspace, 256)),

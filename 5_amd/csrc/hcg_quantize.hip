@@ -49,7 +49,9 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(QuantArgs g) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int i = tid / kAcross, j = tid % kAcross;
   const int64_t tile = hcg::workgroup();
-  const int64_t tr = tile / g.tiles_c, tc = tile - tr * g.tiles_c;
+  // (64-bit division is a long sequence of instructions; few matrices need it.)
+  const int64_t tr = tile >> 32 || g.tiles_c >> 32 ? tile / g.tiles_c : (uint32_t)tile / (uint32_t)g.tiles_c;
+  const int64_t tc = tile - tr * g.tiles_c;
   const int64_t row0 = tr * kBlock + i * kSide, col0 = tc * kBlock + j * kSide;
   const int rows = (int)min((int64_t)kSide, g.rows - row0), cols = (int)min((int64_t)kSide, g.cols - col0);
   if (tr * kBlock >= g.rows) return;  // (a whole workgroup past the grid's last tile)

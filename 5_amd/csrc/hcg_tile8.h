@@ -281,7 +281,9 @@ __global__ __launch_bounds__(64 * WM * WN, waves_per_simd(TM, TN, WM* WN)) void 
   const int quad = lane >> 4;
   static_assert(NI == 2 || NI == 4 || NI == 8, "tokens' scales");
   const int at_x = (nfirst + (lane & (16 * NI - 1) & 63)) * kHeld;
-  const int at_w = by_tile(SC) ? mfirst / kBlock * kHeld : by_power(SC) ? mfirst + (lane & (16 * MI - 1) & 63) : (mfirst + 4 * quad) * kHeld;
+  const int at_w = by_tile(SC)    ? mfirst / kBlock * kHeld
+                   : by_power(SC) ? mfirst + (lane & (16 * MI - 1) & 63)
+                                  : (mfirst + 4 * quad) * kHeld;
   const int rows_w = by_tile(SC) ? (g.V + kBlock - 1) / kBlock : SC == kRow ? (g.V + 3) & ~3 : g.V;
   int block = kbeg / kBlock;  // of the scales that are loaded next
   const int last_block = block + nk - 1;

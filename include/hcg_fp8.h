@@ -67,10 +67,10 @@ int hcg_rms_norm_fp8(int dtype, const void* x, int64_t ldx, int64_t rows, int64_
  * measurements. */
 #define HCG_FP8_AUTO 0
 #define HCG_FP8_STREAM 1 /* operands straight into registers, any alignment */
-#define HCG_FP8_256x256 2 /* tiles of outputs x tokens; 16-bit results that are not scaled by rows in float32 */
+#define HCG_FP8_256x256 2 /* tiles of outputs x tokens; 128x128 for float32 results and weights scaled by rows in float32 */
 #define HCG_FP8_128x128 3
 #define HCG_FP8_128x64 4
-#define HCG_FP8_SPLITS 256 /* times a number up to 16, added to a tile's: K in so many parts */
+#define HCG_FP8_SPLITS 256 /* times a number up to 16, added to a form: K in so many parts */
 
 int64_t hcg_linear_fp8_workspace(int algo, int64_t tokens, int64_t outputs, int64_t inputs, const void* x, int64_t ldx,
                                  const void* weight, int64_t ldw, int scale_dtype, int64_t xs_row, int w_tile,

@@ -93,7 +93,8 @@ def test_quantize_arguments(change, match):
 
 
 @pytest.mark.parametrize("change,match", [
-    ({"algo": 99}, "unknown algo 99"), ({"xdtype": F16}, "x's type 0"), ({"sdtype": F16}, "scales of type 0"),
+    ({"algo": 99}, "unknown algo 99"), ({"algo": -1}, "unknown algo -1"), ({"algo": 256 * 17 + 3}, "unknown algo"),
+    ({"algo": 256 * 2}, "unknown algo 512"), ({"xdtype": F16}, "x's type 0"), ({"sdtype": F16}, "scales of type 0"),
     ({"ydtype": E4M3}, "output's type 3"), ({"tokens": -1}, "out of range"), ({"tokens": 1 << 26}, "out of range"),
     ({"outputs": 1 << 26}, "out of range"), ({"inputs": 4000000}, "out of range"), ({"inputs": 0}, "no inputs"),
     ({"x": None}, "null"), ({"w": None}, "null"), ({"xs": None}, "null"), ({"ws": None}, "null"), ({"y": None}, "null"),
