@@ -8,8 +8,9 @@
 // vectors, all of them in flight, and holds it in registers (8 x 8 values per
 // thread) between the maximum and the result.  Transposed, the bytes pass
 // through LDS, so that both sides are whole lines.  8192 x 8192 float32 by tiles
-// 66.8 us (5.0 TB/s), 8192 x 4096 bf16 transposed 24.4 us (4.1 TB/s; 27.1 with
-// padded instead of swizzled rows in LDS).
+// 63.6 us (5.3 TB/s), 8192 x 4096 bf16 by rows 19.0 (5.3 TB/s), transposed 20.1 (5.0
+// TB/s; 26.5 with loads that waited for each other and scales found by every lane,
+// 2.6 more with padded instead of swizzled rows in LDS), 64 x 8192 bf16 4.5.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -41,6 +42,19 @@ __device__ __forceinline__ uint32_t shfl_max(uint32_t v, int mask) {
   return max(v, (uint32_t)__shfl_xor((int)v, mask));
 }
 
+// Joins 2 H values of two lanes `mask` apart; each is left with H of them, the lane
+// with that bit with the upper ones.  (A scale, with its division, is then found by
+// as few lanes as there are.)
+template <int H>
+__device__ __forceinline__ void halve(uint32_t (&top)[kSide], int lane, int mask) {
+  const bool upper = lane & mask;
+#pragma unroll
+  for (int k = 0; k < H; ++k) {
+    const uint32_t away = upper ? top[k] : top[k + H];
+    top[k] = max(upper ? top[k + H] : top[k], (uint32_t)__shfl_xor((int)away, mask));
+  }
+}
+
 // Thread (i, j) = (tid / 16, tid % 16) holds rows 8 i ... and columns 8 j ... of
 // the workgroup's tile.
 template <class T, bool TRANS, bool TILE>
@@ -50,22 +64,46 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(QuantArgs g) {
   const int i = tid / kAcross, j = tid % kAcross;
   const int64_t tile = hcg::workgroup();
   // (64-bit division is a long sequence of instructions; few matrices need it.)
-  const int64_t tr = tile >> 32 || g.tiles_c >> 32 ? tile / g.tiles_c : (uint32_t)tile / (uint32_t)g.tiles_c;
+  const int64_t tr = tile >> 32 ? tile / g.tiles_c : (uint32_t)tile / (uint32_t)g.tiles_c;
   const int64_t tc = tile - tr * g.tiles_c;
   const int64_t row0 = tr * kBlock + i * kSide, col0 = tc * kBlock + j * kSide;
   const int rows = (int)min((int64_t)kSide, g.rows - row0), cols = (int)min((int64_t)kSide, g.cols - col0);
   if (tr * kBlock >= g.rows) return;  // (a whole workgroup past the grid's last tile)
 
+  // Loads without a branch between them, of the last row where there is none, but in
+  // a last column of tiles: a load that ends a branch is waited for there.
+  constexpr int kEach = hcg::kVec<T>, kParts = kSide / kEach;
+  const T* const x = static_cast<const T*>(g.x) + col0;
+  hcg::raw4 raw[kSide][kParts];
+  if ((tc + 1) * kBlock <= g.cols) {
+#pragma unroll
+    for (int r = 0; r < kSide; ++r)
+#pragma unroll
+      for (int p = 0; p < kParts; ++p)
+        raw[r][p] = hcg::load_raw(x + min(row0 + r, g.rows - 1) * g.ldx + p * kEach, kEach);
+  } else {
+#pragma unroll
+    for (int r = 0; r < kSide; ++r)
+#pragma unroll
+      for (int p = 0; p < kParts; ++p) {
+        raw[r][p] = hcg::raw4{0, 0, 0, 0};
+        if (r < rows && cols > p * kEach)
+          raw[r][p] = hcg::load_raw(x + (row0 + r) * g.ldx + p * kEach, cols - p * kEach);
+        asm volatile("" : "+v"(raw[r][p]));  // (whole words, not values of 16 bits: they took 200 registers)
+      }
+  }
   float v[kSide][kSide];
 #pragma unroll
-  for (int r = 0; r < kSide; ++r) {
-    const int valid = r < rows ? cols : 0;
+  for (int r = 0; r < kSide; ++r)
 #pragma unroll
-    for (int e = 0; e < kSide; ++e) v[r][e] = 0.f;
-    if (valid > 0) hcg::load_floats<T, kSide>(static_cast<const T*>(g.x) + (row0 + r) * g.ldx + col0, valid, v[r]);
-  }
+    for (int p = 0; p < kParts; ++p) {
+      float part[kEach];
+      hcg::unpack<T>(r < rows ? raw[r][p] : hcg::raw4{0, 0, 0, 0}, part);
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) v[r][p * kEach + e] = part[e];
+    }
 
-  hcg::fp8::Scale s[kSide];  // per row of q that the thread holds (TILE: the first alone)
+  float inverse[TILE ? 1 : kSide];  // per row of q that the thread holds
   if constexpr (TILE) {
     uint32_t top = 0;
 #pragma unroll
@@ -77,37 +115,44 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(QuantArgs g) {
     if (lane == 0) meet[wave] = top;
     __syncthreads();
     top = max(max(meet[0], meet[1]), max(meet[2], meet[3]));
-    s[0] = hcg::fp8::scale_of(top, g.out.e5m2, g.out.e8m0);
-    if (tid == 0) hcg::fp8::put_scale(g.out, TRANS ? tc : tr, TRANS ? tr : tc, s[0].held);
+    const hcg::fp8::Scale s = hcg::fp8::scale_of(top, g.out.e5m2, g.out.e8m0);
+    inverse[0] = s.inverse;
+    if (tid == 0) hcg::fp8::put_scale(g.out, TRANS ? tc : tr, TRANS ? tr : tc, s.held);
   } else if constexpr (TRANS) {
     // A row of q is a column of x.
+    __shared__ __attribute__((aligned(16))) float found[kBlock];
+    uint32_t top[kSide] = {};
 #pragma unroll
-    for (int e = 0; e < kSide; ++e) {
-      uint32_t top = 0;
+    for (int e = 0; e < kSide; ++e)
 #pragma unroll
-      for (int r = 0; r < kSide; ++r) top = max(top, hcg::fp8::magnitude(v[r][e]));
-      top = shfl_max(shfl_max(top, 16), 32);
-      if (lane < kAcross) meet[wave * kBlock + j * kSide + e] = top;
+      for (int r = 0; r < kSide; ++r) top[e] = max(top[e], hcg::fp8::magnitude(v[r][e]));
+    halve<4>(top, lane, 16);
+    halve<2>(top, lane, 32);
+    uint32_t* const to = meet + wave * kBlock + j * kSide + (lane & 16 ? 4 : 0) + (lane & 32 ? 2 : 0);
+    to[0] = top[0], to[1] = top[1];
+    __syncthreads();
+    if (tid < kBlock) {
+      const uint32_t most = max(max(meet[tid], meet[kBlock + tid]), max(meet[2 * kBlock + tid], meet[3 * kBlock + tid]));
+      const hcg::fp8::Scale s = hcg::fp8::scale_of(most, g.out.e5m2, g.out.e8m0);
+      if (tc * kBlock + tid < g.cols) hcg::fp8::put_scale(g.out, tc * kBlock + tid, tr, s.held);
+      found[tid] = s.inverse;
     }
     __syncthreads();
 #pragma unroll
-    for (int e = 0; e < kSide; ++e) {
-      const int c = j * kSide + e;
-      const uint32_t top = max(max(meet[c], meet[kBlock + c]), max(meet[2 * kBlock + c], meet[3 * kBlock + c]));
-      s[e] = hcg::fp8::scale_of(top, g.out.e5m2, g.out.e8m0);
-      if (i == 0 && e < cols) hcg::fp8::put_scale(g.out, col0 + e, tr, s[e].held);
-    }
+    for (int e = 0; e < kSide; ++e) inverse[e] = found[j * kSide + e];
   } else {
+    uint32_t top[kSide] = {};
 #pragma unroll
-    for (int r = 0; r < kSide; ++r) {
-      uint32_t top = 0;
+    for (int r = 0; r < kSide; ++r)
 #pragma unroll
-      for (int e = 0; e < kSide; ++e) top = max(top, hcg::fp8::magnitude(v[r][e]));
+      for (int e = 0; e < kSide; ++e) top[r] = max(top[r], hcg::fp8::magnitude(v[r][e]));
+    halve<4>(top, lane, 4);
+    halve<2>(top, lane, 2);
+    halve<1>(top, lane, 1);
+    const hcg::fp8::Scale s = hcg::fp8::scale_of(shfl_max(top[0], 8), g.out.e5m2, g.out.e8m0);  // of row j % 8
+    if (j < rows && j < kSide) hcg::fp8::put_scale(g.out, row0 + j, tc, s.held);
 #pragma unroll
-      for (int m = kAcross / 2; m >= 1; m >>= 1) top = shfl_max(top, m);
-      s[r] = hcg::fp8::scale_of(top, g.out.e5m2, g.out.e8m0);
-      if (j == 0 && r < rows) hcg::fp8::put_scale(g.out, row0 + r, tc, s[r].held);
-    }
+    for (int r = 0; r < kSide; ++r) inverse[r] = __shfl(s.inverse, (lane & -kAcross) + r);
   }
 
   if constexpr (!TRANS) {
@@ -115,7 +160,7 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(QuantArgs g) {
 #pragma unroll
     for (int r = 0; r < kSide; ++r)
       if (r < rows)
-        hcg::fp8::store_q<kSide>(g.out.q + (row0 + r) * g.out.ldq + col0, v[r], s[TILE ? 0 : r].inverse, cols,
+        hcg::fp8::store_q<kSide>(g.out.q + (row0 + r) * g.out.ldq + col0, v[r], inverse[TILE ? 0 : r], cols,
                                  g.out.e5m2);
   } else {
     __shared__ __attribute__((aligned(16))) unsigned char turned[kBlock * kBlock];
@@ -124,7 +169,7 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(QuantArgs g) {
       float f[kSide];
 #pragma unroll
       for (int r = 0; r < kSide; ++r) f[r] = v[r][e];
-      hcg::fp8::store_q<kSide>(turned + turned_at(j * kSide + e, i), f, s[TILE ? 0 : e].inverse, kSide,
+      hcg::fp8::store_q<kSide>(turned + turned_at(j * kSide + e, i), f, inverse[TILE ? 0 : e], kSide,
                                g.out.e5m2);
     }
     __syncthreads();
