@@ -8,9 +8,9 @@
 // vectors, all of them in flight, and holds it in registers (8 x 8 values per
 // thread) between the maximum and the result.  Transposed, the bytes pass
 // through LDS, so that both sides are whole lines.  8192 x 8192 float32 by tiles
-// 63.6 us (5.3 TB/s), 8192 x 4096 bf16 by rows 19.0 (5.3 TB/s), transposed 20.1 (5.0
-// TB/s; 26.5 with loads that waited for each other and scales found by every lane,
-// 2.6 more with padded instead of swizzled rows in LDS), 64 x 8192 bf16 4.5.
+// 64.2 us (5.2 TB/s), 8192 x 4096 bf16 by rows 19.0 (5.3 TB/s), transposed 18.2 (5.6
+// TB/s; 24.5 with loads that waited for each other and scales found by every lane,
+// 27.1 with padded instead of swizzled rows in LDS as well), 64 x 8192 bf16 4.5.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

@@ -11,7 +11,7 @@
 // same function.  The 8-bit form takes each 128 columns' largest magnitude from
 // the 16 or 32 lanes that hold them, by exchanges.  8192 x 4096: to 8 bits with a
 // bf16 residual 45 us (5.2 TB/s), f16 with a float32 residual 82 us (4.9), bf16
-// gradient with the residual's 51.7 us (5.2) and 4.6 for the columns' sums; one row
+// gradient with the residual's 46.5 us (5.8) and 4.7 for the columns' sums; one row
 // 3.8 us, a launch and its latency.
 #include <hip/hip_runtime.h>
 
@@ -50,6 +50,32 @@ struct Raws {
 #pragma unroll
     for (int i = 0; i < kN; ++i)
       v[i] = valid > i * kPer ? hcg::load_raw(p + i * kPer, valid - i * kPer) : raw4{0, 0, 0, 0};
+  }
+  // The same without a branch, of a row of at least kPer elements, in two steps: a
+  // vector past the row's end, or over it, is read as the row's last one, and settle()
+  // moves what it holds of the row (`left` columns) to its place.
+  __device__ __forceinline__ void load_whole(const S* row, int c, int width) {
+    typedef typename hcg::RawAt<sizeof(S)>::type raw4a;
+#pragma unroll
+    for (int i = 0; i < kN; ++i)
+      v[i] = *reinterpret_cast<const raw4a*>(row + min(c + i * kPer, width - kPer));
+  }
+  __device__ __forceinline__ void settle(int left, bool ragged) {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      const int away = kPer - max(min(left - i * kPer, kPer), 0);
+      raw4 r = v[i];
+      if (ragged) {
+        constexpr int kWord = 4 / sizeof(S);  // elements
+        if (away & 2 * kWord) r = raw4{r[2], r[3], 0, 0};
+        if (away & kWord) r = raw4{r[1], r[2], r[3], 0};
+        if constexpr (kWord == 2)
+          if (away & 1) {
+            r = raw4{r[0] >> 16 | r[1] << 16, r[1] >> 16 | r[2] << 16, r[2] >> 16 | r[3] << 16, r[3] >> 16};
+          }
+      }
+      v[i] = away == kPer ? raw4{0, 0, 0, 0} : r;
+    }
   }
   __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -280,7 +306,11 @@ struct RmsGradArgs {
 // workgroup b takes rows b * GROUPS + q, + gridDim.x * GROUPS, ... and keeps its
 // columns' sums of dy xh in registers; the groups' sums meet in LDS once, at the
 // end.  AHEAD: a row's loads go out before the work on the row before it (not by
-// 1024 threads with two vectors each, whose registers do not hold both).
+// 1024 threads with two vectors each, whose registers do not hold both).  Rows hold a
+// vector or more, so that no load is behind a branch: the number of those in flight
+// would not be known after it, and a row would wait for the next row's as well (8192 x
+// 4096 bf16 51.2 -> 46.5 us, 3001 x 1027 float32 12.6 -> 12.0; with the sums 55.2 ->
+// 53.4 and 14.6 -> 13.1).
 template <class T, class H, int LANES, int NV, int GROUPS, bool AHEAD>
 __global__ __launch_bounds__(LANES * GROUPS) void rms_grad_kernel(RmsGradArgs g) {
   constexpr int E = kVec<T>, kWaves = LANES / 64;
@@ -299,6 +329,10 @@ __global__ __launch_bounds__(LANES * GROUPS) void rms_grad_kernel(RmsGradArgs g)
     for (int e = 0; e < E; ++e) dw[i][e] = 0.f;
   }
   const int64_t step = (int64_t)gridDim.x * GROUPS;
+  const bool ragged = g.width % E != 0;
+  // (Without a residual's gradient one vector of h is read in its place, and left out.)
+  const H* const dres_rows = static_cast<const H*>(g.dres ? g.dres : g.h);
+  const int64_t dres_step = g.dres ? g.lddr : 0;
   int parity = 0;
   struct Row {
     float rstd;
@@ -306,18 +340,14 @@ __global__ __launch_bounds__(LANES * GROUPS) void rms_grad_kernel(RmsGradArgs g)
     Raws<H, E> h[NV], dres[NV];
   };
   auto load = [&](Row& r, int64_t row) {
-    const bool live = row < g.rows;
-    const int64_t at = live ? row : 0;
-    r.rstd = live ? g.rstd[at] : 0.f;
+    const int64_t at = min(row, g.rows - 1);
+    r.rstd = g.rstd[at];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = first + i * LANES * E, left = live ? g.width - c : 0;
-      r.dy[i].load(static_cast<const T*>(g.dy) + at * g.lddy + c, left);
-      r.h[i].load(static_cast<const H*>(g.h) + at * g.ldh + c, left);
-      if (g.dres)
-        r.dres[i].load(static_cast<const H*>(g.dres) + at * g.lddr + c, left);
-      else
-        r.dres[i].clear();
+      const int c = first + i * LANES * E;
+      r.dy[i].load_whole(static_cast<const T*>(g.dy) + at * g.lddy, c, g.width);
+      r.h[i].load_whole(static_cast<const H*>(g.h) + at * g.ldh, c, g.width);
+      r.dres[i].load_whole(dres_rows + at * dres_step, g.dres ? c : 0, g.width);
     }
   };
   Row next;
@@ -327,12 +357,16 @@ __global__ __launch_bounds__(LANES * GROUPS) void rms_grad_kernel(RmsGradArgs g)
     const int64_t row = row0 + group;
     const bool live = row < g.rows;
     if constexpr (!AHEAD) load(next, row);
-    const float rstd = next.rstd;
+    const float rstd = live ? next.rstd : 0.f;
     float dy[NV][E], xh[NV][E];
     Raws<H, E> dres[NV];
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
+      const int left = live ? g.width - (first + i * LANES * E) : 0;
+      next.dy[i].settle(left, ragged);
+      next.h[i].settle(left, ragged);
+      next.dres[i].settle(g.dres ? left : 0, ragged);
       next.dy[i].floats(dy[i]);
       next.h[i].floats(xh[i]);
       dres[i] = next.dres[i];
@@ -526,10 +560,19 @@ int launch_rms_grad(const RmsGradArgs& a, hipStream_t s) {
   return (int)wgs;
 }
 
+template <class T, class H>
+int run_rms_grad_wide(const RmsGradArgs& a, hipStream_t s) {
+  rms_grad_wide_kernel<T, H><<<hcg::grid_of(a.rows), 1024, 0, s>>>(a);
+  const int parts = (int)std::min<int64_t>(64, a.rows);
+  if (a.part) rms_columns_kernel<T, H><<<dim3((unsigned)((a.width + 255) / 256), parts), 256, 0, s>>>(a);
+  return parts;
+}
+
 // Returns the number of parts the column sums were left in.
 template <class T, class H>
 int run_rms_grad(const RmsGradArgs& a, hipStream_t s) {
   const int64_t vecs = ((int64_t)a.width + kVec<T> - 1) / kVec<T>;
+  if (a.width < kVec<T>) return run_rms_grad_wide<T, H>(a, s);
   // As few lanes as hold a row, and as many rows as fit 1024 threads (512, where a
   // row is one wave or less): idle lanes are loads that are not in flight.
   if (vecs <= 16) return launch_rms_grad<T, H, 16, 1, 32>(a, s);
@@ -543,10 +586,7 @@ int run_rms_grad(const RmsGradArgs& a, hipStream_t s) {
   if (vecs <= 512) return launch_rms_grad<T, H, 512, 1, 2>(a, s);
   if (vecs <= 1024) return launch_rms_grad<T, H, 512, 2, 1>(a, s);
   if (vecs <= 2048) return launch_rms_grad<T, H, 1024, 2, 1, false>(a, s);
-  rms_grad_wide_kernel<T, H><<<hcg::grid_of(a.rows), 1024, 0, s>>>(a);
-  const int parts = (int)std::min<int64_t>(64, a.rows);
-  if (a.part) rms_columns_kernel<T, H><<<dim3((unsigned)((a.width + 255) / 256), parts), 256, 0, s>>>(a);
-  return parts;
+  return run_rms_grad_wide<T, H>(a, s);
 }
 
 // f(x's type, the residual's type).

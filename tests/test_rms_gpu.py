@@ -110,6 +110,13 @@ def test_grad(rows, width, dtype, wide):
     _close(plain, pwant, ((_depth(width) + 8) * E32) * r * (d.abs() + xh.abs() * pmag) + U[wide] * pwant.abs() + TINY[wide])
 
 
+# Rows that end inside a vector, several to a row group.
+@pytest.mark.parametrize("dtype,wide", TYPES)
+@pytest.mark.parametrize("rows,width", [(4000, 5), (9000, 13), (5000, 130), (2601, 517), (2001, 1027), (521, 4101), (258, 8197)])
+def test_grad_ragged_turns(rows, width, dtype, wide):
+    test_grad(rows, width, dtype, wide)
+
+
 def test_grad_against_differences():
     """The gradient of sum(c * norm(x)) along a direction, by central
     differences of the forward call in float32."""
