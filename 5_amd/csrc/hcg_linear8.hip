@@ -455,6 +455,19 @@ struct Plan {
   int64_t x, w, sx, sw, part, total;                      // offsets into the workspace
 };
 
+// What a plan can be made for, and whether a launch holds it.
+bool algo_ok(int algo) {
+  return algo >= 0 && algo % HCG_FP8_SPLITS <= HCG_FP8_128x64 && algo / HCG_FP8_SPLITS <= kMaxSplits &&
+         (algo % HCG_FP8_SPLITS != HCG_FP8_AUTO || algo == HCG_FP8_AUTO);
+}
+bool sizes_ok(int64_t tokens, int64_t outputs, int64_t inputs) {
+  return tokens >= 0 && tokens < kMaxRows && outputs >= 0 && outputs < kMaxRows && inputs >= 0 && inputs < kMaxInputs;
+}
+bool launch_ok(const Plan& p, const Problem& q) {
+  return p.shape == kStream ? ceil_div(q.tokens, 16) * ceil_div(q.outputs, 16) * p.splits < (int64_t)1 << 32
+                            : tiles_of(p.shape, q) * p.splits < kMaxTiles;
+}
+
 bool in_place(const void* p, int64_t ld, int64_t rows) {
   return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (rows == 1 || ld % 16 == 0);
 }
@@ -541,26 +554,25 @@ extern "C" {
 int64_t hcg_linear_fp8_workspace(int algo, int64_t tokens, int64_t outputs, int64_t inputs, const void* x, int64_t ldx,
                                  const void* weight, int64_t ldw, int scale_dtype, int64_t xs_row, int w_tile,
                                  const void* w_scale, int64_t ws_row, int64_t ws_block, int out_dtype) {
-  if (tokens <= 0 || outputs <= 0 || inputs <= 0) return 0;
-  return make_plan(Problem{algo, tokens, outputs, inputs, x, ldx, weight, ldw, w_tile != 0, scale_dtype == HCG_E8M0,
-                           out_dtype == HCG_F32, xs_row, ws_row, ws_block, w_scale})
-      .total;
+  // (What the call refuses needs none: the call says why.)
+  if (!algo_ok(algo) || !sizes_ok(tokens, outputs, inputs) || tokens == 0 || outputs == 0 || inputs == 0) return 0;
+  const Problem q{algo,        tokens, outputs, inputs, x,
+                  ldx,         weight, ldw,     w_tile != 0, scale_dtype == HCG_E8M0,
+                  out_dtype == HCG_F32, xs_row, ws_row, ws_block, w_scale};
+  const Plan p = make_plan(q);
+  return launch_ok(p, q) ? p.total : 0;
 }
 
 int hcg_linear_fp8(int algo, int x_dtype, const void* x, int64_t ldx, int64_t tokens, const void* weight, int64_t ldw,
                    int64_t outputs, int64_t inputs, int scale_dtype, const void* x_scale, int64_t xs_row,
                    int64_t xs_block, int w_tile, const void* w_scale, int64_t ws_row, int64_t ws_block, int out_dtype,
                    void* y, int64_t ldy, void* workspace, int64_t workspace_bytes, void* stream) {
-  HCG_LM_REQUIRE(algo >= 0 && algo % HCG_FP8_SPLITS <= HCG_FP8_128x64 && algo / HCG_FP8_SPLITS <= kMaxSplits &&
-                     (algo % HCG_FP8_SPLITS != HCG_FP8_AUTO || algo == HCG_FP8_AUTO),
-                 "unknown algo %d", algo);
+  HCG_LM_REQUIRE(algo_ok(algo), "unknown algo %d", algo);
   HCG_LM_REQUIRE(hcg::fp8::type_ok(x_dtype), "x's type %d is not HCG_E4M3 or HCG_E5M2", x_dtype);
   HCG_LM_REQUIRE(hcg::fp8::scale_ok(scale_dtype), "scales of type %d are not HCG_F32 or HCG_E8M0", scale_dtype);
   HCG_LM_REQUIRE(hcg::elem_ok(out_dtype), "the output's type %d is not HCG_F16, HCG_BF16 or HCG_F32", out_dtype);
-  HCG_LM_REQUIRE(tokens >= 0 && tokens < kMaxRows && outputs >= 0 && outputs < kMaxRows && inputs >= 0 &&
-                     inputs < kMaxInputs,
-                 "%lld tokens, %lld outputs and %lld inputs are out of range", (long long)tokens, (long long)outputs,
-                 (long long)inputs);
+  HCG_LM_REQUIRE(sizes_ok(tokens, outputs, inputs), "%lld tokens, %lld outputs and %lld inputs are out of range",
+                 (long long)tokens, (long long)outputs, (long long)inputs);
   if (tokens == 0 || outputs == 0) return HCG_OK;
   HCG_LM_REQUIRE(inputs > 0, "a product over no inputs");
   HCG_LM_REQUIRE(x && weight && x_scale && w_scale && y, "null pointer");
@@ -575,9 +587,8 @@ int hcg_linear_fp8(int algo, int x_dtype, const void* x, int64_t ldx, int64_t to
   const Problem q{algo, tokens, outputs, inputs, x,      ldx,    weight,   ldw,
                   w_tile != 0, e8m0, exact, xs_row, ws_row, ws_block, w_scale};
   const Plan p = make_plan(q);
-  HCG_LM_REQUIRE(p.shape == kStream ? ceil_div(tokens, 16) * ceil_div(outputs, 16) * p.splits < (int64_t)1 << 32
-                                    : tiles_of(p.shape, q) * p.splits < kMaxTiles,
-                 "%lld tokens by %lld outputs are out of range", (long long)tokens, (long long)outputs);
+  HCG_LM_REQUIRE(launch_ok(p, q), "%lld tokens by %lld outputs are out of range", (long long)tokens,
+                 (long long)outputs);
   HCG_LM_REQUIRE(p.total == 0 || (workspace && workspace_bytes >= p.total && hcg::elem_aligned(workspace, 256)),
                  "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)p.total);
   const hipStream_t s = static_cast<hipStream_t>(stream);

@@ -72,6 +72,7 @@ int hcg_rms_norm_fp8(int dtype, const void* x, int64_t ldx, int64_t rows, int64_
 #define HCG_FP8_128x64 4
 #define HCG_FP8_SPLITS 256 /* times a number up to 16, added to a form: K in so many parts */
 
+/* (The scratch of a call that hcg_linear_fp8 refuses is 0: the call says why.) */
 int64_t hcg_linear_fp8_workspace(int algo, int64_t tokens, int64_t outputs, int64_t inputs, const void* x, int64_t ldx,
                                  const void* weight, int64_t ldw, int scale_dtype, int64_t xs_row, int w_tile,
                                  const void* w_scale, int64_t ws_row, int64_t ws_block, int out_dtype);
