@@ -529,7 +529,15 @@ __global__ __launch_bounds__(1024) void rms_reduce_kernel(const float* part, int
 // ---------------------------------------------------------------------------
 
 constexpr int kGradParts = 256;  // workgroups of the gradient, each with one part
+constexpr int kWideParts = 64;   // row sums of the wide form's columns
+constexpr int kMaxVecs = 2048;   // in a row that the gradient holds in registers
 constexpr int64_t kMaxWidth = 1 << 30;
+
+// Parts that the column sums are left in, at most: a row has no more than one, and
+// rows over kMaxVecs vectors of any type are the wide form's.
+int64_t grad_parts(int64_t rows, int64_t width) {
+  return std::min<int64_t>(rows, width > kMaxVecs * kVec<_Float16> ? kWideParts : kGradParts);
+}
 
 template <class T, class H, int LANES, int NV, bool Q>
 void launch_rms(const RmsArgs& a, hipStream_t s) {
@@ -563,7 +571,7 @@ int launch_rms_grad(const RmsGradArgs& a, hipStream_t s) {
 template <class T, class H>
 int run_rms_grad_wide(const RmsGradArgs& a, hipStream_t s) {
   rms_grad_wide_kernel<T, H><<<hcg::grid_of(a.rows), 1024, 0, s>>>(a);
-  const int parts = (int)std::min<int64_t>(64, a.rows);
+  const int parts = (int)std::min<int64_t>(kWideParts, a.rows);
   if (a.part) rms_columns_kernel<T, H><<<dim3((unsigned)((a.width + 255) / 256), parts), 256, 0, s>>>(a);
   return parts;
 }
@@ -585,7 +593,7 @@ int run_rms_grad(const RmsGradArgs& a, hipStream_t s) {
   if (vecs <= 384) return launch_rms_grad<T, H, 384, 1, 2>(a, s);
   if (vecs <= 512) return launch_rms_grad<T, H, 512, 1, 2>(a, s);
   if (vecs <= 1024) return launch_rms_grad<T, H, 512, 2, 1>(a, s);
-  if (vecs <= 2048) return launch_rms_grad<T, H, 1024, 2, 1, false>(a, s);
+  if (vecs <= kMaxVecs) return launch_rms_grad<T, H, 1024, 2, 1, false>(a, s);
   return run_rms_grad_wide<T, H>(a, s);
 }
 
@@ -686,7 +694,7 @@ int hcg_rms_norm_fp8(int dtype, const void* x, int64_t ldx, int64_t rows, int64_
 }
 
 int64_t hcg_rms_norm_grad_workspace(int64_t rows, int64_t width) {
-  return rows > 0 && width > 0 ? (int64_t)kGradParts * width * 4 : 0;
+  return rows > 0 && width > 0 ? grad_parts(rows, width) * width * 4 : 0;
 }
 
 int hcg_rms_norm_grad(int dtype, const void* dy, int64_t lddy, int h_dtype, const void* h, int64_t ldh, int64_t rows,
