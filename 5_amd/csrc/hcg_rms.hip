@@ -508,7 +508,7 @@ template <class P>
 __global__ __launch_bounds__(1024) void rms_reduce_kernel(const float* part, int parts, int width, P* dweight) {
   __shared__ float meet[16][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t c = (int64_t)blockIdx.x * 64 + lane;
+  const int64_t c = hcg::workgroup() * 64 + lane;
   float sum = 0.f;
   if (c < width) {
 #pragma unroll 16
@@ -731,7 +731,7 @@ int hcg_rms_norm_grad(int dtype, const void* dy, int64_t lddy, int h_dtype, cons
     using T = decltype(t);
     const int parts = rows > 0 ? run_rms_grad<T, decltype(r)>(a, s) : 0;
     if (dweight == nullptr) return;
-    const dim3 grid((unsigned)((width + 63) / 64));
+    const dim3 grid = hcg::grid_of((width + 63) / 64);
     if (param_dtype == HCG_F32)
       rms_reduce_kernel<float><<<grid, 1024, 0, s>>>(a.part, parts, (int)width, static_cast<float*>(dweight));
     else
