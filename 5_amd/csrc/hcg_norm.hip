@@ -452,7 +452,15 @@ __global__ __launch_bounds__(1024) void norm_reduce_kernel(const float* part, in
 // ---------------------------------------------------------------------------
 
 constexpr int kGradParts = 256;       // workgroups of the gradient, each with one part
+constexpr int kWideParts = 64;        // row sums of the wide form's columns
+constexpr int kMaxVecs = 2048;        // in a row that the gradient holds in registers
 constexpr int64_t kMaxWidth = 1 << 30;
+
+// Parts that the column sums are left in, at most: a row has no more than one, and
+// rows over kMaxVecs vectors of any type are the wide form's.
+int64_t grad_parts(int64_t rows, int64_t width) {
+  return std::min<int64_t>(rows, width > kMaxVecs * kVec<_Float16> ? kWideParts : kGradParts);
+}
 
 template <class T, class P, int LANES, int NV>
 void launch_norm(const NormArgs& a, hipStream_t s) {
@@ -503,9 +511,9 @@ int run_norm_grad(const NormGradArgs& a, hipStream_t s) {
   if (vecs <= 384) return launch_norm_grad<T, P, 384, 1, 2>(a, s);
   if (vecs <= 512) return launch_norm_grad<T, P, 512, 1, 2>(a, s);
   if (vecs <= 1024) return launch_norm_grad<T, P, 512, 2, 1>(a, s);
-  if (vecs <= 2048) return launch_norm_grad<T, P, 1024, 2, 1, sizeof(T) == 2>(a, s);
+  if (vecs <= kMaxVecs) return launch_norm_grad<T, P, 1024, 2, 1, sizeof(T) == 2>(a, s);
   norm_grad_wide_kernel<T, P><<<hcg::grid_of(a.rows), 1024, 0, s>>>(a);
-  const int parts = (int)std::min<int64_t>(64, a.rows);
+  const int parts = (int)std::min<int64_t>(kWideParts, a.rows);
   if (a.part)
     norm_columns_kernel<T><<<dim3((unsigned)((a.width + 255) / 256), parts), 256, 0, s>>>(a);
   return parts;
@@ -562,7 +570,7 @@ int hcg_layer_norm(int dtype, const void* x, int64_t ldx, int64_t rows, int64_t 
 }
 
 int64_t hcg_layer_norm_grad_workspace(int64_t rows, int64_t width) {
-  return rows > 0 && width > 0 ? (int64_t)kGradParts * 2 * width * 4 : 0;
+  return rows > 0 && width > 0 ? grad_parts(rows, width) * 2 * width * 4 : 0;
 }
 
 int hcg_layer_norm_grad(int dtype, const void* dy, int64_t lddy, const void* x, int64_t ldx, int64_t rows,
