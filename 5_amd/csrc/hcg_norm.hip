@@ -423,17 +423,18 @@ __global__ __launch_bounds__(256) void norm_columns_kernel(NormGradArgs g) {
 // dw and db from the workgroups' sums (8 MB from the L2 at a width of 4096: 4.7
 // us, 3.9 at 1027): 64 columns by 16 waves, wave q adding
 // the parts q, q + 16, ..., the waves' sums added in order.
+// (The grid's third dimension is dw or db.)
 template <class P>
 __global__ __launch_bounds__(1024) void norm_reduce_kernel(const float* part, int parts, int width, P* dweight,
                                                            P* dbias) {
   __shared__ float meet[16][64];
-  P* out = blockIdx.y ? dbias : dweight;
+  P* out = blockIdx.z ? dbias : dweight;
   if (out == nullptr) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t c = (int64_t)blockIdx.x * 64 + lane;
+  const int64_t c = hcg::workgroup() * 64 + lane;
   float sum = 0.f;
   if (c < width) {
-    const float* p = part + (int64_t)blockIdx.y * width + c;
+    const float* p = part + (int64_t)blockIdx.z * width + c;
 #pragma unroll 16
     for (int q = wave; q < parts; q += 16) sum += p[(int64_t)q * 2 * width];
   }
@@ -612,9 +613,11 @@ int hcg_layer_norm_grad(int dtype, const void* dy, int64_t lddy, const void* x, 
     using P = decltype(p);
     if constexpr (std::is_same_v<P, float> || std::is_same_v<P, T>) {
       const int parts = rows > 0 ? run_norm_grad<T, P>(a, s) : 0;
+      dim3 grid = hcg::grid_of((width + 63) / 64);
+      grid.z = 2;
       if (params)
-        norm_reduce_kernel<P><<<dim3((unsigned)((width + 63) / 64), 2), 1024, 0, s>>>(
-            a.part, parts, (int)width, static_cast<P*>(dweight), static_cast<P*>(dbias));
+        norm_reduce_kernel<P><<<grid, 1024, 0, s>>>(a.part, parts, (int)width, static_cast<P*>(dweight),
+                                                    static_cast<P*>(dbias));
     }
     return 0;
   });

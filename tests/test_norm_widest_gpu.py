@@ -46,3 +46,20 @@ def test_rms_norm_grad(width):
         assert torch.equal(dweight[at : at + STEP].double(), (d * x)[0])
         # |d - x mean| < 2, so half a step of float16 is at most 2^-11, and float32's three roundings 3 * 2^-24
         assert float((dh[:, at : at + STEP].double() - (d - x * mean)).abs().max()) <= 2.0**-11 + 3 * 2.0**-24
+
+
+@pytest.mark.parametrize("width", [(1 << 28) - 64, (1 << 28) + 5])
+def test_layer_norm_grad(width):
+    gen = torch.Generator(device=DEV).manual_seed(2)
+    dy, x = _signs(gen, width), _signs(gen, width)
+    one = torch.ones((1,), device=DEV)
+    dx, dweight, dbias = g.layer_norm_grad(dy, x, torch.zeros_like(one), one)
+    along = _dot(dy, x, width) / width
+    mean = sum(float(dy[:, at : at + STEP].sum(dtype=torch.float64)) for at in range(0, width, STEP)) / width
+    assert abs(mean) + abs(along) < 2.0**-5
+    assert torch.equal(dbias, dy[0])
+    for at in range(0, width, STEP):
+        d, v = dy[:, at : at + STEP].double(), x[:, at : at + STEP].double()
+        assert torch.equal(dweight[at : at + STEP].double(), (d * v)[0])
+        # as above, with a division and a subtraction more
+        assert float((dx[:, at : at + STEP].double() - (d - mean - v * along)).abs().max()) <= 2.0**-11 + 5 * 2.0**-24
