@@ -36,6 +36,7 @@ HCG_E8M0 = 5
 FP8_BLOCK = 128  # HCG_FP8_BLOCK
 FP8_ALGOS = {"auto": 0, "stream": 1, "256x256": 2, "128x128": 3, "128x64": 4}  # HCG_FP8_*
 FP8_SPLITS = 256
+FP8_MAX_SPLITS = 16
 
 HCG_ALGO_AUTO = 0
 HCG_ALGO_TILED = 1

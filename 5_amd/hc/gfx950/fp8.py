@@ -146,6 +146,18 @@ def _scale_arg(torch: Any, scale: Any, what: str, index: int) -> int:
     return code
 
 
+def _algo_number(algo: Any) -> int:
+    """HCG_FP8_* of a form's name, or of "128x128/4", K in four parts."""
+    name, _, splits = str(algo).partition("/")
+    number = _native.FP8_ALGOS.get(name)
+    plain = splits.isascii() and splits.isdigit() and len(splits) < 9
+    parts = int(splits) if plain else 0
+    if number is None or (splits and not plain) or parts > _native.FP8_MAX_SPLITS or (number == 0 and parts):
+        raise LaunchError(f"unknown algo {algo!r}; expected one of {', '.join(_native.FP8_ALGOS)}, the forms after auto "
+                          f"also with /1 to /{_native.FP8_MAX_SPLITS} for so many parts of the inputs")
+    return number + _native.FP8_SPLITS * parts
+
+
 def linear_fp8(x: Any, x_scale: Any, weight: Any, weight_scale: Any, *, out_dtype: Any | None = None,
                out: Any | None = None, algo: str = "auto") -> Any:
     """``x @ weight.T`` of two quantised matrices: ``x`` (..., inputs),
@@ -188,11 +200,7 @@ def linear_fp8(x: Any, x_scale: Any, weight: Any, weight_scale: Any, *, out_dtyp
     if not tile and tuple(weight_scale.shape) != (outputs, blocks):
         raise LaunchError(f"weight_scale shape {tuple(weight_scale.shape)} is neither {(outputs, blocks)} (rows) nor "
                           f"{(_blocks(outputs), blocks)} (tiles)")
-    name, _, splits = str(algo).partition("/")  # "128x128/4": K in four parts
-    number = _native.FP8_ALGOS.get(name)
-    if number is None or (splits and not splits.isdigit()):
-        raise LaunchError(f"unknown algo {algo!r}; expected one of {', '.join(_native.FP8_ALGOS)}")
-    number += _native.FP8_SPLITS * int(splits or 0)
+    number = _algo_number(algo)
     if out is not None:
         out_dtype = out.dtype if out_dtype is None and isinstance(out, torch.Tensor) else out_dtype
     out_dtype = torch.bfloat16 if out_dtype is None else out_dtype
