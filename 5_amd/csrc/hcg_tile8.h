@@ -279,8 +279,8 @@ __global__ __launch_bounds__(64 * WM * WN, waves_per_simd(TM, TN, WM* WN)) void 
   // zeros.
   constexpr int kHeld = by_power(SC) ? 1 : 4;
   const int quad = lane >> 4;
-  static_assert(NI == 2 || NI == 4 || NI == 8, "tokens' scales");
-  const int at_x = (nfirst + (lane & (16 * NI - 1) & 63)) * kHeld;
+  static_assert(NI == 2 || NI == 4, "tokens' scales");
+  const int at_x = (nfirst + (lane & (16 * NI - 1))) * kHeld;
   const int at_w = by_tile(SC)    ? mfirst / kBlock * kHeld
                    : by_power(SC) ? mfirst + (lane & (16 * MI - 1) & 63)
                                   : (mfirst + 4 * quad) * kHeld;
@@ -291,7 +291,7 @@ __global__ __launch_bounds__(64 * WM * WN, waves_per_simd(TM, TN, WM* WN)) void 
   // As loaded: of 64 of the wave's tokens or outputs, one a lane (a load for each
   // group of 16 would take as many of the CU's address cycles as a third of the
   // operands' DMA).
-  constexpr int kXs = NI > 4 ? NI / 4 : 1, kEws = SC == kPowerRow && MI > 4 ? MI / 4 : 1;
+  constexpr int kXs = (NI + 3) / 4, kEws = SC == kPowerRow ? (MI + 3) / 4 : 1;
   struct Loaded {
     uint32_t x[kXs], ew[kEws];
     f32x4 w[SC == kRow ? MI : 1];
@@ -493,15 +493,9 @@ __global__ __launch_bounds__(64 * WM * WN, waves_per_simd(TM, TN, WM* WN)) void 
       if constexpr (kLate > 1 && i == kEarly - 1) rz = OpA::frag(sa, base_a, i + 2);
       dma(ic);
       product(Int<i * NI>{}, fa, fb[0], s);
-      if constexpr (NI > 1) product(Int<i * NI + 1>{}, fa, fb[1], s);
+      product(Int<i * NI + 1>{}, fa, fb[1], s);
       if constexpr (NI > 2) product(Int<i * NI + 2>{}, fa, fb[2], s);
       if constexpr (NI > 3) product(Int<i * NI + 3>{}, fa, fb[3], s);
-      if constexpr (NI > 4) {
-        product(Int<i * NI + 4>{}, fa, fb[4], s);
-        product(Int<i * NI + 5>{}, fa, fb[5], s);
-        product(Int<i * NI + 6>{}, fa, fb[6], s);
-        product(Int<i * NI + 7>{}, fa, fb[7], s);
-      }
       if constexpr (i == kHalf - 1) {
         wait_vm<OpA::kInst>();  // the next stage's two units have landed
         if constexpr (i < kEarly - 1) {
@@ -516,7 +510,6 @@ __global__ __launch_bounds__(64 * WM * WN, waves_per_simd(TM, TN, WM* WN)) void 
     if constexpr (kEarly > 3) step(Int<3>{});
     if constexpr (kEarly > 4) step(Int<4>{});
     if constexpr (kEarly > 5) step(Int<5>{});
-    if constexpr (kEarly > 6) step(Int<6>{});
     static_assert(MI == 2 || MI == 4 || MI == 8, "steps");
     wait_lgkm();
     __builtin_amdgcn_s_barrier();
@@ -537,15 +530,9 @@ __global__ __launch_bounds__(64 * WM * WN, waves_per_simd(TM, TN, WM* WN)) void 
       __builtin_amdgcn_sched_barrier(0);
     };
     late(Int<0>{});
-    if constexpr (NI > 1) late(Int<1>{});
+    late(Int<1>{});
     if constexpr (NI > 2) late(Int<2>{});
     if constexpr (NI > 3) late(Int<3>{});
-    if constexpr (NI > 4) {
-      late(Int<4>{});
-      late(Int<5>{});
-      late(Int<6>{});
-      late(Int<7>{});
-    }
     now = spread(next);
     load_scales(next);
     finish(s);
