@@ -431,7 +431,7 @@ __global__ __launch_bounds__(1024) void norm_reduce_kernel(const float* part, in
   P* out = blockIdx.z ? dbias : dweight;
   if (out == nullptr) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t c = hcg::workgroup() * 64 + lane;
+  const int64_t c = hcg::workgroup_short() * 64 + lane;
   float sum = 0.f;
   if (c < width) {
     const float* p = part + (int64_t)blockIdx.z * width + c;

@@ -508,7 +508,7 @@ template <class P>
 __global__ __launch_bounds__(1024) void rms_reduce_kernel(const float* part, int parts, int width, P* dweight) {
   __shared__ float meet[16][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t c = hcg::workgroup() * 64 + lane;
+  const int64_t c = hcg::workgroup_short() * 64 + lane;
   float sum = 0.f;
   if (c < width) {
 #pragma unroll 16

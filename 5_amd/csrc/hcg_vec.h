@@ -156,11 +156,14 @@ __device__ __forceinline__ float wave_max(float v) {
 // The grid of n workgroups, in two dimensions past 2^20 of them (a launch's
 // threads along one are fewer than 2^32), and a workgroup's number in it, which
 // may be n or more.
+constexpr int kGridShift = 20;
 inline dim3 grid_of(int64_t n) {
-  const int64_t x = n < (1 << 20) ? n : 1 << 20;
+  const int64_t x = n < (1 << kGridShift) ? n : 1 << kGridShift;
   return dim3((unsigned)x, (unsigned)((n + x - 1) / x));
 }
 __device__ __forceinline__ int64_t workgroup() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
+// The same for a kernel so short that gridDim, a load, shows.
+__device__ __forceinline__ int64_t workgroup_short() { return ((int64_t)blockIdx.y << kGridShift) + blockIdx.x; }
 
 // Host: the shape and pointer rules that every row-wise entry point has.
 inline int elem_bytes(int dtype) { return dtype == HCG_F32 ? 4 : 2; }
