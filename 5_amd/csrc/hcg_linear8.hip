@@ -110,13 +110,13 @@ __device__ __forceinline__ float scale_at(const void* p, int64_t at) {
   return static_cast<const float*>(p)[at];
 }
 
-// For few tokens, bound by reading the weight (8192 x 8192: one token 12.9 us, 5.2
-// TB/s, 16 tokens 14.7).  A workgroup takes 16 R rows of the weight and 16 NI tokens;
+// For few tokens, bound by reading the weight (8192 x 8192: one token 12.8 us, 5.2
+// TB/s, 16 tokens 14.5).  A workgroup takes 16 R rows of the weight and 16 NI tokens;
 // its waves take the blocks of K in turn, each an own load of both operands, a block
 // ahead, and their sums meet in LDS, in the order of the waves.  Workgroups start at
 // blocks of their own (a golden-ratio sequence) and wrap: rows a power of two apart
 // put what is read at one k on a few HBM channels (4096 x 4096, one token: 5.9 -> 4.7
-// us).
+// us in one run; passes over several weights take 5.4, and 6.8 for 16 tokens).
 // Waves, that is, parts of K: as many again where a workgroup has 16 rows.
 constexpr int stream_waves(int r) { return r == 1 ? 8 : 4; }
 
@@ -352,7 +352,10 @@ constexpr int64_t kMaxTiles = (int64_t)1 << 22;  // of a launch: its threads are
 // eight waves (`fixed`) or by four (`lo`), or the weight from HBM.  Split sums: a
 // launch, and their MB per us.  Fitted to 100000 times of 9000 random sizes of up to
 // 16384, every form and 1 to 16 splits; the pick is within 2.1% of the fastest in the
-// mean, and within 10% at 90% of the sizes.
+// mean, and within 10% at 90% of the sizes.  (It ranks forms and foretells no times:
+// one token by 8192 x 8192 comes out at 18.9 us for 12.8.  Where it loses, us picked /
+// best: 32 tokens by 8192 x 8192 19.2 / 17.2, 64 by it 20.9 / 18.9, 256 by 4096 x 4096
+// 20.4 / 17.6.)
 struct Cost {
   double launch, fixed, lo, hi, join, join_rate, rate;
 };
@@ -387,7 +390,8 @@ struct Problem {
 // 16 rows per workgroup of the streaming form (by eight waves), or 32 (by four),
 // which read x half as often: what gives a CU less to read.  us, 16 / 32 rows, one
 // token by 8192 x 8192 12.2 / 11.4, 16 tokens 16.7 / 12.9, 64 tokens 37.9 / 24.3; one
-// by 4096 x 4096 4.6 / 6.1, 16 by it 5.8 / 7.4.
+// by 4096 x 4096 4.6 / 6.1, 16 by it 5.8 / 7.4 (both sides in one run; passes over
+// several weights take 12.8, 14.5, 5.4 and 6.8).
 int stream_rows(int64_t tokens, int64_t outputs, int splits) {
   const int64_t tiles = ceil_div(tokens, 64) * splits, n = std::min<int64_t>(tokens, 64);
   const int64_t one = ceil_div(ceil_div(outputs, 16) * tiles, kCus) * (16 + n);

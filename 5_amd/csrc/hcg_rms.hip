@@ -12,7 +12,8 @@
 // the 16 or 32 lanes that hold them, by exchanges.  8192 x 4096: to 8 bits with a
 // bf16 residual 45 us (5.2 TB/s), f16 with a float32 residual 82 us (4.9), bf16
 // gradient with the residual's 46.5 us (5.8) and 4.7 for the columns' sums; one row
-// 3.8 us, a launch and its latency.
+// 3.8 us, a launch and its latency.  Wider rows, whole passes: 4096 x 8192 to 8 bits
+// 55, 2048 x 16384 70 (1024 lanes of four vectors, half of them idle).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -305,8 +306,10 @@ struct RmsGradArgs {
 // 256 workgroups, one per CU.  GROUPS row groups of LANES lanes; group q of
 // workgroup b takes rows b * GROUPS + q, + gridDim.x * GROUPS, ... and keeps its
 // columns' sums of dy xh in registers; the groups' sums meet in LDS once, at the
-// end.  AHEAD: a row's loads go out before the work on the row before it (not by
-// 1024 threads with two vectors each, whose registers do not hold both).  Rows hold a
+// end.  AHEAD: a row's loads go out before the work on the row before it.  Not by 1024
+// threads with two vectors each, whose registers do not hold both; with a float32 h
+// beside a 16-bit dy they do not hold one either (22 of them spill): 2048 x 16384 bf16
+// 66.8 us (4.0 TB/s with the sums), with a float32 h 127 (3.7).  Rows hold a
 // vector or more, so that no load is behind a branch: the number of those in flight
 // would not be known after it, and a row would wait for the next row's as well (8192 x
 // 4096 bf16 51.2 -> 46.5 us, 3001 x 1027 float32 12.6 -> 12.0; with the sums 55.2 ->
@@ -442,7 +445,8 @@ __global__ __launch_bounds__(LANES * GROUPS) void rms_grad_kernel(RmsGradArgs g)
 }
 
 // Rows too wide for registers: a workgroup per row for dh (two passes); the
-// column sums follow by rms_columns_kernel.
+// column sums follow by rms_columns_kernel.  Three readings of dy and h: 2048 x 16384
+// float32 174 us, 3.1 TB/s of what one reading takes.
 template <class T, class H>
 __global__ __launch_bounds__(1024) void rms_grad_wide_kernel(RmsGradArgs g) {
   constexpr int E = kVec<T>;

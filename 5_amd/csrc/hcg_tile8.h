@@ -7,24 +7,26 @@
 // the weight's, two for x's (160 KB for 256 x 256).  The 16-byte chunks of an LDS
 // row are XOR-swizzled so that the lanes that an LDS cycle serves cover all banks.
 //
-// 256 x 256 tiles by eight waves, 8192^3: 412 us with float32 scales (2.67
-// PFLOP/s), 361 with e8m0 ones (3.05); a library's product of the same size with one
-// scale for all took 340 to 350 on the same cards (3.2), so that the scaling of a
-// block's sums (16 multiply-adds per lane and four products) costs a seventh.
-// Float32 scales of the weight's rows 594 us in 128 x 128 tiles, a multiplication
-// more per sum; exact products with them 956 (1.15 PFLOP/s; a 16-bit product 742):
-// the conversions and scalings issue as long as the MFMAs take.  Alone on a CU a
-// 256 x 256 stage takes 1.04 us (2500 cycles for 2048 of MFMA issue), on a busy chip
-// 1.47 at a lower clock.  Four-wave and sixteen-wave tiles spill or are slower (478
-// us by sixteen).
+// 256 x 256 tiles by eight waves, 8192^3, passes back to back on one card: 450 us
+// with float32 scales (2.44 PFLOP/s), 398 with e8m0 ones (2.76; 381 on another
+// card); a library's product of the same size with one scale for all 350 (3.14), so
+// that the scaling of a block's sums (16 multiply-adds per lane and four products)
+// costs an eighth.  Float32 scales of the weight's rows 657 us in 128 x 128 tiles, a
+// multiplication more per sum; exact products with them 1039 (1.06 PFLOP/s; a 16-bit
+// product 809): of 21 instructions per 128-deep product 4 are MFMAs, 8 scale and 8
+// convert, every fragment in the two waves that hold it.  Alone on a CU a 256 x 256
+// stage takes 1.04 us (2500 cycles for 2048 of MFMA issue), on a busy chip 1.47 at a
+// lower clock.  Four-wave tiles spill; sixteen-wave ones took 478 us where eight took
+// 412.
 //
 // A 16-bit result takes v_mfma_f32_16x16x128 on the bytes as they are: a block's
 // products in one instruction, whose sum is multiplied by both scales into the
 // accumulators, or whose scales are the instruction's own (e8m0), which then
 // adds up all of K.  The instruction cuts each product of 8 neighbours to
 // multiples of 2^-13 of the largest exponent among them (measured: beside 448 *
-// 448 the bits below 2^3 are lost), 1.5e-5 of a sum of 128 random products: less
-// than a 16-bit result's rounding, but not float32.  So a float32 result (EXACT)
+// 448 the bits below 2^3 are lost), 1.5e-5 of a sum of normal products, and up to 8e-5
+// where one column in a hundred is sixteen times the others: less than a 16-bit
+// result's rounding (2.1e-4 for f16), but not float32.  So a float32 result (EXACT)
 // takes the bytes as f16, which holds both formats, in v_mfma_f32_16x16x32,
 // whose sums are within 2^-22 of the magnitudes.
 #pragma once

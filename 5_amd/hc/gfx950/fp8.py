@@ -170,8 +170,9 @@ def linear_fp8(x: Any, x_scale: Any, weight: Any, weight_scale: Any, *, out_dtyp
     or float32; that of ``out``).  A float32 one has float32 sums of exact
     products, at the rate of 16-bit products.  A 16-bit one comes from the 8-bit
     matrix instructions: sums are float32, but each product is cut below 2^-13 of
-    the largest among 8 neighbours (about 1.5e-5 of the result) before the
-    result's own rounding.  Rows that start at multiples of 16 bytes, as
+    the largest among 8 neighbours (1.5e-5 of the results for normal operands, up
+    to 8e-5 where a few columns are much larger than the others) before the result's
+    own rounding.  ``algo`` forces a form, for measurements.  Rows that start at multiples of 16 bytes, as
     :func:`quantize_fp8` makes them, are read where they lie."""
     torch = _torch()
     if out is None and algo == "auto":

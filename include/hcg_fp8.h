@@ -57,8 +57,10 @@ int hcg_rms_norm_fp8(int dtype, const void* x, int64_t ldx, int64_t rows, int64_
  * each 128 inputs are added up in float32, times both scales (their float32
  * product), and so are the blocks.  For a HCG_F32 y the products are exact.  A
  * 16-bit y is rounded once, and its products come from the 8-bit matrix
- * instructions, which cut each of 8 neighbours below 2^-13 of the largest of them
- * (about 1.5e-5 of a result, at most 2^-10 of the sum of magnitudes).  Operands
+ * instructions, which cut each of 8 neighbours below 2^-13 of the largest of them:
+ * 1.5e-5 of the results for normal operands, up to 8e-5 where a few columns are much
+ * larger than the others, at most 2^-10 of the sum of magnitudes.  (With HCG_E8M0
+ * scales these instructions multiply by them and add up all of inputs.)  Operands
  * need no alignment; rows that start at multiples of 16 bytes are read where they lie,
  * others may be copied to scratch first.  inputs and the row strides are below
  * 4,000,000, tokens and outputs below 2^26.
@@ -72,7 +74,7 @@ int hcg_rms_norm_fp8(int dtype, const void* x, int64_t ldx, int64_t rows, int64_
 #define HCG_FP8_128x64 4
 #define HCG_FP8_SPLITS 256 /* times a number up to 16, added to a form: K in so many parts */
 
-/* (The scratch of a call that hcg_linear_fp8 refuses is 0: the call says why.) */
+/* (0 for sizes and forms that hcg_linear_fp8 refuses, which says why.) */
 int64_t hcg_linear_fp8_workspace(int algo, int64_t tokens, int64_t outputs, int64_t inputs, const void* x, int64_t ldx,
                                  const void* weight, int64_t ldw, int scale_dtype, int64_t xs_row, int w_tile,
                                  const void* w_scale, int64_t ws_row, int64_t ws_block, int out_dtype);
