@@ -16,6 +16,7 @@ where inputs require gradients.
 
 from __future__ import annotations
 
+import math
 import sys
 from typing import Any
 
@@ -91,7 +92,7 @@ def _rows(t: Any, what: str) -> Any:
     next to each other: a view where the strides allow it, else a copy."""
     if t.ndim == 0:
         raise LaunchError(f"{what} must have at least one dimension")
-    m = t if t.ndim == 2 else t.reshape(-1, t.shape[-1]) if t.numel() else t.new_empty((0, t.shape[-1]))
+    m = t if t.ndim == 2 else t.reshape(math.prod(t.shape[:-1]), t.shape[-1])
     rows, width = m.shape
     if (width > 1 and m.stride(1) != 1) or (rows > 1 and m.stride(0) < width):
         m = m.contiguous()
